@@ -389,6 +389,111 @@ int tpp_decode_advance(const int64_t* next_tokens, int64_t* out_ids, int64_t ld_
                        int64_t out_cap, int32_t* positions, int32_t* seqlens, int64_t B,
                        void* stream);
 
+/* ---- draft trees (speculative decoding) ------------------------------------
+ * A step verifies T drafted tokens a sequence at once.  They form a tree: node
+ * 0 is the root (the last token already chosen, whose K/V is not in the cache
+ * yet), parents[i] < i, and node i stands at position ctx_lens[b] + its depth.
+ * The nodes' K and V stay beside the cache, [B, T, Hkv, D]; once the target has
+ * verified the tree the accepted path's rows are copied into the cache.  The
+ * reference has no counterpart (its speculative decoding is a stub). */
+
+/* Per-head q/k RMSNorm (qn_w / kn_w [D], either may be NULL) and rotate-half
+ * RoPE at positions[b, t] of the raw projection rows qkv [B, T, (Hq+2Hkv)*D]
+ * (q heads, then k, then v; batch stride qkv_sb, token stride qkv_st) into
+ * contiguous q_out [B, T, Hq, D] and k_out [B, T, Hkv, D]; the v part needs no
+ * copy.  cos/sin: tables [table_rows, D]; a position outside them gives zero
+ * rows.  D one of 16, 32, 64, 128, 256. */
+int tpp_qk_norm_rope_tree(const void* qkv, int64_t qkv_sb, int64_t qkv_st, const void* qn_w,
+                          const void* kn_w, float eps, const void* cos, const void* sin,
+                          int64_t cs_stride, int64_t table_rows, int cs_dtype,
+                          const int32_t* positions, void* q_out, void* k_out, int64_t B,
+                          int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int dtype,
+                          void* stream);
+
+/* Bytes of workspace tpp_attention_tree(_paged) needs (0: none). */
+int64_t tpp_attention_tree_workspace(int64_t B, int64_t T, int64_t Hq, int64_t Hkv,
+                                     int64_t max_ctx, int64_t D, int64_t window_left);
+
+/* Attention of a tree's T nodes (1..256) over the cache and the tree:
+ *   o[b,i,h] = sum_j w_j v_j / sum_j w_j,   w_j = exp(scale * q[b,i,h].k_j)
+ * over cache rows j < ctx_lens[b] (0 <= ctx_lens[b] <= max_ctx <= cache rows;
+ * values outside are clamped) and the nodes j whose bit j % 64 of
+ * mask[b, i, j / 64] is set (mask uint64 [B or 1][T][ceil(T/64)], batch stride
+ * mask_sb, 0 to share one).  window_left >= 0 drops the cache rows below
+ * p - window_left, where node i's position p is ctx_lens[b] + popcount(mask row)
+ * - 1.  A row that sees nothing gives zeros.  What a row does not see has no
+ * effect on it, NaN and infinities included.  q [B,T,Hq,D], k_tree / v_tree
+ * [B,T,Hkv,D], o [B,T,Hq,D] by (batch, token, head) strides, caches
+ * [B,Hkv,Smax,D] as tpp_attention_decode; D 64 or 128. */
+int tpp_attention_tree(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
+                       const void* k_cache, const void* v_cache, int64_t c_sb, int64_t c_sh,
+                       int64_t c_ss, const void* k_tree, int64_t kt_sb, int64_t kt_st,
+                       int64_t kt_sh, const void* v_tree, int64_t vt_sb, int64_t vt_st,
+                       int64_t vt_sh, const int32_t* ctx_lens, int64_t max_ctx,
+                       const uint64_t* mask, int64_t mask_sb, void* o, int64_t o_sb,
+                       int64_t o_st, int64_t o_sh, int64_t B, int64_t T, int64_t Hq,
+                       int64_t Hkv, int64_t D, int64_t window_left, float scale,
+                       void* workspace, int64_t workspace_bytes, int dtype, void* stream);
+/* The same over block pools [num_blocks][Hkv][64][D] (see the paged cache
+ * above); block_table [B][table_cols], row stride table_stride.  max_ctx <=
+ * 64 * table_cols; a block number outside the pools reads as zeros. */
+int tpp_attention_tree_paged(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
+                             const void* k_pool, const void* v_pool, int64_t num_blocks,
+                             const int32_t* block_table, int64_t table_stride,
+                             const void* k_tree, int64_t kt_sb, int64_t kt_st, int64_t kt_sh,
+                             const void* v_tree, int64_t vt_sb, int64_t vt_st, int64_t vt_sh,
+                             const int32_t* ctx_lens, int64_t max_ctx, const uint64_t* mask,
+                             int64_t mask_sb, void* o, int64_t o_sb, int64_t o_st, int64_t o_sh,
+                             int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                             int64_t window_left, float scale, void* workspace,
+                             int64_t workspace_bytes, int dtype, void* stream);
+
+/* Verifies each sequence's drafted tree against the target's logits
+ * [B, T, V] (f16, bf16 or f32; strides l_sb, l_st), with given uniform numbers
+ * u [B, T] in [0, 1): walking from the root, the children i of the current node
+ * are tried in index order with u[b, i], the walk descends to the first one
+ * accepted, and where none is, the next token is drawn with u[b, 0] from what
+ * is left of the target's distribution there.
+ *   p = softmax(logits[b, node] / temperature)
+ *   no draft logits (proposals without a distribution): child token t is
+ *     accepted if u < p(t) / (mass of p left); rejected, p(t) becomes 0;
+ *   draft logits [B, >= T-1, V] of the draft that drew each node's children
+ *     (same temperature, d_sb, d_st): q = softmax of the node's row; t is
+ *     accepted if u * q(t) < p(t); rejected, p becomes max(p - q, 0) over its
+ *     sum (p stays where that sum is 0).
+ * Either way the emitted tokens follow the target's distribution.
+ * temperature == 0: p is 1 at the largest logit (lowest index on ties; u and
+ * the draft logits are not read and may be NULL).
+ * Sums and cumulative sums run over whole multiples of 2^-40, so results do
+ * not depend on how a row is split.  NaN logits count as -inf; a row
+ * with no weight (all -inf, or +inf at temperature > 0) accepts no child and
+ * draws -1.  tokens int64 [B, T] (stride tok_sb; one outside [0, V) is
+ * rejected), parents int32 (stride par_sb, 0 to share one tree).
+ * Outputs: path int32 [B, T] (accepted nodes from the root on, then -1), count
+ * int32 [B] (nodes on the path, >= 1), next_token int64 [B]. */
+int tpp_verify_tree(const void* logits, int64_t l_sb, int64_t l_st, const void* draft_logits,
+                    int64_t d_sb, int64_t d_st, const int64_t* tokens, int64_t tok_sb,
+                    const int32_t* parents, int64_t par_sb, const float* u, int64_t u_sb,
+                    double temperature, int32_t* path, int32_t* count, int64_t* next_token,
+                    int64_t B, int64_t T, int64_t V, int dtype, void* stream);
+
+/* Copies the accepted path's K/V rows of all L layers into the caches:
+ *   cache[l, b, h, ctx_lens[b] + i, :] = tree[l, b, path[b, i], h, :],
+ * i < count[b] (at most T).  Trees by strides (layer, batch, node, head); caches
+ * [L][B][Hkv][rows][D] by strides c_sl, c_sb, c_sh, c_ss, or, with
+ * block_table, pools [L][num_blocks][Hkv][64][D] (layer stride c_sl; c_sb,
+ * c_sh, c_ss unused, rows = 64 * table columns).  A destination row or
+ * block, or a node, outside its range is skipped.  D a multiple of 8, rows
+ * 16-byte aligned. */
+int tpp_kv_commit(const void* k_tree, int64_t kt_sl, int64_t kt_sb, int64_t kt_st,
+                  int64_t kt_sh, const void* v_tree, int64_t vt_sl, int64_t vt_sb,
+                  int64_t vt_st, int64_t vt_sh, const int32_t* path, int64_t path_sb,
+                  const int32_t* count, const int32_t* ctx_lens, void* k_cache, void* v_cache,
+                  int64_t c_sl, int64_t c_sb, int64_t c_sh, int64_t c_ss, int64_t rows,
+                  int64_t num_blocks, const int32_t* block_table, int64_t table_stride,
+                  int64_t L, int64_t B, int64_t T, int64_t Hkv, int64_t D, int dtype,
+                  void* stream);
+
 /* ---- persistent single-sequence decode step ------------------------------- */
 /* Row pitch of the persistent step's weights: `in` + TPP_PERSISTENT_ROW_PAD
  * elements.  The padding (never read) shifts consecutive rows by 16

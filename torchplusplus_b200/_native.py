@@ -100,6 +100,22 @@ SIGNATURES: dict[str, tuple] = {
                              _i64, _i64, _i64, _i64, _i64, _p, _i32, _p]),
     "tpp_argmax": (_i32, [_p, _i64, _i64, _i64, _p, _i32, _p]),
     "tpp_embedding": (_i32, [_p, _i64, _p, _i64, _i64, _p, _i32, _p]),
+    "tpp_qk_norm_rope_tree": (_i32, [_p, _i64, _i64, _p, _p, _f32, _p, _p, _i64, _i64, _i32, _p,
+                                     _p, _p, _i64, _i64, _i64, _i64, _i64, _i32, _p]),
+    "tpp_attention_tree_workspace": (_i64, [_i64] * 7),
+    "tpp_attention_tree": (_i32, [_p, _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _i64, _i64,
+                                  _i64, _p, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _i64,
+                                  _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _p, _i64, _i32,
+                                  _p]),
+    "tpp_attention_tree_paged": (_i32, [_p, _i64, _i64, _i64, _p, _p, _i64, _p, _i64, _p, _i64,
+                                        _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _p, _i64, _p,
+                                        _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                        _f32, _p, _i64, _i32, _p]),
+    "tpp_verify_tree": (_i32, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _p, _i64, _p, _i64,
+                               C.c_double, _p, _p, _p, _i64, _i64, _i64, _i32, _p]),
+    "tpp_kv_commit": (_i32, [_p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64, _p, _i64, _p,
+                             _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64,
+                             _i64, _i64, _i64, _i32, _p]),
     "tpp_decode_advance": (_i32, [_p, _p, _i64, _i64, _p, _p, _i64, _p]),
 }
 

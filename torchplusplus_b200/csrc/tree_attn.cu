@@ -1,0 +1,574 @@
+// Attention of a drafted tree's nodes over the KV cache and the tree itself
+// (tpp_attention_tree, tpp_attention_tree_paged).
+//
+// The T nodes x G query heads of one kv head are the rows of one unit (b, kv
+// head, row tile): all of them read the same keys, so the cache is streamed
+// once per 16 * RW rows.  Online softmax over tiles of 64 keys, first the cache's
+// (masked only at the context's end and at a window's edge), then the tree's
+// (one 64-bit mask word a row and tile).
+//
+// Warp 4 feeds a ring of K/V tiles by TMA (one request an operand); warps 0-3
+// are RW row groups of 16 rows x KW = 4 / RW key groups, each with its own
+// running maximum and sum (mma.sync m16n8k16 on fragments from ldmatrix, fp32
+// accumulators, exp2 domain); the key groups merge in shared memory at the end.
+//
+// Masked keys: the score becomes -inf and the value is cleared before the
+// product, since 0 * NaN is NaN.  Values that some rows see and others do not
+// (tree tiles, a window's edge) are cleared too where they are not finite, and
+// added afterwards, element by element, to the rows that see them.
+#include <math.h>
+#include "mma_common.cuh"
+#include "tc_common.cuh"
+
+namespace tpp {
+namespace {
+
+constexpr int KT = 64;            // keys of a tile
+constexpr int kThreads = 160;     // 4 compute warps + the producer warp
+constexpr int kMaxNodes = 256;
+constexpr float kRescale = 8.0f;  // log2: the base moves when the maximum grew by 2^8
+
+struct TreeArgs {
+  const void* q; int64_t q_sb, q_st, q_sh;
+  const void* v_cache; int64_t c_sb, c_sh, c_ss;  // for values that are not finite
+  const void* v_tree; int64_t vt_sb, vt_st, vt_sh;
+  const int32_t* ctx_lens; int max_ctx;
+  const uint64_t* mask; int64_t mask_sb;
+  void* o; int64_t o_sb, o_st, o_sh;
+  const int32_t* table; int64_t table_stride; int num_blocks;
+  int64_t window_left;
+  float scale_log2;
+  int B, T, Hq, Hkv, G, W, R, RT, NT;  // W mask words a row, R = T * G rows, NT tree tiles
+  int* err;
+};
+
+template <int D, int RW>
+struct TreeSmem {
+  static constexpr int KW = 4 / RW;
+  static constexpr int kStages = D == 128 ? 3 : 6;
+  static constexpr uint32_t kTile = KT * D * 2;
+  static constexpr uint32_t kRing = kStages * 2 * kTile;
+  static constexpr int kDims = RW == 1 ? D : 64;  // dims merged at a time
+  static constexpr uint32_t kMerge = KW > 1 ? RW * 16 * kDims * 4 : 0;
+  static constexpr uint32_t kMl = 4 * 16 * 2 * 4;  // (m, l) of each warp's rows
+  static constexpr size_t kBytes = 1024 + kRing + kMerge + kMl + 2 * kStages * 8 + 16;
+};
+
+__device__ __forceinline__ uint32_t sw_addr(uint32_t base, int r, int chunk) {
+  return base + (uint32_t)((chunk >> 3) * KT * 128 + r * 128 + (((chunk & 7) ^ (r & 7)) << 4));
+}
+__device__ __forceinline__ void bar_compute() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+template <typename T> struct ExpMask;
+template <> struct ExpMask<__half> { static constexpr uint32_t value = 0x7c00u; };
+template <> struct ExpMask<__nv_bfloat16> { static constexpr uint32_t value = 0x7f80u; };
+
+// Clears the halves of w that are not finite; `bad` collects whether any was.
+template <typename T>
+__device__ __forceinline__ uint32_t finite2(uint32_t w, uint32_t& bad) {
+  constexpr uint32_t E = ExpMask<T>::value;
+  const uint32_t lo = (w & E) == E ? 0xffffu : 0u;
+  const uint32_t hi = (w & (E << 16)) == (E << 16) ? 0xffff0000u : 0u;
+  bad |= lo | hi;
+  return w & ~(lo | hi);
+}
+
+// One sequence's cache tiles: rows [64 * first, ctx), and the bounds below
+// which a window hides rows from all (lo_all) or from some (lo_some) nodes.
+struct Span {
+  int ctx, first, tiles;
+  int64_t lo_all, lo_some;
+};
+__device__ __forceinline__ Span span_of(const TreeArgs& p, int b) {
+  Span s;
+  s.ctx = min(max(p.ctx_lens[b], 0), p.max_ctx);
+  s.lo_all = s.lo_some = 0;
+  if (p.window_left >= 0) {
+    s.lo_all = max((int64_t)0, (int64_t)s.ctx - 1 - p.window_left);
+    s.lo_some = max((int64_t)0, (int64_t)s.ctx + p.T - 1 - p.window_left);
+  }
+  s.first = (int)(s.lo_all / KT);
+  s.tiles = s.ctx > 0 ? (s.ctx + KT - 1) / KT - s.first : 0;
+  return s;
+}
+// The first cache row that the node with mask row `row` sees.
+__device__ __forceinline__ int64_t low_of(const TreeArgs& p, const Span& s, const uint64_t* row) {
+  if (p.window_left < 0) return 0;
+  int seen = 0;
+  for (int w = 0; w < p.W; ++w) {
+    const int n = p.T - 64 * w;
+    seen += __popcll(row[w] & (n < 64 ? (1ull << n) - 1 : ~0ull));
+  }
+  return (int64_t)s.ctx + seen - 1 - p.window_left;
+}
+
+template <typename T, int D, int RW>
+__global__ void __launch_bounds__(kThreads) tree_attn_kernel(
+    const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+    const __grid_constant__ CUtensorMap tm_kt, const __grid_constant__ CUtensorMap tm_vt,
+    const __grid_constant__ TreeArgs p) {
+  using SM = TreeSmem<D, RW>;
+  constexpr int ST = SM::kStages, KW = SM::KW;
+  constexpr int KPW = KT / KW;    // keys of a tile for each warp
+  constexpr int NTL = KPW / 8;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~(uintptr_t)1023);
+  float* mbuf = reinterpret_cast<float*>(smem + SM::kRing);
+  float* ml = reinterpret_cast<float*>(smem + SM::kRing + SM::kMerge);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + SM::kRing + SM::kMerge + SM::kMl);
+  uint64_t* empty = full + ST;
+  volatile uint32_t* odd = reinterpret_cast<volatile uint32_t*>(empty + ST);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tm_k);
+    prefetch_tmap(&tm_v);
+    prefetch_tmap(&tm_kt);
+    prefetch_tmap(&tm_vt);
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 4);
+    }
+    fence_mbar_init();
+    *odd = 0;
+  }
+  __syncthreads();
+  pdl_wait();
+  pdl_trigger();
+
+  const int rt = blockIdx.x % p.RT;
+  const int kvh = blockIdx.x / p.RT;
+  const int b = blockIdx.y;
+  const Span sp = span_of(p, b);
+  const int ntiles = sp.tiles + p.NT;
+  bool ok = true;
+
+  if (warp == 4) {
+    // ---------------- producer ----------------
+    if (lane == 0) {
+      for (int i = 0; i < ntiles && ok; ++i) {
+        const int s = i % ST;
+        if (i >= ST) ok = mbar_wait(&empty[s], ((i / ST) & 1) ^ 1, p.err, 61);
+        if (!ok) break;
+        uint8_t* kd = smem + s * 2 * SM::kTile;
+        uint8_t* vd = kd + SM::kTile;
+        mbar_arrive_expect_tx(&full[s], 2 * SM::kTile);
+        if (i >= sp.tiles) {
+          const int n0 = (i - sp.tiles) * KT;
+          tma_load_5d(kd, &tm_kt, &full[s], 0, n0, 0, kvh, b);
+          tma_load_5d(vd, &tm_vt, &full[s], 0, n0, 0, kvh, b);
+        } else if (p.table) {
+          // a block outside the pool is out of the map's range: zeros
+          int blk = p.table[b * p.table_stride + sp.first + i];
+          if (blk < 0 || blk >= p.num_blocks) blk = p.num_blocks;
+          tma_load_5d(kd, &tm_k, &full[s], 0, 0, 0, kvh, blk);
+          tma_load_5d(vd, &tm_v, &full[s], 0, 0, 0, kvh, blk);
+        } else {
+          tma_load_5d(kd, &tm_k, &full[s], 0, (sp.first + i) * KT, 0, kvh, b);
+          tma_load_5d(vd, &tm_v, &full[s], 0, (sp.first + i) * KT, 0, kvh, b);
+        }
+      }
+    }
+    return;
+  }
+
+  // ---------------- compute ----------------
+  const int g = lane >> 2, c = lane & 3;
+  const int rw = warp / KW, kw = warp % KW;
+  const int kr0 = kw * KPW;
+  int node[2], head[2];
+  bool live[2];
+  const uint64_t* mrow[2];
+  int64_t lo[2];
+#pragma unroll
+  for (int hr = 0; hr < 2; ++hr) {
+    const int r = rt * 16 * RW + rw * 16 + g + 8 * hr;
+    live[hr] = r < p.R;
+    node[hr] = live[hr] ? r / p.G : 0;
+    head[hr] = kvh * p.G + (live[hr] ? r % p.G : 0);
+    mrow[hr] = p.mask + b * p.mask_sb + (int64_t)node[hr] * p.W;
+    lo[hr] = low_of(p, sp, mrow[hr]);
+  }
+  // Q fragments straight from global memory: each value is used by one lane only
+  uint32_t qf[D / 16][4];
+#pragma unroll
+  for (int hr = 0; hr < 2; ++hr) {
+    const uint32_t* src = reinterpret_cast<const uint32_t*>(
+        static_cast<const T*>(p.q) + b * p.q_sb + node[hr] * p.q_st + head[hr] * p.q_sh);
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      qf[ks][hr] = live[hr] ? src[ks * 8 + c] : 0u;
+      qf[ks][hr + 2] = live[hr] ? src[ks * 8 + c + 4] : 0u;
+    }
+  }
+  float o[D / 8][4];
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  float m_r[2] = {-INFINITY, -INFINITY}, l_r[2] = {0.f, 0.f};
+  uint32_t bad = 0;
+
+  for (int i = 0; i < ntiles; ++i) {
+    const int s = i % ST;
+    if (ok) ok = mbar_wait(&full[s], (i / ST) & 1, p.err, 62);
+    const uint32_t kb = smem_u32(smem + s * 2 * SM::kTile), vb = kb + SM::kTile;
+    float sc[NTL][4];
+#pragma unroll
+    for (int j = 0; j < NTL; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+#pragma unroll
+      for (int jp = 0; jp < NTL / 2; ++jp) {
+        uint32_t bf[4];
+        ldsm_x4(sw_addr(kb, kr0 + jp * 16 + (lane & 7) + (lane >> 4) * 8,
+                        ks * 2 + ((lane >> 3) & 1)), bf);
+        mma<T>(sc[2 * jp], qf[ks], bf[0], bf[1]);
+        mma<T>(sc[2 * jp + 1], qf[ks], bf[2], bf[3]);
+      }
+    }
+    const bool tree = i >= sp.tiles;
+    const int64_t key0 = (int64_t)(sp.first + i) * KT;   // of a cache tile
+    const bool careful = tree || key0 + KT > sp.ctx || key0 < sp.lo_some;
+    if (tree) {
+      const int n0 = (i - sp.tiles) * KT, n = p.T - n0;
+      const uint64_t in = n < 64 ? (1ull << n) - 1 : ~0ull;
+      const uint64_t w0 = mrow[0][i - sp.tiles] & in, w1 = mrow[1][i - sp.tiles] & in;
+#pragma unroll
+      for (int j = 0; j < NTL; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int k = kr0 + j * 8 + 2 * c + (e & 1);
+          sc[j][e] = (((e < 2 ? w0 : w1) >> k) & 1) ? sc[j][e] * p.scale_log2 : -INFINITY;
+        }
+    } else if (careful) {
+#pragma unroll
+      for (int j = 0; j < NTL; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int64_t k = key0 + kr0 + j * 8 + 2 * c + (e & 1);
+          sc[j][e] = (k < sp.ctx && k >= lo[e >> 1]) ? sc[j][e] * p.scale_log2 : -INFINITY;
+        }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NTL; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[j][e] *= p.scale_log2;
+    }
+    // Online softmax with a lazy base: m_r moves, and o and l are rescaled,
+    // only when a row's maximum grew by more than 2^8.
+    float corr[2];
+    bool grow = false;
+#pragma unroll
+    for (int hr = 0; hr < 2; ++hr) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < NTL; ++j) mx = fmax3(mx, sc[j][2 * hr], sc[j][2 * hr + 1]);
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      corr[hr] = 1.f;
+      if (mx > m_r[hr] + kRescale) {
+        corr[hr] = ex2_ftz(m_r[hr] - mx);  // 0 when no key was seen yet
+        m_r[hr] = mx;
+        grow = true;
+      }
+      const float base = m_r[hr] == -INFINITY ? 0.f : m_r[hr];
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < NTL; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float pv = ex2_ftz(sc[j][2 * hr + e] - base);
+          sc[j][2 * hr + e] = pv;
+          sum += pv;
+        }
+      l_r[hr] = l_r[hr] * corr[hr] + sum;
+    }
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+      for (int d = 0; d < D / 8; ++d) {
+        o[d][0] *= corr[0]; o[d][1] *= corr[0];
+        o[d][2] *= corr[1]; o[d][3] *= corr[1];
+      }
+    }
+#pragma unroll
+    for (int kk = 0; kk < KPW / 16; ++kk) {
+      // the probabilities are rounded to T for the product: the same relative
+      // error as the values themselves carry
+      uint32_t pa[4];
+      pa[0] = pack2<T>(sc[2 * kk][0], sc[2 * kk][1]);
+      pa[1] = pack2<T>(sc[2 * kk][2], sc[2 * kk][3]);
+      pa[2] = pack2<T>(sc[2 * kk + 1][0], sc[2 * kk + 1][1]);
+      pa[3] = pack2<T>(sc[2 * kk + 1][2], sc[2 * kk + 1][3]);
+      uint32_t keep0 = ~0u, keep1 = ~0u;  // values no row sees: stale rows of a cache
+      if (careful && !tree) {
+        const int64_t k = key0 + kr0 + kk * 16 + 2 * c;
+        auto in = [&](int64_t x) { return x < sp.ctx && x >= sp.lo_all; };
+        keep0 = (in(k) ? 0xffffu : 0u) | (in(k + 1) ? 0xffff0000u : 0u);
+        keep1 = (in(k + 8) ? 0xffffu : 0u) | (in(k + 9) ? 0xffff0000u : 0u);
+      }
+#pragma unroll
+      for (int dp = 0; dp < D / 16; ++dp) {
+        uint32_t bf[4];
+        ldsm_x4_t(sw_addr(vb, kr0 + kk * 16 + (lane & 7) + ((lane >> 3) & 1) * 8,
+                          dp * 2 + (lane >> 4)), bf);
+        if (careful) {
+          bf[0] = finite2<T>(bf[0] & keep0, bad);
+          bf[1] = finite2<T>(bf[1] & keep1, bad);
+          bf[2] = finite2<T>(bf[2] & keep0, bad);
+          bf[3] = finite2<T>(bf[3] & keep1, bad);
+        }
+        mma<T>(o[2 * dp], pa, bf[0], bf[1]);
+        mma<T>(o[2 * dp + 1], pa, bf[2], bf[3]);
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty[s]);
+  }
+  if (bad) *odd = 1;
+
+  // ---------------- merge the key groups ----------------
+#pragma unroll
+  for (int hr = 0; hr < 2; ++hr) {
+    l_r[hr] += __shfl_xor_sync(0xffffffffu, l_r[hr], 1);
+    l_r[hr] += __shfl_xor_sync(0xffffffffu, l_r[hr], 2);
+  }
+  if (KW > 1) {
+    if (c == 0) {
+#pragma unroll
+      for (int hr = 0; hr < 2; ++hr) {
+        ml[(warp * 16 + g + 8 * hr) * 2] = m_r[hr];
+        ml[(warp * 16 + g + 8 * hr) * 2 + 1] = l_r[hr];
+      }
+    }
+    bar_compute();
+#pragma unroll
+    for (int hr = 0; hr < 2; ++hr) {
+      float M = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int w = 0; w < KW; ++w) M = fmaxf(M, ml[((rw * KW + w) * 16 + g + 8 * hr) * 2]);
+      const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {
+        const float* x = ml + ((rw * KW + w) * 16 + g + 8 * hr) * 2;
+        L += x[1] * ex2_ftz(x[0] - base);
+      }
+      const float f = ex2_ftz(m_r[hr] - base);
+#pragma unroll
+      for (int d = 0; d < D / 8; ++d) {
+        o[d][2 * hr] *= f;
+        o[d][2 * hr + 1] *= f;
+      }
+      m_r[hr] = M;
+      l_r[hr] = L;
+    }
+    // group k hands its sum to group k - 1, in this order always
+#pragma unroll
+    for (int k = KW - 1; k > 0; --k)
+#pragma unroll
+      for (int d0 = 0; d0 < D / 8; d0 += SM::kDims / 8) {
+        float2* buf = reinterpret_cast<float2*>(mbuf) + rw * 16 * SM::kDims / 2 + lane;
+        if (kw == k) {
+#pragma unroll
+          for (int d = 0; d < SM::kDims / 8; ++d) {
+            buf[(2 * d) * 32] = make_float2(o[d0 + d][0], o[d0 + d][1]);
+            buf[(2 * d + 1) * 32] = make_float2(o[d0 + d][2], o[d0 + d][3]);
+          }
+        }
+        bar_compute();
+        if (kw == k - 1) {
+#pragma unroll
+          for (int d = 0; d < SM::kDims / 8; ++d) {
+            const float2 x = buf[(2 * d) * 32], y = buf[(2 * d + 1) * 32];
+            o[d0 + d][0] += x.x; o[d0 + d][1] += x.y;
+            o[d0 + d][2] += y.x; o[d0 + d][3] += y.y;
+          }
+        }
+        bar_compute();
+      }
+  }
+  // ---------------- output ----------------
+  if (kw == 0) {
+#pragma unroll
+    for (int hr = 0; hr < 2; ++hr) {
+      if (!live[hr]) continue;
+      const float inv = l_r[hr] == 0.f ? 0.f : 1.f / l_r[hr];  // nothing seen: zeros
+      uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + b * p.o_sb +
+                                                  node[hr] * p.o_st + head[hr] * p.o_sh);
+#pragma unroll
+      for (int d = 0; d < D / 8; ++d)
+        dst[d * 4 + c] = pack2<T>(o[d][2 * hr] * inv, o[d][2 * hr + 1] * inv);
+    }
+  }
+  bar_compute();
+  if (*odd) {
+    // values that are not finite, to the rows that see them
+    const int n = min(16 * RW, p.R - rt * 16 * RW);
+    for (int e = threadIdx.x; e < n * D; e += 128) {
+      const int r = rt * 16 * RW + e / D, d = e % D;
+      const int t = r / p.G, h = kvh * p.G + r % p.G;
+      const uint64_t* row = p.mask + b * p.mask_sb + (int64_t)t * p.W;
+      const int64_t low = max(low_of(p, sp, row), (int64_t)0);
+      float acc = 0.f;
+      auto add = [&](float x) { if (!isfinite(x)) acc += x; };
+      for (int j = 0; j < p.T; ++j)
+        if ((row[j / 64] >> (j % 64)) & 1)
+          add(to_f32(static_cast<const T*>(p.v_tree)[b * p.vt_sb + j * p.vt_st + kvh * p.vt_sh + d]));
+      for (int64_t k = low; k < sp.ctx; ++k) {
+        const int64_t k0 = k / KT * KT;
+        if (k0 + KT <= sp.ctx && k0 >= sp.lo_some) { k = k0 + KT - 1; continue; }
+        int64_t at = b * p.c_sb + kvh * p.c_sh + k * p.c_ss;
+        if (p.table) {
+          const int blk = p.table[b * p.table_stride + k / KT];
+          if (blk < 0 || blk >= p.num_blocks) continue;
+          at = (((int64_t)blk * p.Hkv + kvh) * KT + k % KT) * D;
+        }
+        add(to_f32(static_cast<const T*>(p.v_cache)[at + d]));
+      }
+      if (acc != 0.f) {
+        T* dst = static_cast<T*>(p.o) + b * p.o_sb + t * p.o_st + h * p.o_sh + d;
+        *dst = from_f32<T>(to_f32(*dst) + acc);
+      }
+    }
+  }
+}
+
+struct TreeCall {
+  const void* q; int64_t q_sb, q_st, q_sh;
+  const void* k; const void* v; int64_t c_sb, c_sh, c_ss;
+  int64_t num_blocks; const int32_t* table; int64_t table_stride;
+  const void* kt; int64_t kt_sb, kt_st, kt_sh;
+  const void* vt; int64_t vt_sb, vt_st, vt_sh;
+  const int32_t* ctx_lens; int64_t max_ctx;
+  const uint64_t* mask; int64_t mask_sb;
+  void* o; int64_t o_sb, o_st, o_sh;
+  int64_t B, T, Hq, Hkv, D, window_left;
+  float scale;
+  void* ws; int64_t ws_bytes;
+};
+
+// {64 columns, row, column box (D/64), kv head, batch or block}
+int kv_map(CUtensorMap* m, const void* base, int dtype, int64_t D, int64_t rows, int64_t heads,
+           int64_t outer, int64_t s_row, int64_t s_head, int64_t s_outer) {
+  // a dim of one needs a valid stride all the same
+  auto st = [&](int64_t n, int64_t s) { return (uint64_t)(n > 1 ? s : D) * 2; };
+  const uint64_t dims[5] = {64, (uint64_t)rows, (uint64_t)(D / 64), (uint64_t)heads,
+                            (uint64_t)outer};
+  const uint64_t strides[4] = {st(rows, s_row), 128, st(heads, s_head), st(outer, s_outer)};
+  const uint32_t box[5] = {64, KT, (uint32_t)(D / 64), 1, 1};
+  return make_tmap(m, base, dtype, 5, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+int tree_attention(const TreeCall& c, int dtype, cudaStream_t st) {
+  if (c.B == 0 || c.T == 0) return TPP_OK;
+  TPP_REQUIRE(c.q && c.k && c.v && c.kt && c.vt && c.ctx_lens && c.mask && c.o, TPP_ERR_SHAPE,
+              "null pointer");
+  TPP_REQUIRE(c.B > 0 && c.B <= 65535 && c.T > 0 && c.T <= kMaxNodes && c.Hq > 0 && c.Hkv > 0 &&
+                  c.Hq <= 65535 && c.max_ctx >= 0 && c.max_ctx < (1ll << 31) - 2 * KT &&
+                  c.num_blocks >= 0 && c.num_blocks < (1ll << 31),
+              TPP_ERR_SHAPE, "bad sizes (1..256 nodes, at most 65535 sequences and heads)");
+  TPP_REQUIRE(c.Hq % c.Hkv == 0, TPP_ERR_SHAPE, "Hq must be a multiple of Hkv");
+  TPP_REQUIRE(c.D == 64 || c.D == 128, TPP_ERR_UNSUPPORTED, "head dim must be 64 or 128");
+  TPP_REQUIRE(dtype == TPP_F16 || dtype == TPP_BF16, TPP_ERR_DTYPE,
+              "dtype must be f16 (0) or bf16 (1)");
+  TPP_REQUIRE(((c.q_sb | c.q_st | c.q_sh | c.kt_sb | c.kt_st | c.kt_sh | c.vt_sb | c.vt_st |
+                c.vt_sh) & 7) == 0 &&
+                  ((c.o_sb | c.o_st | c.o_sh) & 1) == 0 && aligned16(c.q) && aligned16(c.k) &&
+                  aligned16(c.v) && aligned16(c.kt) && aligned16(c.vt) &&
+                  (reinterpret_cast<uintptr_t>(c.o) & 3) == 0,
+              TPP_ERR_ALIGN, "rows must be 16-byte aligned (the output's: 4-byte)");
+  CUtensorMap tk, tv, tkt, tvt;
+  const int64_t rows = c.max_ctx > 0 ? c.max_ctx : 1;
+  int rc;
+  if (c.table) {
+    rc = kv_map(&tk, c.k, dtype, c.D, KT, c.Hkv, c.num_blocks, c.D, KT * c.D, c.Hkv * KT * c.D);
+    if (rc == TPP_OK)
+      rc = kv_map(&tv, c.v, dtype, c.D, KT, c.Hkv, c.num_blocks, c.D, KT * c.D, c.Hkv * KT * c.D);
+  } else {
+    rc = kv_map(&tk, c.k, dtype, c.D, rows, c.Hkv, c.B, c.c_ss, c.c_sh, c.c_sb);
+    if (rc == TPP_OK) rc = kv_map(&tv, c.v, dtype, c.D, rows, c.Hkv, c.B, c.c_ss, c.c_sh, c.c_sb);
+  }
+  if (rc == TPP_OK) rc = kv_map(&tkt, c.kt, dtype, c.D, c.T, c.Hkv, c.B, c.kt_st, c.kt_sh, c.kt_sb);
+  if (rc == TPP_OK) rc = kv_map(&tvt, c.vt, dtype, c.D, c.T, c.Hkv, c.B, c.vt_st, c.vt_sh, c.vt_sb);
+  if (rc != TPP_OK) return rc;
+  TreeArgs a;
+  a.q = c.q; a.q_sb = c.q_sb; a.q_st = c.q_st; a.q_sh = c.q_sh;
+  a.v_cache = c.v; a.c_sb = c.c_sb; a.c_sh = c.c_sh; a.c_ss = c.c_ss;
+  a.v_tree = c.vt; a.vt_sb = c.vt_sb; a.vt_st = c.vt_st; a.vt_sh = c.vt_sh;
+  a.ctx_lens = c.ctx_lens; a.max_ctx = (int)c.max_ctx;
+  a.mask = c.mask; a.mask_sb = c.mask_sb;
+  a.o = c.o; a.o_sb = c.o_sb; a.o_st = c.o_st; a.o_sh = c.o_sh;
+  a.table = c.table; a.table_stride = c.table_stride; a.num_blocks = (int)c.num_blocks;
+  a.window_left = c.window_left;
+  a.scale_log2 = c.scale * 1.4426950408889634f;
+  a.B = (int)c.B; a.T = (int)c.T; a.Hq = (int)c.Hq; a.Hkv = (int)c.Hkv;
+  a.G = (int)(c.Hq / c.Hkv); a.W = (a.T + 63) / 64; a.R = a.T * a.G; a.NT = a.W;
+  a.err = device_error_flag();
+  const int rw = a.R <= 16 ? 1 : a.R <= 32 ? 2 : 4;
+  a.RT = (a.R + 16 * rw - 1) / (16 * rw);
+  const dim3 grid((unsigned)(a.Hkv * a.RT), (unsigned)a.B);
+  auto go = [&](auto kern, size_t smem) -> int {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
+        cudaSuccess) {
+      set_error("tree_attn_kernel: cannot reserve shared memory");
+      return TPP_ERR_LAUNCH;
+    }
+    return launch("tree_attn_kernel", kern, grid, dim3(kThreads), smem, st, 0u, tk, tv, tkt, tvt,
+                  a);
+  };
+  return TPP_DISPATCH_HALF(dtype, T, [&]() -> int {
+    if (c.D == 64) {
+      if (rw == 1) return go(tree_attn_kernel<T, 64, 1>, TreeSmem<64, 1>::kBytes);
+      if (rw == 2) return go(tree_attn_kernel<T, 64, 2>, TreeSmem<64, 2>::kBytes);
+      return go(tree_attn_kernel<T, 64, 4>, TreeSmem<64, 4>::kBytes);
+    }
+    if (rw == 1) return go(tree_attn_kernel<T, 128, 1>, TreeSmem<128, 1>::kBytes);
+    if (rw == 2) return go(tree_attn_kernel<T, 128, 2>, TreeSmem<128, 2>::kBytes);
+    return go(tree_attn_kernel<T, 128, 4>, TreeSmem<128, 4>::kBytes);
+  });
+}
+
+}  // namespace
+}  // namespace tpp
+
+using namespace tpp;
+
+extern "C" int64_t tpp_attention_tree_workspace(int64_t, int64_t, int64_t, int64_t, int64_t,
+                                                int64_t, int64_t) {
+  return 0;
+}
+
+extern "C" int tpp_attention_tree(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
+                                  const void* k_cache, const void* v_cache, int64_t c_sb,
+                                  int64_t c_sh, int64_t c_ss, const void* k_tree, int64_t kt_sb,
+                                  int64_t kt_st, int64_t kt_sh, const void* v_tree,
+                                  int64_t vt_sb, int64_t vt_st, int64_t vt_sh,
+                                  const int32_t* ctx_lens, int64_t max_ctx, const uint64_t* mask,
+                                  int64_t mask_sb, void* o, int64_t o_sb, int64_t o_st,
+                                  int64_t o_sh, int64_t B, int64_t T, int64_t Hq, int64_t Hkv,
+                                  int64_t D, int64_t window_left, float scale, void* workspace,
+                                  int64_t workspace_bytes, int dtype, void* stream) {
+  TPP_REQUIRE(((c_sb | c_sh | c_ss) & 7) == 0, TPP_ERR_ALIGN,
+              "cache strides must be multiples of 8 elements");
+  const TreeCall c{q, q_sb, q_st, q_sh, k_cache, v_cache, c_sb, c_sh, c_ss, 0, nullptr, 0,
+                   k_tree, kt_sb, kt_st, kt_sh, v_tree, vt_sb, vt_st, vt_sh, ctx_lens, max_ctx,
+                   mask, mask_sb, o, o_sb, o_st, o_sh, B, T, Hq, Hkv, D, window_left, scale,
+                   workspace, workspace_bytes};
+  return tree_attention(c, dtype, as_stream(stream));
+}
+
+extern "C" int tpp_attention_tree_paged(
+    const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k_pool,
+    const void* v_pool, int64_t num_blocks, const int32_t* block_table, int64_t table_stride,
+    const void* k_tree, int64_t kt_sb, int64_t kt_st, int64_t kt_sh, const void* v_tree,
+    int64_t vt_sb, int64_t vt_st, int64_t vt_sh, const int32_t* ctx_lens, int64_t max_ctx,
+    const uint64_t* mask, int64_t mask_sb, void* o, int64_t o_sb, int64_t o_st, int64_t o_sh,
+    int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t window_left, float scale,
+    void* workspace, int64_t workspace_bytes, int dtype, void* stream) {
+  TPP_REQUIRE(block_table != nullptr && num_blocks > 0, TPP_ERR_SHAPE,
+              "null block table or empty pools");
+  const TreeCall c{q, q_sb, q_st, q_sh, k_pool, v_pool, 0, 0, 0, num_blocks, block_table,
+                   table_stride, k_tree, kt_sb, kt_st, kt_sh, v_tree, vt_sb, vt_st, vt_sh,
+                   ctx_lens, max_ctx, mask, mask_sb, o, o_sb, o_st, o_sh, B, T, Hq, Hkv, D,
+                   window_left, scale, workspace, workspace_bytes};
+  return tree_attention(c, dtype, as_stream(stream));
+}

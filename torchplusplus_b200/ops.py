@@ -681,6 +681,243 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
            N.ptr(positions), dt, N.stream_of(k))
 
 
+# ---------------------------------------------------------------- draft trees
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """t itself if its last dim is contiguous and every row starts on 16 bytes,
+    a contiguous copy otherwise."""
+    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:-1]):
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _i32(t: torch.Tensor, shape: tuple, what: str) -> None:
+    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous int32 {list(shape)}")
+
+
+def qk_norm_rope_tree(qkv: torch.Tensor, q_norm_w: torch.Tensor | None,
+                      k_norm_w: torch.Tensor | None, eps: float, cos: torch.Tensor,
+                      sin: torch.Tensor, positions: torch.Tensor, Hq: int, Hkv: int,
+                      q_out: torch.Tensor | None = None,
+                      k_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """qkv [B,T,(Hq+2Hkv)*D] -> q [B,T,Hq,D], k [B,T,Hkv,D], normed per head and
+    rotated at positions int32 [B,T] (a tree's siblings share one; a position
+    outside the tables gives zero rows).  v is the last part of qkv as it is."""
+    _cuda(qkv, q_norm_w, k_norm_w, cos, sin, positions, q_out, k_out)
+    dt = _half(qkv, "qkv")
+    _same_dtype(qkv, q_norm_w, k_norm_w, q_out, k_out)
+    if qkv.dim() != 3 or Hq <= 0 or Hkv <= 0 or qkv.shape[2] % (Hq + 2 * Hkv):
+        raise ValueError("qkv must be [B, T, (Hq+2Hkv)*D]")
+    B, T, W = qkv.shape
+    D = W // (Hq + 2 * Hkv)
+    _i32(positions, (B, T), "positions")
+    for w in (q_norm_w, k_norm_w):
+        if w is not None and tuple(w.shape) != (D,):
+            raise ValueError(f"norm weights must be [{D}]")
+    qkv = _rows16(qkv)
+    cos, sin, cs_stride, cs_dt = _table(cos, sin, D)
+    q_out = _tree_out(q_out, (B, T, Hq, D), qkv)
+    k_out = _tree_out(k_out, (B, T, Hkv, D), qkv)
+    N.call("tpp_qk_norm_rope_tree", qkv.data_ptr(), qkv.stride(0), qkv.stride(1),
+           N.ptr(q_norm_w), N.ptr(k_norm_w), float(eps), cos.data_ptr(), sin.data_ptr(),
+           cs_stride, cos.shape[0], cs_dt, positions.data_ptr(), q_out.data_ptr(),
+           k_out.data_ptr(), B, T, Hq, Hkv, D, dt, N.stream_of(qkv))
+    return q_out, k_out
+
+
+def _tree_out(out: torch.Tensor | None, shape: tuple, like: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=like.dtype, device=like.device)
+    if tuple(out.shape) != shape or not out.is_contiguous():
+        raise ValueError(f"the output must be contiguous {list(shape)}")
+    return out
+
+
+def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor,
+                uniforms: torch.Tensor | None = None, temperature: float = 1.0,
+                draft_logits: torch.Tensor | None = None
+                ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Which drafted tokens of each sequence's tree the target accepts, and the
+    token after them.  logits [B,T,V] (the target's at every node), tokens int64
+    [B,T] (node 0, the root, is already chosen), parents int32 [T] or [B,T]
+    (parents[i] < i), uniforms float32 [B,T] in [0,1) (one test a node, entry 0
+    for the draw), draft_logits [B,T or T-1,V] if the children of each node were
+    drawn from their softmax at the same temperature.  temperature 0 accepts the
+    argmax (see tpp_verify_tree for the rules).  Returns path int32 [B,T]
+    (accepted nodes from the root, then -1), count int32 [B] (nodes on it, at
+    least the root) and next_token int64 [B] (-1 if the row has no weight)."""
+    _cuda(logits, tokens, parents, uniforms, draft_logits)
+    if logits.dim() != 3:
+        raise ValueError("logits must be [B, T, V]")
+    dt = N.dtype_code(logits.dtype)
+    _same_dtype(logits, draft_logits)
+    B, T, V = logits.shape
+    if logits.stride(2) != 1:
+        logits = logits.contiguous()
+    if tokens.dtype != torch.int64 or tuple(tokens.shape) != (B, T):
+        raise ValueError("tokens must be int64 [B, T]")
+    if parents.dtype != torch.int32 or tuple(parents.shape) not in ((T,), (B, T)):
+        raise ValueError("parents must be int32 [T] or [B, T]")
+    tokens, parents = tokens.contiguous(), parents.contiguous()
+    if temperature > 0:
+        if uniforms is None or uniforms.dtype != torch.float32 or tuple(uniforms.shape) != (B, T):
+            raise ValueError("uniforms must be float32 [B, T]")
+        uniforms = uniforms.contiguous()
+    d_sb = d_st = 0
+    if draft_logits is not None:
+        if draft_logits.dim() != 3 or draft_logits.shape[0] != B or draft_logits.shape[2] != V \
+                or not T - 1 <= draft_logits.shape[1] <= T:
+            raise ValueError("draft_logits must be [B, T or T - 1, V]")
+        if draft_logits.stride(2) != 1:
+            draft_logits = draft_logits.contiguous()
+        d_sb, d_st = draft_logits.stride(0), draft_logits.stride(1)
+    path = torch.empty((B, T), dtype=torch.int32, device=logits.device)
+    count = torch.empty(B, dtype=torch.int32, device=logits.device)
+    nxt = torch.empty(B, dtype=torch.int64, device=logits.device)
+    N.call("tpp_verify_tree", logits.data_ptr(), logits.stride(0), logits.stride(1),
+           N.ptr(draft_logits), d_sb, d_st, tokens.data_ptr(), T, parents.data_ptr(),
+           0 if parents.dim() == 1 else T, N.ptr(uniforms), T, float(temperature),
+           path.data_ptr(), count.data_ptr(), nxt.data_ptr(), B, T, V, dt, N.stream_of(logits))
+    return path, count, nxt
+
+
+def kv_commit(k_tree: torch.Tensor, v_tree: torch.Tensor, path: torch.Tensor,
+              count: torch.Tensor, ctx_lens: torch.Tensor, k_cache: torch.Tensor,
+              v_cache: torch.Tensor, block_table: torch.Tensor | None = None) -> None:
+    """Copies the accepted path's K/V of all layers into the caches, in place:
+    k_tree/v_tree [L,B,T,Hkv,D] node path[b,i] -> row ctx_lens[b] + i, i <
+    count[b], of k_cache/v_cache [L,B,Hkv,Smax,D], or with block_table int32
+    [B,max_blocks] of pools [L,num_blocks,Hkv,64,D].  Rows past the cache are
+    skipped.  path int32 [B,T], count and ctx_lens int32 [B]."""
+    _cuda(k_tree, v_tree, path, count, ctx_lens, k_cache, v_cache, block_table)
+    dt = _half(k_tree, "k_tree")
+    _same_dtype(k_tree, v_tree, k_cache, v_cache)
+    if k_tree.dim() != 5 or v_tree.shape != k_tree.shape:
+        raise ValueError("k_tree and v_tree must be [L, B, T, Hkv, D]")
+    L, B, T, Hkv, D = k_tree.shape
+    if k_cache.dim() != 5 or k_cache.shape != v_cache.shape \
+            or k_cache.stride() != v_cache.stride() or k_cache.stride(4) != 1 \
+            or k_cache.shape[0] != L or k_cache.shape[2] != Hkv or k_cache.shape[4] != D:
+        raise ValueError("caches must be [L, B, Hkv, Smax, D] (pools [L, num_blocks, Hkv, 64, "
+                         "D]) with identical layouts")
+    _i32(path, (B, T), "path")
+    _i32(count, (B,), "count")
+    _i32(ctx_lens, (B,), "ctx_lens")
+    rows, nb, tstride = k_cache.shape[3], 0, 0
+    if block_table is not None:
+        if block_table.dtype != torch.int32 or block_table.dim() != 2 \
+                or block_table.shape[0] != B or block_table.stride(1) != 1:
+            raise ValueError("block_table must be int32 [B, max_blocks] with unit column stride")
+        if rows != 64 or (L > 0 and not k_cache[0].is_contiguous()):
+            raise ValueError("pools must be [L, num_blocks, Hkv, 64, D], each layer contiguous")
+        nb, rows, tstride = k_cache.shape[1], 64 * block_table.shape[1], block_table.stride(0)
+    elif k_cache.shape[1] != B:
+        raise ValueError("the caches' batch must match the tree's")
+    k_tree, v_tree = _rows16(k_tree), _rows16(v_tree)
+    N.call("tpp_kv_commit", k_tree.data_ptr(), *k_tree.stride()[:4], v_tree.data_ptr(),
+           *v_tree.stride()[:4], path.data_ptr(), T, count.data_ptr(), ctx_lens.data_ptr(),
+           k_cache.data_ptr(), v_cache.data_ptr(), *k_cache.stride()[:4], rows, nb,
+           N.ptr(block_table), tstride, L, B, T, Hkv, D, dt, N.stream_of(k_tree))
+
+
+def _tree_args(q, k_tree, v_tree, ctx_lens, mask, max_ctx, out, Hkv, D):
+    """Checks what both forms of tree attention share."""
+    B, T, Hq, Dq = q.shape
+    if Dq != D or Hq % Hkv or tuple(k_tree.shape) != (B, T, Hkv, D) \
+            or v_tree.shape != k_tree.shape:
+        raise ValueError("q must be [B, T, Hq, D] and k_tree/v_tree [B, T, Hkv, D], Hq a "
+                         "multiple of the cache's Hkv")
+    _i32(ctx_lens, (B,), "ctx_lens")
+    W = (T + 63) // 64
+    if mask.dtype != torch.int64 or tuple(mask.shape) not in ((T, W), (B, T, W)):
+        raise ValueError(f"mask must be int64 [{T}, {W}] or [{B}, {T}, {W}]")
+    if max_ctx < 0:
+        raise ValueError("max_ctx must not be negative")
+    if out is None:
+        out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
+    elif tuple(out.shape) != (B, T, Hq, D) or out.dtype != q.dtype or out.stride(3) != 1:
+        raise ValueError("out must be [B, T, Hq, D] of q's dtype")
+    return _rows16(q), _rows16(k_tree), _rows16(v_tree), mask.contiguous(), out
+
+
+def attention_tree_workspace_bytes(B: int, T: int, Hq: int, Hkv: int, max_ctx: int, D: int,
+                                   window_left: int = -1) -> int:
+    return int(N.lib().tpp_attention_tree_workspace(B, T, Hq, Hkv, max_ctx, D, window_left))
+
+
+def _tree_workspace(workspace, q, Hkv, max_ctx, window_left):
+    B, T, Hq, D = q.shape
+    need = attention_tree_workspace_bytes(B, T, Hq, Hkv, max_ctx, D, window_left)
+    if workspace is None and need > 0:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    return N.ptr(workspace), 0 if workspace is None else workspace.numel()
+
+
+def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   k_tree: torch.Tensor, v_tree: torch.Tensor, ctx_lens: torch.Tensor,
+                   max_ctx: int, mask: torch.Tensor, window_left: int = -1,
+                   scale: float | None = None, out: torch.Tensor | None = None,
+                   workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of T drafted nodes a sequence (q [B,T,Hq,D], T <= 256) over the
+    first ctx_lens[b] (int32 [B], at most max_ctx) rows of the caches
+    [B,Hkv,Smax,D] and those nodes of the tree (k_tree/v_tree [B,T,Hkv,D]) that
+    its mask row has: bit j % 64 of mask[.., i, j // 64] (int64 [T,W] or
+    [B,T,W], W = ceil(T/64)) lets node i see node j.  A row that sees nothing
+    gives zeros.  window_left: see tpp_attention_tree."""
+    _cuda(q, k_cache, v_cache, k_tree, v_tree, ctx_lens, mask, out, workspace)
+    dt = _half(q, "q")
+    _same_dtype(q, k_cache, v_cache, k_tree, v_tree)
+    if q.dim() != 4 or k_cache.dim() != 4 or k_cache.shape[0] != q.shape[0] \
+            or v_cache.shape != k_cache.shape or k_cache.stride() != v_cache.stride() \
+            or k_cache.stride(3) != 1:
+        raise ValueError("q must be [B, T, Hq, D], caches [B, Hkv, Smax, D] with identical layouts")
+    B, T, Hq, _ = q.shape
+    Hkv, Smax, D = k_cache.shape[1:]
+    if max_ctx > Smax:
+        raise ValueError("max_ctx exceeds the cache capacity")
+    q, k_tree, v_tree, mask, out = _tree_args(q, k_tree, v_tree, ctx_lens, mask, max_ctx, out,
+                                              Hkv, D)
+    ws, ws_bytes = _tree_workspace(workspace, q, Hkv, max_ctx, window_left)
+    N.call("tpp_attention_tree", q.data_ptr(), *q.stride()[:3], k_cache.data_ptr(),
+           v_cache.data_ptr(), *k_cache.stride()[:3], k_tree.data_ptr(), *k_tree.stride()[:3],
+           v_tree.data_ptr(), *v_tree.stride()[:3], ctx_lens.data_ptr(), int(max_ctx),
+           mask.data_ptr(), 0 if mask.dim() == 2 else mask.stride(0), out.data_ptr(),
+           *out.stride()[:3], B, T, Hq, Hkv, D, int(window_left),
+           1.0 / math.sqrt(D) if scale is None else float(scale), ws, ws_bytes, dt,
+           N.stream_of(q))
+    return out
+
+
+def attention_tree_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                         block_table: torch.Tensor, k_tree: torch.Tensor, v_tree: torch.Tensor,
+                         ctx_lens: torch.Tensor, max_ctx: int, mask: torch.Tensor,
+                         window_left: int = -1, scale: float | None = None,
+                         out: torch.Tensor | None = None,
+                         workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """attention_tree over a paged cache: pools [num_blocks,Hkv,64,D], key k of
+    sequence b in block block_table[b, k // 64], row k % 64."""
+    _cuda(q, k_pool, v_pool, block_table, k_tree, v_tree, ctx_lens, mask, out, workspace)
+    dt = _half(q, "q")
+    _same_dtype(q, k_pool, v_pool, k_tree, v_tree)
+    if q.dim() != 4 or k_pool.dim() != 4:
+        raise ValueError("q must be [B, T, Hq, D] and the pools [num_blocks, Hkv, 64, D]")
+    B, T, Hq, _ = q.shape
+    NB, Hkv, D = _paged_args(k_pool, v_pool, block_table, B)
+    if max_ctx > 64 * block_table.shape[1]:
+        raise ValueError("max_ctx exceeds the block table's capacity")
+    q, k_tree, v_tree, mask, out = _tree_args(q, k_tree, v_tree, ctx_lens, mask, max_ctx, out,
+                                              Hkv, D)
+    ws, ws_bytes = _tree_workspace(workspace, q, Hkv, max_ctx, window_left)
+    N.call("tpp_attention_tree_paged", q.data_ptr(), *q.stride()[:3], k_pool.data_ptr(),
+           v_pool.data_ptr(), NB, block_table.data_ptr(), block_table.stride(0),
+           k_tree.data_ptr(), *k_tree.stride()[:3], v_tree.data_ptr(), *v_tree.stride()[:3],
+           ctx_lens.data_ptr(), int(max_ctx), mask.data_ptr(),
+           0 if mask.dim() == 2 else mask.stride(0), out.data_ptr(), *out.stride()[:3], B, T, Hq,
+           Hkv, D, int(window_left), 1.0 / math.sqrt(D) if scale is None else float(scale), ws,
+           ws_bytes, dt, N.stream_of(q))
+    return out
+
+
 def argmax(logits: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
     """Greedy token per row of logits [B, V] -> int64 [B]."""
     _cuda(logits)
