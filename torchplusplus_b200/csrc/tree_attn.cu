@@ -7,9 +7,17 @@
 // (masked only at the context's end and at a window's edge), then the tree's
 // (one 64-bit mask word a row and tile).
 //
-// Warp 4 feeds a ring of K/V tiles by TMA (one request an operand); warps 0-3
-// are RW row groups of 16 rows x KW = 4 / RW key groups, each with its own
-// running maximum and sum (mma.sync m16n8k16 on fragments from ldmatrix, fp32
+// Split: the tiles of all units form one list, cut into equal parts, one for
+// each CTA, whatever the lengths of the sequences.  A unit that lies within one
+// part is finished there; the pieces of the others go to the workspace as
+// (m, l, o) in fp32 and tree_combine_kernel joins them, in list order.
+//
+// Thread 0 feeds a ring of K/V tiles by TMA (one request an operand), on into the
+// next piece; it refills a stage one tile after its use.  (A producer warp of
+// its own makes 10 warps an SM, three on one scheduler, and so caps the
+// registers of two CTAs at 168: the 64-row form spilled.)  The four warps are RW
+// row groups of 16 rows x KW = 4 / RW key groups, each with its own running
+// maximum and sum (mma.sync m16n8k16 on fragments from ldmatrix, fp32
 // accumulators, exp2 domain); the key groups merge in shared memory at the end.
 //
 // Masked keys: the score becomes -inf and the value is cleared before the
@@ -17,6 +25,7 @@
 // (tree tiles, a window's edge) are cleared too where they are not finite, and
 // added afterwards, element by element, to the rows that see them.
 #include <math.h>
+#include <algorithm>
 #include "mma_common.cuh"
 #include "tc_common.cuh"
 
@@ -24,8 +33,9 @@ namespace tpp {
 namespace {
 
 constexpr int KT = 64;            // keys of a tile
-constexpr int kThreads = 160;     // 4 compute warps + the producer warp
+constexpr int kThreads = 128;
 constexpr int kMaxNodes = 256;
+constexpr int kMinTiles = 4;      // tiles of a part at least
 constexpr float kRescale = 8.0f;  // log2: the base moves when the maximum grew by 2^8
 
 struct TreeArgs {
@@ -39,25 +49,28 @@ struct TreeArgs {
   int64_t window_left;
   float scale_log2;
   int B, T, Hq, Hkv, G, W, R, RT, NT;  // W mask words a row, R = T * G rows, NT tree tiles
+  int ctas, rows;                      // parts at most (0: a unit each), rows of a unit
+  float* ws;                           // pieces: two a part
   int* err;
 };
 
-template <int D, int RW>
-struct TreeSmem {
-  static constexpr int KW = 4 / RW;
-  static constexpr int kStages = D == 128 ? 3 : 6;
-  static constexpr uint32_t kTile = KT * D * 2;
-  static constexpr uint32_t kRing = kStages * 2 * kTile;
-  static constexpr int kDims = RW == 1 ? D : 64;  // dims merged at a time
-  static constexpr uint32_t kMerge = KW > 1 ? RW * 16 * kDims * 4 : 0;
-  static constexpr uint32_t kMl = 4 * 16 * 2 * 4;  // (m, l) of each warp's rows
-  static constexpr size_t kBytes = 1024 + kRing + kMerge + kMl + 2 * kStages * 8 + 16;
-};
+// fp32 words of a piece: o [rows][D], m [rows], l [rows], whether a value that
+// is not finite was met
+__host__ __device__ constexpr int64_t slot_floats(int rows, int D) {
+  return (int64_t)rows * (D + 2) + 4;
+}
 
 __device__ __forceinline__ uint32_t sw_addr(uint32_t base, int r, int chunk) {
   return base + (uint32_t)((chunk >> 3) * KT * 128 + r * 128 + (((chunk & 7) ^ (r & 7)) << 4));
 }
 __device__ __forceinline__ void bar_compute() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ bool bar_compute_or(bool x) {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred a, b;\n\tsetp.ne.u32 a, %1, 0;\n\t"
+               "barrier.cta.red.or.pred b, 1, 128, a;\n\tselp.u32 %0, 1, 0, b;\n\t}"
+               : "=r"(r) : "r"((uint32_t)x) : "memory");
+  return r != 0;
+}
 
 template <typename T> struct ExpMask;
 template <> struct ExpMask<__half> { static constexpr uint32_t value = 0x7c00u; };
@@ -91,6 +104,114 @@ __device__ __forceinline__ Span span_of(const TreeArgs& p, int b) {
   s.tiles = s.ctx > 0 ? (s.ctx + KT - 1) / KT - s.first : 0;
   return s;
 }
+
+// ---- the list of tiles -------------------------------------------------------
+// Units in (b, kv head, row tile) order, each with its cache's tiles, then the
+// tree's.  Part c of n is [total * c / n, total * (c + 1) / n).
+struct Parts { int64_t total; int n; };
+__device__ __forceinline__ int64_t part_start(const Parts& s, int c) { return s.total * c / s.n; }
+
+// The number of tiles before sequence b, by one warp; b = B gives all.
+__device__ __forceinline__ int64_t tiles_before(const TreeArgs& p, int b) {
+  const int lane = threadIdx.x & 31;
+  int64_t n = 0;
+  for (int i = lane; i < b; i += 32) n += span_of(p, i).tiles + p.NT;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  return n * p.Hkv * p.RT;
+}
+__device__ __forceinline__ Parts parts_of(const TreeArgs& p) {
+  Parts s;
+  s.total = tiles_before(p, p.B);
+  s.n = (int)max((int64_t)1, min((int64_t)p.ctas, s.total / kMinTiles));
+  return s;
+}
+// The sequence that tile x of the list belongs to and the tiles before it.
+__device__ __forceinline__ int sequence_of(const TreeArgs& p, int64_t x, int64_t& before) {
+  const int lane = threadIdx.x & 31;
+  before = 0;
+  for (int b0 = 0;; b0 += 32) {
+    const int64_t n = b0 + lane < p.B
+        ? (int64_t)(span_of(p, b0 + lane).tiles + p.NT) * p.Hkv * p.RT : 0;
+    int64_t incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, n > 0 && x < before + incl);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      before += __shfl_sync(0xffffffffu, incl - n, l);
+      return b0 + l;
+    }
+    if (b0 + 32 >= p.B) return p.B;  // past the end
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+}
+// Walks the pieces of units in one CTA's part.
+struct Piece {
+  int64_t pos, end, before;  // in the list; before: tiles of earlier sequences
+  int b, unit, t0, t1;       // tiles [t0, t1) of the unit (kv head, row tile) of b
+  Span sp;
+  bool whole;
+  __device__ __forceinline__ bool start(const TreeArgs& p) {
+    if (p.ctas == 0) {
+      const int u = p.Hkv * p.RT;
+      b = blockIdx.x / u;
+      sp = span_of(p, b);
+      before = pos = (int64_t)blockIdx.x * (sp.tiles + p.NT);  // b's list begins at unit 0
+      before -= (int64_t)(blockIdx.x % u) * (sp.tiles + p.NT);
+      end = pos + sp.tiles + p.NT;
+    } else {
+      const Parts s = parts_of(p);
+      if ((int)blockIdx.x >= s.n) return false;
+      pos = part_start(s, blockIdx.x);
+      end = part_start(s, blockIdx.x + 1);
+      b = sequence_of(p, pos, before);
+      if (b >= p.B) return false;
+      sp = span_of(p, b);
+    }
+    locate(p);
+    return pos < end;
+  }
+  __device__ __forceinline__ void locate(const TreeArgs& p) {
+    const int n = sp.tiles + p.NT;
+    const int64_t at = pos - before;
+    unit = (int)(at / n);
+    t0 = (int)(at - (int64_t)unit * n);
+    t1 = (int)min((int64_t)n, t0 + (end - pos));
+    whole = t0 == 0 && t1 == n;
+  }
+  __device__ __forceinline__ bool next(const TreeArgs& p) {
+    pos += t1 - t0;
+    if (pos >= end) return false;
+    const int n = sp.tiles + p.NT;
+    if (unit == p.Hkv * p.RT - 1 && t1 == n) {
+      before += (int64_t)n * p.Hkv * p.RT;
+      sp = span_of(p, ++b);
+    }
+    locate(p);
+    return true;
+  }
+};
+template <int D, int RW>
+struct TreeSmem {
+  static constexpr int KW = 4 / RW;
+  static constexpr int kStages = D == 128 ? 3 : 6;
+  static constexpr uint32_t kTile = KT * D * 2;
+  static constexpr uint32_t kRing = kStages * 2 * kTile;
+  static constexpr int kDims = RW == 1 ? D : 64;  // dims merged at a time
+  static constexpr uint32_t kMerge = KW > 1 ? RW * 16 * kDims * 4 : 0;
+  static constexpr uint32_t kMl = 4 * 16 * 2 * 4;  // (m, l) of each warp's rows
+  static constexpr size_t kBytes = 1024 + kRing + kMerge + kMl + 2 * kStages * 8 + sizeof(Piece);
+};
+
+// Where part c keeps a piece: the one that starts its unit, or continues one.
+__device__ __forceinline__ float* slot_of(const TreeArgs& p, int D, int c, bool starts) {
+  return p.ws + (int64_t)(2 * c + (starts ? 1 : 0)) * slot_floats(p.rows, D);
+}
+
 // The first cache row that the node with mask row `row` sees.
 __device__ __forceinline__ int64_t low_of(const TreeArgs& p, const Span& s, const uint64_t* row) {
   if (p.window_left < 0) return 0;
@@ -102,8 +223,32 @@ __device__ __forceinline__ int64_t low_of(const TreeArgs& p, const Span& s, cons
   return (int64_t)s.ctx + seen - 1 - p.window_left;
 }
 
+// Sum of the values at dim d that are not finite over the keys that node t sees
+// in the tree and in the cache tiles that were cleared of them.
+template <typename T, int D>
+__device__ float odd_values(const TreeArgs& p, const Span& sp, int b, int kvh, int t, int d) {
+  const uint64_t* row = p.mask + b * p.mask_sb + (int64_t)t * p.W;
+  float acc = 0.f;
+  auto add = [&](float x) { if (!isfinite(x)) acc += x; };
+  for (int j = 0; j < p.T; ++j)
+    if ((row[j / 64] >> (j % 64)) & 1)
+      add(to_f32(static_cast<const T*>(p.v_tree)[b * p.vt_sb + j * p.vt_st + kvh * p.vt_sh + d]));
+  for (int64_t k = max(low_of(p, sp, row), (int64_t)0); k < sp.ctx; ++k) {
+    const int64_t k0 = k / KT * KT;
+    if (k0 + KT <= sp.ctx && k0 >= sp.lo_some) { k = k0 + KT - 1; continue; }
+    int64_t at = b * p.c_sb + kvh * p.c_sh + k * p.c_ss;
+    if (p.table) {
+      const int blk = p.table[b * p.table_stride + k / KT];
+      if (blk < 0 || blk >= p.num_blocks) continue;
+      at = (((int64_t)blk * p.Hkv + kvh) * KT + k % KT) * D;
+    }
+    add(to_f32(static_cast<const T*>(p.v_cache)[at + d]));
+  }
+  return acc;
+}
+
 template <typename T, int D, int RW>
-__global__ void __launch_bounds__(kThreads) tree_attn_kernel(
+__global__ void __launch_bounds__(kThreads, 2) tree_attn_kernel(
     const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
     const __grid_constant__ CUtensorMap tm_kt, const __grid_constant__ CUtensorMap tm_vt,
     const __grid_constant__ TreeArgs p) {
@@ -118,7 +263,6 @@ __global__ void __launch_bounds__(kThreads) tree_attn_kernel(
   float* ml = reinterpret_cast<float*>(smem + SM::kRing + SM::kMerge);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + SM::kRing + SM::kMerge + SM::kMl);
   uint64_t* empty = full + ST;
-  volatile uint32_t* odd = reinterpret_cast<volatile uint32_t*>(empty + ST);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -131,52 +275,59 @@ __global__ void __launch_bounds__(kThreads) tree_attn_kernel(
       mbar_init(&empty[s], 4);
     }
     fence_mbar_init();
-    *odd = 0;
   }
   __syncthreads();
   pdl_wait();
   pdl_trigger();
 
-  const int rt = blockIdx.x % p.RT;
-  const int kvh = blockIdx.x / p.RT;
-  const int b = blockIdx.y;
-  const Span sp = span_of(p, b);
-  const int ntiles = sp.tiles + p.NT;
+  Piece pc;
+  if (!pc.start(p)) return;
   bool ok = true;
-
-  if (warp == 4) {
-    // ---------------- producer ----------------
-    if (lane == 0) {
-      for (int i = 0; i < ntiles && ok; ++i) {
-        const int s = i % ST;
-        if (i >= ST) ok = mbar_wait(&empty[s], ((i / ST) & 1) ^ 1, p.err, 61);
-        if (!ok) break;
-        uint8_t* kd = smem + s * 2 * SM::kTile;
-        uint8_t* vd = kd + SM::kTile;
-        mbar_arrive_expect_tx(&full[s], 2 * SM::kTile);
-        if (i >= sp.tiles) {
-          const int n0 = (i - sp.tiles) * KT;
-          tma_load_5d(kd, &tm_kt, &full[s], 0, n0, 0, kvh, b);
-          tma_load_5d(vd, &tm_vt, &full[s], 0, n0, 0, kvh, b);
-        } else if (p.table) {
-          // a block outside the pool is out of the map's range: zeros
-          int blk = p.table[b * p.table_stride + sp.first + i];
-          if (blk < 0 || blk >= p.num_blocks) blk = p.num_blocks;
-          tma_load_5d(kd, &tm_k, &full[s], 0, 0, 0, kvh, blk);
-          tma_load_5d(vd, &tm_v, &full[s], 0, 0, 0, kvh, blk);
-        } else {
-          tma_load_5d(kd, &tm_k, &full[s], 0, (sp.first + i) * KT, 0, kvh, b);
-          tma_load_5d(vd, &tm_v, &full[s], 0, (sp.first + i) * KT, 0, kvh, b);
-        }
-      }
+  int it = 0;  // tiles so far: the ring's position
+  // The loads run ahead of pc; thread 0 keeps their place in shared memory.
+  Piece* ahead = reinterpret_cast<Piece*>(empty + ST);
+  int issued = 0;
+  auto issue = [&]() {  // thread 0: the next tile of the part, if there is one
+    if (issued < 0) return;
+    const int i = ahead->t0, b = ahead->b, kvh = ahead->unit / p.RT;
+    const int s = issued % ST, first = ahead->sp.first, tiles = ahead->sp.tiles;
+    uint8_t* kd = smem + s * 2 * SM::kTile;
+    uint8_t* vd = kd + SM::kTile;
+    mbar_arrive_expect_tx(&full[s], 2 * SM::kTile);
+    if (i >= tiles) {
+      const int n0 = (i - tiles) * KT;
+      tma_load_5d(kd, &tm_kt, &full[s], 0, n0, 0, kvh, b);
+      tma_load_5d(vd, &tm_vt, &full[s], 0, n0, 0, kvh, b);
+    } else if (p.table) {
+      // a block outside the pool is out of the map's range: zeros
+      int blk = p.table[b * p.table_stride + first + i];
+      if (blk < 0 || blk >= p.num_blocks) blk = p.num_blocks;
+      tma_load_5d(kd, &tm_k, &full[s], 0, 0, 0, kvh, blk);
+      tma_load_5d(vd, &tm_v, &full[s], 0, 0, 0, kvh, blk);
+    } else {
+      tma_load_5d(kd, &tm_k, &full[s], 0, (first + i) * KT, 0, kvh, b);
+      tma_load_5d(vd, &tm_v, &full[s], 0, (first + i) * KT, 0, kvh, b);
     }
-    return;
+    ++issued;
+    if (i + 1 < ahead->t1) {
+      ahead->t0 = i + 1;
+      ahead->pos += 1;
+    } else if (!ahead->next(p)) {
+      issued = -1;
+    }
+  };
+  if (threadIdx.x == 0) {
+    *ahead = pc;
+    for (int s = 0; s < ST; ++s) issue();
   }
 
   // ---------------- compute ----------------
   const int g = lane >> 2, c = lane & 3;
   const int rw = warp / KW, kw = warp % KW;
   const int kr0 = kw * KPW;
+  do {
+  const int b = pc.b, kvh = pc.unit / p.RT, rt = pc.unit % p.RT;
+  const Span& sp = pc.sp;
   int node[2], head[2];
   bool live[2];
   const uint64_t* mrow[2];
@@ -208,9 +359,13 @@ __global__ void __launch_bounds__(kThreads) tree_attn_kernel(
   float m_r[2] = {-INFINITY, -INFINITY}, l_r[2] = {0.f, 0.f};
   uint32_t bad = 0;
 
-  for (int i = 0; i < ntiles; ++i) {
-    const int s = i % ST;
-    if (ok) ok = mbar_wait(&full[s], (i / ST) & 1, p.err, 62);
+  for (int i = pc.t0; i < pc.t1; ++i, ++it) {
+    const int s = it % ST;
+    if (threadIdx.x == 0 && it > 0 && ok && issued >= 0) {
+      ok = mbar_wait(&empty[(it - 1) % ST], ((it - 1) / ST) & 1, p.err, 61);
+      if (ok) issue();
+    }
+    if (ok) ok = mbar_wait(&full[s], (it / ST) & 1, p.err, 62);
     const uint32_t kb = smem_u32(smem + s * 2 * SM::kTile), vb = kb + SM::kTile;
     float sc[NTL][4];
 #pragma unroll
@@ -324,8 +479,6 @@ __global__ void __launch_bounds__(kThreads) tree_attn_kernel(
     __syncwarp();
     if (lane == 0) mbar_arrive(&empty[s]);
   }
-  if (bad) *odd = 1;
-
   // ---------------- merge the key groups ----------------
 #pragma unroll
   for (int hr = 0; hr < 2; ++hr) {
@@ -387,49 +540,102 @@ __global__ void __launch_bounds__(kThreads) tree_attn_kernel(
       }
   }
   // ---------------- output ----------------
+  float* slot = pc.whole ? nullptr : slot_of(p, D, blockIdx.x, pc.t0 == 0);
   if (kw == 0) {
 #pragma unroll
     for (int hr = 0; hr < 2; ++hr) {
       if (!live[hr]) continue;
-      const float inv = l_r[hr] == 0.f ? 0.f : 1.f / l_r[hr];  // nothing seen: zeros
-      uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + b * p.o_sb +
-                                                  node[hr] * p.o_st + head[hr] * p.o_sh);
+      if (pc.whole) {
+        const float inv = l_r[hr] == 0.f ? 0.f : 1.f / l_r[hr];  // nothing seen: zeros
+        uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + b * p.o_sb +
+                                                    node[hr] * p.o_st + head[hr] * p.o_sh);
 #pragma unroll
-      for (int d = 0; d < D / 8; ++d)
-        dst[d * 4 + c] = pack2<T>(o[d][2 * hr] * inv, o[d][2 * hr + 1] * inv);
+        for (int d = 0; d < D / 8; ++d)
+          dst[d * 4 + c] = pack2<T>(o[d][2 * hr] * inv, o[d][2 * hr + 1] * inv);
+      } else {
+        const int r = rw * 16 + g + 8 * hr;
+        float2* dst = reinterpret_cast<float2*>(slot + r * D);
+#pragma unroll
+        for (int d = 0; d < D / 8; ++d)
+          dst[d * 4 + c] = make_float2(o[d][2 * hr], o[d][2 * hr + 1]);
+        if (c == 0) {
+          slot[p.rows * D + r] = m_r[hr];
+          slot[p.rows * (D + 1) + r] = l_r[hr];
+        }
+      }
     }
   }
-  bar_compute();
-  if (*odd) {
-    // values that are not finite, to the rows that see them
+  const bool odd = bar_compute_or(bad != 0);
+  if (!pc.whole) {
+    if (threadIdx.x == 0) slot[p.rows * (D + 2)] = odd ? 1.f : 0.f;
+  } else if (odd) {
     const int n = min(16 * RW, p.R - rt * 16 * RW);
     for (int e = threadIdx.x; e < n * D; e += 128) {
       const int r = rt * 16 * RW + e / D, d = e % D;
       const int t = r / p.G, h = kvh * p.G + r % p.G;
-      const uint64_t* row = p.mask + b * p.mask_sb + (int64_t)t * p.W;
-      const int64_t low = max(low_of(p, sp, row), (int64_t)0);
-      float acc = 0.f;
-      auto add = [&](float x) { if (!isfinite(x)) acc += x; };
-      for (int j = 0; j < p.T; ++j)
-        if ((row[j / 64] >> (j % 64)) & 1)
-          add(to_f32(static_cast<const T*>(p.v_tree)[b * p.vt_sb + j * p.vt_st + kvh * p.vt_sh + d]));
-      for (int64_t k = low; k < sp.ctx; ++k) {
-        const int64_t k0 = k / KT * KT;
-        if (k0 + KT <= sp.ctx && k0 >= sp.lo_some) { k = k0 + KT - 1; continue; }
-        int64_t at = b * p.c_sb + kvh * p.c_sh + k * p.c_ss;
-        if (p.table) {
-          const int blk = p.table[b * p.table_stride + k / KT];
-          if (blk < 0 || blk >= p.num_blocks) continue;
-          at = (((int64_t)blk * p.Hkv + kvh) * KT + k % KT) * D;
-        }
-        add(to_f32(static_cast<const T*>(p.v_cache)[at + d]));
-      }
+      const float acc = odd_values<T, D>(p, sp, b, kvh, t, d);
       if (acc != 0.f) {
         T* dst = static_cast<T*>(p.o) + b * p.o_sb + t * p.o_st + h * p.o_sh + d;
         *dst = from_f32<T>(to_f32(*dst) + acc);
       }
     }
   }
+  } while (pc.next(p));
+}
+
+// Joins the pieces of the units that more than one part holds: a warp a row.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant__ TreeArgs p) {
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31;
+  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (item >= (int64_t)p.B * p.Hkv * p.R) return;
+  const int row = (int)(item % p.R);
+  const int kvh = (int)(item / p.R % p.Hkv), b = (int)(item / p.R / p.Hkv);
+  const Span sp = span_of(p, b);
+  const Parts s = parts_of(p);
+  const int n = sp.tiles + p.NT;
+  const int64_t x0 = tiles_before(p, b) + (int64_t)(kvh * p.RT + row / p.rows) * n;
+  auto part_with = [&](int64_t x) {
+    int c = (int)min((int64_t)s.n - 1, x * s.n / s.total);
+    while (part_start(s, c) > x) --c;
+    while (part_start(s, c + 1) <= x) ++c;
+    return c;
+  };
+  const int c0 = part_with(x0), c1 = part_with(x0 + n - 1);
+  if (c0 == c1) return;
+  const int r = row % p.rows;
+  float M = -INFINITY;
+  for (int c = c0 + lane; c <= c1; c += 32)
+    M = fmaxf(M, slot_of(p, D, c, c == c0)[p.rows * D + r]);
+  M = warp_max(M);
+  const float base = M == -INFINITY ? 0.f : M;
+  float L = 0.f, odd = 0.f;
+  constexpr int PER = D / 32;
+  float o[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) o[i] = 0.f;
+#pragma unroll 4
+  for (int c = c0; c <= c1; ++c) {
+    const float* sl = slot_of(p, D, c, c == c0);
+    const float w = ex2_ftz(sl[p.rows * D + r] - base);
+    L += w * sl[p.rows * (D + 1) + r];
+    odd += sl[p.rows * (D + 2)];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) o[i] = fmaf(w, sl[r * D + lane * PER + i], o[i]);
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  const int t = row / p.G, h = kvh * p.G + row % p.G;
+  T* dst = static_cast<T*>(p.o) + b * p.o_sb + t * p.o_st + h * p.o_sh + lane * PER;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    o[i] *= inv;
+    if (odd != 0.f) o[i] += odd_values<T, D>(p, sp, b, kvh, t, lane * PER + i);
+  }
+#pragma unroll
+  for (int i = 0; i < PER; i += 2)
+    *reinterpret_cast<uint32_t*>(dst + i) = pack2<T>(o[i], o[i + 1]);
 }
 
 struct TreeCall {
@@ -446,6 +652,21 @@ struct TreeCall {
   void* ws; int64_t ws_bytes;
 };
 
+// How a call is cut: the row groups of a CTA and the parts (0: one a unit).
+struct Plan { int rw, rt, ctas; };
+Plan plan_of(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t max_ctx,
+             int64_t window_left) {
+  const int64_t R = T * (Hq / Hkv);
+  Plan pl;
+  pl.rw = R <= 16 ? 1 : R <= 32 ? 2 : 4;
+  pl.rt = (int)((R + 16 * pl.rw - 1) / (16 * pl.rw));
+  int64_t keys = max_ctx;
+  if (window_left >= 0 && window_left + 1 < keys) keys = window_left + KT;
+  const int64_t tiles = (keys + KT - 1) / KT + (T + 63) / 64;
+  pl.ctas = tiles <= kMinTiles ? 0 : (int)std::min<int64_t>(2 * sm_budget(), B * Hkv * pl.rt * tiles);
+  return pl;
+}
+
 // {64 columns, row, column box (D/64), kv head, batch or block}
 int kv_map(CUtensorMap* m, const void* base, int dtype, int64_t D, int64_t rows, int64_t heads,
            int64_t outer, int64_t s_row, int64_t s_head, int64_t s_outer) {
@@ -456,6 +677,10 @@ int kv_map(CUtensorMap* m, const void* base, int dtype, int64_t D, int64_t rows,
   const uint64_t strides[4] = {st(rows, s_row), 128, st(heads, s_head), st(outer, s_outer)};
   const uint32_t box[5] = {64, KT, (uint32_t)(D / 64), 1, 1};
   return make_tmap(m, base, dtype, 5, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+int64_t workspace_of(const Plan& pl, int64_t D) {
+  return pl.ctas ? 2 * pl.ctas * slot_floats(16 * pl.rw, (int)D) * 4 : 0;
 }
 
 int tree_attention(const TreeCall& c, int dtype, cudaStream_t st) {
@@ -503,9 +728,15 @@ int tree_attention(const TreeCall& c, int dtype, cudaStream_t st) {
   a.B = (int)c.B; a.T = (int)c.T; a.Hq = (int)c.Hq; a.Hkv = (int)c.Hkv;
   a.G = (int)(c.Hq / c.Hkv); a.W = (a.T + 63) / 64; a.R = a.T * a.G; a.NT = a.W;
   a.err = device_error_flag();
-  const int rw = a.R <= 16 ? 1 : a.R <= 32 ? 2 : 4;
-  a.RT = (a.R + 16 * rw - 1) / (16 * rw);
-  const dim3 grid((unsigned)(a.Hkv * a.RT), (unsigned)a.B);
+  const Plan pl = plan_of(c.B, c.T, c.Hq, c.Hkv, c.max_ctx, c.window_left);
+  const int rw = pl.rw;
+  a.RT = pl.rt; a.ctas = pl.ctas; a.rows = 16 * rw;
+  a.ws = static_cast<float*>(c.ws);
+  TPP_REQUIRE(pl.ctas == 0 || (c.ws && c.ws_bytes >= workspace_of(pl, c.D) && aligned16(c.ws)),
+              TPP_ERR_WORKSPACE, "workspace missing, too small or not 16-byte aligned");
+  const int64_t units = c.B * c.Hkv * pl.rt;
+  TPP_REQUIRE(units < (1ll << 31), TPP_ERR_SHAPE, "too many rows");
+  const dim3 grid((unsigned)(pl.ctas ? pl.ctas : units));
   auto go = [&](auto kern, size_t smem) -> int {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
         cudaSuccess) {
@@ -515,7 +746,7 @@ int tree_attention(const TreeCall& c, int dtype, cudaStream_t st) {
     return launch("tree_attn_kernel", kern, grid, dim3(kThreads), smem, st, 0u, tk, tv, tkt, tvt,
                   a);
   };
-  return TPP_DISPATCH_HALF(dtype, T, [&]() -> int {
+  rc = TPP_DISPATCH_HALF(dtype, T, [&]() -> int {
     if (c.D == 64) {
       if (rw == 1) return go(tree_attn_kernel<T, 64, 1>, TreeSmem<64, 1>::kBytes);
       if (rw == 2) return go(tree_attn_kernel<T, 64, 2>, TreeSmem<64, 2>::kBytes);
@@ -525,6 +756,12 @@ int tree_attention(const TreeCall& c, int dtype, cudaStream_t st) {
     if (rw == 2) return go(tree_attn_kernel<T, 128, 2>, TreeSmem<128, 2>::kBytes);
     return go(tree_attn_kernel<T, 128, 4>, TreeSmem<128, 4>::kBytes);
   });
+  if (rc != TPP_OK || pl.ctas == 0) return rc;
+  const int64_t blocks = (c.B * c.Hkv * a.R + 7) / 8;
+  return TPP_DISPATCH_HALF(dtype, T, [&]() -> int {
+    auto kern = c.D == 64 ? tree_combine_kernel<T, 64> : tree_combine_kernel<T, 128>;
+    return launch("tree_combine_kernel", kern, dim3((unsigned)blocks), dim3(256), 0, st, 0u, a);
+  });
 }
 
 }  // namespace
@@ -532,9 +769,11 @@ int tree_attention(const TreeCall& c, int dtype, cudaStream_t st) {
 
 using namespace tpp;
 
-extern "C" int64_t tpp_attention_tree_workspace(int64_t, int64_t, int64_t, int64_t, int64_t,
-                                                int64_t, int64_t) {
-  return 0;
+extern "C" int64_t tpp_attention_tree_workspace(int64_t B, int64_t T, int64_t Hq, int64_t Hkv,
+                                                int64_t max_ctx, int64_t D,
+                                                int64_t window_left) {
+  if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || max_ctx < 0) return 0;
+  return workspace_of(plan_of(B, T, Hq, Hkv, max_ctx, window_left), D);
 }
 
 extern "C" int tpp_attention_tree(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
