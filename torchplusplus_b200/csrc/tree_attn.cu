@@ -50,6 +50,7 @@ struct TreeArgs {
   float scale_log2;
   int B, T, Hq, Hkv, G, W, R, RT, NT;  // W mask words a row, R = T * G rows, NT tree tiles
   int ctas, rows;                      // parts at most (0: a unit each), rows of a unit
+  int o_vec;                           // the output's rows start on 16 bytes
   float* ws;                           // pieces: two a part
   int* err;
 };
@@ -583,6 +584,374 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attn_kernel(
   } while (pc.next(p));
 }
 
+// ---- wide trees: tcgen05 ------------------------------------------------------
+// From 33 rows a unit on, the products outgrow mma.sync (64 rows over a 64-key
+// tile are 1050 clocks of MMA an SM, about what the tile takes to arrive), so a
+// unit is a 128-row tile on the 5th-generation tensor core.  Two CTAs an SM, each
+// with its own S, P and O in 256 columns of TMEM: while one waits for its scores
+// the other's softmax runs.
+//   warps 0-3: Q into shared memory, softmax (a row a thread), output
+//   warp 4:    K and V tiles by TMA into two rings, ahead into the next piece
+//   warp 5:    S = Q K^T (M 128, N 64), O += P V (P read from TMEM)
+// S and P share two 64-column buffers; S of tile j+1 is computed under the softmax
+// of tile j.  Dead rows of a narrow unit (R < 128) are skipped by whole warps.
+constexpr int kTcRows = 128;
+constexpr int kTcThreads = 192;
+constexpr int kKSt = 3, kVSt = 2;
+
+template <int D>
+struct TcSmem {
+  static constexpr uint32_t kQ = kTcRows * D * 2;
+  static constexpr uint32_t kTile = KT * D * 2;
+  static constexpr size_t kBytes = kQ + (kKSt + kVSt) * kTile + 1024;
+};
+
+__device__ __forceinline__ bool bar_softmax_or(bool x) {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred a, b;\n\tsetp.ne.u32 a, %1, 0;\n\t"
+               "barrier.cta.red.or.pred b, 2, 128, a;\n\tselp.u32 %0, 1, 0, b;\n\t}"
+               : "=r"(r) : "r"((uint32_t)x) : "memory");
+  return r != 0;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kTcThreads, 2) tree_attn_tc_kernel(
+    const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+    const __grid_constant__ CUtensorMap tm_kt, const __grid_constant__ CUtensorMap tm_vt,
+    const __grid_constant__ TreeArgs p) {
+  using SM = TcSmem<D>;
+  extern __shared__ __align__(1024) uint8_t tc_smem[];
+  uint8_t* sQ = tc_smem;
+  uint8_t* sK = sQ + SM::kQ;
+  uint8_t* sV = sK + kKSt * SM::kTile;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(sV + kVSt * SM::kTile);
+  uint64_t* k_full = q_full + 1;
+  uint64_t* k_empty = k_full + kKSt;
+  uint64_t* v_full = k_empty + kKSt;
+  uint64_t* v_empty = v_full + kVSt;
+  uint64_t* s_full = v_empty + kVSt;   // S of a tile is in its buffer
+  uint64_t* p_full = s_full + 2;       // P has replaced it
+  uint64_t* pv_done = p_full + 2;      // P V is complete: the buffer is free
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tm_k);
+    prefetch_tmap(&tm_v);
+    prefetch_tmap(&tm_kt);
+    prefetch_tmap(&tm_vt);
+    mbar_init(q_full, 4);
+    for (int s = 0; s < kKSt; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); }
+    for (int s = 0; s < kVSt; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&pv_done[i], 1);
+    }
+    fence_mbar_init();
+  }
+  __syncthreads();
+  pdl_wait();
+  pdl_trigger();
+  Piece pc;
+  if (!pc.start(p)) return;
+  if (warp == 5) tmem_alloc(tmem_slot, 256);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  bool ok = true;
+
+  if (warp == 4) {
+    // ---------------- K/V producer ----------------
+    if (lane == 0) {
+      Piece pv = pc;                 // where V is; pc: where K is
+      bool more_k = true, more_v = true;
+      int nk = 0, nv = 0;
+      uint32_t idle = 0;
+      auto load = [&](Piece& at, const CUtensorMap* cache, const CUtensorMap* tree, uint8_t* dst,
+                      uint64_t* full) {
+        const int kvh = at.unit / p.RT, i = at.t0;
+        mbar_arrive_expect_tx(full, SM::kTile);
+        if (i >= at.sp.tiles) {
+          tma_load_5d(dst, tree, full, 0, (i - at.sp.tiles) * KT, 0, kvh, at.b);
+        } else if (p.table) {
+          int blk = p.table[at.b * p.table_stride + at.sp.first + i];
+          if (blk < 0 || blk >= p.num_blocks) blk = p.num_blocks;
+          tma_load_5d(dst, cache, full, 0, 0, 0, kvh, blk);
+        } else {
+          tma_load_5d(dst, cache, full, 0, (at.sp.first + i) * KT, 0, kvh, at.b);
+        }
+        if (i + 1 < at.t1) { at.t0 = i + 1; at.pos += 1; return true; }
+        return at.next(p);
+      };
+      while (ok && more_v) {
+        bool moved = false;
+        if (more_k && (nk < kKSt || mbar_try_wait(&k_empty[nk % kKSt], ((nk / kKSt) & 1) ^ 1))) {
+          const int s = nk % kKSt;
+          more_k = load(pc, &tm_k, &tm_kt, sK + s * SM::kTile, &k_full[s]);
+          ++nk;
+          moved = true;
+        }
+        if (nv < nk && (nv < kVSt || mbar_try_wait(&v_empty[nv % kVSt], ((nv / kVSt) & 1) ^ 1))) {
+          const int s = nv % kVSt;
+          more_v = load(pv, &tm_v, &tm_vt, sV + s * SM::kTile, &v_full[s]);
+          ++nv;
+          moved = true;
+        }
+        if (moved) {
+          idle = 0;
+        } else if (++idle > (kWaitLimit << 2)) {
+          if (p.err) atomicExch(p.err, 63);
+          ok = false;
+        }
+      }
+    }
+  } else if (warp == 5) {
+    // ---------------- MMA issuer ----------------
+    if (lane == 0) {
+      constexpr uint32_t idesc_s = make_idesc_f16(kTcRows, KT, IsBf16<T>::value, 0, 0);
+      constexpr uint32_t idesc_o = make_idesc_f16(kTcRows, D, IsBf16<T>::value, 0, 1);
+      const uint32_t tO = tmem, tS = tmem + 128, qa = smem_u32(sQ);
+      int ns = 0, npv = 0, piece = 0;
+      do {
+        // Q of this piece is written, and O of the piece before it is read
+        ok = mbar_wait(q_full, piece & 1, p.err, 64);
+        ++piece;
+        const int end = npv + (pc.t1 - pc.t0), begin = npv;
+        tc_fence_after();
+        uint32_t idle = 0;
+        while (ok && npv < end) {
+          bool moved = false;
+          // buffer ns % 2 last held P of tile ns - 2
+          if (ns < end && ns < npv + 2 &&
+              (ns < 2 || mbar_try_wait(&pv_done[ns & 1], ((ns - 2) >> 1) & 1)) &&
+              mbar_try_wait(&k_full[ns % kKSt], (ns / kKSt) & 1)) {
+            tc_fence_after();
+            const uint32_t ka = smem_u32(sK + (ns % kKSt) * SM::kTile);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk)
+              tc_mma_f16(tS + (ns & 1) * 64,
+                         make_sdesc(qa + (kk >> 2) * (kTcRows * 128) + (kk & 3) * 32, 16, 1024, 2),
+                         make_sdesc(ka + (kk >> 2) * (KT * 128) + (kk & 3) * 32, 16, 1024, 2),
+                         idesc_s, kk != 0);
+            tc_commit(&s_full[ns & 1]);
+            tc_commit(&k_empty[ns % kKSt]);
+            ++ns;
+            moved = true;
+          }
+          if (npv < ns && mbar_try_wait(&p_full[npv & 1], (npv >> 1) & 1) &&
+              mbar_try_wait(&v_full[npv % kVSt], (npv / kVSt) & 1)) {
+            tc_fence_after();
+            const uint32_t va = smem_u32(sV + (npv % kVSt) * SM::kTile);
+#pragma unroll
+            for (int kk = 0; kk < KT / 16; ++kk)
+              // V is MN-major: 64-dim boxes KT * 128 bytes apart, 8-key groups
+              // 1 KB apart; 16 keys are 2 KB
+              tc_mma_f16_ts(tO, tS + (npv & 1) * 64 + kk * 8,
+                            make_sdesc(va + kk * 2048, KT * 128, 1024, 2), idesc_o,
+                            (npv != begin) || kk != 0);
+            tc_commit(&pv_done[npv & 1]);
+            tc_commit(&v_empty[npv % kVSt]);
+            ++npv;
+            moved = true;
+          }
+          if (moved) {
+            idle = 0;
+          } else if (++idle > (kWaitLimit << 2)) {
+            if (p.err) atomicExch(p.err, 65);
+            ok = false;
+          }
+        }
+      } while (ok && pc.next(p));
+    }
+  } else {
+    // ---------------- softmax and output: thread = row ----------------
+    const int rl = threadIdx.x;
+    const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
+    const uint32_t tO = tmem + lane_off, tS = tmem + 128 + lane_off;
+    int it = 0;
+    do {
+      const int b = pc.b, kvh = pc.unit / p.RT, row0 = (pc.unit % p.RT) * kTcRows;
+      const Span& sp = pc.sp;
+      // Q rows into shared memory, K-major in 128-byte swizzled boxes of 64 dims
+      // (every S of the piece before has been read, so its Q is spent)
+      const T* Q = static_cast<const T*>(p.q) + b * p.q_sb;
+      for (int e = rl; e < kTcRows * (D / 8); e += 128) {
+        const int r = e / (D / 8), ch = e % (D / 8), row = row0 + r;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (row < p.R)
+          x = __ldg(reinterpret_cast<const uint4*>(Q + (row / p.G) * p.q_st +
+                                                   (kvh * p.G + row % p.G) * p.q_sh) + ch);
+        *reinterpret_cast<uint4*>(sQ + (ch >> 3) * (kTcRows * 128) + r * 128 +
+                                  (((ch & 7) ^ (r & 7)) << 4)) = x;
+      }
+      fence_proxy_async_smem();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+      const int row = row0 + rl;
+      const bool live = row < p.R, warp_live = row0 + warp * 32 < p.R;
+      const int node = live ? row / p.G : 0, head = kvh * p.G + (live ? row % p.G : 0);
+      const uint64_t* mrow = p.mask + b * p.mask_sb + (int64_t)node * p.W;
+      const int64_t lo = low_of(p, sp, mrow);
+      float m_ref = -INFINITY, l = 0.f;
+      uint32_t bad = 0;
+      for (int i = pc.t0; i < pc.t1; ++i, ++it) {
+        const int buf = it & 1;
+        if (ok) ok = mbar_wait(&s_full[buf], (it >> 1) & 1, p.err, 66);
+        tc_fence_after();
+        const bool tree = i >= sp.tiles;
+        const int64_t key0 = (int64_t)(sp.first + i) * KT;
+        const bool careful = tree || key0 + KT > sp.ctx || key0 < sp.lo_some;
+        if (warp_live) {
+          float sv[KT];
+          {
+            uint32_t r[KT];
+            tmem_ld32(tS + buf * 64, r);
+            tmem_ld32(tS + buf * 64 + 32, r + 32);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < KT; ++k) sv[k] = __uint_as_float(r[k]);
+          }
+          if (careful) {
+            uint64_t see;
+            if (tree) {
+              const int w = i - sp.tiles, n = p.T - 64 * w;
+              see = mrow[w] & (n < 64 ? (1ull << n) - 1 : ~0ull);
+            } else {
+              const int64_t hi = sp.ctx - key0, from = lo - key0;  // seen: [from, hi)
+              see = hi >= 64 ? ~0ull : (1ull << hi) - 1;
+              if (from > 0) see &= from >= 64 ? 0ull : ~0ull << from;
+            }
+#pragma unroll
+            for (int k = 0; k < KT; ++k)
+              if (!((see >> k) & 1)) sv[k] = -INFINITY;
+          }
+          float pm[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) pm[u] = fmaxf(sv[u], sv[8 + u]);
+#pragma unroll
+          for (int k = 16; k < KT; k += 16)
+#pragma unroll
+            for (int u = 0; u < 8; ++u) pm[u] = fmax3(pm[u], sv[k + u], sv[k + 8 + u]);
+          const float mx = fmax3(fmax3(pm[0], pm[1], pm[2]), fmax3(pm[3], pm[4], pm[5]),
+                                 fmaxf(pm[6], pm[7])) * p.scale_log2;
+          // lazy base, as above; O's rescale is warp-collective, so lanes that
+          // keep their base use the factor 1
+          const bool grow = mx > m_ref + kRescale;
+          const float corr = grow ? ex2_ftz(m_ref - mx) : 1.f;
+          if (grow) { l *= corr; m_ref = mx; }
+          if (i > pc.t0 && __any_sync(0xffffffffu, grow)) {
+            if (ok) ok = mbar_wait(&pv_done[(it - 1) & 1], ((it - 1) >> 1) & 1, p.err, 67);
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+              uint32_t r[32];
+              tmem_ld32(tO + c, r);
+              tmem_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * corr);
+              tmem_st32(tO + c, r);
+            }
+            tmem_wait_st();
+          }
+          const float nm = m_ref == -INFINITY ? 0.f : -m_ref;
+          const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), nm2 = f2_pack(nm, nm);
+          uint64_t ps[4] = {0ull, 0ull, 0ull, 0ull};
+          uint32_t pk[KT / 2];
+#pragma unroll
+          for (int k = 0; k < KT; k += 2) {
+            float a0, a1;
+            f2_unpack(f2_fma(f2_pack(sv[k], sv[k + 1]), sc2, nm2), a0, a1);
+            const float p0 = ex2_ftz(a0), p1 = ex2_ftz(a1);
+            ps[(k >> 1) & 3] = f2_add(ps[(k >> 1) & 3], f2_pack(p0, p1));
+            pk[k / 2] = pack2<T>(p0, p1);
+          }
+          float t0, t1;
+          f2_unpack(f2_add(f2_add(ps[0], ps[1]), f2_add(ps[2], ps[3])), t0, t1);
+          l += t0 + t1;
+          tmem_st32(tS + buf * 64, pk);
+          tmem_wait_st();
+        }
+        if (careful) {
+          // clear the values that no row may take from this tile's V
+          if (ok) ok = mbar_wait(&v_full[it % kVSt], (it / kVSt) & 1, p.err, 68);
+          uint8_t* v = sV + (it % kVSt) * SM::kTile;
+          for (int e = rl; e < KT * (D / 8); e += 128) {
+            const int64_t key = key0 + (e / 8) % KT;
+            uint4* w = reinterpret_cast<uint4*>(v) + e;   // [box][key][8 chunks]
+            uint4 x = *w;
+            if (!tree && (key >= sp.ctx || key < sp.lo_all)) {
+              x = make_uint4(0, 0, 0, 0);
+            } else {
+              x.x = finite2<T>(x.x, bad); x.y = finite2<T>(x.y, bad);
+              x.z = finite2<T>(x.z, bad); x.w = finite2<T>(x.w, bad);
+            }
+            *w = x;
+          }
+          fence_proxy_async_smem();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[buf]);
+      }
+      // ---- the piece's output ----
+      if (ok) ok = mbar_wait(&pv_done[(it - 1) & 1], ((it - 1) >> 1) & 1, p.err, 69);
+      tc_fence_after();
+      float* slot = pc.whole ? nullptr : slot_of(p, D, blockIdx.x, pc.t0 == 0);
+      if (warp_live) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        T* dst = static_cast<T*>(p.o) + b * p.o_sb + node * p.o_st + head * p.o_sh;
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          uint32_t r[32];
+          __syncwarp();
+          tmem_ld32(tO + c, r);
+          tmem_wait_ld();
+          if (!live) {
+          } else if (!pc.whole) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 4)
+              *reinterpret_cast<uint4*>(slot + rl * D + c + k) =
+                  make_uint4(r[k], r[k + 1], r[k + 2], r[k + 3]);
+          } else {
+            uint32_t w[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+              w[k] = pack2<T>(__uint_as_float(r[2 * k]) * inv, __uint_as_float(r[2 * k + 1]) * inv);
+            if (p.o_vec) {
+#pragma unroll
+              for (int k = 0; k < 16; k += 4)
+                *reinterpret_cast<uint4*>(dst + c + 2 * k) = make_uint4(w[k], w[k + 1], w[k + 2], w[k + 3]);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 16; ++k) *reinterpret_cast<uint32_t*>(dst + c + 2 * k) = w[k];
+            }
+          }
+        }
+        if (!pc.whole && live) {
+          slot[p.rows * D + rl] = m_ref;
+          slot[p.rows * (D + 1) + rl] = l;
+        }
+      }
+      const bool odd = bar_softmax_or(bad != 0);
+      if (!pc.whole) {
+        if (rl == 0) slot[p.rows * (D + 2)] = odd ? 1.f : 0.f;
+      } else if (odd && live) {
+        T* dst = static_cast<T*>(p.o) + b * p.o_sb + node * p.o_st + head * p.o_sh;
+        for (int d = 0; d < D; ++d) {
+          const float acc = odd_values<T, D>(p, sp, b, kvh, node, d);
+          if (acc != 0.f) dst[d] = from_f32<T>(to_f32(dst[d]) + acc);
+        }
+      }
+    } while (pc.next(p));
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 5) tmem_dealloc(tmem, 256);
+}
+
 // Joins the pieces of the units that more than one part holds: a warp a row.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant__ TreeArgs p) {
@@ -653,13 +1022,14 @@ struct TreeCall {
 };
 
 // How a call is cut: the row groups of a CTA and the parts (0: one a unit).
-struct Plan { int rw, rt, ctas; };
+struct Plan { int rw, rows, rt, ctas; };  // rw 0: tcgen05
 Plan plan_of(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t max_ctx,
              int64_t window_left) {
   const int64_t R = T * (Hq / Hkv);
   Plan pl;
-  pl.rw = R <= 16 ? 1 : R <= 32 ? 2 : 4;
-  pl.rt = (int)((R + 16 * pl.rw - 1) / (16 * pl.rw));
+  pl.rw = R <= 16 ? 1 : R <= 32 ? 2 : 0;
+  pl.rows = pl.rw ? 16 * pl.rw : kTcRows;
+  pl.rt = (int)((R + pl.rows - 1) / pl.rows);
   int64_t keys = max_ctx;
   if (window_left >= 0 && window_left + 1 < keys) keys = window_left + KT;
   const int64_t tiles = (keys + KT - 1) / KT + (T + 63) / 64;
@@ -680,7 +1050,7 @@ int kv_map(CUtensorMap* m, const void* base, int dtype, int64_t D, int64_t rows,
 }
 
 int64_t workspace_of(const Plan& pl, int64_t D) {
-  return pl.ctas ? 2 * pl.ctas * slot_floats(16 * pl.rw, (int)D) * 4 : 0;
+  return pl.ctas ? 2 * pl.ctas * slot_floats(pl.rows, (int)D) * 4 : 0;
 }
 
 int tree_attention(const TreeCall& c, int dtype, cudaStream_t st) {
@@ -730,31 +1100,32 @@ int tree_attention(const TreeCall& c, int dtype, cudaStream_t st) {
   a.err = device_error_flag();
   const Plan pl = plan_of(c.B, c.T, c.Hq, c.Hkv, c.max_ctx, c.window_left);
   const int rw = pl.rw;
-  a.RT = pl.rt; a.ctas = pl.ctas; a.rows = 16 * rw;
+  a.RT = pl.rt; a.ctas = pl.ctas; a.rows = pl.rows;
+  a.o_vec = aligned16(c.o) && ((c.o_sb | c.o_st | c.o_sh) & 7) == 0;
   a.ws = static_cast<float*>(c.ws);
   TPP_REQUIRE(pl.ctas == 0 || (c.ws && c.ws_bytes >= workspace_of(pl, c.D) && aligned16(c.ws)),
               TPP_ERR_WORKSPACE, "workspace missing, too small or not 16-byte aligned");
   const int64_t units = c.B * c.Hkv * pl.rt;
   TPP_REQUIRE(units < (1ll << 31), TPP_ERR_SHAPE, "too many rows");
   const dim3 grid((unsigned)(pl.ctas ? pl.ctas : units));
-  auto go = [&](auto kern, size_t smem) -> int {
+  auto go = [&](auto kern, int threads, size_t smem) -> int {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
         cudaSuccess) {
       set_error("tree_attn_kernel: cannot reserve shared memory");
       return TPP_ERR_LAUNCH;
     }
-    return launch("tree_attn_kernel", kern, grid, dim3(kThreads), smem, st, 0u, tk, tv, tkt, tvt,
+    return launch("tree_attn_kernel", kern, grid, dim3(threads), smem, st, 0u, tk, tv, tkt, tvt,
                   a);
   };
   rc = TPP_DISPATCH_HALF(dtype, T, [&]() -> int {
     if (c.D == 64) {
-      if (rw == 1) return go(tree_attn_kernel<T, 64, 1>, TreeSmem<64, 1>::kBytes);
-      if (rw == 2) return go(tree_attn_kernel<T, 64, 2>, TreeSmem<64, 2>::kBytes);
-      return go(tree_attn_kernel<T, 64, 4>, TreeSmem<64, 4>::kBytes);
+      if (rw == 1) return go(tree_attn_kernel<T, 64, 1>, kThreads, TreeSmem<64, 1>::kBytes);
+      if (rw == 2) return go(tree_attn_kernel<T, 64, 2>, kThreads, TreeSmem<64, 2>::kBytes);
+      return go(tree_attn_tc_kernel<T, 64>, kTcThreads, TcSmem<64>::kBytes);
     }
-    if (rw == 1) return go(tree_attn_kernel<T, 128, 1>, TreeSmem<128, 1>::kBytes);
-    if (rw == 2) return go(tree_attn_kernel<T, 128, 2>, TreeSmem<128, 2>::kBytes);
-    return go(tree_attn_kernel<T, 128, 4>, TreeSmem<128, 4>::kBytes);
+    if (rw == 1) return go(tree_attn_kernel<T, 128, 1>, kThreads, TreeSmem<128, 1>::kBytes);
+    if (rw == 2) return go(tree_attn_kernel<T, 128, 2>, kThreads, TreeSmem<128, 2>::kBytes);
+    return go(tree_attn_tc_kernel<T, 128>, kTcThreads, TcSmem<128>::kBytes);
   });
   if (rc != TPP_OK || pl.ctas == 0) return rc;
   const int64_t blocks = (c.B * c.Hkv * a.R + 7) / 8;
