@@ -50,6 +50,7 @@ struct TreeArgs {
   float scale_log2;
   int B, T, Hq, Hkv, G, W, R, RT, NT;  // W mask words a row, R = T * G rows, NT tree tiles
   int ctas, rows;                      // parts at most (0: a unit each), rows of a unit
+  int min_tiles;                       // tiles of a part at least
   int o_vec;                           // the output's rows start on 16 bytes
   float* ws;                           // pieces: two a part
   int* err;
@@ -108,52 +109,67 @@ __device__ __forceinline__ Span span_of(const TreeArgs& p, int b) {
 
 // ---- the list of tiles -------------------------------------------------------
 // Units in (b, kv head, row tile) order, each with its cache's tiles, then the
-// tree's.  Part c of n is [total * c / n, total * (c + 1) / n).
-struct Parts { int64_t total; int n; };
-__device__ __forceinline__ int64_t part_start(const Parts& s, int c) { return s.total * c / s.n; }
-
-// The number of tiles before sequence b, by one warp; b = B gives all.
-__device__ __forceinline__ int64_t tiles_before(const TreeArgs& p, int b) {
-  const int lane = threadIdx.x & 31;
-  int64_t n = 0;
-  for (int i = lane; i < b; i += 32) n += span_of(p, i).tiles + p.NT;
+// tree's.  The first `more` of n parts hold each + 1 tiles, the others `each`.
+struct Parts {
+  int n, each, more;
+  __device__ __forceinline__ int start(int c) const { return each * c + min(c, more); }
+  __device__ __forceinline__ int of(int x) const {
+    const int x1 = more * (each + 1);
+    return x < x1 ? x / (each + 1) : more + (x - x1) / each;
+  }
+};
+// The tiles of lane i's sequence (32 * round + i) and of all up to it, by one
+// warp; `before` holds those of earlier rounds.
+__device__ __forceinline__ int tiles_scan(const TreeArgs& p, int round, int& incl) {
+  const int lane = threadIdx.x & 31, b = 32 * round + lane;
+  const int n = b < p.B ? (span_of(p, b).tiles + p.NT) * p.Hkv * p.RT : 0;
+  incl = n;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-  return n * p.Hkv * p.RT;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += up;
+  }
+  return n;
 }
-__device__ __forceinline__ Parts parts_of(const TreeArgs& p) {
+__device__ __forceinline__ Parts parts_of(const TreeArgs& p, int total) {
   Parts s;
-  s.total = tiles_before(p, p.B);
-  s.n = (int)max((int64_t)1, min((int64_t)p.ctas, s.total / kMinTiles));
+  s.n = max(1, min(p.ctas, total / p.min_tiles));
+  s.each = total / s.n;
+  s.more = total - s.each * s.n;
   return s;
 }
-// The sequence that tile x of the list belongs to and the tiles before it.
-__device__ __forceinline__ int sequence_of(const TreeArgs& p, int64_t x, int64_t& before) {
-  const int lane = threadIdx.x & 31;
+// All tiles, and those before sequence b.
+__device__ __forceinline__ int tiles_before(const TreeArgs& p, int b, int& total) {
+  int before = 0;
+  total = 0;
+  for (int r = 0; 32 * r < p.B; ++r) {
+    int incl;
+    const int n = tiles_scan(p, r, incl);
+    if (b / 32 == r) before = total + __shfl_sync(0xffffffffu, incl - n, b % 32);
+    total += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return before;
+}
+// The sequence that tile x of the list belongs to, and the tiles before it.
+__device__ __forceinline__ int sequence_of(const TreeArgs& p, int x, int& before) {
   before = 0;
-  for (int b0 = 0;; b0 += 32) {
-    const int64_t n = b0 + lane < p.B
-        ? (int64_t)(span_of(p, b0 + lane).tiles + p.NT) * p.Hkv * p.RT : 0;
-    int64_t incl = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += up;
-    }
+  for (int r = 0; 32 * r < p.B; ++r) {
+    int incl;
+    const int n = tiles_scan(p, r, incl);
     const unsigned hit = __ballot_sync(0xffffffffu, n > 0 && x < before + incl);
     if (hit) {
       const int l = __ffs(hit) - 1;
       before += __shfl_sync(0xffffffffu, incl - n, l);
-      return b0 + l;
+      return 32 * r + l;
     }
-    if (b0 + 32 >= p.B) return p.B;  // past the end
     before += __shfl_sync(0xffffffffu, incl, 31);
   }
+  return p.B;  // past the end
 }
 // Walks the pieces of units in one CTA's part.
 struct Piece {
-  int64_t pos, end, before;  // in the list; before: tiles of earlier sequences
-  int b, unit, t0, t1;       // tiles [t0, t1) of the unit (kv head, row tile) of b
+  int pos, end, before;  // in the list; before: tiles of earlier sequences
+  int b, unit, t0, t1;   // tiles [t0, t1) of the unit (kv head, row tile) of b
   Span sp;
   bool whole;
   __device__ __forceinline__ bool start(const TreeArgs& p) {
@@ -161,14 +177,16 @@ struct Piece {
       const int u = p.Hkv * p.RT;
       b = blockIdx.x / u;
       sp = span_of(p, b);
-      before = pos = (int64_t)blockIdx.x * (sp.tiles + p.NT);  // b's list begins at unit 0
-      before -= (int64_t)(blockIdx.x % u) * (sp.tiles + p.NT);
+      before = 0;  // a list of b's own
+      pos = (int)(blockIdx.x % u) * (sp.tiles + p.NT);
       end = pos + sp.tiles + p.NT;
     } else {
-      const Parts s = parts_of(p);
+      int total;
+      tiles_before(p, 0, total);
+      const Parts s = parts_of(p, total);
       if ((int)blockIdx.x >= s.n) return false;
-      pos = part_start(s, blockIdx.x);
-      end = part_start(s, blockIdx.x + 1);
+      pos = s.start(blockIdx.x);
+      end = s.start(blockIdx.x + 1);
       b = sequence_of(p, pos, before);
       if (b >= p.B) return false;
       sp = span_of(p, b);
@@ -178,10 +196,9 @@ struct Piece {
   }
   __device__ __forceinline__ void locate(const TreeArgs& p) {
     const int n = sp.tiles + p.NT;
-    const int64_t at = pos - before;
-    unit = (int)(at / n);
-    t0 = (int)(at - (int64_t)unit * n);
-    t1 = (int)min((int64_t)n, t0 + (end - pos));
+    unit = (pos - before) / n;
+    t0 = pos - before - unit * n;
+    t1 = min(n, t0 + (end - pos));
     whole = t0 == 0 && t1 == n;
   }
   __device__ __forceinline__ bool next(const TreeArgs& p) {
@@ -189,7 +206,7 @@ struct Piece {
     if (pos >= end) return false;
     const int n = sp.tiles + p.NT;
     if (unit == p.Hkv * p.RT - 1 && t1 == n) {
-      before += (int64_t)n * p.Hkv * p.RT;
+      before += n * p.Hkv * p.RT;
       sp = span_of(p, ++b);
     }
     locate(p);
@@ -777,14 +794,24 @@ __global__ void __launch_bounds__(kTcThreads, 2) tree_attn_tc_kernel(
       // Q rows into shared memory, K-major in 128-byte swizzled boxes of 64 dims
       // (every S of the piece before has been read, so its Q is spent)
       const T* Q = static_cast<const T*>(p.q) + b * p.q_sb;
-      for (int e = rl; e < kTcRows * (D / 8); e += 128) {
-        const int r = e / (D / 8), ch = e % (D / 8), row = row0 + r;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (row < p.R)
-          x = __ldg(reinterpret_cast<const uint4*>(Q + (row / p.G) * p.q_st +
-                                                   (kvh * p.G + row % p.G) * p.q_sh) + ch);
-        *reinterpret_cast<uint4*>(sQ + (ch >> 3) * (kTcRows * 128) + r * 128 +
-                                  (((ch & 7) ^ (r & 7)) << 4)) = x;
+#pragma unroll
+      for (int e0 = 0; e0 < kTcRows * (D / 8); e0 += 128 * 8) {
+        uint4 x[8];  // eight loads in flight
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int e = e0 + u * 128 + rl, row = row0 + e / (D / 8);
+          x[u] = make_uint4(0, 0, 0, 0);
+          if (row < p.R)
+            x[u] = __ldg(reinterpret_cast<const uint4*>(Q + (row / p.G) * p.q_st +
+                                                        (kvh * p.G + row % p.G) * p.q_sh) +
+                         e % (D / 8));
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int e = e0 + u * 128 + rl, r = e / (D / 8), ch = e % (D / 8);
+          *reinterpret_cast<uint4*>(sQ + (ch >> 3) * (kTcRows * 128) + r * 128 +
+                                    (((ch & 7) ^ (r & 7)) << 4)) = x[u];
+        }
       }
       fence_proxy_async_smem();
       tc_fence_before();
@@ -955,52 +982,69 @@ __global__ void __launch_bounds__(kTcThreads, 2) tree_attn_tc_kernel(
 // Joins the pieces of the units that more than one part holds: a warp a row.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant__ TreeArgs p) {
+  const int lane = threadIdx.x & 31;
+  const int item = blockIdx.x * 8 + (threadIdx.x >> 5);
+  // which pieces: from the lengths alone, which the kernel before this one
+  // only reads
+  const bool in = item < p.B * p.Hkv * p.R;
+  const int row = item % p.R;
+  const int kvh = item / p.R % p.Hkv, b = in ? item / p.R / p.Hkv : 0;
+  const Span sp = span_of(p, b);
+  int total;
+  const int before = tiles_before(p, b, total);
+  const Parts s = parts_of(p, total);
+  const int n = sp.tiles + p.NT;
+  const int x0 = before + (kvh * p.RT + row / p.rows) * n;
+  const int c0 = s.of(x0), c1 = s.of(x0 + n - 1);
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (item >= (int64_t)p.B * p.Hkv * p.R) return;
-  const int row = (int)(item % p.R);
-  const int kvh = (int)(item / p.R % p.Hkv), b = (int)(item / p.R / p.Hkv);
-  const Span sp = span_of(p, b);
-  const Parts s = parts_of(p);
-  const int n = sp.tiles + p.NT;
-  const int64_t x0 = tiles_before(p, b) + (int64_t)(kvh * p.RT + row / p.rows) * n;
-  auto part_with = [&](int64_t x) {
-    int c = (int)min((int64_t)s.n - 1, x * s.n / s.total);
-    while (part_start(s, c) > x) --c;
-    while (part_start(s, c + 1) <= x) ++c;
-    return c;
-  };
-  const int c0 = part_with(x0), c1 = part_with(x0 + n - 1);
-  if (c0 == c1) return;
+  if (!in || c0 == c1) return;
   const int r = row % p.rows;
-  float M = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32)
-    M = fmaxf(M, slot_of(p, D, c, c == c0)[p.rows * D + r]);
-  M = warp_max(M);
-  const float base = M == -INFINITY ? 0.f : M;
-  float L = 0.f, odd = 0.f;
   constexpr int PER = D / 32;
-  float o[PER];
+  float M = -INFINITY, L = 0.f, odd = 0.f, o[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) o[i] = 0.f;
-#pragma unroll 4
-  for (int c = c0; c <= c1; ++c) {
-    const float* sl = slot_of(p, D, c, c == c0);
-    const float w = ex2_ftz(sl[p.rows * D + r] - base);
-    L += w * sl[p.rows * (D + 1) + r];
-    odd += sl[p.rows * (D + 2)];
+  // 32 pieces at a time: a lane takes the weight of one, all take its values
+  for (int k0 = c0; k0 <= c1; k0 += 32) {
+    const int k = k0 + lane, cnt = min(32, c1 - k0 + 1);
+    float m = -INFINITY, l = 0.f;
+    if (k <= c1) {
+      const float* sl = slot_of(p, D, k, k == c0);
+      m = sl[p.rows * D + r];
+      l = sl[p.rows * (D + 1) + r];
+      odd += sl[p.rows * (D + 2)];
+    }
+    const float mx = fmaxf(M, warp_max(m));
+    const float base = mx == -INFINITY ? 0.f : mx;
+    const float w = ex2_ftz(m - base), corr = ex2_ftz(M - base);
+    M = mx;
+    L = L * corr + warp_sum(l * w);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) o[i] = fmaf(w, sl[r * D + lane * PER + i], o[i]);
+    for (int i = 0; i < PER; ++i) o[i] *= corr;
+#pragma unroll 8
+    for (int j = 0; j < cnt; ++j) {
+      const float wj = __shfl_sync(0xffffffffu, w, j);
+      const float* sl = slot_of(p, D, k0 + j, k0 + j == c0) + r * D + lane * PER;
+      float v[PER];
+      if constexpr (PER == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(sl);
+        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+      } else {
+        const float2 x = *reinterpret_cast<const float2*>(sl);
+        v[0] = x.x; v[1] = x.y;
+      }
+#pragma unroll
+      for (int i = 0; i < PER; ++i) o[i] = fmaf(wj, v[i], o[i]);
+    }
   }
+  const bool any_odd = __any_sync(0xffffffffu, odd != 0.f);
   const float inv = L == 0.f ? 0.f : 1.f / L;
   const int t = row / p.G, h = kvh * p.G + row % p.G;
   T* dst = static_cast<T*>(p.o) + b * p.o_sb + t * p.o_st + h * p.o_sh + lane * PER;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     o[i] *= inv;
-    if (odd != 0.f) o[i] += odd_values<T, D>(p, sp, b, kvh, t, lane * PER + i);
+    if (any_odd) o[i] += odd_values<T, D>(p, sp, b, kvh, t, lane * PER + i);
   }
 #pragma unroll
   for (int i = 0; i < PER; i += 2)
@@ -1102,11 +1146,14 @@ int tree_attention(const TreeCall& c, int dtype, cudaStream_t st) {
   const int rw = pl.rw;
   a.RT = pl.rt; a.ctas = pl.ctas; a.rows = pl.rows;
   a.o_vec = aligned16(c.o) && ((c.o_sb | c.o_st | c.o_sh) & 7) == 0;
+  a.min_tiles = kMinTiles;
   a.ws = static_cast<float*>(c.ws);
   TPP_REQUIRE(pl.ctas == 0 || (c.ws && c.ws_bytes >= workspace_of(pl, c.D) && aligned16(c.ws)),
               TPP_ERR_WORKSPACE, "workspace missing, too small or not 16-byte aligned");
   const int64_t units = c.B * c.Hkv * pl.rt;
-  TPP_REQUIRE(units < (1ll << 31), TPP_ERR_SHAPE, "too many rows");
+  TPP_REQUIRE(units * (c.max_ctx / KT + a.NT + 1) < (1ll << 31) &&
+                  c.B * c.Hkv * a.R < (1ll << 31) - 8,
+              TPP_ERR_SHAPE, "too many rows or tiles");
   const dim3 grid((unsigned)(pl.ctas ? pl.ctas : units));
   auto go = [&](auto kern, int threads, size_t smem) -> int {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
