@@ -12,8 +12,9 @@
 // part is finished there; the pieces of the others go to the workspace as
 // (m, l, o) in fp32 and tree_combine_kernel joins them, in list order.
 //
-// Thread 0 feeds a ring of K/V tiles by TMA (one request an operand), on into the
-// next piece; it refills a stage one tile after its use.  (A producer warp of
+// Threads 0 and 32 feed a ring of K and V tiles by TMA (one request a tile; an
+// issuing thread spends about 0.2 us on each), on into the next piece; they refill
+// a stage one tile after its use.  (A producer warp of
 // its own makes 10 warps an SM, three on one scheduler, and so caps the
 // registers of two CTAs at 168: the 64-row form spilled.)  The four warps are RW
 // row groups of 16 rows x KW = 4 / RW key groups, each with its own running
@@ -35,7 +36,6 @@ namespace {
 constexpr int KT = 64;            // keys of a tile
 constexpr int kThreads = 128;
 constexpr int kMaxNodes = 256;
-constexpr int kMinTiles = 4;      // tiles of a part at least
 constexpr float kRescale = 8.0f;  // log2: the base moves when the maximum grew by 2^8
 
 struct TreeArgs {
@@ -150,22 +150,6 @@ __device__ __forceinline__ int tiles_before(const TreeArgs& p, int b, int& total
   }
   return before;
 }
-// The sequence that tile x of the list belongs to, and the tiles before it.
-__device__ __forceinline__ int sequence_of(const TreeArgs& p, int x, int& before) {
-  before = 0;
-  for (int r = 0; 32 * r < p.B; ++r) {
-    int incl;
-    const int n = tiles_scan(p, r, incl);
-    const unsigned hit = __ballot_sync(0xffffffffu, n > 0 && x < before + incl);
-    if (hit) {
-      const int l = __ffs(hit) - 1;
-      before += __shfl_sync(0xffffffffu, incl - n, l);
-      return 32 * r + l;
-    }
-    before += __shfl_sync(0xffffffffu, incl, 31);
-  }
-  return p.B;  // past the end
-}
 // Walks the pieces of units in one CTA's part.
 struct Piece {
   int pos, end, before;  // in the list; before: tiles of earlier sequences
@@ -181,13 +165,26 @@ struct Piece {
       pos = (int)(blockIdx.x % u) * (sp.tiles + p.NT);
       end = pos + sp.tiles + p.NT;
     } else {
-      int total;
-      tiles_before(p, 0, total);
+      int incl, total = 0, rounds = (p.B + 31) / 32;
+      int n = 0;
+      for (int r = 0; r < rounds; ++r) {
+        n = tiles_scan(p, r, incl);
+        total += __shfl_sync(0xffffffffu, incl, 31);
+      }
       const Parts s = parts_of(p, total);
       if ((int)blockIdx.x >= s.n) return false;
       pos = s.start(blockIdx.x);
       end = s.start(blockIdx.x + 1);
-      b = sequence_of(p, pos, before);
+      // the sequence that pos belongs to; the scan of a single round is at hand
+      b = p.B;
+      before = 0;
+      for (int r = 0; r < rounds && b == p.B; ++r) {
+        if (rounds > 1) n = tiles_scan(p, r, incl);
+        const unsigned hit = __ballot_sync(0xffffffffu, n > 0 && pos < before + incl);
+        const int l = hit ? __ffs(hit) - 1 : 31;
+        if (hit) b = 32 * r + l;
+        before += __shfl_sync(0xffffffffu, hit ? incl - n : incl, l);
+      }
       if (b >= p.B) return false;
       sp = span_of(p, b);
     }
@@ -222,7 +219,7 @@ struct TreeSmem {
   static constexpr int kDims = RW == 1 ? D : 64;  // dims merged at a time
   static constexpr uint32_t kMerge = KW > 1 ? RW * 16 * kDims * 4 : 0;
   static constexpr uint32_t kMl = 4 * 16 * 2 * 4;  // (m, l) of each warp's rows
-  static constexpr size_t kBytes = 1024 + kRing + kMerge + kMl + 2 * kStages * 8 + sizeof(Piece);
+  static constexpr size_t kBytes = 1024 + kRing + kMerge + kMl + 2 * kStages * 8 + 2 * sizeof(Piece);
 };
 
 // Where part c keeps a piece: the one that starts its unit, or continues one.
@@ -289,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attn_kernel(
     prefetch_tmap(&tm_kt);
     prefetch_tmap(&tm_vt);
     for (int s = 0; s < ST; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], 2);
       mbar_init(&empty[s], 4);
     }
     fence_mbar_init();
@@ -302,29 +299,27 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attn_kernel(
   if (!pc.start(p)) return;
   bool ok = true;
   int it = 0;  // tiles so far: the ring's position
-  // The loads run ahead of pc; thread 0 keeps their place in shared memory.
-  Piece* ahead = reinterpret_cast<Piece*>(empty + ST);
+  // The loads run ahead of pc; their threads keep the place in shared memory.
+  const bool loader = threadIdx.x == 0 || threadIdx.x == 32;
+  Piece* ahead = reinterpret_cast<Piece*>(empty + ST) + (warp & 1);
+  const CUtensorMap* from = warp == 0 ? &tm_k : &tm_v;
+  const CUtensorMap* from_tree = warp == 0 ? &tm_kt : &tm_vt;
   int issued = 0;
-  auto issue = [&]() {  // thread 0: the next tile of the part, if there is one
+  auto issue = [&]() {  // the next tile of the part, if there is one
     if (issued < 0) return;
     const int i = ahead->t0, b = ahead->b, kvh = ahead->unit / p.RT;
     const int s = issued % ST, first = ahead->sp.first, tiles = ahead->sp.tiles;
-    uint8_t* kd = smem + s * 2 * SM::kTile;
-    uint8_t* vd = kd + SM::kTile;
-    mbar_arrive_expect_tx(&full[s], 2 * SM::kTile);
+    uint8_t* dst = smem + (s * 2 + (warp & 1)) * SM::kTile;
+    mbar_arrive_expect_tx(&full[s], SM::kTile);
     if (i >= tiles) {
-      const int n0 = (i - tiles) * KT;
-      tma_load_5d(kd, &tm_kt, &full[s], 0, n0, 0, kvh, b);
-      tma_load_5d(vd, &tm_vt, &full[s], 0, n0, 0, kvh, b);
+      tma_load_5d(dst, from_tree, &full[s], 0, (i - tiles) * KT, 0, kvh, b);
     } else if (p.table) {
       // a block outside the pool is out of the map's range: zeros
       int blk = p.table[b * p.table_stride + first + i];
       if (blk < 0 || blk >= p.num_blocks) blk = p.num_blocks;
-      tma_load_5d(kd, &tm_k, &full[s], 0, 0, 0, kvh, blk);
-      tma_load_5d(vd, &tm_v, &full[s], 0, 0, 0, kvh, blk);
+      tma_load_5d(dst, from, &full[s], 0, 0, 0, kvh, blk);
     } else {
-      tma_load_5d(kd, &tm_k, &full[s], 0, (first + i) * KT, 0, kvh, b);
-      tma_load_5d(vd, &tm_v, &full[s], 0, (first + i) * KT, 0, kvh, b);
+      tma_load_5d(dst, from, &full[s], 0, (first + i) * KT, 0, kvh, b);
     }
     ++issued;
     if (i + 1 < ahead->t1) {
@@ -334,10 +329,11 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attn_kernel(
       issued = -1;
     }
   };
-  if (threadIdx.x == 0) {
+  if (loader) {
     *ahead = pc;
     for (int s = 0; s < ST; ++s) issue();
   }
+  __syncwarp();
 
   // ---------------- compute ----------------
   const int g = lane >> 2, c = lane & 3;
@@ -379,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attn_kernel(
 
   for (int i = pc.t0; i < pc.t1; ++i, ++it) {
     const int s = it % ST;
-    if (threadIdx.x == 0 && it > 0 && ok && issued >= 0) {
+    if (loader && it > 0 && ok && issued >= 0) {
       ok = mbar_wait(&empty[(it - 1) % ST], ((it - 1) / ST) & 1, p.err, 61);
       if (ok) issue();
     }
@@ -607,8 +603,10 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attn_kernel(
 // unit is a 128-row tile on the 5th-generation tensor core.  Two CTAs an SM, each
 // with its own S, P and O in 256 columns of TMEM: while one waits for its scores
 // the other's softmax runs.
-//   warps 0-3: Q into shared memory, softmax (a row a thread), output
-//   warp 4:    K and V tiles by TMA into two rings, ahead into the next piece
+//   warps 0-3: softmax (a row a thread), output
+//   warp 4:    Q, and K and V tiles into two rings, by TMA, ahead into the next
+//              piece (a unit takes as many whole nodes as 128 rows hold, so that
+//              its Q is one box of nodes x heads for each 64 dims)
 //   warp 5:    S = Q K^T (M 128, N 64), O += P V (P read from TMEM)
 // S and P share two 64-column buffers; S of tile j+1 is computed under the softmax
 // of tile j.  Dead rows of a narrow unit (R < 128) are skipped by whole warps.
@@ -635,14 +633,15 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kTcThreads, 2) tree_attn_tc_kernel(
     const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
     const __grid_constant__ CUtensorMap tm_kt, const __grid_constant__ CUtensorMap tm_vt,
-    const __grid_constant__ TreeArgs p) {
+    const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ TreeArgs p) {
   using SM = TcSmem<D>;
   extern __shared__ __align__(1024) uint8_t tc_smem[];
   uint8_t* sQ = tc_smem;
   uint8_t* sK = sQ + SM::kQ;
   uint8_t* sV = sK + kKSt * SM::kTile;
   uint64_t* q_full = reinterpret_cast<uint64_t*>(sV + kVSt * SM::kTile);
-  uint64_t* k_full = q_full + 1;
+  uint64_t* q_empty = q_full + 1;      // every S of a piece is complete
+  uint64_t* k_full = q_empty + 1;
   uint64_t* k_empty = k_full + kKSt;
   uint64_t* v_full = k_empty + kKSt;
   uint64_t* v_empty = v_full + kVSt;
@@ -657,7 +656,9 @@ __global__ void __launch_bounds__(kTcThreads, 2) tree_attn_tc_kernel(
     prefetch_tmap(&tm_v);
     prefetch_tmap(&tm_kt);
     prefetch_tmap(&tm_vt);
-    mbar_init(q_full, 4);
+    prefetch_tmap(&tm_q);
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
     for (int s = 0; s < kKSt; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); }
     for (int s = 0; s < kVSt; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
     for (int i = 0; i < 2; ++i) {
@@ -683,8 +684,8 @@ __global__ void __launch_bounds__(kTcThreads, 2) tree_attn_tc_kernel(
     // ---------------- K/V producer ----------------
     if (lane == 0) {
       Piece pv = pc;                 // where V is; pc: where K is
-      bool more_k = true, more_v = true;
-      int nk = 0, nv = 0;
+      bool more_k = true, more_v = true, new_piece = true;
+      int nk = 0, nv = 0, nq = 0;
       uint32_t idle = 0;
       auto load = [&](Piece& at, const CUtensorMap* cache, const CUtensorMap* tree, uint8_t* dst,
                       uint64_t* full) {
@@ -704,9 +705,20 @@ __global__ void __launch_bounds__(kTcThreads, 2) tree_attn_tc_kernel(
       };
       while (ok && more_v) {
         bool moved = false;
-        if (more_k && (nk < kKSt || mbar_try_wait(&k_empty[nk % kKSt], ((nk / kKSt) & 1) ^ 1))) {
+        if (new_piece && (nq == 0 || mbar_try_wait(q_empty, (nq - 1) & 1))) {
+          mbar_arrive_expect_tx(q_full, p.rows * D * 2);
+          for (int bx = 0; bx < D / 64; ++bx)
+            tma_load_5d(sQ + bx * (kTcRows * 128), &tm_q, q_full, 0, (pc.unit / p.RT) * p.G,
+                        (pc.unit % p.RT) * (p.rows / p.G), bx, pc.b);
+          ++nq;
+          new_piece = false;
+          moved = true;
+        }
+        if (more_k && !new_piece && (nk < kKSt || mbar_try_wait(&k_empty[nk % kKSt], ((nk / kKSt) & 1) ^ 1))) {
           const int s = nk % kKSt;
+          new_piece = pc.t0 + 1 == pc.t1;
           more_k = load(pc, &tm_k, &tm_kt, sK + s * SM::kTile, &k_full[s]);
+          new_piece = new_piece && more_k;
           ++nk;
           moved = true;
         }
@@ -732,7 +744,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) tree_attn_tc_kernel(
       const uint32_t tO = tmem, tS = tmem + 128, qa = smem_u32(sQ);
       int ns = 0, npv = 0, piece = 0;
       do {
-        // Q of this piece is written, and O of the piece before it is read
+        // (O of the piece before is read by the time the first P is written)
         ok = mbar_wait(q_full, piece & 1, p.err, 64);
         ++piece;
         const int end = npv + (pc.t1 - pc.t0), begin = npv;
@@ -754,6 +766,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) tree_attn_tc_kernel(
                          idesc_s, kk != 0);
             tc_commit(&s_full[ns & 1]);
             tc_commit(&k_empty[ns % kKSt]);
+            if (ns == end - 1) tc_commit(q_empty);
             ++ns;
             moved = true;
           }
@@ -789,36 +802,11 @@ __global__ void __launch_bounds__(kTcThreads, 2) tree_attn_tc_kernel(
     const uint32_t tO = tmem + lane_off, tS = tmem + 128 + lane_off;
     int it = 0;
     do {
-      const int b = pc.b, kvh = pc.unit / p.RT, row0 = (pc.unit % p.RT) * kTcRows;
+      const int b = pc.b, kvh = pc.unit / p.RT, row0 = (pc.unit % p.RT) * p.rows;
       const Span& sp = pc.sp;
-      // Q rows into shared memory, K-major in 128-byte swizzled boxes of 64 dims
-      // (every S of the piece before has been read, so its Q is spent)
-      const T* Q = static_cast<const T*>(p.q) + b * p.q_sb;
-#pragma unroll
-      for (int e0 = 0; e0 < kTcRows * (D / 8); e0 += 128 * 8) {
-        uint4 x[8];  // eight loads in flight
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int e = e0 + u * 128 + rl, row = row0 + e / (D / 8);
-          x[u] = make_uint4(0, 0, 0, 0);
-          if (row < p.R)
-            x[u] = __ldg(reinterpret_cast<const uint4*>(Q + (row / p.G) * p.q_st +
-                                                        (kvh * p.G + row % p.G) * p.q_sh) +
-                         e % (D / 8));
-        }
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int e = e0 + u * 128 + rl, r = e / (D / 8), ch = e % (D / 8);
-          *reinterpret_cast<uint4*>(sQ + (ch >> 3) * (kTcRows * 128) + r * 128 +
-                                    (((ch & 7) ^ (r & 7)) << 4)) = x[u];
-        }
-      }
-      fence_proxy_async_smem();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
       const int row = row0 + rl;
-      const bool live = row < p.R, warp_live = row0 + warp * 32 < p.R;
+      const bool live = rl < p.rows && row < p.R;
+      const bool warp_live = row0 + warp * 32 < p.R;
       const int node = live ? row / p.G : 0, head = kvh * p.G + (live ? row % p.G : 0);
       const uint64_t* mrow = p.mask + b * p.mask_sb + (int64_t)node * p.W;
       const int64_t lo = low_of(p, sp, mrow);
@@ -979,11 +967,15 @@ __global__ void __launch_bounds__(kTcThreads, 2) tree_attn_tc_kernel(
   if (warp == 5) tmem_dealloc(tmem, 256);
 }
 
-// Joins the pieces of the units that more than one part holds: a warp a row.
-template <typename T, int D>
+// Joins the pieces of the units that more than one part holds.  WPR warps a row
+// take every WPR-th piece each; with 33 pieces a row (one long sequence) one warp
+// a row waits on them five round trips long.
+template <typename T, int D, int WPR>
 __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant__ TreeArgs p) {
-  const int lane = threadIdx.x & 31;
-  const int item = blockIdx.x * 8 + (threadIdx.x >> 5);
+  constexpr int PER = D / 32;
+  __shared__ float part[WPR > 1 ? 8 : 1][D + 2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w0 = warp % WPR;
+  const int item = blockIdx.x * (8 / WPR) + warp / WPR;
   // which pieces: from the lengths alone, which the kernel before this one
   // only reads
   const bool in = item < p.B * p.Hkv * p.R;
@@ -998,15 +990,14 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant
   const int c0 = s.of(x0), c1 = s.of(x0 + n - 1);
   pdl_wait();
   pdl_trigger();
-  if (!in || c0 == c1) return;
+  const bool work = in && c0 != c1;
   const int r = row % p.rows;
-  constexpr int PER = D / 32;
   float M = -INFINITY, L = 0.f, odd = 0.f, o[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) o[i] = 0.f;
   // 32 pieces at a time: a lane takes the weight of one, all take its values
-  for (int k0 = c0; k0 <= c1; k0 += 32) {
-    const int k = k0 + lane, cnt = min(32, c1 - k0 + 1);
+  for (int k0 = c0 + w0; work && k0 <= c1; k0 += 32 * WPR) {
+    const int k = k0 + lane * WPR, cnt = min(32, (c1 - k0) / WPR + 1);
     float m = -INFINITY, l = 0.f;
     if (k <= c1) {
       const float* sl = slot_of(p, D, k, k == c0);
@@ -1024,7 +1015,8 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant
 #pragma unroll 8
     for (int j = 0; j < cnt; ++j) {
       const float wj = __shfl_sync(0xffffffffu, w, j);
-      const float* sl = slot_of(p, D, k0 + j, k0 + j == c0) + r * D + lane * PER;
+      const int kj = k0 + j * WPR;
+      const float* sl = slot_of(p, D, kj, kj == c0) + r * D + lane * PER;
       float v[PER];
       if constexpr (PER == 4) {
         const float4 x = *reinterpret_cast<const float4*>(sl);
@@ -1037,7 +1029,31 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant
       for (int i = 0; i < PER; ++i) o[i] = fmaf(wj, v[i], o[i]);
     }
   }
-  const bool any_odd = __any_sync(0xffffffffu, odd != 0.f);
+  bool any_odd = __any_sync(0xffffffffu, odd != 0.f);
+  if (WPR > 1) {  // the row's warps, in order
+    if (lane == 0) {
+      part[warp][D] = M;
+      part[warp][D + 1] = L;
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) part[warp][lane * PER + i] = o[i];
+    any_odd = __syncthreads_or(any_odd);
+    if (w0 != 0) return;
+    float mx = M;
+    for (int w = 1; w < WPR; ++w) mx = fmaxf(mx, part[warp + w][D]);
+    const float base = mx == -INFINITY ? 0.f : mx;
+    const float f0 = ex2_ftz(M - base);
+    L *= f0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) o[i] *= f0;
+    for (int w = 1; w < WPR; ++w) {
+      const float f = ex2_ftz(part[warp + w][D] - base);
+      L += part[warp + w][D + 1] * f;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) o[i] += part[warp + w][lane * PER + i] * f;
+    }
+  }
+  if (!work) return;
   const float inv = L == 0.f ? 0.f : 1.f / L;
   const int t = row / p.G, h = kvh * p.G + row % p.G;
   T* dst = static_cast<T*>(p.o) + b * p.o_sb + t * p.o_st + h * p.o_sh + lane * PER;
@@ -1066,18 +1082,21 @@ struct TreeCall {
 };
 
 // How a call is cut: the row groups of a CTA and the parts (0: one a unit).
-struct Plan { int rw, rows, rt, ctas; };  // rw 0: tcgen05
+struct Plan { int rw, rows, rt, min_tiles, ctas; };  // rw 0: tcgen05
 Plan plan_of(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t max_ctx,
              int64_t window_left) {
   const int64_t R = T * (Hq / Hkv);
   Plan pl;
-  pl.rw = R <= 16 ? 1 : R <= 32 ? 2 : 0;
-  pl.rows = pl.rw ? 16 * pl.rw : kTcRows;
+  const int64_t G = Hq / Hkv;
+  // (more than 128 query heads a kv head: no whole node fits a tcgen05 tile)
+  pl.rw = R <= 16 ? 1 : R <= 32 || G > kTcRows ? 2 : 0;
+  pl.rows = pl.rw ? 16 * pl.rw : (int)(kTcRows / G * G);
   pl.rt = (int)((R + pl.rows - 1) / pl.rows);
+  pl.min_tiles = pl.rw ? 4 : 8;
   int64_t keys = max_ctx;
   if (window_left >= 0 && window_left + 1 < keys) keys = window_left + KT;
   const int64_t tiles = (keys + KT - 1) / KT + (T + 63) / 64;
-  pl.ctas = tiles <= kMinTiles ? 0 : (int)std::min<int64_t>(2 * sm_budget(), B * Hkv * pl.rt * tiles);
+  pl.ctas = tiles <= pl.min_tiles ? 0 : (int)std::min<int64_t>(2 * sm_budget(), B * Hkv * pl.rt * tiles);
   return pl;
 }
 
@@ -1146,38 +1165,59 @@ int tree_attention(const TreeCall& c, int dtype, cudaStream_t st) {
   const int rw = pl.rw;
   a.RT = pl.rt; a.ctas = pl.ctas; a.rows = pl.rows;
   a.o_vec = aligned16(c.o) && ((c.o_sb | c.o_st | c.o_sh) & 7) == 0;
-  a.min_tiles = kMinTiles;
+  a.min_tiles = pl.min_tiles;
   a.ws = static_cast<float*>(c.ws);
   TPP_REQUIRE(pl.ctas == 0 || (c.ws && c.ws_bytes >= workspace_of(pl, c.D) && aligned16(c.ws)),
               TPP_ERR_WORKSPACE, "workspace missing, too small or not 16-byte aligned");
   const int64_t units = c.B * c.Hkv * pl.rt;
   TPP_REQUIRE(units * (c.max_ctx / KT + a.NT + 1) < (1ll << 31) &&
-                  c.B * c.Hkv * a.R < (1ll << 31) - 8,
+                  c.B * c.Hkv * a.R < (1ll << 29) - 8,
               TPP_ERR_SHAPE, "too many rows or tiles");
   const dim3 grid((unsigned)(pl.ctas ? pl.ctas : units));
-  auto go = [&](auto kern, int threads, size_t smem) -> int {
+  CUtensorMap tq;
+  if (pl.rw == 0) {
+    // {64 columns, head, node, column box, batch}
+    auto sb = [&](int64_t n, int64_t s) { return (uint64_t)(n > 1 ? s : c.D) * 2; };
+    const uint64_t dims[5] = {64, (uint64_t)c.Hq, (uint64_t)c.T, (uint64_t)(c.D / 64), (uint64_t)c.B};
+    const uint64_t strides[4] = {sb(c.Hq, c.q_sh), sb(c.T, c.q_st), 128, sb(c.B, c.q_sb)};
+    const uint32_t box[5] = {64, (uint32_t)a.G, (uint32_t)(pl.rows / a.G), 1, 1};
+    rc = make_tmap(&tq, c.q, dtype, 5, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc != TPP_OK) return rc;
+  }
+  auto go_tc = [&](auto kern, size_t smem) -> int {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
+        cudaSuccess) {
+      set_error("tree_attn_tc_kernel: cannot reserve shared memory");
+      return TPP_ERR_LAUNCH;
+    }
+    return launch("tree_attn_tc_kernel", kern, grid, dim3(kTcThreads), smem, st, 0u, tk, tv, tkt,
+                  tvt, tq, a);
+  };
+  auto go = [&](auto kern, size_t smem) -> int {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
         cudaSuccess) {
       set_error("tree_attn_kernel: cannot reserve shared memory");
       return TPP_ERR_LAUNCH;
     }
-    return launch("tree_attn_kernel", kern, grid, dim3(threads), smem, st, 0u, tk, tv, tkt, tvt,
+    return launch("tree_attn_kernel", kern, grid, dim3(kThreads), smem, st, 0u, tk, tv, tkt, tvt,
                   a);
   };
   rc = TPP_DISPATCH_HALF(dtype, T, [&]() -> int {
     if (c.D == 64) {
-      if (rw == 1) return go(tree_attn_kernel<T, 64, 1>, kThreads, TreeSmem<64, 1>::kBytes);
-      if (rw == 2) return go(tree_attn_kernel<T, 64, 2>, kThreads, TreeSmem<64, 2>::kBytes);
-      return go(tree_attn_tc_kernel<T, 64>, kTcThreads, TcSmem<64>::kBytes);
+      if (rw == 1) return go(tree_attn_kernel<T, 64, 1>, TreeSmem<64, 1>::kBytes);
+      if (rw == 2) return go(tree_attn_kernel<T, 64, 2>, TreeSmem<64, 2>::kBytes);
+      return go_tc(tree_attn_tc_kernel<T, 64>, TcSmem<64>::kBytes);
     }
-    if (rw == 1) return go(tree_attn_kernel<T, 128, 1>, kThreads, TreeSmem<128, 1>::kBytes);
-    if (rw == 2) return go(tree_attn_kernel<T, 128, 2>, kThreads, TreeSmem<128, 2>::kBytes);
-    return go(tree_attn_tc_kernel<T, 128>, kTcThreads, TcSmem<128>::kBytes);
+    if (rw == 1) return go(tree_attn_kernel<T, 128, 1>, TreeSmem<128, 1>::kBytes);
+    if (rw == 2) return go(tree_attn_kernel<T, 128, 2>, TreeSmem<128, 2>::kBytes);
+    return go_tc(tree_attn_tc_kernel<T, 128>, TcSmem<128>::kBytes);
   });
   if (rc != TPP_OK || pl.ctas == 0) return rc;
-  const int64_t blocks = (c.B * c.Hkv * a.R + 7) / 8;
+  const int wpr = pl.ctas >= 4 * units ? 4 : 1;  // four pieces a unit and more
+  const int64_t blocks = (c.B * c.Hkv * a.R * wpr + 7) / 8;
   return TPP_DISPATCH_HALF(dtype, T, [&]() -> int {
-    auto kern = c.D == 64 ? tree_combine_kernel<T, 64> : tree_combine_kernel<T, 128>;
+    auto kern = c.D == 64 ? (wpr == 4 ? tree_combine_kernel<T, 64, 4> : tree_combine_kernel<T, 64, 1>)
+                          : (wpr == 4 ? tree_combine_kernel<T, 128, 4> : tree_combine_kernel<T, 128, 1>);
     return launch("tree_combine_kernel", kern, dim3((unsigned)blocks), dim3(256), 0, st, 0u, a);
   });
 }
