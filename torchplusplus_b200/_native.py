@@ -171,7 +171,9 @@ def dtype_code(t: torch.dtype) -> int:
 
 
 def stream_of(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    # the handle itself: torch.cuda.current_stream() builds a Stream object
+    # around it, which costs 2.2 us a call (this: 0.1)
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -27,6 +27,9 @@
 // added afterwards, element by element, to the rows that see them.
 #include <math.h>
 #include <algorithm>
+#include <mutex>
+#include <set>
+#include <utility>
 #include "mma_common.cuh"
 #include "tc_common.cuh"
 
@@ -1081,6 +1084,23 @@ struct TreeCall {
   void* ws; int64_t ws_bytes;
 };
 
+// cudaFuncSetAttribute once a kernel and device (0.5 us a call otherwise).
+int reserve_smem(const void* kern, size_t smem) {
+  static std::mutex lock;
+  static std::set<std::pair<const void*, int>> done;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> hold(lock);
+  if (done.count({kern, dev})) return TPP_OK;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
+      cudaSuccess) {
+    set_error("tree attention: cannot reserve shared memory");
+    return TPP_ERR_LAUNCH;
+  }
+  done.insert({kern, dev});
+  return TPP_OK;
+}
+
 // How a call is cut: the row groups of a CTA and the parts (0: one a unit).
 struct Plan { int rw, rows, rt, min_tiles, ctas; };  // rw 0: tcgen05
 Plan plan_of(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t max_ctx,
@@ -1185,20 +1205,12 @@ int tree_attention(const TreeCall& c, int dtype, cudaStream_t st) {
     if (rc != TPP_OK) return rc;
   }
   auto go_tc = [&](auto kern, size_t smem) -> int {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
-        cudaSuccess) {
-      set_error("tree_attn_tc_kernel: cannot reserve shared memory");
-      return TPP_ERR_LAUNCH;
-    }
+    if (const int e = reserve_smem(reinterpret_cast<const void*>(kern), smem)) return e;
     return launch("tree_attn_tc_kernel", kern, grid, dim3(kTcThreads), smem, st, 0u, tk, tv, tkt,
                   tvt, tq, a);
   };
   auto go = [&](auto kern, size_t smem) -> int {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
-        cudaSuccess) {
-      set_error("tree_attn_kernel: cannot reserve shared memory");
-      return TPP_ERR_LAUNCH;
-    }
+    if (const int e = reserve_smem(reinterpret_cast<const void*>(kern), smem)) return e;
     return launch("tree_attn_kernel", kern, grid, dim3(kThreads), smem, st, 0u, tk, tv, tkt, tvt,
                   a);
   };

@@ -682,17 +682,51 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
 
 
 # ---------------------------------------------------------------- draft trees
+# These run once a layer and step on small tensors, where the host's time is the
+# call's: each check below reads an attribute once and no torch op runs unless an
+# operand has to be copied.
+_DT = {torch.float16: 0, torch.bfloat16: 1}
+
+
+def _half_alike(what: str, x: torch.Tensor, *ts: torch.Tensor | None) -> int:
+    """The dtype code of x (16 bits), which all of ts share; all on CUDA."""
+    dt = x.dtype
+    code = _DT.get(dt)
+    if not x.is_cuda:
+        _cuda(x)
+    if code is None:
+        _half(x, what)
+    for t in ts:
+        if t is not None and (t.dtype is not dt or not t.is_cuda):
+            _cuda(t)
+            _same_dtype(x, t)
+    return code
+
+
 def _rows16(t: torch.Tensor) -> torch.Tensor:
     """t itself if its last dim is contiguous and every row starts on 16 bytes,
     a contiguous copy otherwise."""
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:-1]):
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
+    if not t.data_ptr() & 15:
+        if t.is_contiguous() and not t.shape[-1] & 7:
+            return t
+        *lead, last = t.stride()
+        if last == 1 and not any(s & 7 for s in lead):
+            return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _i32(t: torch.Tensor, shape: tuple, what: str) -> None:
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous() or not t.is_cuda:
+        _cuda(t)
         raise ValueError(f"{what} must be contiguous int32 {list(shape)}")
+
+
+def _tree_out(out: torch.Tensor | None, shape: tuple, like: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return like.new_empty(shape)
+    if out.shape != shape or not out.is_contiguous():
+        raise ValueError(f"the output must be contiguous {list(shape)}")
+    return out
 
 
 def qk_norm_rope_tree(qkv: torch.Tensor, q_norm_w: torch.Tensor | None,
@@ -703,34 +737,27 @@ def qk_norm_rope_tree(qkv: torch.Tensor, q_norm_w: torch.Tensor | None,
     """qkv [B,T,(Hq+2Hkv)*D] -> q [B,T,Hq,D], k [B,T,Hkv,D], normed per head and
     rotated at positions int32 [B,T] (a tree's siblings share one; a position
     outside the tables gives zero rows).  v is the last part of qkv as it is."""
-    _cuda(qkv, q_norm_w, k_norm_w, cos, sin, positions, q_out, k_out)
-    dt = _half(qkv, "qkv")
-    _same_dtype(qkv, q_norm_w, k_norm_w, q_out, k_out)
+    dt = _half_alike("qkv", qkv, q_norm_w, k_norm_w, q_out, k_out)
     if qkv.dim() != 3 or Hq <= 0 or Hkv <= 0 or qkv.shape[2] % (Hq + 2 * Hkv):
         raise ValueError("qkv must be [B, T, (Hq+2Hkv)*D]")
     B, T, W = qkv.shape
     D = W // (Hq + 2 * Hkv)
     _i32(positions, (B, T), "positions")
     for w in (q_norm_w, k_norm_w):
-        if w is not None and tuple(w.shape) != (D,):
-            raise ValueError(f"norm weights must be [{D}]")
+        if w is not None and (w.shape != (D,) or not w.is_contiguous()):
+            raise ValueError(f"norm weights must be contiguous [{D}]")
+    if not (cos.is_cuda and sin.is_cuda):
+        _cuda(cos, sin)
     qkv = _rows16(qkv)
     cos, sin, cs_stride, cs_dt = _table(cos, sin, D)
     q_out = _tree_out(q_out, (B, T, Hq, D), qkv)
     k_out = _tree_out(k_out, (B, T, Hkv, D), qkv)
-    N.call("tpp_qk_norm_rope_tree", qkv.data_ptr(), qkv.stride(0), qkv.stride(1),
-           N.ptr(q_norm_w), N.ptr(k_norm_w), float(eps), cos.data_ptr(), sin.data_ptr(),
-           cs_stride, cos.shape[0], cs_dt, positions.data_ptr(), q_out.data_ptr(),
-           k_out.data_ptr(), B, T, Hq, Hkv, D, dt, N.stream_of(qkv))
+    sb, st, _ = qkv.stride()
+    N.call("tpp_qk_norm_rope_tree", qkv.data_ptr(), sb, st, N.ptr(q_norm_w), N.ptr(k_norm_w),
+           eps, cos.data_ptr(), sin.data_ptr(), cs_stride, cos.shape[0], cs_dt,
+           positions.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), B, T, Hq, Hkv, D, dt,
+           N.stream_of(qkv))
     return q_out, k_out
-
-
-def _tree_out(out: torch.Tensor | None, shape: tuple, like: torch.Tensor) -> torch.Tensor:
-    if out is None:
-        return torch.empty(shape, dtype=like.dtype, device=like.device)
-    if tuple(out.shape) != shape or not out.is_contiguous():
-        raise ValueError(f"the output must be contiguous {list(shape)}")
-    return out
 
 
 def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor,
@@ -746,38 +773,41 @@ def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
     argmax (see tpp_verify_tree for the rules).  Returns path int32 [B,T]
     (accepted nodes from the root, then -1), count int32 [B] (nodes on it, at
     least the root) and next_token int64 [B] (-1 if the row has no weight)."""
-    _cuda(logits, tokens, parents, uniforms, draft_logits)
+    if not (logits.is_cuda and tokens.is_cuda and parents.is_cuda):
+        _cuda(logits, tokens, parents)
     if logits.dim() != 3:
         raise ValueError("logits must be [B, T, V]")
     dt = N.dtype_code(logits.dtype)
-    _same_dtype(logits, draft_logits)
     B, T, V = logits.shape
     if logits.stride(2) != 1:
         logits = logits.contiguous()
-    if tokens.dtype != torch.int64 or tuple(tokens.shape) != (B, T):
+    if tokens.dtype is not torch.int64 or tokens.shape != (B, T):
         raise ValueError("tokens must be int64 [B, T]")
-    if parents.dtype != torch.int32 or tuple(parents.shape) not in ((T,), (B, T)):
+    if parents.dtype is not torch.int32 or (parents.shape != (B, T) and parents.shape != (T,)):
         raise ValueError("parents must be int32 [T] or [B, T]")
     tokens, parents = tokens.contiguous(), parents.contiguous()
     if temperature > 0:
-        if uniforms is None or uniforms.dtype != torch.float32 or tuple(uniforms.shape) != (B, T):
+        if uniforms is None or uniforms.dtype is not torch.float32 or uniforms.shape != (B, T):
             raise ValueError("uniforms must be float32 [B, T]")
+        _cuda(uniforms)
         uniforms = uniforms.contiguous()
     d_sb = d_st = 0
     if draft_logits is not None:
+        _cuda(draft_logits)
+        _same_dtype(logits, draft_logits)
         if draft_logits.dim() != 3 or draft_logits.shape[0] != B or draft_logits.shape[2] != V \
                 or not T - 1 <= draft_logits.shape[1] <= T:
             raise ValueError("draft_logits must be [B, T or T - 1, V]")
         if draft_logits.stride(2) != 1:
             draft_logits = draft_logits.contiguous()
-        d_sb, d_st = draft_logits.stride(0), draft_logits.stride(1)
-    path = torch.empty((B, T), dtype=torch.int32, device=logits.device)
-    count = torch.empty(B, dtype=torch.int32, device=logits.device)
-    nxt = torch.empty(B, dtype=torch.int64, device=logits.device)
-    N.call("tpp_verify_tree", logits.data_ptr(), logits.stride(0), logits.stride(1),
-           N.ptr(draft_logits), d_sb, d_st, tokens.data_ptr(), T, parents.data_ptr(),
-           0 if parents.dim() == 1 else T, N.ptr(uniforms), T, float(temperature),
-           path.data_ptr(), count.data_ptr(), nxt.data_ptr(), B, T, V, dt, N.stream_of(logits))
+        d_sb, d_st, _ = draft_logits.stride()
+    path, count = parents.new_empty((B, T)), parents.new_empty(B)
+    nxt = tokens.new_empty(B)
+    l_sb, l_st, _ = logits.stride()
+    N.call("tpp_verify_tree", logits.data_ptr(), l_sb, l_st, N.ptr(draft_logits), d_sb, d_st,
+           tokens.data_ptr(), T, parents.data_ptr(), 0 if parents.dim() == 1 else T,
+           N.ptr(uniforms), T, temperature, path.data_ptr(), count.data_ptr(), nxt.data_ptr(), B,
+           T, V, dt, N.stream_of(logits))
     return path, count, nxt
 
 
@@ -789,68 +819,77 @@ def kv_commit(k_tree: torch.Tensor, v_tree: torch.Tensor, path: torch.Tensor,
     count[b], of k_cache/v_cache [L,B,Hkv,Smax,D], or with block_table int32
     [B,max_blocks] of pools [L,num_blocks,Hkv,64,D].  Rows past the cache are
     skipped.  path int32 [B,T], count and ctx_lens int32 [B]."""
-    _cuda(k_tree, v_tree, path, count, ctx_lens, k_cache, v_cache, block_table)
-    dt = _half(k_tree, "k_tree")
-    _same_dtype(k_tree, v_tree, k_cache, v_cache)
+    dt = _half_alike("k_tree", k_tree, v_tree, k_cache, v_cache)
     if k_tree.dim() != 5 or v_tree.shape != k_tree.shape:
         raise ValueError("k_tree and v_tree must be [L, B, T, Hkv, D]")
     L, B, T, Hkv, D = k_tree.shape
-    if k_cache.dim() != 5 or k_cache.shape != v_cache.shape \
-            or k_cache.stride() != v_cache.stride() or k_cache.stride(4) != 1 \
-            or k_cache.shape[0] != L or k_cache.shape[2] != Hkv or k_cache.shape[4] != D:
-        raise ValueError("caches must be [L, B, Hkv, Smax, D] (pools [L, num_blocks, Hkv, 64, "
-                         "D]) with identical layouts")
+    if k_cache.dim() != 5 or k_cache.shape != v_cache.shape:
+        raise ValueError("caches must be [L, B, Hkv, Smax, D] (pools [L, num_blocks, Hkv, 64, D])")
+    cL, cB, cH, rows, cD = k_cache.shape
+    cs = k_cache.stride()
+    if cL != L or cH != Hkv or cD != D or cs[4] != 1 or v_cache.stride() != cs:
+        raise ValueError("the caches must match the trees' layers, heads and head dim and share "
+                         "one layout")
     _i32(path, (B, T), "path")
     _i32(count, (B,), "count")
     _i32(ctx_lens, (B,), "ctx_lens")
-    rows, nb, tstride = k_cache.shape[3], 0, 0
+    nb = tstride = 0
     if block_table is not None:
-        if block_table.dtype != torch.int32 or block_table.dim() != 2 \
+        _cuda(block_table)
+        if block_table.dtype is not torch.int32 or block_table.dim() != 2 \
                 or block_table.shape[0] != B or block_table.stride(1) != 1:
             raise ValueError("block_table must be int32 [B, max_blocks] with unit column stride")
         if rows != 64 or (L > 0 and not k_cache[0].is_contiguous()):
             raise ValueError("pools must be [L, num_blocks, Hkv, 64, D], each layer contiguous")
-        nb, rows, tstride = k_cache.shape[1], 64 * block_table.shape[1], block_table.stride(0)
-    elif k_cache.shape[1] != B:
+        nb, rows, tstride = cB, 64 * block_table.shape[1], block_table.stride(0)
+    elif cB != B:
         raise ValueError("the caches' batch must match the tree's")
     k_tree, v_tree = _rows16(k_tree), _rows16(v_tree)
-    N.call("tpp_kv_commit", k_tree.data_ptr(), *k_tree.stride()[:4], v_tree.data_ptr(),
-           *v_tree.stride()[:4], path.data_ptr(), T, count.data_ptr(), ctx_lens.data_ptr(),
-           k_cache.data_ptr(), v_cache.data_ptr(), *k_cache.stride()[:4], rows, nb,
+    ks, vs = k_tree.stride(), v_tree.stride()
+    N.call("tpp_kv_commit", k_tree.data_ptr(), ks[0], ks[1], ks[2], ks[3], v_tree.data_ptr(),
+           vs[0], vs[1], vs[2], vs[3], path.data_ptr(), T, count.data_ptr(), ctx_lens.data_ptr(),
+           k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2], cs[3], rows, nb,
            N.ptr(block_table), tstride, L, B, T, Hkv, D, dt, N.stream_of(k_tree))
 
 
-def _tree_args(q, k_tree, v_tree, ctx_lens, mask, max_ctx, out, Hkv, D):
-    """Checks what both forms of tree attention share."""
+def _tree_call(q, k_tree, v_tree, ctx_lens, mask, max_ctx, window_left, out, workspace, Hkv, D):
+    """Checks what both forms of tree attention share; the operands as the kernels
+    take them, with the workspace."""
     B, T, Hq, Dq = q.shape
-    if Dq != D or Hq % Hkv or tuple(k_tree.shape) != (B, T, Hkv, D) \
-            or v_tree.shape != k_tree.shape:
+    if Dq != D or Hq % Hkv or k_tree.shape != (B, T, Hkv, D) or v_tree.shape != k_tree.shape:
         raise ValueError("q must be [B, T, Hq, D] and k_tree/v_tree [B, T, Hkv, D], Hq a "
                          "multiple of the cache's Hkv")
     _i32(ctx_lens, (B,), "ctx_lens")
     W = (T + 63) // 64
-    if mask.dtype != torch.int64 or tuple(mask.shape) not in ((T, W), (B, T, W)):
+    if mask.dtype is not torch.int64 or (mask.shape != (B, T, W) and mask.shape != (T, W)) \
+            or not mask.is_cuda:
+        _cuda(mask)
         raise ValueError(f"mask must be int64 [{T}, {W}] or [{B}, {T}, {W}]")
     if max_ctx < 0:
         raise ValueError("max_ctx must not be negative")
+    q = _rows16(q)
     if out is None:
-        out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
-    elif tuple(out.shape) != (B, T, Hq, D) or out.dtype != q.dtype or out.stride(3) != 1:
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((B, T, Hq, D))
+    elif out.shape != (B, T, Hq, D) or out.dtype is not q.dtype or out.stride(3) != 1 \
+            or not out.is_cuda:
         raise ValueError("out must be [B, T, Hq, D] of q's dtype")
-    return _rows16(q), _rows16(k_tree), _rows16(v_tree), mask.contiguous(), out
+    ws, nbytes = None, 0
+    if workspace is None:
+        nbytes = attention_tree_workspace_bytes(B, T, Hq, Hkv, max_ctx, D, window_left)
+        if nbytes > 0:
+            workspace = q.new_empty(nbytes // 2)  # 2-byte elements
+            ws = workspace.data_ptr()
+    else:
+        _cuda(workspace)
+        ws, nbytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    mask = mask.contiguous()
+    return (q, _rows16(k_tree), _rows16(v_tree), mask, 0 if mask.dim() == 2 else T * W, out,
+            workspace, ws, nbytes)
 
 
 def attention_tree_workspace_bytes(B: int, T: int, Hq: int, Hkv: int, max_ctx: int, D: int,
                                    window_left: int = -1) -> int:
-    return int(N.lib().tpp_attention_tree_workspace(B, T, Hq, Hkv, max_ctx, D, window_left))
-
-
-def _tree_workspace(workspace, q, Hkv, max_ctx, window_left):
-    B, T, Hq, D = q.shape
-    need = attention_tree_workspace_bytes(B, T, Hq, Hkv, max_ctx, D, window_left)
-    if workspace is None and need > 0:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    return N.ptr(workspace), 0 if workspace is None else workspace.numel()
+    return N.lib().tpp_attention_tree_workspace(B, T, Hq, Hkv, max_ctx, D, window_left)
 
 
 def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -864,27 +903,23 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     its mask row has: bit j % 64 of mask[.., i, j // 64] (int64 [T,W] or
     [B,T,W], W = ceil(T/64)) lets node i see node j.  A row that sees nothing
     gives zeros.  window_left: see tpp_attention_tree."""
-    _cuda(q, k_cache, v_cache, k_tree, v_tree, ctx_lens, mask, out, workspace)
-    dt = _half(q, "q")
-    _same_dtype(q, k_cache, v_cache, k_tree, v_tree)
-    if q.dim() != 4 or k_cache.dim() != 4 or k_cache.shape[0] != q.shape[0] \
-            or v_cache.shape != k_cache.shape or k_cache.stride() != v_cache.stride() \
-            or k_cache.stride(3) != 1:
+    dt = _half_alike("q", q, k_cache, v_cache, k_tree, v_tree)
+    cs = k_cache.stride()
+    if q.dim() != 4 or len(cs) != 4 or k_cache.shape[0] != q.shape[0] \
+            or v_cache.shape != k_cache.shape or cs != v_cache.stride() or cs[3] != 1:
         raise ValueError("q must be [B, T, Hq, D], caches [B, Hkv, Smax, D] with identical layouts")
     B, T, Hq, _ = q.shape
-    Hkv, Smax, D = k_cache.shape[1:]
+    _, Hkv, Smax, D = k_cache.shape
     if max_ctx > Smax:
         raise ValueError("max_ctx exceeds the cache capacity")
-    q, k_tree, v_tree, mask, out = _tree_args(q, k_tree, v_tree, ctx_lens, mask, max_ctx, out,
-                                              Hkv, D)
-    ws, ws_bytes = _tree_workspace(workspace, q, Hkv, max_ctx, window_left)
-    N.call("tpp_attention_tree", q.data_ptr(), *q.stride()[:3], k_cache.data_ptr(),
-           v_cache.data_ptr(), *k_cache.stride()[:3], k_tree.data_ptr(), *k_tree.stride()[:3],
-           v_tree.data_ptr(), *v_tree.stride()[:3], ctx_lens.data_ptr(), int(max_ctx),
-           mask.data_ptr(), 0 if mask.dim() == 2 else mask.stride(0), out.data_ptr(),
-           *out.stride()[:3], B, T, Hq, Hkv, D, int(window_left),
-           1.0 / math.sqrt(D) if scale is None else float(scale), ws, ws_bytes, dt,
-           N.stream_of(q))
+    q, k_tree, v_tree, mask, mask_sb, out, keep, ws, ws_bytes = _tree_call(
+        q, k_tree, v_tree, ctx_lens, mask, max_ctx, window_left, out, workspace, Hkv, D)
+    qs, ks, vs, os_ = q.stride(), k_tree.stride(), v_tree.stride(), out.stride()
+    N.call("tpp_attention_tree", q.data_ptr(), qs[0], qs[1], qs[2], k_cache.data_ptr(),
+           v_cache.data_ptr(), cs[0], cs[1], cs[2], k_tree.data_ptr(), ks[0], ks[1], ks[2],
+           v_tree.data_ptr(), vs[0], vs[1], vs[2], ctx_lens.data_ptr(), max_ctx,
+           mask.data_ptr(), mask_sb, out.data_ptr(), os_[0], os_[1], os_[2], B, T, Hq, Hkv, D,
+           window_left, D ** -0.5 if scale is None else scale, ws, ws_bytes, dt, N.stream_of(q))
     return out
 
 
@@ -896,25 +931,23 @@ def attention_tree_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
                          workspace: torch.Tensor | None = None) -> torch.Tensor:
     """attention_tree over a paged cache: pools [num_blocks,Hkv,64,D], key k of
     sequence b in block block_table[b, k // 64], row k % 64."""
-    _cuda(q, k_pool, v_pool, block_table, k_tree, v_tree, ctx_lens, mask, out, workspace)
-    dt = _half(q, "q")
-    _same_dtype(q, k_pool, v_pool, k_tree, v_tree)
+    dt = _half_alike("q", q, k_pool, v_pool, k_tree, v_tree)
     if q.dim() != 4 or k_pool.dim() != 4:
         raise ValueError("q must be [B, T, Hq, D] and the pools [num_blocks, Hkv, 64, D]")
+    _cuda(block_table)
     B, T, Hq, _ = q.shape
     NB, Hkv, D = _paged_args(k_pool, v_pool, block_table, B)
     if max_ctx > 64 * block_table.shape[1]:
         raise ValueError("max_ctx exceeds the block table's capacity")
-    q, k_tree, v_tree, mask, out = _tree_args(q, k_tree, v_tree, ctx_lens, mask, max_ctx, out,
-                                              Hkv, D)
-    ws, ws_bytes = _tree_workspace(workspace, q, Hkv, max_ctx, window_left)
-    N.call("tpp_attention_tree_paged", q.data_ptr(), *q.stride()[:3], k_pool.data_ptr(),
+    q, k_tree, v_tree, mask, mask_sb, out, keep, ws, ws_bytes = _tree_call(
+        q, k_tree, v_tree, ctx_lens, mask, max_ctx, window_left, out, workspace, Hkv, D)
+    qs, ks, vs, os_ = q.stride(), k_tree.stride(), v_tree.stride(), out.stride()
+    N.call("tpp_attention_tree_paged", q.data_ptr(), qs[0], qs[1], qs[2], k_pool.data_ptr(),
            v_pool.data_ptr(), NB, block_table.data_ptr(), block_table.stride(0),
-           k_tree.data_ptr(), *k_tree.stride()[:3], v_tree.data_ptr(), *v_tree.stride()[:3],
-           ctx_lens.data_ptr(), int(max_ctx), mask.data_ptr(),
-           0 if mask.dim() == 2 else mask.stride(0), out.data_ptr(), *out.stride()[:3], B, T, Hq,
-           Hkv, D, int(window_left), 1.0 / math.sqrt(D) if scale is None else float(scale), ws,
-           ws_bytes, dt, N.stream_of(q))
+           k_tree.data_ptr(), ks[0], ks[1], ks[2], v_tree.data_ptr(), vs[0], vs[1], vs[2],
+           ctx_lens.data_ptr(), max_ctx, mask.data_ptr(), mask_sb, out.data_ptr(), os_[0],
+           os_[1], os_[2], B, T, Hq, Hkv, D, window_left, D ** -0.5 if scale is None else scale,
+           ws, ws_bytes, dt, N.stream_of(q))
     return out
 
 
