@@ -475,7 +475,11 @@ int tpp_verify_tree(const void* logits, int64_t l_sb, int64_t l_st, const void* 
                     int64_t d_sb, int64_t d_st, const int64_t* tokens, int64_t tok_sb,
                     const int32_t* parents, int64_t par_sb, const float* u, int64_t u_sb,
                     double temperature, int32_t* path, int32_t* count, int64_t* next_token,
-                    int64_t B, int64_t T, int64_t V, int dtype, void* stream);
+                    int64_t B, int64_t T, int64_t V, void* workspace, int64_t workspace_bytes,
+                    int dtype, void* stream);
+/* Bytes of workspace that needs (0: none), with_draft 1 if draft logits are given. */
+int64_t tpp_verify_tree_workspace(int64_t B, int64_t T, int64_t V, int with_draft,
+                                  double temperature, int dtype);
 
 /* Copies the accepted path's K/V rows of all L layers into the caches:
  *   cache[l, b, h, ctx_lens[b] + i, :] = tree[l, b, path[b, i], h, :],

@@ -112,7 +112,8 @@ SIGNATURES: dict[str, tuple] = {
                                         _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                         _f32, _p, _i64, _i32, _p]),
     "tpp_verify_tree": (_i32, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _p, _i64, _p, _i64,
-                               C.c_double, _p, _p, _p, _i64, _i64, _i64, _i32, _p]),
+                               C.c_double, _p, _p, _p, _i64, _i64, _i64, _p, _i64, _i32, _p]),
+    "tpp_verify_tree_workspace": (_i64, [_i64, _i64, _i64, _i32, C.c_double, _i32]),
     "tpp_kv_commit": (_i32, [_p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64, _p, _i64, _p,
                              _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64,
                              _i64, _i64, _i64, _i32, _p]),

@@ -801,13 +801,15 @@ def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
         if draft_logits.stride(2) != 1:
             draft_logits = draft_logits.contiguous()
         d_sb, d_st, _ = draft_logits.stride()
+    nbytes = N.lib().tpp_verify_tree_workspace(B, T, V, draft_logits is not None, temperature, dt)
+    workspace = tokens.new_empty(nbytes // 8) if nbytes > 0 else None
     path, count = parents.new_empty((B, T)), parents.new_empty(B)
     nxt = tokens.new_empty(B)
     l_sb, l_st, _ = logits.stride()
     N.call("tpp_verify_tree", logits.data_ptr(), l_sb, l_st, N.ptr(draft_logits), d_sb, d_st,
            tokens.data_ptr(), T, parents.data_ptr(), 0 if parents.dim() == 1 else T,
            N.ptr(uniforms), T, temperature, path.data_ptr(), count.data_ptr(), nxt.data_ptr(), B,
-           T, V, dt, N.stream_of(logits))
+           T, V, N.ptr(workspace), max(nbytes, 0), dt, N.stream_of(logits))
     return path, count, nxt
 
 
