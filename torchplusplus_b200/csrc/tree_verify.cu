@@ -1,23 +1,24 @@
 // Verification of a drafted tree against the target's logits (tpp_verify_tree).
 //
-// One cluster of 8 CTAs walks one sequence's tree from the root.  At a node it
-// needs the softmax of one row of logits (and of the draft's row, where the
-// children were drawn from one).  Every CTA of the cluster holds an eighth of the
-// row; every thread makes the same decisions from the exchanged sums.
+// One cluster walks one sequence's tree from the root.  At a node it needs the
+// softmax of one row of logits (and of the draft's row, where the children were
+// drawn from one).  Every CTA of the cluster holds its part of the row; every
+// thread makes the same decisions from the exchanged sums.
 //
 // Weights are exp((l - max) / temperature) in fp32; sums and cumulative sums of
 // weights run over 64-bit integers, round(w * 2^40), so they are exact and a
 // result does not depend on the order or the split of a row (fp32 cumulative
 // sums over 150k tokens move the boundaries of a draw by about 1e-6).
 //
-// What a walk costs is its chain of passes and exchanges, two a node (the maximum,
-// the sum).  An exchange is one remote store a warp and CTA (st.async, counted by
-// the receiver's mbarrier) and no barrier of the CTA or the cluster.  For small
-// batches verify_stats_kernel first takes every row's maximum and an fp32 sum on
-// all SMs; the walk decides from those, and goes through the exact sums only where
-// a test comes within the fp32 sum's error of a tie, and for the draw.  For larger
-// ones reading the rows off the path costs more than the exchanges: rows are then
-// read as the walk reaches them.
+// What a walk costs is its chain of passes and exchanges, and the exact weights
+// are 23 instructions an element.  So a node's tests go by its maximum and an fp32
+// sum, taken in one pass of 7 instructions an element and one exchange; the exact
+// sums follow only where a test comes within the fp32 sum's error of a tie, and
+// at the last node, for the draw.  For small batches verify_stats_kernel takes
+// these of all rows ahead of the walk, on all SMs; for larger ones reading the rows
+// off the path would cost more than it saves.  An exchange is one remote store a
+// warp and CTA (st.async, counted by the receiver's mbarrier) and no barrier of the
+// CTA or the cluster.
 #include <limits.h>
 #include <math.h>
 #include <cstdlib>
@@ -29,16 +30,12 @@ namespace cg = cooperative_groups;
 namespace tpp {
 namespace {
 
-constexpr int kCluster = 8;
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
 constexpr int kMaxNodes = 256;
-constexpr int kUnroll = 5;           // groups a lane has in flight: all of its
-                                     // share of 160k tokens of 16 bits
 constexpr int kSlice = 1024;         // groups of a row for a CTA of the statistics
 constexpr double kFix = 1099511627776.0;  // 2^40
-// Relative error of the statistics' sums: fp32 sums of at most 32 + 13 + 512 / 32
-// terms in a row and an exponential within 2^-21 of exact (its argument rounded at
+// Relative error of the fp32 sums: the worst chain of additions is a lane's 1024
+// terms at 2^22 tokens (and a few dozen at 150k), which in practice err like its
+// root; the exponential is within 2^-21 of exact (its argument is rounded at
 // |x| < 32; weights below e^-32 do not count).
 constexpr float kSumError = 1e-5f;
 using ull = unsigned long long;
@@ -79,19 +76,16 @@ __device__ __forceinline__ void unpack_group<float>(const uint4& w, float* f) {
   f[2] = __uint_as_float(w.z); f[3] = __uint_as_float(w.w);
 }
 
-// Elements [e0, e0 + VE) of a row of V as they are stored, -inf outside it.  The
-// slow way is for a row's ends, and for a draft row whose start is aligned
-// otherwise than the target's.
+// Elements [e0, e0 + VE) of a row of V as they are stored, -inf outside it, one by
+// one: a row's ends, and a draft row whose start is aligned otherwise than the
+// target's.
 template <typename T>
-__device__ __forceinline__ uint4 load_group(const T* row, int e0, int V) {
+__device__ __noinline__ uint4 load_edge(const T* row, int e0, int V) {
   constexpr int VE = 16 / sizeof(T);
-  const T* a = row + e0;
-  if (e0 >= 0 && e0 + VE <= V && (reinterpret_cast<uintptr_t>(a) & 15) == 0)
-    return __ldg(reinterpret_cast<const uint4*>(a));
   ull w[2] = {0, 0};
 #pragma unroll 1
   for (int j = 0; j < VE; ++j) {
-    const T x = e0 + j >= 0 && e0 + j < V ? a[j] : from_f32<T>(-INFINITY);
+    const T x = e0 + j >= 0 && e0 + j < V ? row[e0 + j] : from_f32<T>(-INFINITY);
     ull bits;
     if constexpr (sizeof(T) == 4) bits = __float_as_uint(x);
     else bits = *reinterpret_cast<const unsigned short*>(&x);
@@ -101,6 +95,13 @@ __device__ __forceinline__ uint4 load_group(const T* row, int e0, int V) {
   }
   return make_uint4((uint32_t)w[0], (uint32_t)(w[0] >> 32), (uint32_t)w[1],
                     (uint32_t)(w[1] >> 32));
+}
+template <typename T>
+__device__ __forceinline__ uint4 load_group(const T* row, int e0, int V) {
+  const T* a = row + e0;
+  if (e0 >= 0 && e0 + (int)(16 / sizeof(T)) <= V && (reinterpret_cast<uintptr_t>(a) & 15) == 0)
+    return __ldg(reinterpret_cast<const uint4*>(a));
+  return load_edge<T>(row, e0, V);
 }
 
 // exp((l - m) / temperature), 0 where that is NaN (NaN logits; no finite max).
@@ -132,6 +133,24 @@ __device__ __forceinline__ ull warp_sum_u64(ull v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+
+// A thread's sum of integer weights: at most 2^22 / 4096 of them, so that either
+// half fits 32 bits.
+struct Sum {
+  uint32_t hi = 0;
+  int lo = 0;
+  template <int N> __device__ __forceinline__ void add(const float* w) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      uint32_t h;
+      int l;
+      fixed_parts(w[j], h, l);
+      hi += h;
+      lo += l;
+    }
+  }
+  __device__ __forceinline__ ull warp() const { return warp_sum_u64(fixed_sum(hi, lo)); }
+};
 
 // ---- every row's maximum and sum ---------------------------------------------
 // Row r < B*T: the target's at (r / T, r % T); after those, the draft's.
@@ -189,8 +208,9 @@ __global__ void __launch_bounds__(256) verify_stats_kernel(VerifyArgs p) {
 // ---- the walk ----------------------------------------------------------------
 struct __align__(16) Part { ull a, b; };  // a warp's part of an exchange
 
+template <int PARTS>
 struct Shared {
-  Part in[2][kCluster * kWarps];  // every warp's part, by the exchange's parity
+  Part in[2][PARTS];       // every warp's part, by the exchange's parity
   ull bar[2];
   float stage[kMaxNodes];  // sums of the residual after each rejection
   int out[kMaxNodes];      // rejected tokens
@@ -199,30 +219,88 @@ struct Shared {
   float u[kMaxNodes];
   float lt[kMaxNodes], qt[kMaxNodes];  // a node's own logit in its parent's rows
   float m[kMaxNodes], z[kMaxNodes], mq[kMaxNodes], zq[kMaxNodes];  // from the statistics
+  float pt[kMaxNodes], uq[kMaxNodes];  // and from those, a node's own test
 };
 
 // How the cluster's warps share a row: `gc` groups a CTA, of which this warp owns
 // [g0, g1) (counted from the row's first, whatever its alignment).
 struct Share { int first, g0, g1; };
 
-// f(group, values) over the warp's groups of a row, kUnroll loads at a time; the
-// second pass over a row finds it in L1.
-template <typename T, typename F>
+// f(group, values) over the warp's groups of a row.  The first pass over a row has
+// U loads in flight (5: with 8 CTAs of 512, all of a lane's part of 160k 16-bit
+// logits); the later ones find it in L1 or L2 and keep two, since their code, run
+// once or twice a walk, costs more to fetch than to run when it is unrolled (half
+// of the stalls of a single sequence's walk were instruction fetches).  The row's
+// first and last groups go apart, so that the loop holds plain loads and arithmetic.
+template <typename T, int U, typename F>
 __device__ __forceinline__ void each(const Share& sh, const T* src, int mis, int V, F f) {
   constexpr int VE = 16 / sizeof(T);
-  for (int k0 = sh.g0 + (threadIdx.x & 31); k0 < sh.g1; k0 += 32 * kUnroll) {
-    uint4 raw[kUnroll];
+  const int lane = threadIdx.x & 31;
+  const bool plain = (reinterpret_cast<uintptr_t>(src - mis) & 15) == 0;
+  // whole groups: those from 1 on that end within the row
+  const int lo = plain ? min(max(sh.g0, 1), sh.g1) : sh.g0;
+  const int hi = plain ? max(min(sh.g1, (V + mis) / VE), lo) : sh.g0;
+  const uint4* at = reinterpret_cast<const uint4*>(src - mis);
+  if constexpr (U > 1) {
+    for (int k0 = lo + lane; k0 < hi; k0 += 32 * U) {
+      uint4 raw[U];
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i)
-      if (k0 + 32 * i < sh.g1) raw[i] = load_group<T>(src, (k0 + 32 * i) * VE - mis, V);
+      for (int i = 0; i < U; ++i)
+        if (k0 + 32 * i < hi) raw[i] = __ldg(at + k0 + 32 * i);
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i)
-      if (k0 + 32 * i < sh.g1) {
-        float v[VE];
-        unpack_group<T>(raw[i], v);
-        f(k0 + 32 * i, v);
-      }
+      for (int i = 0; i < U; ++i)
+        if (k0 + 32 * i < hi) {
+          float v[VE];
+          unpack_group<T>(raw[i], v);
+          f(k0 + 32 * i, v);
+        }
+    }
   }
+  // with U = 1 all groups take this loop, the plain ones with a load ahead
+  const int n = U > 1 ? lo - sh.g0 + sh.g1 - hi : sh.g1 - sh.g0;
+  auto group = [&](int j) { return U > 1 && j >= lo - sh.g0 ? hi + j - (lo - sh.g0) : sh.g0 + j; };
+  auto load = [&](int k) {
+    return k >= lo && k < hi ? __ldg(at + k) : load_edge<T>(src, k * VE - mis, V);
+  };
+  uint4 raw = make_uint4(0, 0, 0, 0);
+  if (lane < n) raw = load(group(lane));
+#pragma unroll 1
+  for (int j = lane; j < n; j += 32) {
+    uint4 next = raw;
+    if (j + 32 < n) next = load(group(j + 32));
+    float v[VE];
+    unpack_group<T>(raw, v);
+    f(group(j), v);
+    raw = next;
+  }
+}
+__device__ __forceinline__ ull pack_f2(float x, float y) {
+  return (ull)__float_as_uint(y) << 32 | __float_as_uint(x);
+}
+// The maximum of the warp's part of a row and the fp32 sum of its weights over
+// that maximum.  (A NaN argument, of a NaN logit or of inf - inf, is clamped to a
+// weight of 0.)
+template <typename T>
+__device__ __noinline__ ull approx_of(Share sh, const T* src, int mis, int V, float inv_t) {
+  constexpr int VE = 16 / sizeof(T);
+  const float c = inv_t * 1.4426950408889634f;
+  float m = -INFINITY, s = 0.f;
+  each<T, 5>(sh, src, mis, V, [&](int, const float* v) {
+    float top = m;
+#pragma unroll
+    for (int j = 0; j < VE; ++j) top = fmaxf(top, v[j]);
+    if (top > m) {
+      s *= ex2_ftz((m - top) * c);
+      m = top;
+    }
+    // (subtracted first: a product with logits near the type's lowest value
+    // would overflow)
+#pragma unroll
+    for (int j = 0; j < VE; ++j) s += ex2_ftz(fmaxf((v[j] - m) * c, -200.f));
+  });
+  const float top = warp_max(m);
+  s = warp_sum(s * ex2_ftz(fmaxf((m - top) * c, -200.f)));
+  return pack_f2(top, s);
 }
 // The maximum of the warp's part of a row and the lowest index that has it.
 template <typename T>
@@ -230,10 +308,17 @@ __device__ __noinline__ ull max_of(Share sh, const T* src, int mis, int V) {
   constexpr int VE = 16 / sizeof(T);
   float m = -INFINITY;
   int ix = INT_MAX;
-  each<T>(sh, src, mis, V, [&](int k, const float* v) {
+  each<T, 5>(sh, src, mis, V, [&](int k, const float* v) {
+    float top = v[0];
 #pragma unroll
-    for (int j = 0; j < VE; ++j)
-      if (v[j] > m) { m = v[j]; ix = k * VE - mis + j; }
+    for (int j = 1; j < VE; ++j) top = fmaxf(top, v[j]);
+    const int e0 = k * VE - mis;
+    if (top > m || (top == m && e0 < ix)) {  // (the row's first group comes late)
+      m = top;
+#pragma unroll
+      for (int j = VE - 1; j >= 0; --j)
+        if (v[j] == top) ix = e0 + j;
+    }
   });
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -248,68 +333,96 @@ template <typename T>
 __device__ __noinline__ ull sum_weights(Share sh, const T* src, int mis, int V, float top,
                                         float inv_t) {
   constexpr int VE = 16 / sizeof(T);
-  ull hi = 0;
-  long long lo = 0;
-  each<T>(sh, src, mis, V, [&](int, const float* v) {
-    uint32_t h = 0;
-    int l = 0;
+  Sum s;
+  each<T, 1>(sh, src, mis, V, [&](int, const float* v) {
+    float x[VE];
 #pragma unroll
-    for (int j = 0; j < VE; ++j) {
-      uint32_t hj;
-      int lj;
-      fixed_parts(weight(v[j], top, inv_t), hj, lj);
-      h += hj;
-      l += lj;
-    }
-    hi += h;
-    lo += l;
+    for (int j = 0; j < VE; ++j) x[j] = weight(v[j], top, inv_t);
+    s.add<VE>(x);
   });
-  return warp_sum_u64(fixed_sum(hi, lo));
+  return s.warp();
 }
 // With a draft, what is left of p is kept in `cache`, this CTA's part of the row:
 // shares() puts the warp's part of p = w / z there, reject() takes p = max(p / s - q,
 // 0) (s 0: p as it is), and both return the sum of the integer weights; scale()
 // that of p / s without changing it.
+//
+// Many quotients by one divisor: with r = 1 / b rounded to nearest, q = a r and one
+// correction by the exact remainder a - q b give a / b rounded to nearest
+// (Markstein, Computation of elementary functions on the IBM RISC System/6000,
+// 1990), three instructions.  Numerators below 2^-80, 40 powers of two under what
+// an integer weight can show, are set to 0: their remainders could be denormal.
+struct Divisor {
+  float b, r;
+  __device__ __forceinline__ explicit Divisor(float by) {
+    b = by;
+    r = by > 0.f ? __fdiv_rn(1.f, by) : 0.f;
+  }
+  __device__ __forceinline__ float of(float a) const {
+    const float q = __fmul_rn(a, r);
+    const float x = __fmaf_rn(__fmaf_rn(-q, b, a), r, q);
+    return a >= 8.271806e-25f ? x : 0.f;
+  }
+};
 template <typename T>
 __device__ __noinline__ ull shares(Share sh, const T* src, int mis, int V, float top, float z,
                                    float inv_t, float* cache) {
   constexpr int VE = 16 / sizeof(T);
-  ull s = 0;
-  each<T>(sh, src, mis, V, [&](int k, const float* v) {
+  Sum s;
+  const Divisor by(z);
+  each<T, 1>(sh, src, mis, V, [&](int k, const float* v) {
     float* c = cache + (k - sh.first) * VE;
+    float x[VE];
 #pragma unroll
-    for (int j = 0; j < VE; ++j) {
-      c[j] = share(weight(v[j], top, inv_t), z);
-      s += fixed(c[j]);
-    }
+    for (int j = 0; j < VE; ++j) x[j] = by.of(weight(v[j], top, inv_t));
+    s.add<VE>(x);
+#pragma unroll
+    for (int j = 0; j < VE; j += 4)
+      *reinterpret_cast<float4*>(c + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
   });
-  return warp_sum_u64(s);
+  return s.warp();
 }
-__device__ __forceinline__ float scaled(float p, float s) { return s > 0.f ? __fdiv_rn(p, s) : p; }
 template <typename T>
 __device__ __noinline__ ull reject(Share sh, const T* src, int mis, int V, float top, float zq,
                                    float inv_t, float s, float* cache) {
   constexpr int VE = 16 / sizeof(T);
-  ull sum = 0;
-  each<T>(sh, src, mis, V, [&](int k, const float* v) {
+  Sum sum;
+  const Divisor by(zq), over(s > 0.f ? s : 1.f);
+  each<T, 1>(sh, src, mis, V, [&](int k, const float* v) {
     float* c = cache + (k - sh.first) * VE;
+    float x[VE];
 #pragma unroll
-    for (int j = 0; j < VE; ++j) {
-      c[j] = fmaxf(scaled(c[j], s) - share(weight(v[j], top, inv_t), zq), 0.f);
-      sum += fixed(c[j]);
+    for (int j = 0; j < VE; j += 4) {
+      const float4 y = *reinterpret_cast<const float4*>(c + j);
+      x[j] = y.x; x[j + 1] = y.y; x[j + 2] = y.z; x[j + 3] = y.w;
     }
+#pragma unroll
+    for (int j = 0; j < VE; ++j)
+      x[j] = fmaxf(over.of(x[j]) - by.of(weight(v[j], top, inv_t)), 0.f);
+    sum.add<VE>(x);
+#pragma unroll
+    for (int j = 0; j < VE; j += 4)
+      *reinterpret_cast<float4*>(c + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
   });
-  return warp_sum_u64(sum);
+  return sum.warp();
 }
 template <int VE>
 __device__ __noinline__ ull scale(Share sh, float s, const float* cache) {
-  ull sum = 0;
+  Sum sum;
+  const Divisor over(s > 0.f ? s : 1.f);
+#pragma unroll 1
   for (int k = sh.g0 + (threadIdx.x & 31); k < sh.g1; k += 32) {
     const float* c = cache + (k - sh.first) * VE;
+    float x[VE];
 #pragma unroll
-    for (int j = 0; j < VE; ++j) sum += fixed(scaled(c[j], s));
+    for (int j = 0; j < VE; j += 4) {
+      const float4 y = *reinterpret_cast<const float4*>(c + j);
+      x[j] = over.of(y.x); x[j + 1] = over.of(y.y);
+      x[j + 2] = over.of(y.z); x[j + 3] = over.of(y.w);
+    }
+    sum.add<VE>(x);
   }
-  return warp_sum_u64(sum);
+  return sum.warp();
 }
 // The element of the warp's part at which the cumulative weight, `before` ahead
 // of the part, passes `at`: in one lane, -1 in the others.  `weights` gives a
@@ -318,6 +431,7 @@ template <int VE, typename F>
 __device__ __forceinline__ long long find_at(const Share& sh, int mis, ull before, ull at,
                                              F weights) {
   const int lane = threadIdx.x & 31;
+#pragma unroll 1
   for (int k0 = sh.g0; k0 < sh.g1; k0 += 32) {
     const int k = k0 + lane;
     ull w[VE], sum = 0;
@@ -350,17 +464,59 @@ __device__ __forceinline__ long long find_at(const Share& sh, int mis, ull befor
   return -1;
 }
 
+// A token's share of a row's weights.
+__device__ __noinline__ float share_of(float l, float m, float z, float inv_t) {
+  return share(weight(l, m, inv_t), z);
+}
+// p of a token after the rejections so far, from its p and q before them.
+__device__ __noinline__ float left_of(float pv, float qv, int nst, const float* stage) {
+  for (int k = 0; k < nst; ++k)
+    if (stage[k] > 0.f) pv = __fdiv_rn(fmaxf(pv - qv, 0.f), stage[k]);
+  return pv;
+}
+// The first child of `cur` after node `after`, n if there is none.
+__device__ __noinline__ int next_child(const int* par, int n, int cur, int after) {
+  for (int base = (after + 1) & ~31; base < n; base += 32) {
+    const int j = base + (threadIdx.x & 31);
+    const unsigned hit = __ballot_sync(0xffffffffu, j > after && j < n && par[j] == cur);
+    if (hit) return base + __ffs(hit) - 1;
+  }
+  return n;
+}
+// Whether an earlier child had node i's token (and so took its weight).
+__device__ __noinline__ bool seen_before(const int* par, const int* tok, int cur, int i) {
+  bool s = false;
+  for (int j = cur + 1 + (threadIdx.x & 31); j < i; j += 32) s |= par[j] == cur && tok[j] == tok[i];
+  return __any_sync(0xffffffffu, s) != 0;
+}
+// Sums of all parts' a and b.
+template <int PARTS>
+__device__ __noinline__ Part total(const Part* in) {
+  Part r = {0, 0};
+#pragma unroll 4
+  for (int i = 0; i < PARTS / 32; ++i) {
+    r.a += in[(threadIdx.x & 31) + 32 * i].a;
+    r.b += in[(threadIdx.x & 31) + 32 * i].b;
+  }
+  r.a = warp_sum_u64(r.a);
+  r.b = warp_sum_u64(r.b);
+  return r;
+}
+
 // Gives this warp's part (in every lane) to all CTAs of the cluster and waits for
 // all parts of the same turn.  A buffer is written again two turns later, when
 // every warp has given its part of the turn between, and so has read this one's.
-__device__ __noinline__ const Part* exchange(Shared& sm, int turn, int rank, ull a, ull b, int* err) {
+template <int C, int PARTS>
+__device__ __noinline__ const Part* exchange(Shared<PARTS>& sm, int turn, int rank, ull a, ull b,
+                                             int* err) {
+  constexpr int W = PARTS / C;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   Part* in = sm.in[turn & 1];
   uint64_t* bar = reinterpret_cast<uint64_t*>(&sm.bar[turn & 1]);
-  if (threadIdx.x == 0) mbar_arrive_expect_tx(bar, sizeof(Part) * kCluster * kWarps);
-  if (lane < kCluster) {
+  if (threadIdx.x == 0) mbar_arrive_expect_tx(bar, sizeof(Part) * PARTS);
+  if (lane < C) {
     uint32_t to, tb;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(in + rank * kWarps + warp)), "r"(lane));
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(in + rank * W + warp)), "r"(lane));
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(tb) : "r"(smem_u32(bar)), "r"(lane));
     asm volatile(
         "st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to),
@@ -383,14 +539,14 @@ __device__ __noinline__ const Part* exchange(Shared& sm, int turn, int rank, ull
   return in;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) __cluster_dims__(kCluster, 1, 1)
-    verify_tree_kernel(VerifyArgs p) {
-  constexpr int VE = 16 / sizeof(T);
-  __shared__ Shared sm;
+// C CTAs of TH threads a sequence; rank = blockIdx.y.
+template <typename T, int C, int TH>
+__global__ void __launch_bounds__(TH, 1024 / TH) verify_tree_kernel(VerifyArgs p) {
+  constexpr int VE = 16 / sizeof(T), W = TH / 32, PARTS = C * W;
+  __shared__ Shared<PARTS> sm;
   extern __shared__ __align__(16) float cache[];
   cg::cluster_group cluster = cg::this_cluster();
-  const int rank = blockIdx.x, b = blockIdx.y;
+  const int rank = blockIdx.y, b = blockIdx.x;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const bool with_q = p.draft != nullptr && !p.greedy;
   if (tid == 0) {
@@ -402,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, 2) __cluster_dims__(kCluster, 1, 1)
   pdl_trigger();
   const T* lb = static_cast<const T*>(p.logits) + b * p.l_sb;
   const T* db = with_q ? static_cast<const T*>(p.draft) + b * p.d_sb : nullptr;
-  for (int i = tid; i < p.T; i += kThreads) {
+  for (int i = tid; i < p.T; i += TH) {
     const int par = p.parents[b * p.par_sb + i];
     const int64_t t = p.tokens[b * p.tok_sb + i];
     const bool known = i > 0 && par >= 0 && par < i && t >= 0 && t < p.V;
@@ -415,7 +571,7 @@ __global__ void __launch_bounds__(kThreads, 2) __cluster_dims__(kCluster, 1, 1)
   if (p.stats) {
     // a warp a row: its slices' maxima and sums
     const int rows = p.T + (with_q ? p.T - 1 : 0);
-    for (int i = warp; i < rows; i += kWarps) {
+    for (int i = warp; i < rows; i += W) {
       const int r = i < p.T ? b * p.T + i : p.B * p.T + b * (p.T - 1) + i - p.T;
       const float2* st = p.stats + (int64_t)r * p.slices;
       float m = -INFINITY, s = 0.f;
@@ -432,31 +588,28 @@ __global__ void __launch_bounds__(kThreads, 2) __cluster_dims__(kCluster, 1, 1)
       }
     }
   }
+  if (p.stats) {
+    __syncthreads();
+    for (int i = tid; i < p.T; i += TH) {
+      const int par = max(sm.par[i], 0);
+      const float w = weight(sm.lt[i], sm.m[par], p.inv_t);
+      sm.pt[i] = with_q ? share(w, sm.z[par]) : w;
+      if (with_q && i > 0)
+        sm.uq[i] = __fmul_rn(sm.u[i], share(weight(sm.qt[i], sm.mq[par], p.inv_t), sm.zq[par]));
+    }
+  }
   cluster.sync();  // all CTAs run: their shared memory can be written
 
-  const int gc = ((p.V + 2 * VE - 2) / VE + kCluster - 1) / kCluster;
-  const int gw = (gc + kWarps - 1) / kWarps;
+  const int gc = ((p.V + 2 * VE - 2) / VE + C - 1) / C;
+  const int gw = (gc + W - 1) / W;
   Share sh;
   sh.first = rank * gc;
   sh.g0 = min(sh.first + warp * gw, sh.first + gc);
   sh.g1 = min(sh.g0 + gw, sh.first + gc);
   int turn = 0;  // exchanges so far
-  // sums of a and b over all parts
-  auto total = [&](const Part* in, ull& a, ull& c) {
-    a = c = 0;
-#pragma unroll
-    for (int i = 0; i < kCluster * kWarps / 32; ++i) {
-      a += in[lane + 32 * i].a;
-      c += in[lane + 32 * i].b;
-    }
-    a = warp_sum_u64(a);
-    c = warp_sum_u64(c);
-  };
   auto sum1 = [&](ull mine) {
-    ull a, c;
-    total(exchange(sm, turn, rank, mine, 0, p.err), a, c);
-    ++turn;
-    return a;
+    const Part* in = exchange<C>(sm, turn++, rank, mine, 0, p.err);
+    return total<PARTS>(in).a;
   };
 
   int32_t* path = p.path + (int64_t)b * p.T;
@@ -473,12 +626,11 @@ __global__ void __launch_bounds__(kThreads, 2) __cluster_dims__(kCluster, 1, 1)
     auto sums = [&]() {   // the exact sums of the node's weights
       const ull s = sum_weights<T>(sh, row, mis, p.V, m, p.inv_t);
       const ull sq = qrow ? sum_weights<T>(sh, qrow, mis, p.V, mq, p.inv_t) : 0;
-      ull a, c;
-      total(exchange(sm, turn, rank, s, sq, p.err), a, c);
-      ++turn;
-      left = a;
-      z = unfixed(a);
-      zq = unfixed(c);
+      const Part* in = exchange<C>(sm, turn++, rank, s, sq, p.err);
+      const Part r = total<PARTS>(in);
+      left = r.a;
+      z = unfixed(r.a);
+      zq = unfixed(r.b);
       summed = true;
     };
     if (p.stats) {
@@ -486,19 +638,16 @@ __global__ void __launch_bounds__(kThreads, 2) __cluster_dims__(kCluster, 1, 1)
       z = sm.z[cur];
       if (qrow) { mq = sm.mq[cur]; zq = sm.zq[cur]; }
       left = (ull)((double)z * kFix);
-    } else {
-      const ull a = max_of<T>(sh, row, mis, p.V);
-      const ull c = qrow ? max_of<T>(sh, qrow, mis, p.V) : __float_as_uint(-INFINITY);
-      const Part* in = exchange(sm, turn, rank, a, c, p.err);
+    } else if (p.greedy) {
+      const Part* in = exchange<C>(sm, turn, rank, max_of<T>(sh, row, mis, p.V), 0, p.err);
       ++turn;
       m = -INFINITY;
       int ix = INT_MAX;
-#pragma unroll
-      for (int i = 0; i < kCluster * kWarps / 32; ++i) {  // (ascending indexes)
-        const Part o = in[lane * (kCluster * kWarps / 32) + i];
-        const float x = __uint_as_float((uint32_t)o.a);
-        if (x > m) { m = x; ix = (int)(o.a >> 32); }
-        mq = fmaxf(mq, __uint_as_float((uint32_t)o.b));
+#pragma unroll 4
+      for (int i = 0; i < PARTS / 32; ++i) {  // (ascending indexes)
+        const ull o = in[lane * (PARTS / 32) + i].a;
+        const float x = __uint_as_float((uint32_t)o);
+        if (x > m) { m = x; ix = (int)(o >> 32); }
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
@@ -506,63 +655,66 @@ __global__ void __launch_bounds__(kThreads, 2) __cluster_dims__(kCluster, 1, 1)
         const int oi = __shfl_xor_sync(0xffffffffu, ix, o);
         if (om > m || (om == m && oi < ix)) { m = om; ix = oi; }
       }
-      mq = warp_max(mq);
       best = m > -INFINITY ? ix : -1;
-      if (!p.greedy) sums();
-    }
-    // p and q of child i's token, after nst rejections
-    auto p_of = [&](int i) {
-      float pv = share(weight(sm.lt[i], m, p.inv_t), z);
-      const float qv = share(weight(sm.qt[i], mq, p.inv_t), zq);
-      for (int k = 0; k < nst; ++k)
-        if (sm.stage[k] > 0.f) pv = __fdiv_rn(fmaxf(pv - qv, 0.f), sm.stage[k]);
-      return pv;
-    };
-    auto uq_of = [&](int i) {
-      return __fmul_rn(sm.u[i], share(weight(sm.qt[i], mq, p.inv_t), zq));
-    };
-    auto next_child = [&](int after) {
-      for (int base = (after + 1) & ~31; base < p.T; base += 32) {
-        const int j = base + lane;
-        const unsigned hit = __ballot_sync(0xffffffffu, j > after && j < p.T && sm.par[j] == cur);
-        if (hit) return base + __ffs(hit) - 1;
+    } else {
+      const ull a = approx_of<T>(sh, row, mis, p.V, p.inv_t);
+      const ull c = qrow ? approx_of<T>(sh, qrow, mis, p.V, p.inv_t) : pack_f2(-INFINITY, 0.f);
+      const Part* in = exchange<C>(sm, turn, rank, a, c, p.err);
+      ++turn;
+      const float sc = p.inv_t * 1.4426950408889634f;
+      m = -INFINITY;
+#pragma unroll 4
+      for (int i = 0; i < PARTS / 32; ++i) {
+        m = fmaxf(m, __uint_as_float((uint32_t)in[lane + 32 * i].a));
+        mq = fmaxf(mq, __uint_as_float((uint32_t)in[lane + 32 * i].b));
       }
-      return p.T;
-    };
-    // whether an earlier child had node i's token (and so took its weight)
-    auto seen = [&](int i) {
-      bool s = false;
-      for (int j = cur + 1 + lane; j < i; j += 32) s |= sm.par[j] == cur && sm.tok[j] == sm.tok[i];
-      return __any_sync(0xffffffffu, s) != 0;
-    };
+      m = warp_max(m);
+      mq = warp_max(mq);
+#pragma unroll 4
+      for (int i = 0; i < PARTS / 32; ++i) {
+        const Part o = in[lane + 32 * i];
+        z += __uint_as_float((uint32_t)(o.a >> 32)) *
+             ex2_ftz(fmaxf((__uint_as_float((uint32_t)o.a) - m) * sc, -200.f));
+        zq += __uint_as_float((uint32_t)(o.b >> 32)) *
+              ex2_ftz(fmaxf((__uint_as_float((uint32_t)o.b) - mq) * sc, -200.f));
+      }
+      z = warp_sum(z);
+      zq = warp_sum(zq);
+      left = (ull)((double)z * kFix);
+    }
     // ---- the children, in index order ----
     bool down = false;
-    for (int i = next_child(last); i < p.T; i = next_child(last)) {
-      last = i;
+    for (int i = next_child(sm.par, p.T, cur, last); i < p.T;) {
       const int t = sm.tok[i];
-      bool ok = false;
+      bool ok = false, again = false;  // again: with the exact sums
       if (p.greedy) {
         ok = t == best && best >= 0;
       } else if (with_q) {
         if (t >= 0) {
-          float uq = uq_of(i), pt = p_of(i);
-          if (!summed && fabsf(uq - pt) <= 3.f * kSumError * fmaxf(uq, pt)) {
-            sums();
-            uq = uq_of(i);
-            pt = p_of(i);
+          float uq, pt;
+          if (p.stats && !summed) {
+            uq = sm.uq[i];
+            pt = sm.pt[i];
+          } else {
+            const float qv = share_of(sm.qt[i], mq, zq, p.inv_t);
+            uq = __fmul_rn(sm.u[i], qv);
+            pt = left_of(share_of(sm.lt[i], m, z, p.inv_t), qv, nst, sm.stage);
           }
+          again = !summed && fabsf(uq - pt) <= 3.f * kSumError * fmaxf(uq, pt);
           ok = uq < pt;
         }
-        if (!ok) {
-          if (!summed) sums();
+        again |= !summed && !ok;  // the residual needs them
+        if (!again && !ok) {
           if (nst == 0) shares<T>(sh, row, mis, p.V, m, z, p.inv_t, cache);
           const ull r = sum1(reject<T>(sh, qrow, mis, p.V, mq, zq, p.inv_t, over, cache));
           sm.stage[nst] = unfixed(r);  // (all threads write the same)
           if (r > 0) {
             over = unfixed(r);
-          } else {  // nothing left: p stays as it was, rebuilt stage by stage
+          } else {
+            // nothing left: p stays as it was, rebuilt stage by stage
             shares<T>(sh, row, mis, p.V, m, z, p.inv_t, cache);
             float s = 0.f;
+#pragma unroll 1
             for (int k = 0; k < nst; ++k)
               if (sm.stage[k] > 0.f) {
                 reject<T>(sh, qrow, mis, p.V, mq, zq, p.inv_t, s, cache);
@@ -572,16 +724,22 @@ __global__ void __launch_bounds__(kThreads, 2) __cluster_dims__(kCluster, 1, 1)
           ++nst;
         }
       } else {
-        const ull w = t >= 0 && !seen(i) ? fixed(weight(sm.lt[i], m, p.inv_t)) : 0;
+        const ull w = t < 0 || seen_before(sm.par, sm.tok, cur, i) ? 0
+                      : fixed(p.stats ? sm.pt[i] : weight(sm.lt[i], m, p.inv_t));
         const double u = (double)sm.u[i];
-        if (!summed && fabs(u * (double)left - (double)w) <= u * kSumError * kFix * (double)z) {
-          sums();
-          for (int j = next_child(cur); j < i; j = next_child(j))
-            if (sm.tok[j] >= 0 && !seen(j)) left -= fixed(weight(sm.lt[j], m, p.inv_t));
-        }
         ok = u * (double)left < (double)w;
-        if (!ok) left -= min(left, w);
+        again = !summed && fabs(u * (double)left - (double)w) <= u * kSumError * kFix * (double)z;
+        if (!again && !ok) left -= min(left, w);
       }
+      if (again) {
+        sums();
+        if (!with_q)  // less what the earlier children took
+          for (int j = next_child(sm.par, p.T, cur, cur); j < i; j = next_child(sm.par, p.T, cur, j))
+            if (sm.tok[j] >= 0 && !seen_before(sm.par, sm.tok, cur, j))
+              left -= fixed(weight(sm.lt[j], m, p.inv_t));
+        continue;  // the same child
+      }
+      last = i;
       if (ok) {
         if (rank == 0 && tid == 0) path[n] = i;
         ++n;
@@ -589,6 +747,7 @@ __global__ void __launch_bounds__(kThreads, 2) __cluster_dims__(kCluster, 1, 1)
         down = true;
         break;
       }
+      i = next_child(sm.par, p.T, cur, last);
     }
     if (down) continue;
 
@@ -604,15 +763,15 @@ __global__ void __launch_bounds__(kThreads, 2) __cluster_dims__(kCluster, 1, 1)
         sum1(nst == 0 ? shares<T>(sh, row, mis, p.V, m, z, p.inv_t, cache)
                       : scale<VE>(sh, over, cache));
       } else {
-        for (int j = next_child(cur); j < p.T; j = next_child(j))
-          if (sm.tok[j] >= 0 && !seen(j)) sm.out[nout++] = j;  // (all threads write the same)
+        for (int j = next_child(sm.par, p.T, cur, cur); j < p.T; j = next_child(sm.par, p.T, cur, j))
+          if (sm.tok[j] >= 0 && !seen_before(sm.par, sm.tok, cur, j)) sm.out[nout++] = j;  // (all threads write the same)
       }
       // the parts of the last exchange, less the rejected tokens
       const Part* in = sm.in[(turn - 1) & 1];
-      const int me = rank * kWarps + warp;
+      const int me = rank * W + warp;
       ull all = 0, before = 0, mine = in[me].a;
 #pragma unroll
-      for (int i = 0; i < kCluster * kWarps / 32; ++i) {
+      for (int i = 0; i < PARTS / 32; ++i) {
         const int e = lane + 32 * i;
         all += in[e].a;
         if (e < me) before += in[e].a;
@@ -622,7 +781,7 @@ __global__ void __launch_bounds__(kThreads, 2) __cluster_dims__(kCluster, 1, 1)
       for (int j = 0; j < nout; ++j) {
         const int i = sm.out[j], k = (sm.tok[i] + mis) / VE;
         const ull w = fixed(weight(sm.lt[i], m, p.inv_t));
-        const int e = k / gc * kWarps + k % gc / gw;
+        const int e = k / gc * W + k % gc / gw;
         all -= w;
         if (e < me) before -= w;
         if (e == me) mine -= w;
@@ -633,10 +792,11 @@ __global__ void __launch_bounds__(kThreads, 2) __cluster_dims__(kCluster, 1, 1)
         owner = false;
         if (at >= before && at < before + mine) {  // in this warp's part
           if (with_q) {
+            const Divisor by(over > 0.f ? over : 1.f);
             next = find_at<VE>(sh, mis, before, at, [&](int k, ull* w) {
               const float* c = cache + (k - sh.first) * VE;
 #pragma unroll
-              for (int j = 0; j < VE; ++j) w[j] = fixed(scaled(c[j], over));
+              for (int j = 0; j < VE; ++j) w[j] = fixed(by.of(c[j]));
             });
           } else {
             next = find_at<VE>(sh, mis, before, at, [&](int k, ull* w) {
@@ -662,22 +822,56 @@ __global__ void __launch_bounds__(kThreads, 2) __cluster_dims__(kCluster, 1, 1)
   }
   if (rank == 0) {
     if (tid == 0) { path[0] = 0; p.count[b] = n; }
-    for (int i = n + tid; i < p.T; i += kThreads) path[i] = -1;
+    for (int i = n + tid; i < p.T; i += TH) path[i] = -1;
   }
   cluster.sync();  // a CTA's shared memory outlives its writers
 }
 
-// Rows are read ahead of the walk where all of them are at most this many bytes:
-// measured (8 CTAs a sequence): see the launch below.
+// Rows are read ahead of the walk where all of them are at most this many bytes.
 constexpr int64_t kStatsBytes = 32 << 20;
 
 int stats_slices(int64_t V, int64_t item) {
   return (int)((V * item / 16 + 1 + kSlice) / kSlice);  // whatever the rows' alignment
 }
-int64_t stats_limit() { const char* e = getenv("TSTATS"); return e ? atoll(e) << 20 : kStatsBytes; }
 bool use_stats(int64_t B, int64_t T, int64_t V, int with_q, int64_t item) {
   const int64_t rows = B * (T + (with_q ? T - 1 : 0));
-  return T > 1 && rows <= 65535 && rows * V * item <= stats_limit();
+  return T > 1 && rows <= 65535 && rows * V * item <= (getenv("TSTATS") ? atoll(getenv("TSTATS")) << 20 : kStatsBytes);
+}
+
+// CTAs a sequence and their threads.  Few sequences: as many threads as a cluster
+// can have; many: small CTAs, all of which fit the SMs at once.
+struct Shape { int cluster, threads; };
+Shape shape_of(int64_t B, int64_t row_bytes) {
+  if (const char* e = getenv("TSHAPE")) { int v = atoi(e); return v == 0 ? Shape{16, 1024} : v == 1 ? Shape{8, 512} : Shape{8, 256}; }
+  if (B <= 8 && row_bytes >= 65536) return {16, 1024};
+  return {8, B * 16 <= 2 * num_sms() ? 512 : 256};
+}
+
+template <typename T, int C, int TH>
+int walk_launch(const VerifyArgs& a, int64_t B, cudaStream_t st) {
+  auto kern = verify_tree_kernel<T, C, TH>;
+  constexpr int VE = 16 / sizeof(T);
+  // the cache of what is left of p, a CTA's part of a row (with a draft)
+  const size_t cache = a.draft && !a.greedy
+      ? (size_t)((a.V + 2 * VE - 2) / VE + C - 1) / C * VE * sizeof(float) : 0;
+  if (cache > 16 * 1024 &&
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cache) !=
+          cudaSuccess) {
+    set_error("verify_tree_kernel: cannot reserve shared memory");
+    return TPP_ERR_LAUNCH;
+  }
+  if (C > 8 && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) !=
+                   cudaSuccess) {
+    set_error("verify_tree_kernel: clusters of 16 are not allowed");
+    return TPP_ERR_LAUNCH;
+  }
+  return launch("verify_tree_kernel", kern, dim3((unsigned)B, C), dim3(TH), cache, st, C, a);
+}
+template <typename T>
+int walk_as(const VerifyArgs& a, Shape sh, int64_t B, cudaStream_t st) {
+  if (sh.cluster == 16) return walk_launch<T, 16, 1024>(a, B, st);
+  if (sh.threads == 512) return walk_launch<T, 8, 512>(a, B, st);
+  return walk_launch<T, 8, 256>(a, B, st);
 }
 
 }  // namespace
@@ -728,30 +922,22 @@ extern "C" int tpp_verify_tree(const void* logits, int64_t l_sb, int64_t l_st,
   a.stats = need ? static_cast<float2*>(workspace) : nullptr;
   a.slices = stats_slices(V, dtype == TPP_F32 ? 4 : 2);
   a.err = device_error_flag();
-  // the cache of what is left of p, a CTA's part of a row (with a draft)
-  const int64_t ve = dtype == TPP_F32 ? 4 : 8;
-  const size_t cache = draft_logits && !a.greedy
-      ? ((V + 2 * ve - 2) / ve + kCluster - 1) / kCluster * ve * sizeof(float) : 0;
-  TPP_REQUIRE(cache <= 200 * 1024, TPP_ERR_UNSUPPORTED,
-              "draft logits need a vocabulary of at most 409600 tokens");
-  auto go = [&](auto stats, auto walk) -> int {
-    if (need) {
-      const int64_t rows = B * (T + (draft_logits ? T - 1 : 0));
-      const int rc = launch("verify_stats_kernel", stats, dim3((unsigned)a.slices, (unsigned)rows),
-                            dim3(256), 0, as_stream(stream), 0u, a);
-      if (rc != TPP_OK) return rc;
-    }
-    if (cache > 32 * 1024 &&
-        cudaFuncSetAttribute(walk, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cache) !=
-            cudaSuccess) {
-      set_error("verify_tree_kernel: cannot reserve shared memory");
-      return TPP_ERR_LAUNCH;
-    }
-    return launch("verify_tree_kernel", walk, dim3(kCluster, (unsigned)B), dim3(kThreads), cache,
-                  as_stream(stream), 0u, a);
-  };
-  if (dtype == TPP_F16) return go(verify_stats_kernel<__half>, verify_tree_kernel<__half>);
-  if (dtype == TPP_BF16)
-    return go(verify_stats_kernel<__nv_bfloat16>, verify_tree_kernel<__nv_bfloat16>);
-  return go(verify_stats_kernel<float>, verify_tree_kernel<float>);
+  const int64_t item = dtype == TPP_F32 ? 4 : 2;
+  TPP_REQUIRE(!draft_logits || a.greedy || V <= 400000, TPP_ERR_UNSUPPORTED,
+              "draft logits need a vocabulary of at most 400000 tokens");
+  if (need) {
+    const int64_t rows = B * (T + (draft_logits ? T - 1 : 0));
+    const dim3 grid((unsigned)a.slices, (unsigned)rows);
+    auto stats = [&](auto kern) {
+      return launch("verify_stats_kernel", kern, grid, dim3(256), 0, as_stream(stream), 0u, a);
+    };
+    const int rc = dtype == TPP_F16 ? stats(verify_stats_kernel<__half>)
+                 : dtype == TPP_BF16 ? stats(verify_stats_kernel<__nv_bfloat16>)
+                                     : stats(verify_stats_kernel<float>);
+    if (rc != TPP_OK) return rc;
+  }
+  const Shape sh = shape_of(B, V * item);
+  if (dtype == TPP_F16) return walk_as<__half>(a, sh, B, as_stream(stream));
+  if (dtype == TPP_BF16) return walk_as<__nv_bfloat16>(a, sh, B, as_stream(stream));
+  return walk_as<float>(a, sh, B, as_stream(stream));
 }
