@@ -28,68 +28,82 @@ struct RopeTreeArgs {
   int T, Hq, Hkv;
 };
 
-// y = rope(x * rsqrt(mean(x^2) + eps) * w) of one head row: a group of G = D/8
-// lanes owns a row, lane l holds elements [8l, 8l+8); the rotate-half partner
-// chunk lives in lane l ^ (G/2).  fp32 throughout, one rounding at the store.
-template <typename T, typename CS, int G>
+// y = rope(x * rsqrt(mean(x^2) + eps) * w) of a token's head rows: a group of G =
+// D/8 lanes owns HPG head rows of one token, lane l elements [8l, 8l+8) of each; the
+// rotate-half partner chunk lives in lane l ^ (G/2).  fp32 throughout, one rounding
+// at the store.  Bound by HBM at many tokens, so a group keeps the loads of HPG rows
+// in flight and takes the token's table rows and the norm weights once for all of
+// them; at few tokens by latency, where HPG = 1 spreads the rows.
+template <typename T, typename CS, int G, int HPG>
 __global__ void __launch_bounds__(256) qk_norm_rope_tree_kernel(RopeTreeArgs p) {
   pdl_wait();
   pdl_trigger();
   constexpr int D = G * 8;
-  const int heads = p.Hq + p.Hkv;
+  const int heads = p.Hq + p.Hkv, per = (heads + HPG - 1) / HPG;
   const int64_t item = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
   const int lane = threadIdx.x % G;
-  const bool valid = item < p.tokens * heads;
-  const int64_t it = valid ? item : 0;
-  const int64_t tok = it / heads;
-  const int h = (int)(it - tok * heads);
+  const bool valid = item < p.tokens * per;  // (lanes past the end take part in the shuffles)
+  const int64_t tok = valid ? item / per : 0;
+  const int h0 = valid ? (int)(item - tok * per) * HPG : 0;
   const int64_t b = tok / p.T, t = tok - b * p.T;
-  const bool is_q = h < p.Hq;
-  float v[8];
-  unpack8<T>(ldg_nc_v4(static_cast<const T*>(p.qkv) + b * p.qkv_sb + t * p.qkv_st +
-                       (int64_t)h * D + lane * 8), v);
+  const T* row = static_cast<const T*>(p.qkv) + b * p.qkv_sb + t * p.qkv_st + lane * 8;
+  uint4 raw[HPG];
+#pragma unroll
+  for (int i = 0; i < HPG; ++i) raw[i] = ldg_nc_v4(row + (int64_t)min(h0 + i, heads - 1) * D);
   const int64_t pos = p.positions[tok];
   const bool known = pos >= 0 && pos < p.table_rows;
-  const void* nw = is_q ? p.qn : p.kn;
-  float ss = 0.f;
+  float c8[8], s8[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) ss += v[j] * v[j];
-#pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  if (nw != nullptr) {
-    const float inv = rsqrtf(ss / (float)D + p.eps);
-    float g[8];
-    unpack8<T>(__ldg(static_cast<const uint4*>(nw) + lane), g);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = v[j] * inv * g[j];
-  }
-  float r[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) r[j] = __shfl_xor_sync(0xffffffffu, v[j], G / 2);
-  if (!valid) return;
+  for (int j = 0; j < 8; ++j) c8[j] = s8[j] = 0.f;
   if (known) {
-    float c8[8], s8[8];
     load_table8<CS>(static_cast<const CS*>(p.cosp) + pos * p.cs_stride + lane * 8, c8);
     load_table8<CS>(static_cast<const CS*>(p.sinp) + pos * p.cs_stride + lane * 8, s8);
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      v[j] = lane < G / 2 ? v[j] * c8[j] - r[j] * s8[j] : v[j] * c8[j] + r[j] * s8[j];
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = 0.f;
   }
-  T* dst = is_q ? static_cast<T*>(p.q_out) + (tok * p.Hq + h) * D
-                : static_cast<T*>(p.k_out) + (tok * p.Hkv + h - p.Hq) * D;
-  *reinterpret_cast<uint4*>(dst + lane * 8) = pack8<T>(v);
+#pragma unroll
+  for (int i = 0; i < HPG; ++i) {
+    const int h = min(h0 + i, heads - 1);
+    const bool is_q = h < p.Hq;
+    float v[8];
+    unpack8<T>(raw[i], v);
+    const void* nw = is_q ? p.qn : p.kn;
+    float ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss += v[j] * v[j];
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (nw != nullptr) {
+      const float inv = rsqrtf(ss / (float)D + p.eps);
+      float g[8];
+      unpack8<T>(__ldg(static_cast<const uint4*>(nw) + lane), g);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = v[j] * inv * g[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float r = __shfl_xor_sync(0xffffffffu, v[j], G / 2);
+      v[j] = lane < G / 2 ? v[j] * c8[j] - r * s8[j] : v[j] * c8[j] + r * s8[j];
+      if (!known) v[j] = 0.f;  // (0 * inf is NaN)
+    }
+    if (valid && h0 + i < heads) {
+      T* dst = is_q ? static_cast<T*>(p.q_out) + (tok * p.Hq + h) * D
+                    : static_cast<T*>(p.k_out) + (tok * p.Hkv + h - p.Hq) * D;
+      *reinterpret_cast<uint4*>(dst + lane * 8) = pack8<T>(v);
+    }
+  }
 }
 
 template <typename T, typename CS>
 int rope_tree_launch(const RopeTreeArgs& a, int64_t D, cudaStream_t st) {
   auto go = [&](auto tag) -> int {
     constexpr int G = decltype(tag)::value;
-    const int64_t grid = (a.tokens * (a.Hq + a.Hkv) + 256 / G - 1) / (256 / G);
+    // four rows a group from where they fill the SMs' threads (148 * 2048) on
+    const int64_t heads = a.Hq + a.Hkv;
+    const int hpg = a.tokens * heads * G >= 4 * 2048 * (int64_t)num_sms() ? 4 : 1;
+    const int64_t grid = (a.tokens * ((heads + hpg - 1) / hpg) + 256 / G - 1) / (256 / G);
     TPP_REQUIRE(grid < (1ll << 31), TPP_ERR_SHAPE, "too many rows");
-    return launch("qk_norm_rope_tree_kernel", qk_norm_rope_tree_kernel<T, CS, G>,
+    return launch("qk_norm_rope_tree_kernel",
+                  hpg == 4 ? qk_norm_rope_tree_kernel<T, CS, G, 4>
+                           : qk_norm_rope_tree_kernel<T, CS, G, 1>,
                   dim3((unsigned)grid), dim3(256), 0, st, 0u, a);
   };
   switch (D) {
@@ -104,6 +118,8 @@ int rope_tree_launch(const RopeTreeArgs& a, int64_t D, cudaStream_t st) {
   }
 }
 
+constexpr int kMaxPath = 256;
+
 struct CommitArgs {
   const uint4* src[2];                       // k, v trees
   int64_t s_sl[2], s_sb[2], s_st[2], s_sh[2];  // in 16-byte words
@@ -117,32 +133,59 @@ struct CommitArgs {
   int B, T, Hkv, words;                      // words: 16-byte words of a row
 };
 
-// One block copies the rows of one (layer, sequence, k or v).
+// One block copies the rows of one (layer, sequence, k or v), four words a thread
+// in flight: a copy of a few KB a block, bound by the latency of its chain count ->
+// path -> row -> store at one sequence and by HBM at many.
 __global__ void __launch_bounds__(256) kv_commit_kernel(CommitArgs p) {
+  constexpr int U = 4;
   pdl_wait();
   pdl_trigger();
-  const int64_t l = blockIdx.x / p.B, b = blockIdx.x % p.B;
+  const int l = blockIdx.x / p.B, b = blockIdx.x - l * p.B;
   const int kv = blockIdx.y;
+  __shared__ int64_t from[kMaxPath], to[kMaxPath];  // words, of head 0
   const int n = min(p.count[b], p.T);
   const int64_t ctx = p.ctx_lens[b];
   const uint4* src = p.src[kv] + l * p.s_sl[kv] + b * p.s_sb[kv];
   uint4* dst = p.dst[kv] + l * p.c_sl + (p.table ? 0 : b * p.c_sb);
   const int per = p.Hkv * p.words;
-  for (int e = threadIdx.x; e < n * per; e += blockDim.x) {
-    const int i = e / per, r = e - i * per;
-    const int h = r / p.words, w = r - h * p.words;
-    const int node = p.path[b * p.path_sb + i];
-    const int64_t row = ctx + i;
-    if (node < 0 || node >= p.T || row < 0 || row >= p.rows) continue;
-    int64_t at;
-    if (p.table) {
-      const int64_t blk = p.table[b * p.table_stride + row / 64];
-      if (blk < 0 || blk >= p.num_blocks) continue;
-      at = ((blk * p.Hkv + h) * 64 + row % 64) * p.words;
-    } else {
-      at = h * p.c_sh + row * p.c_ss;
+  const int64_t head = p.table ? 64 * p.words : p.c_sh;
+  for (int i0 = 0; i0 < n; i0 += kMaxPath) {
+    const int m = min(kMaxPath, n - i0);
+    if (i0 > 0) __syncthreads();
+    for (int i = threadIdx.x; i < m; i += blockDim.x) {
+      const int node = p.path[b * p.path_sb + i0 + i];
+      const int64_t row = ctx + i0 + i;
+      int64_t at = -1;
+      if (node >= 0 && node < p.T && row >= 0 && row < p.rows) {
+        if (p.table) {
+          const int64_t blk = p.table[b * p.table_stride + row / 64];
+          if (blk >= 0 && blk < p.num_blocks) at = (blk * p.Hkv * 64 + row % 64) * p.words;
+        } else {
+          at = row * p.c_ss;
+        }
+      }
+      from[i] = node * p.s_st[kv];
+      to[i] = at;
     }
-    dst[at + w] = src[node * p.s_st[kv] + h * p.s_sh[kv] + w];
+    __syncthreads();
+    for (int e0 = threadIdx.x; e0 < m * per; e0 += U * blockDim.x) {
+      uint4 x[U];
+      int64_t at[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int e = e0 + u * blockDim.x;
+        at[u] = -1;
+        if (e >= m * per) continue;
+        const int i = e / per, r = e - i * per;
+        const int h = r / p.words, w = r - h * p.words;
+        if (to[i] < 0) continue;
+        at[u] = to[i] + h * head + w;
+        x[u] = src[from[i] + h * p.s_sh[kv] + w];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (at[u] >= 0) dst[at[u]] = x[u];
+    }
   }
 }
 

@@ -14,14 +14,17 @@
 // are 23 instructions an element.  So a node's tests go by its maximum and an fp32
 // sum, taken in one pass of 7 instructions an element and one exchange; the exact
 // sums follow only where a test comes within the fp32 sum's error of a tie, and
-// at the last node, for the draw.  For small batches verify_stats_kernel takes
-// these of all rows ahead of the walk, on all SMs; for larger ones reading the rows
-// off the path would cost more than it saves.  An exchange is one remote store a
+// at the last node, for the draw.  For chains with a draft verify_stats_kernel takes
+// these of all rows ahead of the walk, on all SMs.  An exchange is one remote store a
 // warp and CTA (st.async, counted by the receiver's mbarrier) and no barrier of the
-// CTA or the cluster.
+// CTA or the cluster, 1.0 us.
+//
+// Bound by latency: one chain of 5 nodes over 151936 tokens with its draft takes
+// 28.0 us (first form 123), of which statistics 5, set-up 3, tests 3, exact sums 6,
+// residual 8, draw 4; 32 trees of 32 nodes 32 us (49).  Code fetched once a walk
+// counts: unrolling the second passes' loops over a lane's groups cost 8 us.
 #include <limits.h>
 #include <math.h>
-#include <cstdlib>
 #include <cooperative_groups.h>
 #include "tc_common.cuh"
 
@@ -33,11 +36,6 @@ namespace {
 constexpr int kMaxNodes = 256;
 constexpr int kSlice = 1024;         // groups of a row for a CTA of the statistics
 constexpr double kFix = 1099511627776.0;  // 2^40
-// Relative error of the fp32 sums: the worst chain of additions is a lane's 1024
-// terms at 2^22 tokens (and a few dozen at 150k), which in practice err like its
-// root; the exponential is within 2^-21 of exact (its argument is rounded at
-// |x| < 32; weights below e^-32 do not count).
-constexpr float kSumError = 1e-5f;
 using ull = unsigned long long;
 
 struct VerifyArgs {
@@ -51,8 +49,9 @@ struct VerifyArgs {
   int32_t* path; int32_t* count; int64_t* next;
   int B, T; int V;
   float2* stats;                           // [row][slices] of (max, sum), or null
-  int* err;
   int slices;
+  float sum_error;                         // relative error of the fp32 sums, at most
+  int* err;
 };
 
 // A row in groups of 16 bytes: group k holds elements [k*VE - mis, k*VE - mis
@@ -274,6 +273,40 @@ __device__ __forceinline__ void each(const Share& sh, const T* src, int mis, int
     raw = next;
   }
 }
+// f(group, values, other row's values) over the warp's groups of two rows, one
+// group's loads ahead.
+template <typename T, typename F>
+__device__ __forceinline__ void each2(const Share& sh, const T* src, const T* other, int mis, int V,
+                                      F f) {
+  constexpr int VE = 16 / sizeof(T);
+  const bool plain = (reinterpret_cast<uintptr_t>(src - mis) & 15) == 0;
+  const bool plain2 = (reinterpret_cast<uintptr_t>(other - mis) & 15) == 0;
+  const int whole = (V + mis) / VE;  // groups 1 .. whole - 1 lie within the row
+  auto load = [&](const T* s, bool pl, int k) {
+    return pl && k > 0 && k < whole ? __ldg(reinterpret_cast<const uint4*>(s - mis) + k)
+                                    : load_edge<T>(s, k * VE - mis, V);
+  };
+  int k = sh.g0 + (threadIdx.x & 31);
+  uint4 a = make_uint4(0, 0, 0, 0), b = a;
+  if (k < sh.g1) {
+    a = load(src, plain, k);
+    b = load(other, plain2, k);
+  }
+#pragma unroll 1
+  for (; k < sh.g1; k += 32) {
+    uint4 a1 = a, b1 = b;
+    if (k + 32 < sh.g1) {
+      a1 = load(src, plain, k + 32);
+      b1 = load(other, plain2, k + 32);
+    }
+    float v[VE], w[VE];
+    unpack_group<T>(a, v);
+    unpack_group<T>(b, w);
+    f(k, v, w);
+    a = a1;
+    b = b1;
+  }
+}
 __device__ __forceinline__ ull pack_f2(float x, float y) {
   return (ull)__float_as_uint(y) << 32 | __float_as_uint(x);
 }
@@ -328,24 +361,37 @@ __device__ __noinline__ ull max_of(Share sh, const T* src, int mis, int V) {
   }
   return (ull)(uint32_t)ix << 32 | __float_as_uint(m);
 }
-// The sum of the integer weights of the warp's part of a row.
+// The sums of the integer weights of the warp's parts of a row and, if there is
+// one, of the draft's.
 template <typename T>
-__device__ __noinline__ ull sum_weights(Share sh, const T* src, int mis, int V, float top,
-                                        float inv_t) {
+__device__ __noinline__ Part sum_weights(Share sh, const T* src, const T* other, int mis, int V,
+                                         float top, float top2, float inv_t) {
   constexpr int VE = 16 / sizeof(T);
-  Sum s;
-  each<T, 1>(sh, src, mis, V, [&](int, const float* v) {
-    float x[VE];
+  Sum s, s2;
+  if (other) {
+    each2<T>(sh, src, other, mis, V, [&](int, const float* v, const float* w) {
+      float x[VE];
 #pragma unroll
-    for (int j = 0; j < VE; ++j) x[j] = weight(v[j], top, inv_t);
-    s.add<VE>(x);
-  });
-  return s.warp();
+      for (int j = 0; j < VE; ++j) x[j] = weight(v[j], top, inv_t);
+      s.add<VE>(x);
+#pragma unroll
+      for (int j = 0; j < VE; ++j) x[j] = weight(w[j], top2, inv_t);
+      s2.add<VE>(x);
+    });
+  } else {
+    each<T, 1>(sh, src, mis, V, [&](int, const float* v) {
+      float x[VE];
+#pragma unroll
+      for (int j = 0; j < VE; ++j) x[j] = weight(v[j], top, inv_t);
+      s.add<VE>(x);
+    });
+  }
+  return {s.warp(), s2.warp()};
 }
 // With a draft, what is left of p is kept in `cache`, this CTA's part of the row:
 // shares() puts the warp's part of p = w / z there, reject() takes p = max(p / s - q,
-// 0) (s 0: p as it is), and both return the sum of the integer weights; scale()
-// that of p / s without changing it.
+// 0) (s 0: p as it is; s < 0: p = w / z is taken from the row), and both return the
+// sum of the integer weights; scale() that of p / s without changing it.
 //
 // Many quotients by one divisor: with r = 1 / b rounded to nearest, q = a r and one
 // correction by the exact remainder a - q b give a / b rounded to nearest
@@ -383,22 +429,29 @@ __device__ __noinline__ ull shares(Share sh, const T* src, int mis, int V, float
   return s.warp();
 }
 template <typename T>
-__device__ __noinline__ ull reject(Share sh, const T* src, int mis, int V, float top, float zq,
-                                   float inv_t, float s, float* cache) {
+__device__ __noinline__ ull reject(Share sh, const T* src, const T* other, int mis, int V,
+                                   float top, float z, float top2, float zq, float inv_t, float s,
+                                   float* cache) {
   constexpr int VE = 16 / sizeof(T);
   Sum sum;
-  const Divisor by(zq), over(s > 0.f ? s : 1.f);
-  each<T, 1>(sh, src, mis, V, [&](int k, const float* v) {
+  const bool first = s < 0.f;
+  const Divisor by(zq), over(first ? z : s > 0.f ? s : 1.f);
+  each2<T>(sh, src, other, mis, V, [&](int k, const float* v, const float* w) {
     float* c = cache + (k - sh.first) * VE;
     float x[VE];
+    if (first) {
 #pragma unroll
-    for (int j = 0; j < VE; j += 4) {
-      const float4 y = *reinterpret_cast<const float4*>(c + j);
-      x[j] = y.x; x[j + 1] = y.y; x[j + 2] = y.z; x[j + 3] = y.w;
+      for (int j = 0; j < VE; ++j) x[j] = weight(v[j], top, inv_t);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VE; j += 4) {
+        const float4 y = *reinterpret_cast<const float4*>(c + j);
+        x[j] = y.x; x[j + 1] = y.y; x[j + 2] = y.z; x[j + 3] = y.w;
+      }
     }
 #pragma unroll
     for (int j = 0; j < VE; ++j)
-      x[j] = fmaxf(over.of(x[j]) - by.of(weight(v[j], top, inv_t)), 0.f);
+      x[j] = fmaxf(over.of(x[j]) - by.of(weight(w[j], top2, inv_t)), 0.f);
     sum.add<VE>(x);
 #pragma unroll
     for (int j = 0; j < VE; j += 4)
@@ -624,9 +677,8 @@ __global__ void __launch_bounds__(TH, 1024 / TH) verify_tree_kernel(VerifyArgs p
     int nst = 0;          // rejections with a draft: stages of the residual
     float over = 0.f;     // the cache holds p times this (0: p itself)
     auto sums = [&]() {   // the exact sums of the node's weights
-      const ull s = sum_weights<T>(sh, row, mis, p.V, m, p.inv_t);
-      const ull sq = qrow ? sum_weights<T>(sh, qrow, mis, p.V, mq, p.inv_t) : 0;
-      const Part* in = exchange<C>(sm, turn++, rank, s, sq, p.err);
+      const Part s = sum_weights<T>(sh, row, qrow, mis, p.V, m, mq, p.inv_t);
+      const Part* in = exchange<C>(sm, turn++, rank, s.a, s.b, p.err);
       const Part r = total<PARTS>(in);
       left = r.a;
       z = unfixed(r.a);
@@ -700,13 +752,13 @@ __global__ void __launch_bounds__(TH, 1024 / TH) verify_tree_kernel(VerifyArgs p
             uq = __fmul_rn(sm.u[i], qv);
             pt = left_of(share_of(sm.lt[i], m, z, p.inv_t), qv, nst, sm.stage);
           }
-          again = !summed && fabsf(uq - pt) <= 3.f * kSumError * fmaxf(uq, pt);
+          again = !summed && fabsf(uq - pt) <= 3.f * p.sum_error * fmaxf(uq, pt);
           ok = uq < pt;
         }
         again |= !summed && !ok;  // the residual needs them
         if (!again && !ok) {
-          if (nst == 0) shares<T>(sh, row, mis, p.V, m, z, p.inv_t, cache);
-          const ull r = sum1(reject<T>(sh, qrow, mis, p.V, mq, zq, p.inv_t, over, cache));
+          const ull r = sum1(reject<T>(sh, row, qrow, mis, p.V, m, z, mq, zq, p.inv_t,
+                                       nst == 0 ? -1.f : over, cache));
           sm.stage[nst] = unfixed(r);  // (all threads write the same)
           if (r > 0) {
             over = unfixed(r);
@@ -717,7 +769,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) verify_tree_kernel(VerifyArgs p
 #pragma unroll 1
             for (int k = 0; k < nst; ++k)
               if (sm.stage[k] > 0.f) {
-                reject<T>(sh, qrow, mis, p.V, mq, zq, p.inv_t, s, cache);
+                reject<T>(sh, row, qrow, mis, p.V, m, z, mq, zq, p.inv_t, s, cache);
                 s = sm.stage[k];
               }
           }
@@ -728,7 +780,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) verify_tree_kernel(VerifyArgs p
                       : fixed(p.stats ? sm.pt[i] : weight(sm.lt[i], m, p.inv_t));
         const double u = (double)sm.u[i];
         ok = u * (double)left < (double)w;
-        again = !summed && fabs(u * (double)left - (double)w) <= u * kSumError * kFix * (double)z;
+        again = !summed && fabs(u * (double)left - (double)w) <= u * p.sum_error * kFix * (double)z;
         if (!again && !ok) left -= min(left, w);
       }
       if (again) {
@@ -827,24 +879,23 @@ __global__ void __launch_bounds__(TH, 1024 / TH) verify_tree_kernel(VerifyArgs p
   cluster.sync();  // a CTA's shared memory outlives its writers
 }
 
-// Rows are read ahead of the walk where all of them are at most this many bytes.
-constexpr int64_t kStatsBytes = 32 << 20;
-
 int stats_slices(int64_t V, int64_t item) {
   return (int)((V * item / 16 + 1 + kSlice) / kSlice);  // whatever the rows' alignment
 }
-bool use_stats(int64_t B, int64_t T, int64_t V, int with_q, int64_t item) {
-  const int64_t rows = B * (T + (with_q ? T - 1 : 0));
-  return T > 1 && rows <= 65535 && rows * V * item <= (getenv("TSTATS") ? atoll(getenv("TSTATS")) << 20 : kStatsBytes);
+// Statistics ahead of the walk, or as it goes: ahead where a node takes two rows
+// (a draft's too) and the rows off the path are few.  Measured (us, ahead / going):
+// 1 chain of 5 nodes over 151936 tokens with its draft 28.0 / 44.9, 64 of 9 over
+// 32003 51.8 / 79.3, 32 of 16 over 151936 126.7 / 168.3; 8 trees of 32 with a draft
+// 94.5 / 74.0; without a draft 1 tree of 32 19.5 / 16.6, 32 of them 106 / 32.
+bool use_stats(int64_t B, int64_t T, int with_q) {
+  return with_q && T > 1 && T <= 16 && B * (2 * T - 1) <= 65535;
 }
 
-// CTAs a sequence and their threads.  Few sequences: as many threads as a cluster
-// can have; many: small CTAs, all of which fit the SMs at once.
-struct Shape { int cluster, threads; };
-Shape shape_of(int64_t B, int64_t row_bytes) {
-  if (const char* e = getenv("TSHAPE")) { int v = atoi(e); return v == 0 ? Shape{16, 1024} : v == 1 ? Shape{8, 512} : Shape{8, 256}; }
-  if (B <= 8 && row_bytes >= 65536) return {16, 1024};
-  return {8, B * 16 <= 2 * num_sms() ? 512 : 256};
+// 8 CTAs a sequence, of 512 threads for few sequences, of 256 for more, so that all
+// of them fit the SMs at once: 64 chains of 9 nodes over 32003 tokens 69.8 us with 512,
+// 52.6 with 256; 1 chain of 5 over 151936 28.2 and 33.8.  (16 CTAs of 1024: 31.4.)
+int walk_threads(int64_t B) {
+  return 16 * B <= 2 * num_sms() ? 512 : 256;
 }
 
 template <typename T, int C, int TH>
@@ -860,18 +911,11 @@ int walk_launch(const VerifyArgs& a, int64_t B, cudaStream_t st) {
     set_error("verify_tree_kernel: cannot reserve shared memory");
     return TPP_ERR_LAUNCH;
   }
-  if (C > 8 && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) !=
-                   cudaSuccess) {
-    set_error("verify_tree_kernel: clusters of 16 are not allowed");
-    return TPP_ERR_LAUNCH;
-  }
   return launch("verify_tree_kernel", kern, dim3((unsigned)B, C), dim3(TH), cache, st, C, a);
 }
 template <typename T>
-int walk_as(const VerifyArgs& a, Shape sh, int64_t B, cudaStream_t st) {
-  if (sh.cluster == 16) return walk_launch<T, 16, 1024>(a, B, st);
-  if (sh.threads == 512) return walk_launch<T, 8, 512>(a, B, st);
-  return walk_launch<T, 8, 256>(a, B, st);
+int walk_as(const VerifyArgs& a, int64_t B, cudaStream_t st) {
+  return walk_threads(B) == 512 ? walk_launch<T, 8, 512>(a, B, st) : walk_launch<T, 8, 256>(a, B, st);
 }
 
 }  // namespace
@@ -883,7 +927,7 @@ extern "C" int64_t tpp_verify_tree_workspace(int64_t B, int64_t T, int64_t V, in
                                              double temperature, int dtype) {
   const int64_t item = dtype == TPP_F32 ? 4 : 2;
   if (B <= 0 || T <= 0 || V <= 0 || temperature <= 0.0) return 0;
-  if (!use_stats(B, T, V, with_draft, item)) return 0;
+  if (!use_stats(B, T, with_draft)) return 0;
   return B * (2 * T - 1) * stats_slices(V, item) * (int64_t)sizeof(float2);
 }
 
@@ -921,13 +965,15 @@ extern "C" int tpp_verify_tree(const void* logits, int64_t l_sb, int64_t l_st,
   a.B = (int)B; a.T = (int)T; a.V = (int)V;
   a.stats = need ? static_cast<float2*>(workspace) : nullptr;
   a.slices = stats_slices(V, dtype == TPP_F32 ? 4 : 2);
+  // A lane adds V / 2048 terms (8 CTAs of 256) one by one, then some dozens of
+  // partial sums; an exponential's argument is rounded thrice at |x| <= 46 (smaller
+  // weights do not count), itself twice.
+  a.sum_error = 8e-6f + (float)(V / 2048 + 64) * 5.9604645e-8f;
   a.err = device_error_flag();
-  const int64_t item = dtype == TPP_F32 ? 4 : 2;
   TPP_REQUIRE(!draft_logits || a.greedy || V <= 400000, TPP_ERR_UNSUPPORTED,
               "draft logits need a vocabulary of at most 400000 tokens");
   if (need) {
-    const int64_t rows = B * (T + (draft_logits ? T - 1 : 0));
-    const dim3 grid((unsigned)a.slices, (unsigned)rows);
+    const dim3 grid((unsigned)a.slices, (unsigned)(B * (2 * T - 1)));
     auto stats = [&](auto kern) {
       return launch("verify_stats_kernel", kern, grid, dim3(256), 0, as_stream(stream), 0u, a);
     };
@@ -936,8 +982,7 @@ extern "C" int tpp_verify_tree(const void* logits, int64_t l_sb, int64_t l_st,
                                      : stats(verify_stats_kernel<float>);
     if (rc != TPP_OK) return rc;
   }
-  const Shape sh = shape_of(B, V * item);
-  if (dtype == TPP_F16) return walk_as<__half>(a, sh, B, as_stream(stream));
-  if (dtype == TPP_BF16) return walk_as<__nv_bfloat16>(a, sh, B, as_stream(stream));
-  return walk_as<float>(a, sh, B, as_stream(stream));
+  if (dtype == TPP_F16) return walk_as<__half>(a, B, as_stream(stream));
+  if (dtype == TPP_BF16) return walk_as<__nv_bfloat16>(a, B, as_stream(stream));
+  return walk_as<float>(a, B, as_stream(stream));
 }
