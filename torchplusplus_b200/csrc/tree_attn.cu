@@ -10,7 +10,11 @@
 // Split: the tiles of all units form one list, cut into equal parts, one for
 // each CTA, whatever the lengths of the sequences.  A unit that lies within one
 // part is finished there; the pieces of the others go to the workspace as
-// (m, l, o) in fp32 and tree_combine_kernel joins them, in list order.
+// (m, l, o) in fp32 and tree_combine_kernel joins them, in list order.  Where there
+// are units enough and each is short, a CTA takes a unit instead: no pieces, and
+// the next unit's start-up hides under its neighbours' work (32 x 8 nodes over up to
+// 640 keys 25.2 us cut, 19.7 not; 64 x 8 46.0 and 34.6; but 8 x 8 over 2000 keys 21.4
+// and 34.2).
 //
 // Threads 0 and 32 feed a ring of K and V tiles by TMA (one request a tile; an
 // issuing thread spends about 0.2 us on each), on into the next piece; they refill
@@ -39,6 +43,7 @@ namespace {
 constexpr int KT = 64;            // keys of a tile
 constexpr int kThreads = 128;
 constexpr int kMaxNodes = 256;
+constexpr int kTcRows = 128;      // rows of a unit on tcgen05
 constexpr float kRescale = 8.0f;  // log2: the base moves when the maximum grew by 2^8
 
 struct TreeArgs {
@@ -53,7 +58,7 @@ struct TreeArgs {
   float scale_log2;
   int B, T, Hq, Hkv, G, W, R, RT, NT;  // W mask words a row, R = T * G rows, NT tree tiles
   int ctas, rows;                      // parts at most (0: a unit each), rows of a unit
-  int min_tiles;                       // tiles of a part at least
+  int whole_tiles;                     // a CTA takes a unit where none has more tiles
   int o_vec;                           // the output's rows start on 16 bytes
   float* ws;                           // pieces: two a part
   int* err;
@@ -114,7 +119,7 @@ __device__ __forceinline__ Span span_of(const TreeArgs& p, int b) {
 // Units in (b, kv head, row tile) order, each with its cache's tiles, then the
 // tree's.  The first `more` of n parts hold each + 1 tiles, the others `each`.
 struct Parts {
-  int n, each, more;
+  int n, each, more;  // n = 0: a CTA a unit
   __device__ __forceinline__ int start(int c) const { return each * c + min(c, more); }
   __device__ __forceinline__ int of(int x) const {
     const int x1 = more * (each + 1);
@@ -134,23 +139,30 @@ __device__ __forceinline__ int tiles_scan(const TreeArgs& p, int round, int& inc
   }
   return n;
 }
-__device__ __forceinline__ Parts parts_of(const TreeArgs& p, int total) {
+// From all tiles and the longest unit's.
+__device__ __forceinline__ Parts parts_of(const TreeArgs& p, int total, int longest) {
   Parts s;
-  s.n = max(1, min(p.ctas, total / p.min_tiles));
+  s.n = s.each = s.more = 0;
+  if (longest <= p.whole_tiles) return s;
+  s.n = max(1, min(p.ctas, total / 2));
+  // a wide tree's piece is 64 KB of fp32 a part: below 8 tiles a part, one CTA an SM
+  if (p.rows > 32 && total < 8 * p.ctas) s.n = min(s.n, max(p.ctas / 2, 1));
   s.each = total / s.n;
   s.more = total - s.each * s.n;
   return s;
 }
-// All tiles, and those before sequence b.
-__device__ __forceinline__ int tiles_before(const TreeArgs& p, int b, int& total) {
+// All tiles, those before sequence b, and the longest unit's.
+__device__ __forceinline__ int tiles_before(const TreeArgs& p, int b, int& total, int& longest) {
   int before = 0;
-  total = 0;
+  total = longest = 0;
   for (int r = 0; 32 * r < p.B; ++r) {
     int incl;
     const int n = tiles_scan(p, r, incl);
     if (b / 32 == r) before = total + __shfl_sync(0xffffffffu, incl - n, b % 32);
     total += __shfl_sync(0xffffffffu, incl, 31);
+    longest = max(longest, __reduce_max_sync(0xffffffffu, n));
   }
+  longest /= p.Hkv * p.RT;
   return before;
 }
 // Walks the pieces of units in one CTA's part.
@@ -160,21 +172,26 @@ struct Piece {
   Span sp;
   bool whole;
   __device__ __forceinline__ bool start(const TreeArgs& p) {
-    if (p.ctas == 0) {
+    Parts s;
+    s.n = 0;
+    int incl = 0, total = 0, n = 0, longest = 0, rounds = (p.B + 31) / 32;
+    if (p.ctas > 0) {
+      for (int r = 0; r < rounds; ++r) {
+        n = tiles_scan(p, r, incl);
+        total += __shfl_sync(0xffffffffu, incl, 31);
+        longest = max(longest, __reduce_max_sync(0xffffffffu, n));
+      }
+      s = parts_of(p, total, longest / (p.Hkv * p.RT));
+    }
+    if (s.n == 0) {
       const int u = p.Hkv * p.RT;
       b = blockIdx.x / u;
+      if (b >= p.B) return false;
       sp = span_of(p, b);
       before = 0;  // a list of b's own
       pos = (int)(blockIdx.x % u) * (sp.tiles + p.NT);
       end = pos + sp.tiles + p.NT;
     } else {
-      int incl, total = 0, rounds = (p.B + 31) / 32;
-      int n = 0;
-      for (int r = 0; r < rounds; ++r) {
-        n = tiles_scan(p, r, incl);
-        total += __shfl_sync(0xffffffffu, incl, 31);
-      }
-      const Parts s = parts_of(p, total);
       if ((int)blockIdx.x >= s.n) return false;
       pos = s.start(blockIdx.x);
       end = s.start(blockIdx.x + 1);
@@ -613,7 +630,6 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attn_kernel(
 //   warp 5:    S = Q K^T (M 128, N 64), O += P V (P read from TMEM)
 // S and P share two 64-column buffers; S of tile j+1 is computed under the softmax
 // of tile j.  Dead rows of a narrow unit (R < 128) are skipped by whole warps.
-constexpr int kTcRows = 128;
 constexpr int kTcThreads = 192;
 constexpr int kKSt = 3, kVSt = 2;
 
@@ -985,9 +1001,14 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant
   const int row = item % p.R;
   const int kvh = item / p.R % p.Hkv, b = in ? item / p.R / p.Hkv : 0;
   const Span sp = span_of(p, b);
-  int total;
-  const int before = tiles_before(p, b, total);
-  const Parts s = parts_of(p, total);
+  int total, longest;
+  const int before = tiles_before(p, b, total, longest);
+  const Parts s = parts_of(p, total, longest);
+  if (s.n == 0) {
+    pdl_wait();
+    pdl_trigger();
+    return;
+  }
   const int n = sp.tiles + p.NT;
   const int x0 = before + (kvh * p.RT + row / p.rows) * n;
   const int c0 = s.of(x0), c1 = s.of(x0 + n - 1);
@@ -1101,8 +1122,9 @@ int reserve_smem(const void* kern, size_t smem) {
   return TPP_OK;
 }
 
-// How a call is cut: the row groups of a CTA and the parts (0: one a unit).
-struct Plan { int rw, rows, rt, min_tiles, ctas; };  // rw 0: tcgen05
+// How a call is cut: the row groups of a CTA (0: tcgen05), a unit's rows and row
+// tiles, and the parts at most (0: a CTA takes a unit, whatever the lengths).
+struct Plan { int rw, rows, rt, whole_tiles, ctas, grid; };
 Plan plan_of(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t max_ctx,
              int64_t window_left) {
   const int64_t R = T * (Hq / Hkv);
@@ -1112,11 +1134,18 @@ Plan plan_of(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t max_ctx,
   pl.rw = R <= 16 ? 1 : R <= 32 || G > kTcRows ? 2 : 0;
   pl.rows = pl.rw ? 16 * pl.rw : (int)(kTcRows / G * G);
   pl.rt = (int)((R + pl.rows - 1) / pl.rows);
-  pl.min_tiles = pl.rw ? 4 : 8;
   int64_t keys = max_ctx;
   if (window_left >= 0 && window_left + 1 < keys) keys = window_left + KT;
   const int64_t tiles = (keys + KT - 1) / KT + (T + 63) / 64;
-  pl.ctas = tiles <= pl.min_tiles ? 0 : (int)std::min<int64_t>(2 * sm_budget(), B * Hkv * pl.rt * tiles);
+  const int64_t units = B * Hkv * pl.rt, ctas = 2 * sm_budget();
+  // a unit a CTA up to so many tiles (us, whole / cut): 64 units and more, 16 (8 x 5
+  // nodes over 400 keys 12.1 / 12.8; above); fewer of a narrow tree, 5 (4 x 5 over 400
+  // keys, 8 tiles, 12.1 / 10.5); of a wide one, 12 (64 nodes over 500 keys, 9 tiles,
+  // 15.3 / 18.0; over 2000, 33 tiles, 37.0 / 20.5)
+  pl.whole_tiles = units >= 64 ? 16 : pl.rw ? 5 : 12;
+  pl.ctas = tiles <= pl.whole_tiles ? 0 : (int)std::min<int64_t>(ctas, std::max<int64_t>(units * tiles / 2, 1));
+  // (the lengths are on the device: they may turn out short, so each unit has a CTA)
+  pl.grid = (int)std::max<int64_t>(units, pl.ctas);
   return pl;
 }
 
@@ -1185,15 +1214,15 @@ int tree_attention(const TreeCall& c, int dtype, cudaStream_t st) {
   const int rw = pl.rw;
   a.RT = pl.rt; a.ctas = pl.ctas; a.rows = pl.rows;
   a.o_vec = aligned16(c.o) && ((c.o_sb | c.o_st | c.o_sh) & 7) == 0;
-  a.min_tiles = pl.min_tiles;
+  a.whole_tiles = pl.whole_tiles;
   a.ws = static_cast<float*>(c.ws);
   TPP_REQUIRE(pl.ctas == 0 || (c.ws && c.ws_bytes >= workspace_of(pl, c.D) && aligned16(c.ws)),
               TPP_ERR_WORKSPACE, "workspace missing, too small or not 16-byte aligned");
   const int64_t units = c.B * c.Hkv * pl.rt;
-  TPP_REQUIRE(units * (c.max_ctx / KT + a.NT + 1) < (1ll << 31) &&
+  TPP_REQUIRE(units < (1ll << 31) && units * (c.max_ctx / KT + a.NT + 1) < (1ll << 31) &&
                   c.B * c.Hkv * a.R < (1ll << 29) - 8,
               TPP_ERR_SHAPE, "too many rows or tiles");
-  const dim3 grid((unsigned)(pl.ctas ? pl.ctas : units));
+  const dim3 grid((unsigned)pl.grid);
   CUtensorMap tq;
   if (pl.rw == 0) {
     // {64 columns, head, node, column box, batch}
