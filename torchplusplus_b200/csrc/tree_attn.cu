@@ -29,6 +29,7 @@
 // product, since 0 * NaN is NaN.  Values that some rows see and others do not
 // (tree tiles, a window's edge) are cleared too where they are not finite, and
 // added afterwards, element by element, to the rows that see them.
+#include <limits.h>
 #include <math.h>
 #include <algorithm>
 #include <mutex>
@@ -59,7 +60,8 @@ struct TreeArgs {
   int B, T, Hq, Hkv, G, W, R, RT, NT;  // W mask words a row, R = T * G rows, NT tree tiles
   int ctas, rows;                      // parts at most (0: a unit each), rows of a unit
   int whole_tiles;                     // a CTA takes a unit where none has more tiles
-  int o_vec;                           // the output's rows start on 16 bytes
+  int by_unit;                         // few wide units: try cutting each by itself
+  int o_vec;                           // the output's rows start on 32 bytes
   float* ws;                           // pieces: two a part
   int* err;
 };
@@ -67,7 +69,7 @@ struct TreeArgs {
 // fp32 words of a piece: o [rows][D], m [rows], l [rows], whether a value that
 // is not finite was met
 __host__ __device__ constexpr int64_t slot_floats(int rows, int D) {
-  return (int64_t)rows * (D + 2) + 4;
+  return ((int64_t)rows * (D + 2) + 8) / 8 * 8;  // (a slot starts on 32 bytes)
 }
 
 __device__ __forceinline__ uint32_t sw_addr(uint32_t base, int r, int chunk) {
@@ -165,12 +167,38 @@ __device__ __forceinline__ int tiles_before(const TreeArgs& p, int b, int& total
   longest /= p.Hkv * p.RT;
   return before;
 }
+// A part of wide units that straddles two of them pays for two starts and two
+// outputs of 64 KB (4 x 64 nodes over 32768 keys: 31 of 296 CTAs, 9 us after all
+// others).  So where the longest part is then only a few tiles longer, each unit of
+// sequence b is cut by itself, into n_b equal parts.  (Narrow units are not: their
+// pieces are small, and the code cost their kernel more.)
+__device__ __forceinline__ int unit_parts(const Parts& s, int total, int tiles) {
+  return (int)((int64_t)s.n * tiles / total);
+}
+__device__ __forceinline__ bool cut_by_unit(const TreeArgs& p, const Parts& s, int total) {
+  if (!p.by_unit || s.n == 0) return false;
+  int worst = 0;
+  for (int b = threadIdx.x & 31; b < p.B; b += 32) {
+    const int n = span_of(p, b).tiles + p.NT, k = unit_parts(s, total, n);
+    worst = max(worst, k == 0 ? INT_MAX : (n + k - 1) / k);
+  }
+  return __reduce_max_sync(0xffffffffu, worst) <= s.each + 5;
+}
+// Parts of the sequences before b, so cut.
+__device__ __forceinline__ int unit_parts_before(const TreeArgs& p, const Parts& s, int total,
+                                                 int b) {
+  int n = 0;
+  for (int i = threadIdx.x & 31; i < b; i += 32)
+    n += unit_parts(s, total, span_of(p, i).tiles + p.NT) * p.Hkv * p.RT;
+  return __reduce_add_sync(0xffffffffu, n);
+}
 // Walks the pieces of units in one CTA's part.
 struct Piece {
   int pos, end, before;  // in the list; before: tiles of earlier sequences
   int b, unit, t0, t1;   // tiles [t0, t1) of the unit (kv head, row tile) of b
   Span sp;
   bool whole;
+  template <bool WIDE>
   __device__ __forceinline__ bool start(const TreeArgs& p) {
     Parts s;
     s.n = 0;
@@ -191,6 +219,36 @@ struct Piece {
       before = 0;  // a list of b's own
       pos = (int)(blockIdx.x % u) * (sp.tiles + p.NT);
       end = pos + sp.tiles + p.NT;
+    } else if (WIDE && cut_by_unit(p, s, total)) {
+      // one piece, in a list of b's own
+      const int u = p.Hkv * p.RT, lane = threadIdx.x & 31;
+      int base = 0, at = -1, tiles = 0, k = 0;
+      for (int r = 0; r < rounds && at < 0; ++r) {
+        const int i = 32 * r + lane, m = i < p.B ? span_of(p, i).tiles + p.NT : 0;
+        const int parts = unit_parts(s, total, m);
+        int scan = parts * u;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, scan, o);
+          if (lane >= o) scan += up;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, (int)blockIdx.x < base + scan);
+        if (hit) {
+          const int l = __ffs(hit) - 1;
+          b = 32 * r + l;
+          tiles = __shfl_sync(0xffffffffu, m, l);
+          k = __shfl_sync(0xffffffffu, parts, l);
+          at = (int)blockIdx.x - base - __shfl_sync(0xffffffffu, scan - parts * u, l);
+        } else {
+          base += __shfl_sync(0xffffffffu, scan, 31);
+        }
+      }
+      if (at < 0) return false;
+      sp = span_of(p, b);
+      const int un = at / k, part = at - un * k;
+      before = 0;
+      pos = un * tiles + (int)((int64_t)tiles * part / k);
+      end = un * tiles + (int)((int64_t)tiles * (part + 1) / k);
     } else {
       if ((int)blockIdx.x >= s.n) return false;
       pos = s.start(blockIdx.x);
@@ -316,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attn_kernel(
   pdl_trigger();
 
   Piece pc;
-  if (!pc.start(p)) return;
+  if (!pc.start<false>(p)) return;
   bool ok = true;
   int it = 0;  // tiles so far: the ring's position
   // The loads run ahead of pc; their threads keep the place in shared memory.
@@ -631,7 +689,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attn_kernel(
 // S and P share two 64-column buffers; S of tile j+1 is computed under the softmax
 // of tile j.  Dead rows of a narrow unit (R < 128) are skipped by whole warps.
 constexpr int kTcThreads = 192;
-constexpr int kKSt = 3, kVSt = 2;
+constexpr int kKSt = 2, kVSt = 3;
 
 template <int D>
 struct TcSmem {
@@ -646,6 +704,14 @@ __device__ __forceinline__ bool bar_softmax_or(bool x) {
                "barrier.cta.red.or.pred b, 2, 128, a;\n\tselp.u32 %0, 1, 0, b;\n\t}"
                : "=r"(r) : "r"((uint32_t)x) : "memory");
   return r != 0;
+}
+
+// 32 bytes at once: a lane writes its own row, so narrower stores would leave half
+// a sector each (a piece's 64 KB took 5 us).
+__device__ __forceinline__ void store8(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]),
+               "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
 }
 
 template <typename T, int D>
@@ -691,7 +757,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) tree_attn_tc_kernel(
   pdl_wait();
   pdl_trigger();
   Piece pc;
-  if (!pc.start(p)) return;
+  if (!pc.start<true>(p)) return;
   if (warp == 5) tmem_alloc(tmem_slot, 256);
   tc_fence_before();
   __syncthreads();
@@ -946,9 +1012,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) tree_attn_tc_kernel(
           if (!live) {
           } else if (!pc.whole) {
 #pragma unroll
-            for (int k = 0; k < 32; k += 4)
-              *reinterpret_cast<uint4*>(slot + rl * D + c + k) =
-                  make_uint4(r[k], r[k + 1], r[k + 2], r[k + 3]);
+            for (int k = 0; k < 32; k += 8) store8(slot + rl * D + c + k, r + k);
           } else {
             uint32_t w[16];
 #pragma unroll
@@ -956,8 +1020,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) tree_attn_tc_kernel(
               w[k] = pack2<T>(__uint_as_float(r[2 * k]) * inv, __uint_as_float(r[2 * k + 1]) * inv);
             if (p.o_vec) {
 #pragma unroll
-              for (int k = 0; k < 16; k += 4)
-                *reinterpret_cast<uint4*>(dst + c + 2 * k) = make_uint4(w[k], w[k + 1], w[k + 2], w[k + 3]);
+              for (int k = 0; k < 16; k += 8) store8(dst + c + 2 * k, w + k);
             } else {
 #pragma unroll
               for (int k = 0; k < 16; ++k) *reinterpret_cast<uint32_t*>(dst + c + 2 * k) = w[k];
@@ -1010,8 +1073,16 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant
     return;
   }
   const int n = sp.tiles + p.NT;
-  const int x0 = before + (kvh * p.RT + row / p.rows) * n;
-  const int c0 = s.of(x0), c1 = s.of(x0 + n - 1);
+  const int unit = kvh * p.RT + row / p.rows;
+  int c0, c1;
+  if (cut_by_unit(p, s, total)) {
+    const int k = unit_parts(s, total, n);
+    c0 = unit_parts_before(p, s, total, b) + unit * k;
+    c1 = c0 + k - 1;
+  } else {
+    c0 = s.of(before + unit * n);
+    c1 = s.of(before + unit * n + n - 1);
+  }
   pdl_wait();
   pdl_trigger();
   const bool work = in && c0 != c1;
@@ -1213,11 +1284,13 @@ int tree_attention(const TreeCall& c, int dtype, cudaStream_t st) {
   const Plan pl = plan_of(c.B, c.T, c.Hq, c.Hkv, c.max_ctx, c.window_left);
   const int rw = pl.rw;
   a.RT = pl.rt; a.ctas = pl.ctas; a.rows = pl.rows;
-  a.o_vec = aligned16(c.o) && ((c.o_sb | c.o_st | c.o_sh) & 7) == 0;
+  a.o_vec = (reinterpret_cast<uintptr_t>(c.o) & 31) == 0 && ((c.o_sb | c.o_st | c.o_sh) & 15) == 0;
   a.whole_tiles = pl.whole_tiles;
+  a.by_unit = pl.rw == 0 && 4 * c.B * c.Hkv * pl.rt <= pl.ctas;
   a.ws = static_cast<float*>(c.ws);
-  TPP_REQUIRE(pl.ctas == 0 || (c.ws && c.ws_bytes >= workspace_of(pl, c.D) && aligned16(c.ws)),
-              TPP_ERR_WORKSPACE, "workspace missing, too small or not 16-byte aligned");
+  TPP_REQUIRE(pl.ctas == 0 || (c.ws && c.ws_bytes >= workspace_of(pl, c.D) &&
+                                (reinterpret_cast<uintptr_t>(c.ws) & 31) == 0),
+              TPP_ERR_WORKSPACE, "workspace missing, too small or not 32-byte aligned");
   const int64_t units = c.B * c.Hkv * pl.rt;
   TPP_REQUIRE(units < (1ll << 31) && units * (c.max_ctx / KT + a.NT + 1) < (1ll << 31) &&
                   c.B * c.Hkv * a.R < (1ll << 29) - 8,
