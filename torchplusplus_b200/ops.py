@@ -749,7 +749,13 @@ def qk_norm_rope_tree(qkv: torch.Tensor, q_norm_w: torch.Tensor | None,
     if not (cos.is_cuda and sin.is_cuda):
         _cuda(cos, sin)
     qkv = _rows16(qkv)
-    cos, sin, cs_stride, cs_dt = _table(cos, sin, D)
+    cs_dt = N.DTYPE_CODE.get(cos.dtype)
+    if cs_dt is None or cos.shape != sin.shape or cos.dtype is not sin.dtype \
+            or cos.shape[-1] != D or not (cos.is_contiguous() and sin.is_contiguous()) \
+            or cos.dim() != 2:
+        cos, sin, cs_stride, cs_dt = _table(cos, sin, D)
+    else:
+        cs_stride = D
     q_out = _tree_out(q_out, (B, T, Hq, D), qkv)
     k_out = _tree_out(k_out, (B, T, Hkv, D), qkv)
     sb, st, _ = qkv.stride()
