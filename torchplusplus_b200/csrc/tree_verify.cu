@@ -165,11 +165,14 @@ __global__ void __launch_bounds__(256) verify_stats_kernel(VerifyArgs p) {
       ? static_cast<const T*>(p.logits) + (r / p.T) * p.l_sb + (r % p.T) * p.l_st
       : static_cast<const T*>(p.draft) + ((r - nt) / nd) * p.d_sb + ((r - nt) % nd) * p.d_st;
   const Row<T> row(src, p.V);
+  const uint4* at = reinterpret_cast<const uint4*>(row.p - row.mis);
+  const int whole = (p.V + row.mis) / VE;  // groups 1 .. whole - 1 lie within the row
   uint4 raw[U];
 #pragma unroll
   for (int i = 0; i < U; ++i) {
     const int k = blockIdx.x * kSlice + i * 256 + tid;
-    raw[i] = load_group<T>(row.p, k < row.groups ? k * VE - row.mis : p.V, p.V);
+    raw[i] = k > 0 && k < whole ? __ldg(at + k)
+                                : load_edge<T>(row.p, k < row.groups ? k * VE - row.mis : p.V, p.V);
   }
   float m = -INFINITY;
 #pragma unroll
@@ -177,24 +180,30 @@ __global__ void __launch_bounds__(256) verify_stats_kernel(VerifyArgs p) {
     float f[VE];
     unpack_group<T>(raw[i], f);
 #pragma unroll
-    for (int j = 0; j < VE; ++j) m = fmaxf(m, f[j]);
+    for (int j = 0; j < VE; j += 2) m = fmax3(m, f[j], f[j + 1]);
   }
   m = warp_max(m);
   if ((tid & 31) == 0) sm[tid >> 5] = m;
   __syncthreads();
   for (int w = 0; w < 8; ++w) m = fmaxf(m, sm[w]);
-  float s = 0.f;
+  // pairs on the two-lane fp32 pipe; a NaN argument is clamped to a weight of 0
   const float c = p.inv_t * 1.4426950408889634f;
+  const uint64_t m2 = f2_pack(-m, -m), c2 = f2_pack(c, c), zero = f2_pack(0.f, 0.f);
+  uint64_t s2 = zero;
 #pragma unroll
   for (int i = 0; i < U; ++i) {
     float f[VE];
     unpack_group<T>(raw[i], f);
 #pragma unroll
-    for (int j = 0; j < VE; ++j) {
-      const float w = ex2_ftz((f[j] - m) * c);
-      s += w == w ? w : 0.f;
+    for (int j = 0; j < VE; j += 2) {
+      float x, y;
+      f2_unpack(f2_fma(f2_add(f2_pack(f[j], f[j + 1]), m2), c2, zero), x, y);
+      s2 = f2_add(s2, f2_pack(ex2_ftz(fmaxf(x, -200.f)), ex2_ftz(fmaxf(y, -200.f))));
     }
   }
+  float s, s_hi;
+  f2_unpack(s2, s, s_hi);
+  s += s_hi;
   s = warp_sum(s);
   if ((tid & 31) == 0) ss[tid >> 5] = s;
   __syncthreads();
