@@ -267,6 +267,37 @@ def test_attention_shared_mask_lengths_out_of_range_and_missing_blocks():
     assert ((o.double().cpu() - ref).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("T", [3, 40])
+def test_attention_empty_cache_wide_windows_and_shared_operands(T):
+    from torchplusplus_b200 import ops
+    g = torch.Generator().manual_seed(17)
+    B, D = 2, 128
+    q, kc, vc, kt, vt, see = make(g, B, T, 4, 2, D, [100, 60], BF16)
+    # a cache without rows
+    none = [x[:0] for x in kc]
+    ref, tol = attention_oracle(q, none, none, kt, vt, [0, 0], see, -1, D ** -0.5)
+    e = torch.zeros(B, 2, 0, D, dtype=BF16, device="cuda")
+    z = torch.zeros(B, dtype=torch.int32, device="cuda")
+    o = ops.attention_tree(q.cuda(), e, e, kt.cuda(), vt.cuda(), z, 0, pack(see).cuda())
+    assert ((o.double().cpu() - ref).abs() <= tol).all()
+    # windows that reach past every row
+    k, v = contiguous_cache(kc, 100), contiguous_cache(vc, 100)
+    lens = torch.tensor([100, 60], dtype=torch.int32, device="cuda")
+    call = lambda **kw: ops.attention_tree(q.cuda(), k, v, kt.cuda(), vt.cuda(), lens, 100,
+                                           pack(see).cuda(), **kw)
+    full = call()
+    for w in (100 + T, 2 ** 31, 2 ** 63 - 1):
+        assert torch.equal(call(window_left=w), full)
+    # every sequence the same tree: q, k and v expanded over the batch
+    one = [x[:1].cuda() for x in (q, kt, vt)]
+    a = ops.attention_tree(one[0].expand(B, T, 4, D), k, v, one[1].expand(B, T, 2, D),
+                           one[2].expand(B, T, 2, D), lens, 100, pack(see)[0].cuda())
+    b = ops.attention_tree(*(x.repeat(B, 1, 1, 1) if i in (0, 3, 4) else x for i, x in
+                             enumerate((one[0], k, v, one[1], one[2]))), lens, 100,
+                           pack(see)[:1].repeat(B, 1, 1).cuda())
+    assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("T", [4, 40])
 def test_attention_offsets_past_32_bits(T):
     """A cache of more than 2^31 elements a sequence, read at its end."""
@@ -584,6 +615,17 @@ def test_verify_does_not_depend_on_the_batch():
         one = ops.verify_tree(*(x[b:b + 1].clone() for x in (logits, tokens, par, u)), 1.0,
                               d[b:b + 1, :6].clone())
         assert all(torch.equal(x[b:b + 1], y) for x, y in zip(all_, one))
+
+
+def test_verify_uniforms_outside_the_unit_interval_are_its_ends():
+    from torchplusplus_b200 import ops
+    lg = torch.randn(4, 1, 3000, device="cuda")
+    lg[:, :, :5] = -math.inf
+    tok = torch.zeros(4, 1, dtype=torch.int64, device="cuda")
+    par = torch.full((1,), -1, dtype=torch.int32, device="cuda")
+    u = torch.tensor([[-1.0], [0.0], [1.0], [7.0]], device="cuda")
+    nxt = ops.verify_tree(lg, tok, par, u)[2].tolist()
+    assert nxt[0] == 5 and nxt[1] == 5 and nxt[2] == 2999 and nxt[3] == 2999
 
 
 def test_verify_refusals():

@@ -32,9 +32,7 @@
 #include <limits.h>
 #include <math.h>
 #include <algorithm>
-#include <mutex>
-#include <set>
-#include <utility>
+#include <atomic>
 #include "mma_common.cuh"
 #include "tc_common.cuh"
 
@@ -1176,20 +1174,20 @@ struct TreeCall {
   void* ws; int64_t ws_bytes;
 };
 
-// cudaFuncSetAttribute once a kernel and device (0.5 us a call otherwise).
-int reserve_smem(const void* kern, size_t smem) {
-  static std::mutex lock;
-  static std::set<std::pair<const void*, int>> done;
+// cudaFuncSetAttribute once a kernel (`id` of 12) and device: 0.5 us a call
+// otherwise.  (Two threads may both make it the first time.)
+int reserve_smem(const void* kern, int id, size_t smem) {
+  static std::atomic<bool> done[64][12];
   int dev = 0;
   cudaGetDevice(&dev);
-  std::lock_guard<std::mutex> hold(lock);
-  if (done.count({kern, dev})) return TPP_OK;
+  std::atomic<bool>* d = dev >= 0 && dev < 64 ? &done[dev][id] : nullptr;
+  if (d && d->load(std::memory_order_acquire)) return TPP_OK;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
       cudaSuccess) {
     set_error("tree attention: cannot reserve shared memory");
     return TPP_ERR_LAUNCH;
   }
-  done.insert({kern, dev});
+  if (d) d->store(true, std::memory_order_release);
   return TPP_OK;
 }
 
@@ -1236,8 +1234,15 @@ int64_t workspace_of(const Plan& pl, int64_t D) {
   return pl.ctas ? 2 * pl.ctas * slot_floats(pl.rows, (int)D) * 4 : 0;
 }
 
-int tree_attention(const TreeCall& c, int dtype, cudaStream_t st) {
+int tree_attention(TreeCall c, int dtype, cudaStream_t st) {
   if (c.B == 0 || c.T == 0) return TPP_OK;
+  if (c.max_ctx == 0 && !c.table) {  // no rows are read: an empty cache has no address
+    c.k = c.kt;
+    c.v = c.vt;
+    c.c_sb = c.c_sh = c.c_ss = c.D;
+  }
+  // a window that reaches past every row is none (and cannot overflow below)
+  if (c.window_left >= c.max_ctx + c.T) c.window_left = -1;
   TPP_REQUIRE(c.q && c.k && c.v && c.kt && c.vt && c.ctx_lens && c.mask && c.o, TPP_ERR_SHAPE,
               "null pointer");
   TPP_REQUIRE(c.B > 0 && c.B <= 65535 && c.T > 0 && c.T <= kMaxNodes && c.Hq > 0 && c.Hkv > 0 &&
@@ -1306,25 +1311,26 @@ int tree_attention(const TreeCall& c, int dtype, cudaStream_t st) {
     rc = make_tmap(&tq, c.q, dtype, 5, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != TPP_OK) return rc;
   }
-  auto go_tc = [&](auto kern, size_t smem) -> int {
-    if (const int e = reserve_smem(reinterpret_cast<const void*>(kern), smem)) return e;
+  auto go_tc = [&](auto kern, int id, size_t smem) -> int {
+    if (const int e = reserve_smem(reinterpret_cast<const void*>(kern), id, smem)) return e;
     return launch("tree_attn_tc_kernel", kern, grid, dim3(kTcThreads), smem, st, 0u, tk, tv, tkt,
                   tvt, tq, a);
   };
-  auto go = [&](auto kern, size_t smem) -> int {
-    if (const int e = reserve_smem(reinterpret_cast<const void*>(kern), smem)) return e;
+  auto go = [&](auto kern, int id, size_t smem) -> int {
+    if (const int e = reserve_smem(reinterpret_cast<const void*>(kern), id, smem)) return e;
     return launch("tree_attn_kernel", kern, grid, dim3(kThreads), smem, st, 0u, tk, tv, tkt, tvt,
                   a);
   };
   rc = TPP_DISPATCH_HALF(dtype, T, [&]() -> int {
+    const int id = 6 * IsBf16<T>::value;
     if (c.D == 64) {
-      if (rw == 1) return go(tree_attn_kernel<T, 64, 1>, TreeSmem<64, 1>::kBytes);
-      if (rw == 2) return go(tree_attn_kernel<T, 64, 2>, TreeSmem<64, 2>::kBytes);
-      return go_tc(tree_attn_tc_kernel<T, 64>, TcSmem<64>::kBytes);
+      if (rw == 1) return go(tree_attn_kernel<T, 64, 1>, id, TreeSmem<64, 1>::kBytes);
+      if (rw == 2) return go(tree_attn_kernel<T, 64, 2>, id + 1, TreeSmem<64, 2>::kBytes);
+      return go_tc(tree_attn_tc_kernel<T, 64>, id + 2, TcSmem<64>::kBytes);
     }
-    if (rw == 1) return go(tree_attn_kernel<T, 128, 1>, TreeSmem<128, 1>::kBytes);
-    if (rw == 2) return go(tree_attn_kernel<T, 128, 2>, TreeSmem<128, 2>::kBytes);
-    return go_tc(tree_attn_tc_kernel<T, 128>, TcSmem<128>::kBytes);
+    if (rw == 1) return go(tree_attn_kernel<T, 128, 1>, id + 3, TreeSmem<128, 1>::kBytes);
+    if (rw == 2) return go(tree_attn_kernel<T, 128, 2>, id + 4, TreeSmem<128, 2>::kBytes);
+    return go_tc(tree_attn_tc_kernel<T, 128>, id + 5, TcSmem<128>::kBytes);
   });
   if (rc != TPP_OK || pl.ctas == 0) return rc;
   const int wpr = pl.ctas >= 4 * units ? 4 : 1;  // four pieces a unit and more

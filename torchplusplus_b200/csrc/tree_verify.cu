@@ -848,7 +848,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) verify_tree_kernel(VerifyArgs p
         if (e == me) mine -= w;
       }
       if (all > 0) {
-        ull at = (ull)((double)sm.u[0] * (double)all);
+        ull at = (ull)(fmax((double)sm.u[0], 0.0) * (double)all);  // (u outside [0, 1): its ends)
         if (at >= all) at = all - 1;
         owner = false;
         if (at >= before && at < before + mine) {  // in this warp's part

@@ -704,13 +704,13 @@ def _half_alike(what: str, x: torch.Tensor, *ts: torch.Tensor | None) -> int:
 
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """t itself if its last dim is contiguous and every row starts on 16 bytes,
-    a contiguous copy otherwise."""
+    """t itself if its last dim is contiguous, every row starts on 16 bytes and no
+    rows share memory, a contiguous copy otherwise."""
     if not t.data_ptr() & 15:
         if t.is_contiguous() and not t.shape[-1] & 7:
             return t
         *lead, last = t.stride()
-        if last == 1 and not any(s & 7 for s in lead):
+        if last == 1 and not any(s & 7 or s == 0 for s in lead):
             return t
     return t.clone(memory_format=torch.contiguous_format)
 
