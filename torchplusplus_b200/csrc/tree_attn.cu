@@ -1194,7 +1194,7 @@ int reserve_smem(const void* kern, int id, size_t smem) {
 // How a call is cut: the row groups of a CTA (0: tcgen05), a unit's rows and row
 // tiles, and the parts at most (0: a CTA takes a unit, whatever the lengths).
 struct Plan { int rw, rows, rt, whole_tiles, ctas, grid; };
-Plan plan_of(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t max_ctx,
+Plan plan_of(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t max_ctx, int64_t D,
              int64_t window_left) {
   const int64_t R = T * (Hq / Hkv);
   Plan pl;
@@ -1207,11 +1207,20 @@ Plan plan_of(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t max_ctx,
   if (window_left >= 0 && window_left + 1 < keys) keys = window_left + KT;
   const int64_t tiles = (keys + KT - 1) / KT + (T + 63) / 64;
   const int64_t units = B * Hkv * pl.rt, ctas = 2 * sm_budget();
-  // a unit a CTA up to so many tiles (us, whole / cut): 64 units and more, 16 (8 x 5
-  // nodes over 400 keys 12.1 / 12.8; above); fewer of a narrow tree, 5 (4 x 5 over 400
-  // keys, 8 tiles, 12.1 / 10.5); of a wide one, 12 (64 nodes over 500 keys, 9 tiles,
-  // 15.3 / 18.0; over 2000, 33 tiles, 37.0 / 20.5)
-  pl.whole_tiles = units >= 64 ? 16 : pl.rw ? 5 : 12;
+  // A unit a CTA up to so many tiles (us, whole / cut).  Few units: a narrow tree's 5
+  // (4 x 5 nodes over 400 keys, 8 tiles, 12.1 / 10.5), a wide one's 12 (64 nodes over
+  // 500 keys, 9 tiles, 15.3 / 18.0; over 2000, 33 tiles, 37.0 / 20.5); 64 units, 16 (8 x
+  // 5 over 400 keys 12.1 / 12.8; 16 x 8 over 2000 36.6 / 30.5).  Narrow units that fill
+  // most of the slots, 32 (32 x 8 over 2000 keys 43.5 / 46.5; 64 x 4 over 4096 140 /
+  // 126).  Wide ones, whose pieces cost more, 100 (32 x 32 over 4000 81 / 90; 64 x 13
+  // over 4096 146 / 153), but 40 where the last wave of CTAs is nearly empty (48 x 32
+  // over 5000 159 / 143; 40 x 32 over 1500 55 / 63) or the keys are narrow (64 x 32 over
+  // 6000 keys of 64 dims 156 / 142).
+  const bool last_full = units <= ctas || units >= 3 * ctas || units % ctas * 10 >= 7 * ctas;
+  if (units < 64) pl.whole_tiles = pl.rw ? 5 : 12;
+  else if (2 * units < ctas) pl.whole_tiles = 16;
+  else if (pl.rw) pl.whole_tiles = 10 * units >= 8 * ctas ? 32 : 16;
+  else pl.whole_tiles = last_full && D == 128 ? 100 : 40;
   pl.ctas = tiles <= pl.whole_tiles ? 0 : (int)std::min<int64_t>(ctas, std::max<int64_t>(units * tiles / 2, 1));
   // (the lengths are on the device: they may turn out short, so each unit has a CTA)
   pl.grid = (int)std::max<int64_t>(units, pl.ctas);
@@ -1286,7 +1295,7 @@ int tree_attention(TreeCall c, int dtype, cudaStream_t st) {
   a.B = (int)c.B; a.T = (int)c.T; a.Hq = (int)c.Hq; a.Hkv = (int)c.Hkv;
   a.G = (int)(c.Hq / c.Hkv); a.W = (a.T + 63) / 64; a.R = a.T * a.G; a.NT = a.W;
   a.err = device_error_flag();
-  const Plan pl = plan_of(c.B, c.T, c.Hq, c.Hkv, c.max_ctx, c.window_left);
+  const Plan pl = plan_of(c.B, c.T, c.Hq, c.Hkv, c.max_ctx, c.D, c.window_left);
   const int rw = pl.rw;
   a.RT = pl.rt; a.ctas = pl.ctas; a.rows = pl.rows;
   a.o_vec = (reinterpret_cast<uintptr_t>(c.o) & 31) == 0 && ((c.o_sb | c.o_st | c.o_sh) & 15) == 0;
@@ -1351,7 +1360,7 @@ extern "C" int64_t tpp_attention_tree_workspace(int64_t B, int64_t T, int64_t Hq
                                                 int64_t max_ctx, int64_t D,
                                                 int64_t window_left) {
   if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || max_ctx < 0) return 0;
-  return workspace_of(plan_of(B, T, Hq, Hkv, max_ctx, window_left), D);
+  return workspace_of(plan_of(B, T, Hq, Hkv, max_ctx, D, window_left), D);
 }
 
 extern "C" int tpp_attention_tree(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
