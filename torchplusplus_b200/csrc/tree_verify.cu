@@ -20,8 +20,8 @@
 // CTA or the cluster, 1.0 us.
 //
 // Bound by latency: one chain of 5 nodes over 151936 tokens with its draft takes
-// 28.0 us (first form 123), of which statistics 5, set-up 3, tests 3, exact sums 6,
-// residual 8, draw 4; 32 trees of 32 nodes 32 us (49).  Code fetched once a walk
+// 26.6 us (first form 123), of which statistics 5, set-up 3, tests 3, exact sums 6,
+// residual 7, draw 3; 32 trees of 32 nodes 32 us (49).  Code fetched once a walk
 // counts: unrolling the second passes' loops over a lane's groups cost 8 us.
 #include <limits.h>
 #include <math.h>
@@ -77,23 +77,26 @@ __device__ __forceinline__ void unpack_group<float>(const uint4& w, float* f) {
 
 // Elements [e0, e0 + VE) of a row of V as they are stored, -inf outside it, one by
 // one: a row's ends, and a draft row whose start is aligned otherwise than the
-// target's.
+// target's.  (All loads first: one after the other they held up the CTAs at a row's
+// ends by some 3 us a pass.)
 template <typename T>
 __device__ __noinline__ uint4 load_edge(const T* row, int e0, int V) {
   constexpr int VE = 16 / sizeof(T);
-  ull w[2] = {0, 0};
-#pragma unroll 1
-  for (int j = 0; j < VE; ++j) {
-    const T x = e0 + j >= 0 && e0 + j < V ? row[e0 + j] : from_f32<T>(-INFINITY);
-    ull bits;
-    if constexpr (sizeof(T) == 4) bits = __float_as_uint(x);
-    else bits = *reinterpret_cast<const unsigned short*>(&x);
-    bits <<= (j * sizeof(T) * 8) & 63;
-    if (j < VE / 2) w[0] |= bits;
-    else w[1] |= bits;
+  T x[VE];
+#pragma unroll
+  for (int j = 0; j < VE; ++j)
+    x[j] = e0 + j >= 0 && e0 + j < V ? row[e0 + j] : from_f32<T>(-INFINITY);
+  uint32_t w[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if constexpr (sizeof(T) == 4) {
+      w[q] = __float_as_uint(x[q]);
+    } else {
+      w[q] = (uint32_t)*reinterpret_cast<const unsigned short*>(&x[2 * q]) |
+             (uint32_t)*reinterpret_cast<const unsigned short*>(&x[2 * q + 1]) << 16;
+    }
   }
-  return make_uint4((uint32_t)w[0], (uint32_t)(w[0] >> 32), (uint32_t)w[1],
-                    (uint32_t)(w[1] >> 32));
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 template <typename T>
 __device__ __forceinline__ uint4 load_group(const T* row, int e0, int V) {
