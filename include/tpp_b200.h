@@ -395,7 +395,8 @@ int tpp_decode_advance(const int64_t* next_tokens, int64_t* out_ids, int64_t ld_
  * yet), parents[i] < i, and node i stands at position ctx_lens[b] + its depth.
  * The nodes' K and V stay beside the cache, [B, T, Hkv, D]; once the target has
  * verified the tree the accepted path's rows are copied into the cache.  The
- * reference has no counterpart (its speculative decoding is a stub). */
+ * reference accepts and rejects a draft chain in Python, without a KV cache
+ * (torchpp/llmops/spec_decoding.py:62). */
 
 /* Per-head q/k RMSNorm (qn_w / kn_w [D], either may be NULL) and rotate-half
  * RoPE at positions[b, t] of the raw projection rows qkv [B, T, (Hq+2Hkv)*D]
@@ -410,7 +411,8 @@ int tpp_qk_norm_rope_tree(const void* qkv, int64_t qkv_sb, int64_t qkv_st, const
                           int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int dtype,
                           void* stream);
 
-/* Bytes of workspace tpp_attention_tree(_paged) needs (0: none). */
+/* Bytes of workspace (32-byte aligned) tpp_attention_tree(_paged) needs (0:
+ * none). */
 int64_t tpp_attention_tree_workspace(int64_t B, int64_t T, int64_t Hq, int64_t Hkv,
                                      int64_t max_ctx, int64_t D, int64_t window_left);
 
@@ -477,7 +479,8 @@ int tpp_verify_tree(const void* logits, int64_t l_sb, int64_t l_st, const void* 
                     double temperature, int32_t* path, int32_t* count, int64_t* next_token,
                     int64_t B, int64_t T, int64_t V, void* workspace, int64_t workspace_bytes,
                     int dtype, void* stream);
-/* Bytes of workspace that needs (0: none), with_draft 1 if draft logits are given. */
+/* Bytes of workspace (8-byte aligned) that needs (0: none); with_draft: 1 if
+ * draft logits are given. */
 int64_t tpp_verify_tree_workspace(int64_t B, int64_t T, int64_t V, int with_draft,
                                   double temperature, int dtype);
 

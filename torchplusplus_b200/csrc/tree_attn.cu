@@ -422,260 +422,260 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attn_kernel(
   const int rw = warp / KW, kw = warp % KW;
   const int kr0 = kw * KPW;
   do {
-  const int b = pc.b, kvh = pc.unit / p.RT, rt = pc.unit % p.RT;
-  const Span& sp = pc.sp;
-  int node[2], head[2];
-  bool live[2];
-  const uint64_t* mrow[2];
-  int64_t lo[2];
-#pragma unroll
-  for (int hr = 0; hr < 2; ++hr) {
-    const int r = rt * 16 * RW + rw * 16 + g + 8 * hr;
-    live[hr] = r < p.R;
-    node[hr] = live[hr] ? r / p.G : 0;
-    head[hr] = kvh * p.G + (live[hr] ? r % p.G : 0);
-    mrow[hr] = p.mask + b * p.mask_sb + (int64_t)node[hr] * p.W;
-    lo[hr] = low_of(p, sp, mrow[hr]);
-  }
-  // Q fragments straight from global memory: each value is used by one lane only
-  uint32_t qf[D / 16][4];
-#pragma unroll
-  for (int hr = 0; hr < 2; ++hr) {
-    const uint32_t* src = reinterpret_cast<const uint32_t*>(
-        static_cast<const T*>(p.q) + b * p.q_sb + node[hr] * p.q_st + head[hr] * p.q_sh);
-#pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) {
-      qf[ks][hr] = live[hr] ? src[ks * 8 + c] : 0u;
-      qf[ks][hr + 2] = live[hr] ? src[ks * 8 + c + 4] : 0u;
-    }
-  }
-  float o[D / 8][4];
-#pragma unroll
-  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  float m_r[2] = {-INFINITY, -INFINITY}, l_r[2] = {0.f, 0.f};
-  uint32_t bad = 0;
-
-  for (int i = pc.t0; i < pc.t1; ++i, ++it) {
-    const int s = it % ST;
-    if (loader && it > 0 && ok && issued >= 0) {
-      ok = mbar_wait(&empty[(it - 1) % ST], ((it - 1) / ST) & 1, p.err, 61);
-      if (ok) issue();
-    }
-    if (ok) ok = mbar_wait(&full[s], (it / ST) & 1, p.err, 62);
-    const uint32_t kb = smem_u32(smem + s * 2 * SM::kTile), vb = kb + SM::kTile;
-    float sc[NTL][4];
-#pragma unroll
-    for (int j = 0; j < NTL; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) {
-#pragma unroll
-      for (int jp = 0; jp < NTL / 2; ++jp) {
-        uint32_t bf[4];
-        ldsm_x4(sw_addr(kb, kr0 + jp * 16 + (lane & 7) + (lane >> 4) * 8,
-                        ks * 2 + ((lane >> 3) & 1)), bf);
-        mma<T>(sc[2 * jp], qf[ks], bf[0], bf[1]);
-        mma<T>(sc[2 * jp + 1], qf[ks], bf[2], bf[3]);
-      }
-    }
-    const bool tree = i >= sp.tiles;
-    const int64_t key0 = (int64_t)(sp.first + i) * KT;   // of a cache tile
-    const bool careful = tree || key0 + KT > sp.ctx || key0 < sp.lo_some;
-    if (tree) {
-      const int n0 = (i - sp.tiles) * KT, n = p.T - n0;
-      const uint64_t in = n < 64 ? (1ull << n) - 1 : ~0ull;
-      const uint64_t w0 = mrow[0][i - sp.tiles] & in, w1 = mrow[1][i - sp.tiles] & in;
-#pragma unroll
-      for (int j = 0; j < NTL; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int k = kr0 + j * 8 + 2 * c + (e & 1);
-          sc[j][e] = (((e < 2 ? w0 : w1) >> k) & 1) ? sc[j][e] * p.scale_log2 : -INFINITY;
-        }
-    } else if (careful) {
-#pragma unroll
-      for (int j = 0; j < NTL; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int64_t k = key0 + kr0 + j * 8 + 2 * c + (e & 1);
-          sc[j][e] = (k < sp.ctx && k >= lo[e >> 1]) ? sc[j][e] * p.scale_log2 : -INFINITY;
-        }
-    } else {
-#pragma unroll
-      for (int j = 0; j < NTL; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sc[j][e] *= p.scale_log2;
-    }
-    // Online softmax with a lazy base: m_r moves, and o and l are rescaled,
-    // only when a row's maximum grew by more than 2^8.
-    float corr[2];
-    bool grow = false;
+    const int b = pc.b, kvh = pc.unit / p.RT, rt = pc.unit % p.RT;
+    const Span& sp = pc.sp;
+    int node[2], head[2];
+    bool live[2];
+    const uint64_t* mrow[2];
+    int64_t lo[2];
 #pragma unroll
     for (int hr = 0; hr < 2; ++hr) {
-      float mx = -INFINITY;
+      const int r = rt * 16 * RW + rw * 16 + g + 8 * hr;
+      live[hr] = r < p.R;
+      node[hr] = live[hr] ? r / p.G : 0;
+      head[hr] = kvh * p.G + (live[hr] ? r % p.G : 0);
+      mrow[hr] = p.mask + b * p.mask_sb + (int64_t)node[hr] * p.W;
+      lo[hr] = low_of(p, sp, mrow[hr]);
+    }
+    // Q fragments straight from global memory: each value is used by one lane only
+    uint32_t qf[D / 16][4];
 #pragma unroll
-      for (int j = 0; j < NTL; ++j) mx = fmax3(mx, sc[j][2 * hr], sc[j][2 * hr + 1]);
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      corr[hr] = 1.f;
-      if (mx > m_r[hr] + kRescale) {
-        corr[hr] = ex2_ftz(m_r[hr] - mx);  // 0 when no key was seen yet
-        m_r[hr] = mx;
-        grow = true;
+    for (int hr = 0; hr < 2; ++hr) {
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(
+          static_cast<const T*>(p.q) + b * p.q_sb + node[hr] * p.q_st + head[hr] * p.q_sh);
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        qf[ks][hr] = live[hr] ? src[ks * 8 + c] : 0u;
+        qf[ks][hr + 2] = live[hr] ? src[ks * 8 + c + 4] : 0u;
       }
-      const float base = m_r[hr] == -INFINITY ? 0.f : m_r[hr];
-      float sum = 0.f;
+    }
+    float o[D / 8][4];
 #pragma unroll
-      for (int j = 0; j < NTL; ++j)
+    for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m_r[2] = {-INFINITY, -INFINITY}, l_r[2] = {0.f, 0.f};
+    uint32_t bad = 0;
+
+    for (int i = pc.t0; i < pc.t1; ++i, ++it) {
+      const int s = it % ST;
+      if (loader && it > 0 && ok && issued >= 0) {
+        ok = mbar_wait(&empty[(it - 1) % ST], ((it - 1) / ST) & 1, p.err, 61);
+        if (ok) issue();
+      }
+      if (ok) ok = mbar_wait(&full[s], (it / ST) & 1, p.err, 62);
+      const uint32_t kb = smem_u32(smem + s * 2 * SM::kTile), vb = kb + SM::kTile;
+      float sc[NTL][4];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float pv = ex2_ftz(sc[j][2 * hr + e] - base);
-          sc[j][2 * hr + e] = pv;
-          sum += pv;
+      for (int j = 0; j < NTL; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+#pragma unroll
+        for (int jp = 0; jp < NTL / 2; ++jp) {
+          uint32_t bf[4];
+          ldsm_x4(sw_addr(kb, kr0 + jp * 16 + (lane & 7) + (lane >> 4) * 8,
+                          ks * 2 + ((lane >> 3) & 1)), bf);
+          mma<T>(sc[2 * jp], qf[ks], bf[0], bf[1]);
+          mma<T>(sc[2 * jp + 1], qf[ks], bf[2], bf[3]);
         }
-      l_r[hr] = l_r[hr] * corr[hr] + sum;
-    }
-    if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-      for (int d = 0; d < D / 8; ++d) {
-        o[d][0] *= corr[0]; o[d][1] *= corr[0];
-        o[d][2] *= corr[1]; o[d][3] *= corr[1];
       }
-    }
+      const bool tree = i >= sp.tiles;
+      const int64_t key0 = (int64_t)(sp.first + i) * KT;   // of a cache tile
+      const bool careful = tree || key0 + KT > sp.ctx || key0 < sp.lo_some;
+      if (tree) {
+        const int n0 = (i - sp.tiles) * KT, n = p.T - n0;
+        const uint64_t in = n < 64 ? (1ull << n) - 1 : ~0ull;
+        const uint64_t w0 = mrow[0][i - sp.tiles] & in, w1 = mrow[1][i - sp.tiles] & in;
 #pragma unroll
-    for (int kk = 0; kk < KPW / 16; ++kk) {
-      // the probabilities are rounded to T for the product: the same relative
-      // error as the values themselves carry
-      uint32_t pa[4];
-      pa[0] = pack2<T>(sc[2 * kk][0], sc[2 * kk][1]);
-      pa[1] = pack2<T>(sc[2 * kk][2], sc[2 * kk][3]);
-      pa[2] = pack2<T>(sc[2 * kk + 1][0], sc[2 * kk + 1][1]);
-      pa[3] = pack2<T>(sc[2 * kk + 1][2], sc[2 * kk + 1][3]);
-      uint32_t keep0 = ~0u, keep1 = ~0u;  // values no row sees: stale rows of a cache
-      if (careful && !tree) {
-        const int64_t k = key0 + kr0 + kk * 16 + 2 * c;
-        auto in = [&](int64_t x) { return x < sp.ctx && x >= sp.lo_all; };
-        keep0 = (in(k) ? 0xffffu : 0u) | (in(k + 1) ? 0xffff0000u : 0u);
-        keep1 = (in(k + 8) ? 0xffffu : 0u) | (in(k + 9) ? 0xffff0000u : 0u);
+        for (int j = 0; j < NTL; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int k = kr0 + j * 8 + 2 * c + (e & 1);
+            sc[j][e] = (((e < 2 ? w0 : w1) >> k) & 1) ? sc[j][e] * p.scale_log2 : -INFINITY;
+          }
+      } else if (careful) {
+#pragma unroll
+        for (int j = 0; j < NTL; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int64_t k = key0 + kr0 + j * 8 + 2 * c + (e & 1);
+            sc[j][e] = (k < sp.ctx && k >= lo[e >> 1]) ? sc[j][e] * p.scale_log2 : -INFINITY;
+          }
+      } else {
+#pragma unroll
+        for (int j = 0; j < NTL; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[j][e] *= p.scale_log2;
       }
-#pragma unroll
-      for (int dp = 0; dp < D / 16; ++dp) {
-        uint32_t bf[4];
-        ldsm_x4_t(sw_addr(vb, kr0 + kk * 16 + (lane & 7) + ((lane >> 3) & 1) * 8,
-                          dp * 2 + (lane >> 4)), bf);
-        if (careful) {
-          bf[0] = finite2<T>(bf[0] & keep0, bad);
-          bf[1] = finite2<T>(bf[1] & keep1, bad);
-          bf[2] = finite2<T>(bf[2] & keep0, bad);
-          bf[3] = finite2<T>(bf[3] & keep1, bad);
-        }
-        mma<T>(o[2 * dp], pa, bf[0], bf[1]);
-        mma<T>(o[2 * dp + 1], pa, bf[2], bf[3]);
-      }
-    }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&empty[s]);
-  }
-  // ---------------- merge the key groups ----------------
-#pragma unroll
-  for (int hr = 0; hr < 2; ++hr) {
-    l_r[hr] += __shfl_xor_sync(0xffffffffu, l_r[hr], 1);
-    l_r[hr] += __shfl_xor_sync(0xffffffffu, l_r[hr], 2);
-  }
-  if (KW > 1) {
-    if (c == 0) {
+      // Online softmax with a lazy base: m_r moves, and o and l are rescaled,
+      // only when a row's maximum grew by more than 2^8.
+      float corr[2];
+      bool grow = false;
 #pragma unroll
       for (int hr = 0; hr < 2; ++hr) {
-        ml[(warp * 16 + g + 8 * hr) * 2] = m_r[hr];
-        ml[(warp * 16 + g + 8 * hr) * 2 + 1] = l_r[hr];
+        float mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < NTL; ++j) mx = fmax3(mx, sc[j][2 * hr], sc[j][2 * hr + 1]);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        corr[hr] = 1.f;
+        if (mx > m_r[hr] + kRescale) {
+          corr[hr] = ex2_ftz(m_r[hr] - mx);  // 0 when no key was seen yet
+          m_r[hr] = mx;
+          grow = true;
+        }
+        const float base = m_r[hr] == -INFINITY ? 0.f : m_r[hr];
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < NTL; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float pv = ex2_ftz(sc[j][2 * hr + e] - base);
+            sc[j][2 * hr + e] = pv;
+            sum += pv;
+          }
+        l_r[hr] = l_r[hr] * corr[hr] + sum;
       }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int d = 0; d < D / 8; ++d) {
+          o[d][0] *= corr[0]; o[d][1] *= corr[0];
+          o[d][2] *= corr[1]; o[d][3] *= corr[1];
+        }
+      }
+#pragma unroll
+      for (int kk = 0; kk < KPW / 16; ++kk) {
+        // the probabilities are rounded to T for the product: the same relative
+        // error as the values themselves carry
+        uint32_t pa[4];
+        pa[0] = pack2<T>(sc[2 * kk][0], sc[2 * kk][1]);
+        pa[1] = pack2<T>(sc[2 * kk][2], sc[2 * kk][3]);
+        pa[2] = pack2<T>(sc[2 * kk + 1][0], sc[2 * kk + 1][1]);
+        pa[3] = pack2<T>(sc[2 * kk + 1][2], sc[2 * kk + 1][3]);
+        uint32_t keep0 = ~0u, keep1 = ~0u;  // values no row sees: stale rows of a cache
+        if (careful && !tree) {
+          const int64_t k = key0 + kr0 + kk * 16 + 2 * c;
+          auto in = [&](int64_t x) { return x < sp.ctx && x >= sp.lo_all; };
+          keep0 = (in(k) ? 0xffffu : 0u) | (in(k + 1) ? 0xffff0000u : 0u);
+          keep1 = (in(k + 8) ? 0xffffu : 0u) | (in(k + 9) ? 0xffff0000u : 0u);
+        }
+#pragma unroll
+        for (int dp = 0; dp < D / 16; ++dp) {
+          uint32_t bf[4];
+          ldsm_x4_t(sw_addr(vb, kr0 + kk * 16 + (lane & 7) + ((lane >> 3) & 1) * 8,
+                            dp * 2 + (lane >> 4)), bf);
+          if (careful) {
+            bf[0] = finite2<T>(bf[0] & keep0, bad);
+            bf[1] = finite2<T>(bf[1] & keep1, bad);
+            bf[2] = finite2<T>(bf[2] & keep0, bad);
+            bf[3] = finite2<T>(bf[3] & keep1, bad);
+          }
+          mma<T>(o[2 * dp], pa, bf[0], bf[1]);
+          mma<T>(o[2 * dp + 1], pa, bf[2], bf[3]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[s]);
     }
-    bar_compute();
+    // ---------------- merge the key groups ----------------
 #pragma unroll
     for (int hr = 0; hr < 2; ++hr) {
-      float M = -INFINITY, L = 0.f;
-#pragma unroll
-      for (int w = 0; w < KW; ++w) M = fmaxf(M, ml[((rw * KW + w) * 16 + g + 8 * hr) * 2]);
-      const float base = M == -INFINITY ? 0.f : M;
-#pragma unroll
-      for (int w = 0; w < KW; ++w) {
-        const float* x = ml + ((rw * KW + w) * 16 + g + 8 * hr) * 2;
-        L += x[1] * ex2_ftz(x[0] - base);
-      }
-      const float f = ex2_ftz(m_r[hr] - base);
-#pragma unroll
-      for (int d = 0; d < D / 8; ++d) {
-        o[d][2 * hr] *= f;
-        o[d][2 * hr + 1] *= f;
-      }
-      m_r[hr] = M;
-      l_r[hr] = L;
+      l_r[hr] += __shfl_xor_sync(0xffffffffu, l_r[hr], 1);
+      l_r[hr] += __shfl_xor_sync(0xffffffffu, l_r[hr], 2);
     }
-    // group k hands its sum to group k - 1, in this order always
+    if (KW > 1) {
+      if (c == 0) {
 #pragma unroll
-    for (int k = KW - 1; k > 0; --k)
+        for (int hr = 0; hr < 2; ++hr) {
+          ml[(warp * 16 + g + 8 * hr) * 2] = m_r[hr];
+          ml[(warp * 16 + g + 8 * hr) * 2 + 1] = l_r[hr];
+        }
+      }
+      bar_compute();
 #pragma unroll
-      for (int d0 = 0; d0 < D / 8; d0 += SM::kDims / 8) {
-        float2* buf = reinterpret_cast<float2*>(mbuf) + rw * 16 * SM::kDims / 2 + lane;
-        if (kw == k) {
+      for (int hr = 0; hr < 2; ++hr) {
+        float M = -INFINITY, L = 0.f;
 #pragma unroll
-          for (int d = 0; d < SM::kDims / 8; ++d) {
-            buf[(2 * d) * 32] = make_float2(o[d0 + d][0], o[d0 + d][1]);
-            buf[(2 * d + 1) * 32] = make_float2(o[d0 + d][2], o[d0 + d][3]);
+        for (int w = 0; w < KW; ++w) M = fmaxf(M, ml[((rw * KW + w) * 16 + g + 8 * hr) * 2]);
+        const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int w = 0; w < KW; ++w) {
+          const float* x = ml + ((rw * KW + w) * 16 + g + 8 * hr) * 2;
+          L += x[1] * ex2_ftz(x[0] - base);
+        }
+        const float f = ex2_ftz(m_r[hr] - base);
+#pragma unroll
+        for (int d = 0; d < D / 8; ++d) {
+          o[d][2 * hr] *= f;
+          o[d][2 * hr + 1] *= f;
+        }
+        m_r[hr] = M;
+        l_r[hr] = L;
+      }
+      // group k hands its sum to group k - 1, in this order always
+#pragma unroll
+      for (int k = KW - 1; k > 0; --k)
+#pragma unroll
+        for (int d0 = 0; d0 < D / 8; d0 += SM::kDims / 8) {
+          float2* buf = reinterpret_cast<float2*>(mbuf) + rw * 16 * SM::kDims / 2 + lane;
+          if (kw == k) {
+#pragma unroll
+            for (int d = 0; d < SM::kDims / 8; ++d) {
+              buf[(2 * d) * 32] = make_float2(o[d0 + d][0], o[d0 + d][1]);
+              buf[(2 * d + 1) * 32] = make_float2(o[d0 + d][2], o[d0 + d][3]);
+            }
+          }
+          bar_compute();
+          if (kw == k - 1) {
+#pragma unroll
+            for (int d = 0; d < SM::kDims / 8; ++d) {
+              const float2 x = buf[(2 * d) * 32], y = buf[(2 * d + 1) * 32];
+              o[d0 + d][0] += x.x; o[d0 + d][1] += x.y;
+              o[d0 + d][2] += y.x; o[d0 + d][3] += y.y;
+            }
+          }
+          bar_compute();
+        }
+    }
+    // ---------------- output ----------------
+    float* slot = pc.whole ? nullptr : slot_of(p, D, blockIdx.x, pc.t0 == 0);
+    if (kw == 0) {
+#pragma unroll
+      for (int hr = 0; hr < 2; ++hr) {
+        if (!live[hr]) continue;
+        if (pc.whole) {
+          const float inv = l_r[hr] == 0.f ? 0.f : 1.f / l_r[hr];  // nothing seen: zeros
+          uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + b * p.o_sb +
+                                                      node[hr] * p.o_st + head[hr] * p.o_sh);
+#pragma unroll
+          for (int d = 0; d < D / 8; ++d)
+            dst[d * 4 + c] = pack2<T>(o[d][2 * hr] * inv, o[d][2 * hr + 1] * inv);
+        } else {
+          const int r = rw * 16 + g + 8 * hr;
+          float2* dst = reinterpret_cast<float2*>(slot + r * D);
+#pragma unroll
+          for (int d = 0; d < D / 8; ++d)
+            dst[d * 4 + c] = make_float2(o[d][2 * hr], o[d][2 * hr + 1]);
+          if (c == 0) {
+            slot[p.rows * D + r] = m_r[hr];
+            slot[p.rows * (D + 1) + r] = l_r[hr];
           }
         }
-        bar_compute();
-        if (kw == k - 1) {
-#pragma unroll
-          for (int d = 0; d < SM::kDims / 8; ++d) {
-            const float2 x = buf[(2 * d) * 32], y = buf[(2 * d + 1) * 32];
-            o[d0 + d][0] += x.x; o[d0 + d][1] += x.y;
-            o[d0 + d][2] += y.x; o[d0 + d][3] += y.y;
-          }
-        }
-        bar_compute();
       }
-  }
-  // ---------------- output ----------------
-  float* slot = pc.whole ? nullptr : slot_of(p, D, blockIdx.x, pc.t0 == 0);
-  if (kw == 0) {
-#pragma unroll
-    for (int hr = 0; hr < 2; ++hr) {
-      if (!live[hr]) continue;
-      if (pc.whole) {
-        const float inv = l_r[hr] == 0.f ? 0.f : 1.f / l_r[hr];  // nothing seen: zeros
-        uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + b * p.o_sb +
-                                                    node[hr] * p.o_st + head[hr] * p.o_sh);
-#pragma unroll
-        for (int d = 0; d < D / 8; ++d)
-          dst[d * 4 + c] = pack2<T>(o[d][2 * hr] * inv, o[d][2 * hr + 1] * inv);
-      } else {
-        const int r = rw * 16 + g + 8 * hr;
-        float2* dst = reinterpret_cast<float2*>(slot + r * D);
-#pragma unroll
-        for (int d = 0; d < D / 8; ++d)
-          dst[d * 4 + c] = make_float2(o[d][2 * hr], o[d][2 * hr + 1]);
-        if (c == 0) {
-          slot[p.rows * D + r] = m_r[hr];
-          slot[p.rows * (D + 1) + r] = l_r[hr];
+    }
+    const bool odd = bar_compute_or(bad != 0);
+    if (!pc.whole) {
+      if (threadIdx.x == 0) slot[p.rows * (D + 2)] = odd ? 1.f : 0.f;
+    } else if (odd) {
+      const int n = min(16 * RW, p.R - rt * 16 * RW);
+      for (int e = threadIdx.x; e < n * D; e += 128) {
+        const int r = rt * 16 * RW + e / D, d = e % D;
+        const int t = r / p.G, h = kvh * p.G + r % p.G;
+        const float acc = odd_values<T, D>(p, sp, b, kvh, t, d);
+        if (acc != 0.f) {
+          T* dst = static_cast<T*>(p.o) + b * p.o_sb + t * p.o_st + h * p.o_sh + d;
+          *dst = from_f32<T>(to_f32(*dst) + acc);
         }
       }
     }
-  }
-  const bool odd = bar_compute_or(bad != 0);
-  if (!pc.whole) {
-    if (threadIdx.x == 0) slot[p.rows * (D + 2)] = odd ? 1.f : 0.f;
-  } else if (odd) {
-    const int n = min(16 * RW, p.R - rt * 16 * RW);
-    for (int e = threadIdx.x; e < n * D; e += 128) {
-      const int r = rt * 16 * RW + e / D, d = e % D;
-      const int t = r / p.G, h = kvh * p.G + r % p.G;
-      const float acc = odd_values<T, D>(p, sp, b, kvh, t, d);
-      if (acc != 0.f) {
-        T* dst = static_cast<T*>(p.o) + b * p.o_sb + t * p.o_st + h * p.o_sh + d;
-        *dst = from_f32<T>(to_f32(*dst) + acc);
-      }
-    }
-  }
   } while (pc.next(p));
 }
 

@@ -11,8 +11,8 @@ whatever was drafted.
 
 The drafts here come from the sequence's own history (the continuations of
 earlier occurrences of its last tokens), so no second model is needed; `draft`
-may be any function of the same form.  The reference's speculative decoding is a
-stub (its README lists it as future work)."""
+may be any function of the same form.  The reference accepts and rejects a draft
+model's chain in Python, without a KV cache (torchpp/llmops/spec_decoding.py:62)."""
 from __future__ import annotations
 
 from typing import Callable, List, Optional, Sequence
