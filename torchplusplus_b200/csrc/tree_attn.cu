@@ -765,13 +765,15 @@ __global__ void __launch_bounds__(kTcThreads, 2) tree_attn_tc_kernel(
   }
   __syncthreads();
   pdl_wait();
-  pdl_trigger();
   Piece pc;
   if (!pc.start<true>(p)) return;
   if (warp == 5) tmem_alloc(tmem_slot, 256);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // Only now: a dependent kernel that allocates TMEM ahead of its own wait could take
+  // what this CTA still lacks, and keep it until this kernel has ended.
+  pdl_trigger();
   const uint32_t tmem = *tmem_slot;
   bool ok = true;
 
