@@ -120,6 +120,7 @@ class SpeculativeDecoder:
         self.temperature = 0.0
         self._graph: Optional[torch.cuda.CUDAGraph] = None
         self._graph_temperature: Optional[float] = None
+        self._graph_weights: List[torch.Tensor] = []
         self.path = self.count = self.next = None
         self.steps = 0
 
@@ -152,24 +153,50 @@ class SpeculativeDecoder:
         ops.kv_commit(self.k_tree, self.v_tree, self.path, self.count, self.ctx, self.k, self.v)
         self.ctx.add_(self.count * self.active)
 
-    def step(self) -> None:
-        """One verified step of the trees in the static buffers, as a CUDA graph
-        (recorded again when the temperature changes)."""
-        if self._graph is None or self._graph_temperature != self.temperature:
-            side = torch.cuda.Stream(self.device)
-            side.wait_stream(torch.cuda.current_stream(self.device))
-            ctx = self.ctx.clone()
-            with torch.cuda.stream(side):
-                self._step()  # warm-up: library set-up does not belong into a graph
-                self.ctx.copy_(ctx)
-                side.synchronize()
-                g = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(g, stream=side):
-                    self._step()
-            torch.cuda.current_stream(self.device).wait_stream(side)
-            self._graph, self._graph_temperature = g, self.temperature
+    def _weights(self) -> List[torch.Tensor]:
+        """Every tensor of the model that a step reads (concatenations that a
+        changed weight has made stale are rebuilt)."""
+        m = self.model
+        ws = [m.tok_embed.weight, m.final_rmsnorm.weight, m.out_head.weight, m.cos, m.sin]
+        for blk in m.transformer_blocs:
+            a = blk.attn
+            ws += [blk.rms_norm1.weight, a._qkv.get(a.Wq.weight, a.Wk.weight, a.Wv.weight),
+                   a.out_projection.weight, blk.rms_norm2.weight, blk.ffn.gate_up_weight(),
+                   blk.ffn.linear_layer2.weight]
+            ws += [n.weight for n in (a.q_norm, a.k_norm) if n is not None]
+        return ws
+
+    def _record(self) -> None:
+        """Records the step as a CUDA graph where there is none yet, the
+        temperature differs or the model's weights have moved."""
+        # A graph reads the addresses it was recorded with: it holds the storages
+        # behind them, so none is freed or handed out again while it lives.
+        ws = [w.detach() for w in self._weights()]
+        if self._graph is not None and self._graph_temperature == self.temperature and \
+                [w.data_ptr() for w in ws] == [w.data_ptr() for w in self._graph_weights]:
+            return
+        side = torch.cuda.Stream(self.device)
+        side.wait_stream(torch.cuda.current_stream(self.device))
+        ctx = self.ctx.clone()
+        with torch.cuda.stream(side):
+            self._step()  # warm-up: library set-up does not belong into a graph
+            self.ctx.copy_(ctx)
+            side.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                self._step()
+        torch.cuda.current_stream(self.device).wait_stream(side)
+        self._graph, self._graph_temperature, self._graph_weights = g, self.temperature, ws
+
+    def _replay(self) -> None:
         self._graph.replay()
         self.steps += 1
+
+    def step(self) -> None:
+        """One verified step of the trees in the static buffers, as a CUDA graph
+        (recorded again when the temperature or the model's weights change)."""
+        self._record()
+        self._replay()
 
     def set_trees(self, trees: "list[tuple[List[int], List[int]]]", roots: Sequence[int]) -> None:
         """Puts each sequence's root token and drafted (tokens, parents) into the
@@ -223,7 +250,9 @@ class SpeculativeDecoder:
             self.active.copy_(torch.tensor([0 if d else 1 for d in done], dtype=torch.int32))
             if self.temperature > 0:
                 self.uniforms.uniform_(generator=gen)
-            self.step()
+            if self.steps == 0:   # weights are looked over once a request
+                self._record()
+            self._replay()
             path, count, nxt, tok = (t.tolist() for t in (self.path, self.count, self.next,
                                                           self.tokens))
             for b, h in enumerate(history):
