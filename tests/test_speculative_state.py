@@ -74,3 +74,27 @@ def test_changed_weights_reach_the_next_request(temperature):
     for blk in m.transformer_blocs:
         blk.rms_norm1.weight.data.fill_(1.0)
     assert run(dec) == first
+
+
+@pytest.mark.gpu
+def test_recording_leaves_the_lengths_as_they_were(monkeypatch):
+    """Work that the caller's stream gets after the recording stream has been
+    tied to it (here a pause of some 50 ms) has no part in what is saved."""
+    m = small_model(torch.device("cuda", 0))
+    dec = SpeculativeDecoder(m, 3, 64, nodes=2)
+    dec.ctx.copy_(torch.tensor([3, 9, 0], dtype=torch.int32))
+    dec.set_trees([([5], [0])] * 3, [1, 2, 3])
+    tie = torch.cuda.Stream.wait_stream
+
+    def tie_then_pause(self, other):
+        tie(self, other)
+        with torch.cuda.stream(other):
+            torch.cuda._sleep(100_000_000)
+
+    torch.cuda.synchronize()
+    monkeypatch.setattr(torch.cuda.Stream, "wait_stream", tie_then_pause)
+    dec._record()
+    torch.cuda.synchronize()
+    assert dec.ctx.tolist() == [3, 9, 0]
+    dec._replay()
+    assert dec.ctx.tolist() == [3 + int(dec.count[0]), 9 + int(dec.count[1]), int(dec.count[2])]

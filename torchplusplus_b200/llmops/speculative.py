@@ -177,8 +177,8 @@ class SpeculativeDecoder:
             return
         side = torch.cuda.Stream(self.device)
         side.wait_stream(torch.cuda.current_stream(self.device))
-        ctx = self.ctx.clone()
         with torch.cuda.stream(side):
+            ctx = self.ctx.clone()  # in the order of side, ahead of what changes it
             self._step()  # warm-up: library set-up does not belong into a graph
             self.ctx.copy_(ctx)
             side.synchronize()
