@@ -61,6 +61,7 @@ struct TreeArgs {
   const int32_t* table; int64_t table_stride; int num_blocks;
   int64_t window_left;
   float scale_log2;
+  float exp_scale;  // scale_log2 if that is positive, 1 otherwise
   int B, T, Hq, Hkv, G, W, R, RT, NT;  // W mask words a row, R = T * G rows, NT tree tiles
   int ctas, rows;                      // parts at most (0: a unit each), rows of a unit
   int whole_tiles;                     // a CTA takes a unit where none has more tiles
@@ -926,6 +927,12 @@ __global__ void __launch_bounds__(kTcThreads, 2) tree_attn_tc_kernel(
 #pragma unroll
             for (int k = 0; k < KT; ++k) sv[k] = __uint_as_float(r[k]);
           }
+          // The scale goes into the exponent's fma, behind the mask and the maximum,
+          // which only a positive one leaves as they are: others are applied here.
+          if (!(p.scale_log2 > 0.f)) {
+#pragma unroll
+            for (int k = 0; k < KT; ++k) sv[k] *= p.scale_log2;
+          }
           if (careful) {
             uint64_t see;
             if (tree) {
@@ -948,7 +955,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) tree_attn_tc_kernel(
 #pragma unroll
             for (int u = 0; u < 8; ++u) pm[u] = fmax3(pm[u], sv[k + u], sv[k + 8 + u]);
           const float mx = fmax3(fmax3(pm[0], pm[1], pm[2]), fmax3(pm[3], pm[4], pm[5]),
-                                 fmaxf(pm[6], pm[7])) * p.scale_log2;
+                                 fmaxf(pm[6], pm[7])) * p.exp_scale;
           // lazy base, as above; O's rescale is warp-collective, so lanes that
           // keep their base use the factor 1
           const bool grow = mx > m_ref + kRescale;
@@ -969,7 +976,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) tree_attn_tc_kernel(
             tmem_wait_st();
           }
           const float nm = m_ref == -INFINITY ? 0.f : -m_ref;
-          const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), nm2 = f2_pack(nm, nm);
+          const uint64_t sc2 = f2_pack(p.exp_scale, p.exp_scale), nm2 = f2_pack(nm, nm);
           uint64_t ps[4] = {0ull, 0ull, 0ull, 0ull};
           uint32_t pk[KT / 2];
 #pragma unroll
@@ -1306,6 +1313,7 @@ int tree_attention(TreeCall c, int dtype, cudaStream_t st) {
   a.table = c.table; a.table_stride = c.table_stride; a.num_blocks = (int)c.num_blocks;
   a.window_left = c.window_left;
   a.scale_log2 = c.scale * 1.4426950408889634f;
+  a.exp_scale = a.scale_log2 > 0.f ? a.scale_log2 : 1.f;
   a.B = (int)c.B; a.T = (int)c.T; a.Hq = (int)c.Hq; a.Hkv = (int)c.Hkv;
   a.G = (int)(c.Hq / c.Hkv); a.W = (a.T + 63) / 64; a.R = a.T * a.G; a.NT = a.W;
   a.err = device_error_flag();
