@@ -3,7 +3,8 @@ ordinary: against the definitions in 64 bits of test_tree_gpu."""
 import pytest
 import torch
 
-from .test_tree_gpu import BF16, attention_oracle, contiguous_cache, make, pack, paged_cache
+from .test_tree_gpu import (BF16, F16, UNIT, attention_oracle, contiguous_cache, make, pack,
+                            paged_cache)
 
 pytestmark = pytest.mark.gpu
 
@@ -27,6 +28,29 @@ def attention(g, q, kc, vc, kt, vt, ctx, see, max_ctx=None, paged=False, mask=No
                               kt.cuda(), vt.cuda(), lens, most, mask, **kw)
 
 
+def oracle(q, kc, vc, kt, vt, ctx, see, scale):
+    """attention_oracle without a window, a head of a sequence at a time."""
+    B, T, Hq, D = q.shape
+    G, u = Hq // kt.shape[2], UNIT[q.dtype]
+    out = torch.zeros(B, T, Hq, D, dtype=torch.float64)
+    tol = torch.zeros_like(out)
+    for b in range(B):
+        n = int(ctx[b])
+        hide = torch.zeros(T, n + T, dtype=torch.float64)
+        hide[:, n:][~see[b]] = float("-inf")
+        for h in range(Hq):
+            k = torch.cat([kc[b][:, h // G], kt[b, :, h // G]]).double()
+            v = torch.cat([vc[b][:, h // G], vt[b, :, h // G]]).double()
+            x = q[b, :, h].double()
+            w = torch.softmax(x @ k.T * scale + hide, 1)
+            out[b, :, h] = o = w @ v
+            a = w @ v.abs()
+            big = (x.abs() @ k.abs().T * abs(scale) + hide).amax(1, keepdim=True)
+            tol[b, :, h] = u * (a + o.abs()) + (2 * (D + 8) * 2.0 ** -24 * big + 2.0 ** -19) * a \
+                + 2.0 ** -24
+    return out, tol
+
+
 # ------------------------------------------------------------------ the scale's sign
 @pytest.mark.parametrize("scale", [-0.07, 0.0])
 @pytest.mark.parametrize("B,T,Hq,Hkv,D,ctx", [
@@ -40,3 +64,65 @@ def test_attention_takes_any_scale(B, T, Hq, Hkv, D, ctx, scale):
     ref, tol = attention_oracle(q, kc, vc, kt, vt, ctx, see, -1, scale)
     o = attention(g, q, kc, vc, kt, vt, ctx, see, scale=scale).double().cpu()
     assert ((o - ref).abs() <= tol).all(), ((o - ref).abs() - tol).max()
+
+
+# ------------------------------------------------------------------ the plans
+# B, T, Hq, Hkv, D, ctx, capacity (None: the longest length)
+PLANS = [
+    (1, 64, 16, 8, 128, [3000], None),              # wide, each unit cut by itself
+    (1, 64, 16, 8, 64, [2500], None),
+    (2, 33, 2, 2, 128, [1900, 1500], None),         # 33 rows of 128
+    (4, 40, 8, 2, 128, [3000, 10, 700, 0], None),   # wide, parts that straddle units
+    (4, 40, 8, 2, 64, [3000, 10, 700, 0], None),
+    (3, 20, 14, 2, 128, [40, 2900, 1111], None),    # 126 rows a unit, two row tiles
+    (40, 40, 4, 2, 128, [2000 if b % 9 == 4 else 37 * b % 300 for b in range(40)], None),
+    (70, 3, 4, 2, 128, [2500 if b % 23 == 7 else 41 * b % 350 for b in range(70)], None),
+    (33, 16, 4, 2, 64, [0] * 32 + [3000], None),    # 32 rows, the last of two rounds
+    (2, 5, 4, 2, 128, [200, 0], 4000),              # room for a cut that the lengths
+    (2, 40, 4, 2, 128, [200, 700], 4000),           # turn out not to need
+    (36, 4, 4, 2, 128, [9 * b for b in range(36)], 3000),
+    (36, 40, 4, 2, 64, [9 * b for b in range(36)], 6000),
+    (1, 8, 16, 8, 128, [2900], 30000),              # cut, far below the room
+    (1, 50, 16, 8, 128, [2900], 30000),
+]
+
+
+@pytest.mark.parametrize("paged", [False, True])
+@pytest.mark.parametrize("case", PLANS, ids=lambda c: f"B{c[0]}T{c[1]}H{c[2]}/{c[3]}D{c[4]}"
+                                                        f"n{max(c[5])}of{c[6]}")
+def test_attention_of_every_plan(case, paged):
+    B, T, Hq, Hkv, D, ctx, room = case
+    dtype = F16 if paged else BF16
+    g = torch.Generator().manual_seed(B * 1000 + T)
+    q, kc, vc, kt, vt, see = make(g, B, T, Hq, Hkv, D, ctx, dtype)
+    ref, tol = oracle(q, kc, vc, kt, vt, ctx, see, D ** -0.5)
+    o = attention(g, q, kc, vc, kt, vt, ctx, see, room, paged).double().cpu()
+    assert o.isfinite().all() and ((o - ref).abs() <= tol).all(), ((o - ref).abs() - tol).max()
+
+
+@pytest.mark.parametrize("T,ctx,window", [(64, [3000], 2100), (40, [2000, 0, 900], 700),
+                                          (8, [3000, 64], 1500)])
+def test_attention_of_a_window_that_is_cut(T, ctx, window):
+    g = torch.Generator().manual_seed(T)
+    q, kc, vc, kt, vt, see = make(g, len(ctx), T, 4, 2, 128, ctx, BF16)
+    ref, tol = attention_oracle(q, kc, vc, kt, vt, ctx, see, window, 128 ** -0.5)
+    o = attention(g, q, kc, vc, kt, vt, ctx, see, window_left=window).double().cpu()
+    assert ((o - ref).abs() <= tol).all(), ((o - ref).abs() - tol).max()
+
+
+@pytest.mark.parametrize("B,T,Hq", [(1, 64, 4), (3, 40, 4), (1, 8, 4)])
+def test_attention_nonfinite_values_of_a_unit_that_is_cut(B, T, Hq):
+    """They reach the rows that see them and no others, whichever piece has them."""
+    g = torch.Generator().manual_seed(41)
+    ctx, D = [2900, 100, 1300][:B], 128
+    q, kc, vc, kt, vt, see = make(g, B, T, Hq, 2, D, ctx, BF16)
+    see[:, :, 2] = False
+    see[:, 4, 2] = True
+    ref, tol = attention_oracle(q, kc, vc, kt, vt, ctx, see, -1, D ** -0.5)
+    vt[:, 2, :, 5] = float("inf")
+    vt[:, 2, :, 70] = float("nan")
+    o = attention(g, q, kc, vc, kt, vt, ctx, see).double().cpu()
+    clean = torch.ones(B, T, Hq, D, dtype=torch.bool)
+    clean[:, 4, :, 5] = clean[:, 4, :, 70] = False
+    assert ((o - ref).abs() <= tol)[clean].all()
+    assert (o[:, 4, :, 5] == float("inf")).all() and o[:, 4, :, 70].isnan().all()
