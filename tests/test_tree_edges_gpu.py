@@ -126,3 +126,40 @@ def test_attention_nonfinite_values_of_a_unit_that_is_cut(B, T, Hq):
     clean[:, 4, :, 5] = clean[:, 4, :, 70] = False
     assert ((o - ref).abs() <= tol)[clean].all()
     assert (o[:, 4, :, 5] == float("inf")).all() and o[:, 4, :, 70].isnan().all()
+
+
+# ------------------------------------------------------------------ verification
+def test_verify_from_two_threads_with_different_vocabularies():
+    """Each launch has the shared memory that its vocabulary takes, whatever the
+    other thread's calls are."""
+    import threading
+    from torchplusplus_b200 import _native as N
+    f = N.lib().tpp_verify_tree
+    failed, keep = [], []
+
+    def work(args, stream):
+        for i in range(4000):
+            if f(*args) != 0:
+                failed.append(N.lib().tpp_last_error())
+                return
+            if i % 100 == 99:
+                stream.synchronize()
+
+    threads = []
+    for V in (151936, 40000):
+        lg = torch.zeros(1, 1, V, dtype=BF16, device="cuda")
+        i64, i32 = (torch.zeros(2, dtype=t, device="cuda") for t in (torch.int64, torch.int32))
+        path, count, nxt, u = i32.clone(), i32.clone(), i64.clone(), torch.zeros(1, device="cuda")
+        stream = torch.cuda.Stream()
+        keep.append((lg, i64, i32, path, count, nxt, u))
+        args = (lg.data_ptr(), V, V, lg.data_ptr(), V, V, i64.data_ptr(), 1, i32.data_ptr(), 0,
+                u.data_ptr(), 1, 1.0, path.data_ptr(), count.data_ptr(), nxt.data_ptr(), 1, 1, V,
+                None, 0, N.dtype_code(BF16), stream.cuda_stream)
+        threads.append(threading.Thread(target=work, args=(args, stream)))
+    torch.cuda.synchronize()
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, failed[0]

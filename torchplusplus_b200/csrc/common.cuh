@@ -4,6 +4,7 @@
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>
 #include <stdint.h>
+#include <atomic>
 #include <string>
 #include <utility>
 #include "../../include/tpp_b200.h"
@@ -198,6 +199,25 @@ __device__ __forceinline__ void pdl_trigger() {
 
 // PDL on unless the environment sets TPP_PDL=0 (for A/B measurements).
 bool pdl_enabled();
+
+// Lets a kernel take up to `bytes` of dynamic shared memory.  The limit belongs to the
+// kernel, not to a launch: give the most that any launch of it takes, so that no
+// other thread's launch meets a smaller one.  Asked for once a device (0.5 us a
+// call otherwise); `done` is the kernel's own, and two threads may both be first.
+inline int reserve_smem(const void* kern, std::atomic<bool> (&done)[64], size_t bytes,
+                        const char* what) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::atomic<bool>* d = dev >= 0 && dev < 64 ? &done[dev] : nullptr;
+  if (d && d->load(std::memory_order_acquire)) return TPP_OK;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) !=
+      cudaSuccess) {
+    set_error(std::string(what) + ": cannot reserve shared memory");
+    return TPP_ERR_LAUNCH;
+  }
+  if (d) d->store(true, std::memory_order_release);
+  return TPP_OK;
+}
 
 template <typename... KArgs, typename... Args>
 int launch(const char* what, void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,

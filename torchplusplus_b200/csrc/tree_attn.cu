@@ -38,7 +38,6 @@
 #include <limits.h>
 #include <math.h>
 #include <algorithm>
-#include <atomic>
 #include "mma_common.cuh"
 #include "tc_common.cuh"
 
@@ -1195,22 +1194,7 @@ struct TreeCall {
   void* ws; int64_t ws_bytes;
 };
 
-// cudaFuncSetAttribute once a kernel (`id` of 12) and device: 0.5 us a call
-// otherwise.  (Two threads may both make it the first time.)
-int reserve_smem(const void* kern, int id, size_t smem) {
-  static std::atomic<bool> done[64][12];
-  int dev = 0;
-  cudaGetDevice(&dev);
-  std::atomic<bool>* d = dev >= 0 && dev < 64 ? &done[dev][id] : nullptr;
-  if (d && d->load(std::memory_order_acquire)) return TPP_OK;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
-      cudaSuccess) {
-    set_error("tree attention: cannot reserve shared memory");
-    return TPP_ERR_LAUNCH;
-  }
-  if (d) d->store(true, std::memory_order_release);
-  return TPP_OK;
-}
+std::atomic<bool> g_reserved[12][64];  // by kernel
 
 // How a call is cut: the row groups of a CTA (0: tcgen05), a unit's rows and row
 // tiles, and the parts at most (0: a CTA takes a unit, whatever the lengths).
@@ -1343,12 +1327,16 @@ int tree_attention(TreeCall c, int dtype, cudaStream_t st) {
     if (rc != TPP_OK) return rc;
   }
   auto go_tc = [&](auto kern, int id, size_t smem) -> int {
-    if (const int e = reserve_smem(reinterpret_cast<const void*>(kern), id, smem)) return e;
+    if (const int e = reserve_smem(reinterpret_cast<const void*>(kern), g_reserved[id], smem,
+                                   "tree_attn_tc_kernel"))
+      return e;
     return launch("tree_attn_tc_kernel", kern, grid, dim3(kTcThreads), smem, st, 0u, tk, tv, tkt,
                   tvt, tq, a);
   };
   auto go = [&](auto kern, int id, size_t smem) -> int {
-    if (const int e = reserve_smem(reinterpret_cast<const void*>(kern), id, smem)) return e;
+    if (const int e = reserve_smem(reinterpret_cast<const void*>(kern), g_reserved[id], smem,
+                                   "tree_attn_kernel"))
+      return e;
     return launch("tree_attn_kernel", kern, grid, dim3(kThreads), smem, st, 0u, tk, tv, tkt, tvt,
                   a);
   };

@@ -34,6 +34,7 @@ namespace tpp {
 namespace {
 
 constexpr int kMaxNodes = 256;
+constexpr int kMaxDraftVocab = 400000;  // with a draft: 196 KB of cache a CTA
 constexpr int kSlice = 1024;         // groups of a row for a CTA of the statistics
 constexpr double kFix = 1099511627776.0;  // 2^40
 using ull = unsigned long long;
@@ -136,8 +137,9 @@ __device__ __forceinline__ ull warp_sum_u64(ull v) {
   return v;
 }
 
-// A thread's sum of integer weights: at most 2^22 / 4096 of them, so that either
-// half fits 32 bits.
+// A thread's sum of integer weights: some 2^22 / 2048 of them at most (8 CTAs of 256
+// threads, to whole groups) of up to 1, so that either half's sum (of 2^20 and of
+// 2^19) fits 32 bits.
 struct Sum {
   uint32_t hi = 0;
   int lo = 0;
@@ -910,19 +912,21 @@ int walk_threads(int64_t B) {
   return 16 * B <= 2 * num_sms() ? 512 : 256;
 }
 
+// Bytes of the cache of what is left of p: a CTA's part of a row, in fp32.
+template <typename T, int C>
+constexpr size_t cache_bytes(int V) {
+  constexpr int VE = 16 / sizeof(T);
+  return (size_t)((V + 2 * VE - 2) / VE + C - 1) / C * VE * sizeof(float);
+}
 template <typename T, int C, int TH>
 int walk_launch(const VerifyArgs& a, int64_t B, cudaStream_t st) {
+  static std::atomic<bool> reserved[64];
   auto kern = verify_tree_kernel<T, C, TH>;
-  constexpr int VE = 16 / sizeof(T);
-  // the cache of what is left of p, a CTA's part of a row (with a draft)
-  const size_t cache = a.draft && !a.greedy
-      ? (size_t)((a.V + 2 * VE - 2) / VE + C - 1) / C * VE * sizeof(float) : 0;
-  if (cache > 16 * 1024 &&
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cache) !=
-          cudaSuccess) {
-    set_error("verify_tree_kernel: cannot reserve shared memory");
-    return TPP_ERR_LAUNCH;
-  }
+  const size_t cache = a.draft && !a.greedy ? cache_bytes<T, C>(a.V) : 0;
+  if (cache > 16 * 1024)
+    if (const int e = reserve_smem(reinterpret_cast<const void*>(kern), reserved,
+                                   cache_bytes<T, C>(kMaxDraftVocab), "verify_tree_kernel"))
+      return e;
   return launch("verify_tree_kernel", kern, dim3((unsigned)B, C), dim3(TH), cache, st, C, a);
 }
 template <typename T>
@@ -982,7 +986,7 @@ extern "C" int tpp_verify_tree(const void* logits, int64_t l_sb, int64_t l_st,
   // weights do not count), itself twice.
   a.sum_error = 8e-6f + (float)(V / 2048 + 64) * 5.9604645e-8f;
   a.err = device_error_flag();
-  TPP_REQUIRE(!draft_logits || a.greedy || V <= 400000, TPP_ERR_UNSUPPORTED,
+  TPP_REQUIRE(!draft_logits || a.greedy || V <= kMaxDraftVocab, TPP_ERR_UNSUPPORTED,
               "draft logits need a vocabulary of at most 400000 tokens");
   if (need) {
     const dim3 grid((unsigned)a.slices, (unsigned)(B * (2 * T - 1)));
