@@ -163,3 +163,14 @@ def test_verify_from_two_threads_with_different_vocabularies():
         t.join()
     torch.cuda.synchronize()
     assert not failed, failed[0]
+
+
+@pytest.mark.parametrize("T", [8, 64])
+def test_attention_of_the_widest_window_over_many_keys(T):
+    g = torch.Generator().manual_seed(61)
+    ctx = [5000]
+    q, kc, vc, kt, vt, see = make(g, 1, T, 16, 8, 128, ctx, BF16)
+    call = lambda w: attention(g, q, kc, vc, kt, vt, ctx, see, window_left=w)
+    full = call(-1)
+    for w in (5000 + T, 2 ** 63 - 1):
+        assert torch.equal(call(w), full)

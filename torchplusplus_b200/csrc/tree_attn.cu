@@ -1209,7 +1209,7 @@ Plan plan_of(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t max_ctx, int
   pl.rows = pl.rw ? 16 * pl.rw : (int)(kTcRows / G * G);
   pl.rt = (int)((R + pl.rows - 1) / pl.rows);
   int64_t keys = max_ctx;
-  if (window_left >= 0 && window_left + 1 < keys) keys = window_left + KT;
+  if (window_left >= 0 && window_left < keys - 1) keys = window_left + KT;
   const int64_t tiles = (keys + KT - 1) / KT + (T + 63) / 64;
   const int64_t units = B * Hkv * pl.rt, ctas = 2 * sm_budget();
   // A unit a CTA up to so many tiles (us, whole / cut).  Few units: a narrow tree's 5
