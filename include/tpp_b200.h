@@ -469,8 +469,9 @@ int tpp_attention_tree_paged(const void* q, int64_t q_sb, int64_t q_st, int64_t 
  * Sums and cumulative sums run over whole multiples of 2^-40, so results do
  * not depend on how a row is split.  NaN logits count as -inf; a row
  * with no weight (all -inf, or +inf at temperature > 0) accepts no child and
- * draws -1.  tokens int64 [B, T] (stride tok_sb; one outside [0, V) is
- * rejected), parents int32 (stride par_sb, 0 to share one tree).
+ * draws -1.  tokens int64 [B, T] (stride tok_sb; a node whose token is
+ * outside [0, V) is passed over, as if it were not there), parents int32
+ * (stride par_sb, 0 to share one tree).
  * Outputs: path int32 [B, T] (accepted nodes from the root on, then -1), count
  * int32 [B] (nodes on the path, >= 1), next_token int64 [B]. */
 int tpp_verify_tree(const void* logits, int64_t l_sb, int64_t l_st, const void* draft_logits,

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from .test_tree_gpu import (BF16, F16, UNIT, attention_oracle, contiguous_cache, make, pack,
-                            paged_cache)
+                            paged_cache, verify_inputs)
 
 pytestmark = pytest.mark.gpu
 
@@ -174,3 +174,55 @@ def test_attention_of_the_widest_window_over_many_keys(T):
     full = call(-1)
     for w in (5000 + T, 2 ** 63 - 1):
         assert torch.equal(call(w), full)
+
+
+@pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("T,pads,V", [(2, 1, 501), (4, 3, 5003), (9, 20, 1001)])
+def test_verify_nodes_without_a_token_change_nothing(draft, T, pads, V):
+    """Trees filled up with nodes that hold no token (before and behind the real
+    children, children of theirs among them) end as the trees without them: nothing
+    was drawn for them, so they take nothing from the target's distribution."""
+    from torchplusplus_b200 import ops
+    g = torch.Generator().manual_seed(71 + T)
+    B = 40
+    logits, tokens, par, u, d = (x if x is None else x.cuda() for x in
+                                 verify_inputs(g, B, T, V, BF16, False, draft))
+    path, count, nxt = ops.verify_tree(logits, tokens, par, u, 1.0, d)
+    # the first `lead` pads come right behind the root, the others last
+    lead, N = pads // 2, T + pads
+    at = torch.tensor([0] + list(range(1 + lead, T + lead)), device="cuda")    # of the real nodes
+    big = [torch.randn(B, N, V, generator=g).to(BF16).cuda() for _ in range(2)]
+    big[0][:, at] = logits
+    if draft:
+        big[1][:, at] = d
+    tok2 = torch.full((B, N), -1, dtype=torch.int64, device="cuda")
+    tok2[:, 1::2] = V + 3
+    tok2[:, at] = tokens
+    par2 = torch.zeros(B, N, dtype=torch.int32, device="cuda")
+    par2[:, N - 1] = N - 2 if pads > 2 else 0
+    par2[:, at] = torch.where(par >= 0, at[par.clamp_min(0).long()].int(), -1)
+    u2 = torch.rand(B, N, generator=g).cuda()
+    u2[:, at] = u
+    path2, count2, nxt2 = ops.verify_tree(big[0], tok2, par2, u2, 1.0, big[1] if draft else None)
+    assert torch.equal(count2, count) and torch.equal(nxt2, nxt)
+    want = torch.where(path >= 0, at[path.clamp_min(0).long()].int(), -1)
+    assert torch.equal(path2[:, :T], want) and (path2[:, T:] == -1).all()
+
+
+def test_verify_emits_the_targets_distribution_from_padded_trees():
+    """As the test of whole trees: chi-square with 9 degrees of freedom, 33.7 is
+    passed once in 10^4."""
+    from torchplusplus_b200 import ops
+    g = torch.Generator().manual_seed(13)
+    n, V = 60000, 10
+    t = torch.randn(V, generator=g) * 1.2
+    d = t + 0.8 * torch.randn(V, generator=g)
+    want = torch.softmax(t.double(), 0) * n
+    kid = torch.multinomial(torch.softmax(d, 0), n, True, generator=g)[:, None]
+    tokens = torch.cat([torch.zeros_like(kid), kid, torch.full((n, 3), -1)], 1).cuda()
+    par = torch.tensor([-1, 0, 0, 0, 0], dtype=torch.int32, device="cuda")
+    lg, dl = (x.expand(1, 5, V).contiguous().cuda().expand(n, 5, V) for x in (t, d))
+    path, count, nxt = ops.verify_tree(lg, tokens, par, torch.rand(n, 5, generator=g).cuda(), 1.0, dl)
+    first = torch.where(count > 1, tokens.gather(1, path[:, 1:2].clamp_min(0).long())[:, 0], nxt)
+    seen = torch.bincount(first.cpu(), minlength=V).double()
+    assert float(((seen - want) ** 2 / want).sum()) < 33.7

@@ -629,7 +629,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) verify_tree_kernel(VerifyArgs p
     const int par = p.parents[b * p.par_sb + i];
     const int64_t t = p.tokens[b * p.tok_sb + i];
     const bool known = i > 0 && par >= 0 && par < i && t >= 0 && t < p.V;
-    sm.par[i] = i > 0 && par < i ? par : -1;
+    sm.par[i] = known ? par : -1;  // (a node without a token is nobody's child)
     sm.tok[i] = known ? (int)t : -1;
     sm.u[i] = p.greedy ? 0.f : p.u[b * p.u_sb + i];
     sm.lt[i] = known ? to_f32(lb[par * p.l_st + t]) : -INFINITY;
@@ -637,7 +637,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) verify_tree_kernel(VerifyArgs p
   }
   if (p.stats) {
     // a warp a row: its slices' maxima and sums
-    const int rows = p.T + (with_q ? p.T - 1 : 0);
+    const int rows = 2 * p.T - 1;  // (they are taken with a draft only)
     for (int i = warp; i < rows; i += W) {
       const int r = i < p.T ? b * p.T + i : p.B * p.T + b * (p.T - 1) + i - p.T;
       const float2* st = p.stats + (int64_t)r * p.slices;
@@ -660,8 +660,8 @@ __global__ void __launch_bounds__(TH, 1024 / TH) verify_tree_kernel(VerifyArgs p
     for (int i = tid; i < p.T; i += TH) {
       const int par = max(sm.par[i], 0);
       const float w = weight(sm.lt[i], sm.m[par], p.inv_t);
-      sm.pt[i] = with_q ? share(w, sm.z[par]) : w;
-      if (with_q && i > 0)
+      sm.pt[i] = share(w, sm.z[par]);
+      if (i > 0)
         sm.uq[i] = __fmul_rn(sm.u[i], share(weight(sm.qt[i], sm.mq[par], p.inv_t), sm.zq[par]));
     }
   }
@@ -756,19 +756,17 @@ __global__ void __launch_bounds__(TH, 1024 / TH) verify_tree_kernel(VerifyArgs p
       if (p.greedy) {
         ok = t == best && best >= 0;
       } else if (with_q) {
-        if (t >= 0) {
-          float uq, pt;
-          if (p.stats && !summed) {
-            uq = sm.uq[i];
-            pt = sm.pt[i];
-          } else {
-            const float qv = share_of(sm.qt[i], mq, zq, p.inv_t);
-            uq = __fmul_rn(sm.u[i], qv);
-            pt = left_of(share_of(sm.lt[i], m, z, p.inv_t), qv, nst, sm.stage);
-          }
-          again = !summed && fabsf(uq - pt) <= 3.f * p.sum_error * fmaxf(uq, pt);
-          ok = uq < pt;
+        float uq, pt;
+        if (p.stats && !summed) {
+          uq = sm.uq[i];
+          pt = sm.pt[i];
+        } else {
+          const float qv = share_of(sm.qt[i], mq, zq, p.inv_t);
+          uq = __fmul_rn(sm.u[i], qv);
+          pt = left_of(share_of(sm.lt[i], m, z, p.inv_t), qv, nst, sm.stage);
         }
+        again = !summed && fabsf(uq - pt) <= 3.f * p.sum_error * fmaxf(uq, pt);
+        ok = uq < pt;
         again |= !summed && !ok;  // the residual needs them
         if (!again && !ok) {
           const ull r = sum1(reject<T>(sh, row, qrow, mis, p.V, m, z, mq, zq, p.inv_t,
@@ -790,8 +788,8 @@ __global__ void __launch_bounds__(TH, 1024 / TH) verify_tree_kernel(VerifyArgs p
           ++nst;
         }
       } else {
-        const ull w = t < 0 || seen_before(sm.par, sm.tok, cur, i) ? 0
-                      : fixed(p.stats ? sm.pt[i] : weight(sm.lt[i], m, p.inv_t));
+        const ull w = seen_before(sm.par, sm.tok, cur, i)
+                          ? 0 : fixed(weight(sm.lt[i], m, p.inv_t));
         const double u = (double)sm.u[i];
         ok = u * (double)left < (double)w;
         again = !summed && fabs(u * (double)left - (double)w) <= u * p.sum_error * kFix * (double)z;
@@ -801,7 +799,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) verify_tree_kernel(VerifyArgs p
         sums();
         if (!with_q)  // less what the earlier children took
           for (int j = next_child(sm.par, p.T, cur, cur); j < i; j = next_child(sm.par, p.T, cur, j))
-            if (sm.tok[j] >= 0 && !seen_before(sm.par, sm.tok, cur, j))
+            if (!seen_before(sm.par, sm.tok, cur, j))
               left -= fixed(weight(sm.lt[j], m, p.inv_t));
         continue;  // the same child
       }
@@ -830,7 +828,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) verify_tree_kernel(VerifyArgs p
                       : scale<VE>(sh, over, cache));
       } else {
         for (int j = next_child(sm.par, p.T, cur, cur); j < p.T; j = next_child(sm.par, p.T, cur, j))
-          if (sm.tok[j] >= 0 && !seen_before(sm.par, sm.tok, cur, j)) sm.out[nout++] = j;  // (all threads write the same)
+          if (!seen_before(sm.par, sm.tok, cur, j)) sm.out[nout++] = j;  // (all threads write the same)
       }
       // the parts of the last exchange, less the rejected tokens
       const Part* in = sm.in[(turn - 1) & 1];

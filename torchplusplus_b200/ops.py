@@ -772,8 +772,8 @@ def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
                 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Which drafted tokens of each sequence's tree the target accepts, and the
     token after them.  logits [B,T,V] (the target's at every node), tokens int64
-    [B,T] (node 0, the root, is already chosen), parents int32 [T] or [B,T]
-    (parents[i] < i), uniforms float32 [B,T] in [0,1) (one test a node, entry 0
+    [B,T] (node 0, the root, is already chosen; a node whose token is outside
+    [0, V) is as good as absent), parents int32 [T] or [B,T] (parents[i] < i), uniforms float32 [B,T] in [0,1) (one test a node, entry 0
     for the draw), draft_logits [B,T or T-1,V] if the children of each node were
     drawn from their softmax at the same temperature.  temperature 0 accepts the
     argmax (see tpp_verify_tree for the rules).  Returns path int32 [B,T]
