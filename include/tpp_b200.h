@@ -452,7 +452,7 @@ int tpp_attention_tree_paged(const void* q, int64_t q_sb, int64_t q_st, int64_t 
 
 /* Verifies each sequence's drafted tree against the target's logits
  * [B, T, V] (f16, bf16 or f32; strides l_sb, l_st), with given uniform numbers
- * u [B, T] in [0, 1): walking from the root, the children i of the current node
+ * u [B, T] in [0, 1) (others count as its ends): walking from the root, the children i of the current node
  * are tried in index order with u[b, i], the walk descends to the first one
  * accepted, and where none is, the next token is drawn with u[b, 0] from what
  * is left of the target's distribution there.

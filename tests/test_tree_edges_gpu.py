@@ -226,3 +226,38 @@ def test_verify_emits_the_targets_distribution_from_padded_trees():
     first = torch.where(count > 1, tokens.gather(1, path[:, 1:2].clamp_min(0).long())[:, 0], nxt)
     seen = torch.bincount(first.cpu(), minlength=V).double()
     assert float(((seen - want) ** 2 / want).sum()) < 33.7
+
+
+@pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("T,chain", [(5, True), (12, False), (20, True)])
+def test_verify_negative_uniforms_stand_for_zero(T, chain, draft):
+    """For the tests of the children as for the draw: a token without weight is
+    not accepted by them."""
+    from torchplusplus_b200 import ops
+    g = torch.Generator().manual_seed(81)
+    logits, tokens, par, u, d = (x if x is None else x.cuda() for x in
+                                 verify_inputs(g, 16, T, 777, BF16, chain, draft))
+    none = torch.rand(16, T, generator=g) < 0.5       # their tokens have no weight
+    none[0, 1:] = True
+    for b, i in none[:, 1:].nonzero().tolist():
+        logits[b, int(par[b, i + 1]), int(tokens[b, i + 1])] = float("-inf")
+    low = torch.where(torch.rand(16, T, generator=g).cuda() < 0.5, u, -u)
+    low[0], low[1] = -1.0, float("-inf")
+    got = ops.verify_tree(logits, tokens, par, low, 1.0, d)
+    assert int(got[1][0]) == 1
+    for x, y in zip(got, ops.verify_tree(logits, tokens, par, low.clamp_min(0.0), 1.0, d)):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("draft", [False, True])
+def test_verify_uniforms_from_one_on_accept_the_only_token(draft):
+    from torchplusplus_b200 import ops
+    T = 4
+    lg = torch.full((3, T, 300), float("-inf"), device="cuda")
+    lg[:, :, 17] = 0.5
+    u = torch.tensor([1.0, 3.0, float("inf")], device="cuda")[:, None].expand(3, T)
+    path, count, nxt = ops.verify_tree(
+        lg, torch.full((3, T), 17, device="cuda"),
+        torch.arange(-1, T - 1, dtype=torch.int32, device="cuda"), u, 1.0, lg if draft else None)
+    # with the draft's row equal to the target's, u * q < p holds for every u in [0, 1)
+    assert count.tolist() == [T] * 3 and nxt.tolist() == [17] * 3

@@ -631,7 +631,10 @@ __global__ void __launch_bounds__(TH, 1024 / TH) verify_tree_kernel(VerifyArgs p
     const bool known = i > 0 && par >= 0 && par < i && t >= 0 && t < p.V;
     sm.par[i] = known ? par : -1;  // (a node without a token is nobody's child)
     sm.tok[i] = known ? (int)t : -1;
-    sm.u[i] = p.greedy ? 0.f : p.u[b * p.u_sb + i];
+    const float u = p.greedy ? 0.f : p.u[b * p.u_sb + i];
+    // outside [0, 1) its ends: a test would accept a token without weight, or reject
+    // the only one left (the draw, with node 0's, sees to that itself)
+    sm.u[i] = i == 0 ? u : u < 0.f ? 0.f : u >= 1.f ? 0x1.fffffep-1f : u;
     sm.lt[i] = known ? to_f32(lb[par * p.l_st + t]) : -INFINITY;
     sm.qt[i] = known && with_q ? to_f32(db[par * p.d_st + t]) : -INFINITY;
   }
