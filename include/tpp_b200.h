@@ -423,7 +423,10 @@ int64_t tpp_attention_tree_workspace(int64_t B, int64_t T, int64_t Hq, int64_t H
  * mask[b, i, j / 64] is set (mask uint64 [B or 1][T][ceil(T/64)], batch stride
  * mask_sb, 0 to share one).  window_left >= 0 drops the cache rows below
  * p - window_left, where node i's position p is ctx_lens[b] + popcount(mask row)
- * - 1.  A row that sees nothing gives zeros.  What a row does not see has no
+ * - 1; nodes it drops not, they go by the mask alone.  A sliding window over both
+ * is this with masks that leave out ancestors more than window_left above a node:
+ * a node deeper than that has window_left + 1 bits left, and so no cache row, the
+ * others all of theirs.  A row that sees nothing gives zeros.  What a row does not see has no
  * effect on it, NaN and infinities included.  q [B,T,Hq,D], k_tree / v_tree
  * [B,T,Hkv,D], o [B,T,Hq,D] by (batch, token, head) strides, caches
  * [B,Hkv,Smax,D] as tpp_attention_decode; D 64 or 128. */
@@ -452,10 +455,10 @@ int tpp_attention_tree_paged(const void* q, int64_t q_sb, int64_t q_st, int64_t 
 
 /* Verifies each sequence's drafted tree against the target's logits
  * [B, T, V] (f16, bf16 or f32; strides l_sb, l_st), with given uniform numbers
- * u [B, T] in [0, 1) (others count as its ends): walking from the root, the children i of the current node
- * are tried in index order with u[b, i], the walk descends to the first one
- * accepted, and where none is, the next token is drawn with u[b, 0] from what
- * is left of the target's distribution there.
+ * u [B, T] in [0, 1) (others count as its ends): walking from the root, the
+ * children i of the current node are tried in index order with u[b, i], the walk
+ * descends to the first one accepted, and where none is, the next token is
+ * drawn with u[b, 0] from what is left of the target's distribution there.
  *   p = softmax(logits[b, node] / temperature)
  *   no draft logits (proposals without a distribution): child token t is
  *     accepted if u < p(t) / (mass of p left); rejected, p(t) becomes 0;

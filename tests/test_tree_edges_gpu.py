@@ -261,3 +261,62 @@ def test_verify_uniforms_from_one_on_accept_the_only_token(draft):
         torch.arange(-1, T - 1, dtype=torch.int32, device="cuda"), u, 1.0, lg if draft else None)
     # with the draft's row equal to the target's, u * q < p holds for every u in [0, 1)
     assert count.tolist() == [T] * 3 and nxt.tolist() == [17] * 3
+
+
+# ------------------------------------------------------------------ sliding windows
+@pytest.mark.parametrize("paged", [False, True])
+@pytest.mark.parametrize("T,Hq,ctx,window", [(12, 4, [300, 2], 4), (12, 4, [50, 9], 0),
+                                             (40, 4, [130, 0], 7), (70, 4, [500, 3], 65),
+                                             (200, 2, [90, 1000], 100), (8, 4, [3000, 5], 1000)])
+def test_attention_of_a_sliding_window_is_decodes(T, Hq, ctx, window, paged):
+    """A chain's nodes see what decoding its tokens one after another with the
+    same window sees: the keys [p - window, p], of the cache and of the tree."""
+    from torchplusplus_b200 import ops
+    from torchplusplus_b200.llmops import tree_mask
+    g = torch.Generator().manual_seed(91)
+    D = 128
+    q, kc, vc, kt, vt, _ = make(g, 2, T, Hq, 2, D, ctx, BF16)
+    par = torch.arange(-1, T - 1)
+    o = attention(g, q, kc, vc, kt, vt, ctx, None, paged=paged, window_left=window,
+                  mask=tree_mask(par, window)[0]).double().cpu()
+    kall = [torch.cat([k, kt[b]]) for b, k in enumerate(kc)]
+    vall = [torch.cat([v, vt[b]]) for b, v in enumerate(vc)]
+    nobody = torch.zeros(2, 1, 1, dtype=torch.bool)
+    cap = max(ctx) + T
+    # (decode's caches are zero where nothing was written, as the framework makes them)
+    kd, vd = contiguous_cache(kall, cap, 0.0), contiguous_cache(vall, cap, 0.0)
+    for t in range(0, T, 1 if T < 50 else 9):
+        # the oracle for the token at p = ctx + t: keys p - window to p, all its own cache
+        lens = [n + t + 1 for n in ctx]
+        low = [max(0, n + t - window) for n in ctx]
+        part = [[x[b][low[b]:lens[b]] for b in range(2)] for x in (kall, vall)]
+        ref, tol = attention_oracle(q[:, t:t + 1], *part, kt[:, :1], vt[:, :1],
+                                    [len(x) for x in part[0]], nobody, -1, D ** -0.5)
+        assert ((o[:, t:t + 1] - ref).abs() <= tol).all(), t
+        d = ops.attention_decode(q[:, t].cuda(), kd, vd, torch.tensor(lens, dtype=torch.int32).cuda(),
+                                 cap, window_left=window).double().cpu()
+        assert ((d - o[:, t]).abs() <= 2 * tol[:, 0]).all(), t
+
+
+def test_attention_of_a_sliding_window_over_a_branching_tree():
+    from torchplusplus_b200.llmops import tree_mask
+    g = torch.Generator().manual_seed(92)
+    T, ctx, window, D = 48, [100, 3], 3, 128
+    q, kc, vc, kt, vt, _ = make(g, 2, T, 4, 2, D, ctx, F16)
+    par = torch.full((2, T), -1, dtype=torch.int32)
+    for i in range(1, T):
+        par[:, i] = (i * torch.rand(2, generator=g) ** 0.3).int()     # deep ones
+    mask, depth = tree_mask(par, window)
+    assert int(depth.max()) > 2 * window
+    o = attention(g, q, kc, vc, kt, vt, ctx, None, window_left=window, mask=mask).double().cpu()
+    for b in range(2):
+        for t in range(T):
+            path = [t]
+            while par[b, path[-1]] >= 0:
+                path.append(int(par[b, path[-1]]))
+            path = path[::-1]                                         # the root first
+            k, v = torch.cat([kc[b], kt[b, path]]), torch.cat([vc[b], vt[b, path]])
+            k, v = k[-1 - window:], v[-1 - window:]
+            ref, tol = attention_oracle(q[b:b + 1, t:t + 1], [k], [v], kt[:1, :1], vt[:1, :1],
+                                        [len(k)], torch.zeros(1, 1, 1, dtype=torch.bool), -1, D ** -0.5)
+            assert ((o[b, t] - ref[0, 0]).abs() <= tol[0, 0]).all(), (b, t)

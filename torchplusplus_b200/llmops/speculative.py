@@ -27,10 +27,12 @@ from .kvcache import KVCache
 Draft = Callable[[Sequence[int], int], "tuple[List[int], List[int]]"]
 
 
-def tree_mask(parents: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+def tree_mask(parents: torch.Tensor, window_left: int = -1) -> tuple[torch.Tensor, torch.Tensor]:
     """parents int [T] or [B,T] (any value < 0 at a root, parents[i] < i) ->
     (mask int64 [.., T, ceil(T/64)] for ops.attention_tree: each node sees its
-    ancestors and itself, depth int32 [.., T]).  Computed on the host."""
+    ancestors and itself, depth int32 [.., T]).  With a sliding window
+    (window_left >= 0, the one given to ops.attention_tree) a node sees of them
+    those at most window_left above it.  Computed on the host."""
     par = parents.cpu().long()
     flat = par.reshape(-1, par.shape[-1])
     B, T = flat.shape
@@ -42,10 +44,13 @@ def tree_mask(parents: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
             raise ValueError("a parent must come before its children")
         see[:, i] = see[rows, p.clamp_min(0)] & (p >= 0)[:, None]
         see[:, i, i] = True
+    depth = see.sum(-1) - 1
+    if window_left >= 0:
+        see[..., :T] &= depth[:, None, :] >= depth[..., None] - window_left
     words = see.view(B, T, -1, 64).long() << torch.arange(64)
-    depth = (see.sum(-1) - 1).to(torch.int32)
     shape = par.shape
-    return words.sum(-1).view(*shape, -1).to(parents.device), depth.view(shape).to(parents.device)
+    return (words.sum(-1).view(*shape, -1).to(parents.device),
+            depth.to(torch.int32).view(shape).to(parents.device))
 
 
 def lookup_draft(history: Sequence[int], nodes: int, ngram: int = 3, branches: int = 3

@@ -910,7 +910,10 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     [B,Hkv,Smax,D] and those nodes of the tree (k_tree/v_tree [B,T,Hkv,D]) that
     its mask row has: bit j % 64 of mask[.., i, j // 64] (int64 [T,W] or
     [B,T,W], W = ceil(T/64)) lets node i see node j.  A row that sees nothing
-    gives zeros.  window_left: see tpp_attention_tree."""
+    gives zeros.  window_left >= 0 drops the cache rows below p - window_left,
+    p = ctx_lens[b] + a node's bits in the mask - 1; it drops no nodes: for a
+    sliding window over the tree too the mask leaves out the ancestors more than
+    window_left above a node (llmops.tree_mask(parents, window_left))."""
     dt = _half_alike("q", q, k_cache, v_cache, k_tree, v_tree)
     cs = k_cache.stride()
     if q.dim() != 4 or len(cs) != 4 or k_cache.shape[0] != q.shape[0] \
