@@ -98,3 +98,19 @@ def test_recording_leaves_the_lengths_as_they_were(monkeypatch):
     assert dec.ctx.tolist() == [3, 9, 0]
     dec._replay()
     assert dec.ctx.tolist() == [3 + int(dec.count[0]), 9 + int(dec.count[1]), int(dec.count[2])]
+
+
+@pytest.mark.gpu
+def test_the_norms_own_eps_is_used():
+    m = small_model(torch.device("cuda", 0))
+    for blk in m.transformer_blocs:
+        blk.attn.q_norm.eps = blk.attn.k_norm.eps = 10.0
+    ids = torch.arange(24).view(2, 12)
+    dec = SpeculativeDecoder(m, 2, 64, nodes=5)
+    new = dec.generate(ids, 20)
+    ref = SpeculativeDecoder(m, 2, 64, nodes=5)
+    n = 12 + 15                                     # rows that both surely hold
+    ref.generate(torch.cat([ids, torch.tensor(new)], 1)[:, :n], 1)
+    a, b = dec.k[:, :, :, :n].float(), ref.k[:, :, :, :n].float()
+    # bf16 rows computed in another order of sums, two layers deep
+    assert (a - b).abs().max() <= 2.0 ** -8 * 8 * b.abs().max()

@@ -20,6 +20,7 @@ from typing import Callable, List, Optional, Sequence
 import torch
 
 from .. import ops
+from ..attention._core import norm_eps
 from .kvcache import KVCache
 
 # history -> (tokens, parents) of at most `nodes` - 1 drafted nodes; parents count
@@ -144,7 +145,8 @@ class SpeculativeDecoder:
             ops.linear(h, a._qkv.get(a.Wq.weight, a.Wk.weight, a.Wv.weight), out=self.qkv[l])
             q, _ = ops.qk_norm_rope_tree(
                 self.qkv[l], None if a.q_norm is None else a.q_norm.weight,
-                None if a.k_norm is None else a.k_norm.weight, 1e-6, m.cos, m.sin,
+                None if a.k_norm is None else a.k_norm.weight,
+                1e-6 if a.q_norm is None else norm_eps(a.q_norm), m.cos, m.sin,
                 self.positions, Hq, Hkv, k_out=self.k_tree[l])
             o = ops.attention_tree(q, self.k[l], self.v[l], self.k_tree[l], self.v_tree[l],
                                    self.ctx, self.max_seq_len, self.mask)
