@@ -114,3 +114,14 @@ def test_the_norms_own_eps_is_used():
     a, b = dec.k[:, :, :, :n].float(), ref.k[:, :, :, :n].float()
     # bf16 rows computed in another order of sums, two layers deep
     assert (a - b).abs().max() <= 2.0 ** -8 * 8 * b.abs().max()
+
+
+@pytest.mark.gpu
+def test_no_new_tokens():
+    m = small_model(torch.device("cuda", 0))
+    dec = SpeculativeDecoder(m, 2, 64, nodes=5)
+    ids = torch.arange(24).view(2, 12)
+    assert dec.generate(ids, 0) == [[], []] and dec.steps == 0
+    assert [len(n) for n in dec.generate(ids, 1)] == [1, 1]
+    with pytest.raises(ValueError):
+        dec.generate(ids, -1)

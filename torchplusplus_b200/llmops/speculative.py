@@ -232,6 +232,10 @@ class SpeculativeDecoder:
         B, S = input_ids.shape
         if B != self.batch_size or S + max_new_token > self.max_seq_len:
             raise ValueError("prompt + max_new_token does not fit the decoder")
+        if max_new_token < 0:
+            raise ValueError("max_new_token must not be negative")
+        if max_new_token == 0:
+            return [[] for _ in range(B)]
         m = self.model
         self.temperature = float(temperature)
         gen = torch.Generator(device=self.device).manual_seed(seed)
@@ -249,7 +253,7 @@ class SpeculativeDecoder:
         first = ops.verify_tree(logits[:, None], root, torch.full_like(root, -1, dtype=torch.int32),
                                 u, self.temperature)[2].tolist()
         history = [ids + [t] for ids, t in zip(input_ids.tolist(), first)]
-        done = [max_new_token <= 1 or h[-1] == eos_token_id for h in history]
+        done = [max_new_token == 1 or h[-1] == eos_token_id for h in history]
         self.steps = 0
         while not all(done):
             self.set_trees([([], []) if d else self.draft(h, self.nodes)
