@@ -320,3 +320,20 @@ def test_attention_of_a_sliding_window_over_a_branching_tree():
             ref, tol = attention_oracle(q[b:b + 1, t:t + 1], [k], [v], kt[:1, :1], vt[:1, :1],
                                         [len(k)], torch.zeros(1, 1, 1, dtype=torch.bool), -1, D ** -0.5)
             assert ((o[b, t] - ref[0, 0]).abs() <= tol[0, 0]).all(), (b, t)
+
+
+# ------------------------------------------------------------------ q/k norm + RoPE
+@pytest.mark.parametrize("B,T", [(1, 3), (64, 64)])
+def test_qk_norm_rope_positions_outside_the_table_are_zero_without_an_eps(B, T):
+    from torchplusplus_b200 import ops
+    D = 128
+    g = torch.Generator().manual_seed(101)
+    qkv = torch.randn(B, T, 8 * D, generator=g).to(BF16).cuda()
+    w = torch.ones(D, dtype=BF16, device="cuda")
+    cos = torch.ones(10, D, device="cuda")
+    pos = torch.randint(0, 10, (B, T), generator=g).int()
+    pos[0, 1], pos[-1, -1] = -1, 10
+    q, k = ops.qk_norm_rope_tree(qkv, w, w, 0.0, cos, cos, pos.cuda(), 4, 2)
+    out = (pos < 0) | (pos >= 10)
+    for x in (q, k):
+        assert (x.cpu()[out] == 0).all() and x.isfinite().all()

@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_tree_kernel(RopeTreeArgs p) 
 #pragma unroll
     for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     if (nw != nullptr) {
-      const float inv = rsqrtf(ss / (float)D + p.eps);
+      const float inv = known ? rsqrtf(ss / (float)D + p.eps) : 0.f;  // (eps may be 0)
       float g[8];
       unpack8<T>(__ldg(static_cast<const uint4*>(nw) + lane), g);
 #pragma unroll
