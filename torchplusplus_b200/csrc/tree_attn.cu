@@ -25,11 +25,14 @@
 // maximum and sum (mma.sync m16n8k16 on fragments from ldmatrix, fp32
 // accumulators, exp2 domain); the key groups merge in shared memory at the end.
 //
-// Bound by HBM on the cache from some 8 tiles a unit on: 64 x 4 nodes over 4096 keys
-// 172 us, 6.24 TB/s (96% of a copy's); 16 x 16 over 8192 (32 rows, the most of this
-// form) 102 us, 5.3 TB/s.  Short calls are latency: 5 nodes over 130 keys 8.2 us, of
-// which 0.5 the lengths, 1.0 the first loads' issue, 1.0 their arrival, 3.6 four tiles,
-// 1.1 the merge.
+// Bound by HBM on the cache from some 8 tiles a unit on (16 query heads, 8 kv heads of
+// 128 dims here and below, unless said otherwise): 64 x 4 nodes over 4096 keys each
+// 172 us, 6.27 TB/s (96% of a copy's; 175 paged); 16 x 16 over 8192 (32 rows, the most
+// of this form) 102 us, 5.3 TB/s.  Short calls are latency: 5 nodes over 130 keys 8.1
+// us, of which 0.5 the lengths, 1.0 the first loads' issue, 1.0 their arrival, 3.6 four
+// tiles, 1.1 the merge.  With room for many more keys than the lengths have, where
+// tree_combine_kernel is launched to find nothing to do, 2 us more (32 x 8 over up to
+// 640 in room for 4096 22.1 us, 20.0 in room for 640).
 //
 // Masked keys: the score becomes -inf and the value is cleared before the
 // product, since 0 * NaN is NaN.  Values that some rows see and others do not
@@ -692,7 +695,9 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attn_kernel(
 //   warp 5:    S = Q K^T (M 128, N 64), O += P V (P read from TMEM)
 // S and P share two 64-column buffers; S of tile j+1 is computed under the softmax
 // of tile j.  Rows that a narrow unit (R < 128) lacks are skipped by whole warps.
-// 4 x 64 nodes over 32768 keys: 113 us, 609 TFLOP/s, 4.78 TB/s; in mid-course a CTA
+// Two CTAs of 192 threads leave 168 registers a thread, of which the softmax warps
+// spill 112 bytes.
+// 4 x 64 nodes over 32768 keys: 114 us, 604 TFLOP/s, 4.74 TB/s; in mid-course a CTA
 // takes 1.3 to 1.5 us a tile, which for all 296 is 7.4 to 6.5 TB/s; the rest is
 // the start (5 us), the pieces' output (4) and the combine kernel (4).  Measured and
 // not kept: P in shared memory, so that S of tile j+2 need not wait for the product
@@ -1068,8 +1073,9 @@ __global__ void __launch_bounds__(kTcThreads, 2) tree_attn_tc_kernel(
 }
 
 // Joins the pieces of the units that more than one part holds.  WPR warps a row
-// take every WPR-th piece each; with 33 pieces a row (one long sequence) one warp
-// a row waits on them five round trips long.
+// take every WPR-th piece each: the few units of one long sequence have up to 37
+// pieces (narrow trees over 8192 keys; wide ones 18), on which one warp a row would
+// wait several round trips long.
 template <typename T, int D, int WPR>
 __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant__ TreeArgs p) {
   constexpr int PER = D / 32;
@@ -1216,9 +1222,9 @@ Plan plan_of(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t max_ctx, int
   // (4 x 5 nodes over 400 keys, 8 tiles, 12.1 / 10.5), a wide one's 12 (64 nodes over
   // 500 keys, 9 tiles, 15.3 / 18.0; over 2000, 33 tiles, 37.0 / 20.5); 64 units, 16 (8 x
   // 5 over 400 keys 12.1 / 12.8; 16 x 8 over 2000 36.6 / 30.5).  Narrow units that fill
-  // most of the slots, 32 (32 x 8 over 2000 keys 43.5 / 46.5; 64 x 4 over 4096 140 /
-  // 126).  Wide ones, whose pieces cost more, 100 (32 x 32 over 4000 81 / 90; 64 x 13
-  // over 4096 146 / 153), but 40 where the last wave of CTAs is nearly empty (48 x 32
+  // most of the slots, 32 (32 x 8 over 2000 keys 43.5 / 46.5; 64 x 4 over ragged lengths
+  // up to 4096 140 / 126).  Wide ones, whose pieces cost more, 100 (32 x 32 over 4000 81
+  // / 90; 64 x 13 of 32 query heads over ragged lengths up to 4096 146 / 153), but 40 where the last wave of CTAs is nearly empty (48 x 32
   // over 5000 159 / 143; 40 x 32 over 1500 55 / 63) or the keys are narrow (64 x 32 over
   // 6000 keys of 64 dims 156 / 142).
   const bool last_full = units <= ctas || units >= 3 * ctas || units % ctas * 10 >= 7 * ctas;

@@ -141,7 +141,8 @@ struct CommitArgs {
 // One block copies the rows of one (layer, sequence, k or v), four words a thread
 // in flight.  One sequence: 2.2 us, the latency of the chain count -> path -> row ->
 // store.  28 layers of 64 sequences, 4.5 rows each: 15.9 us, 4.15 TB/s (64% of a
-// copy's): the destination's rows are 256 bytes a head, 16 KB apart.  (Four layers a
+// copy's), issue slots 64% busy: two divisions a word, four dependent loads a block, the
+// destination's rows of 256 bytes 16 KB apart; their shares are not known.  (Four layers a
 // block, so that all blocks start at once, 17.3; a thread for each word of a row
 // instead of divisions, 16.9.)
 __global__ void __launch_bounds__(256) kv_commit_kernel(CommitArgs p) {

@@ -21,8 +21,10 @@
 //
 // Bound by latency: one chain of 5 nodes over 151936 tokens with its draft takes
 // 26.6 us (first form 123), of which statistics 5, set-up 3, tests 3, exact sums 6,
-// residual 7, draw 3; 32 trees of 32 nodes 32 us (49).  Code fetched once a walk
-// counts: unrolling the second passes' loops over a lane's groups cost 8 us.
+// residual 7, draw 3; 32 trees of 32 nodes 31 us (49), greedily 48 (longer paths).
+// Code fetched once a walk counts: unrolling the second passes' loops over a lane's
+// groups cost 8 us.  With 64 registers a thread, for 1024 threads an SM, the walk
+// spills some 200 bytes.
 #include <limits.h>
 #include <math.h>
 #include <cooperative_groups.h>
