@@ -505,6 +505,62 @@ int tpp_kv_commit(const void* k_tree, int64_t kt_sl, int64_t kt_sb, int64_t kt_s
                   int64_t L, int64_t B, int64_t T, int64_t Hkv, int64_t D, int dtype,
                   void* stream);
 
+/* ---- packed prompts and their scores ---------------------------------------- */
+/* Prompts of different lengths in one row dimension: sequence b is rows
+ * cu_seqlens[b] .. cu_seqlens[b+1] - 1 (int32 [B+1], ascending, inside [0, N]; on the
+ * device).  Rows of no sequence are neither read for others nor written. */
+
+/* q/k RMSNorm (weights may be NULL) + RoPE of the projection rows qkv
+ * [N, (Hq+2Hkv)*D] (row stride qkv_sn) at each row's position in its sequence (a
+ * position outside the tables [table_rows, D] gives zero rows) -> q_out [N, Hq, D] and
+ * k_out [N, Hkv, D], contiguous.  With k_cache / v_cache (both or none; strides c_sb,
+ * c_sh, c_ss) k and v are also written to row `position` of sequence b of caches
+ * [B][Hkv][rows][D], or, with block_table, of pools [num_blocks][Hkv][64][D] (c_sb,
+ * c_sh, c_ss unused, rows = 64 * table columns); rows and blocks outside the cache are
+ * skipped.  D 16, 32, 64, 128 or 256. */
+int tpp_qk_norm_rope_packed(const void* qkv, int64_t qkv_sn, const void* qn_w,
+                            const void* kn_w, float eps, const void* cos, const void* sin,
+                            int64_t cs_stride, int64_t table_rows, int cs_dtype,
+                            const int32_t* cu_seqlens, int64_t B, void* q_out, void* k_out,
+                            void* k_cache, void* v_cache, int64_t c_sb, int64_t c_sh,
+                            int64_t c_ss, int64_t rows, int64_t num_blocks,
+                            const int32_t* block_table, int64_t table_stride, int64_t N,
+                            int64_t Hq, int64_t Hkv, int64_t D, int dtype, void* stream);
+
+/* Attention of every packed row over its own sequence: q [N, Hq, D], k, v
+ * [N, Hkv, D], o [N, Hq, D] by row and head strides (multiples of 8 elements).  causal: keys up to the
+ * row itself; window_left >= 0: keys from the row's position - window_left on.  D 64 or
+ * 128, Hq / Hkv <= 128.  What a row does not see does not affect it, NaN and
+ * infinities included. */
+int tpp_attention_packed(const void* q, int64_t q_sn, int64_t q_sh, const void* k, int64_t k_sn,
+                         int64_t k_sh, const void* v, int64_t v_sn, int64_t v_sh,
+                         const int32_t* cu_seqlens, int64_t B, void* o, int64_t o_sn,
+                         int64_t o_sh, int64_t N, int64_t Hq, int64_t Hkv, int64_t D,
+                         int causal, int64_t window_left, float scale, int dtype, void* stream);
+
+/* Of each row of logits [N, V] (f16, bf16 or f32, row stride ld), x = logits / temperature:
+ * logprobs[n] = log softmax(x)[tokens[n]], entropy[n] = -sum p log p (nats), ranks[n] =
+ * 1 + the number of logits above the token's, and the `top` (at most 32 and V) largest
+ * logits' log probabilities and tokens [N, top] in descending order (the lower index
+ * first on ties).  A token outside [0, V) gives log probability 0 and rank 0.  Logits
+ * of -inf weigh nothing; a row of nothing else gives log probabilities -inf and entropy
+ * 0.  NaN (the largest, as for tpp_argmax) or +inf in a row make its log probabilities
+ * and entropy NaN. */
+int tpp_token_logprobs(const void* logits, int64_t ld, int64_t N, int64_t V,
+                       const int64_t* tokens, double temperature, int64_t top, float* logprobs,
+                       float* entropy, int64_t* ranks, float* top_logprobs, int64_t* top_tokens,
+                       int dtype, void* stream);
+
+/* The log probabilities and entropies of tpp_token_logprobs for the logits
+ * x [N, E] . w [V, E]^T, summed in 32 bits and never written (row strides ldx, ldw; f16
+ * or bf16; E a multiple of 8, rows 16-byte aligned).  An infinite or NaN logit makes its row NaN.
+ * workspace: tpp_linear_logprobs_workspace bytes, 4-byte aligned. */
+int tpp_linear_logprobs(const void* x, int64_t ldx, const void* w, int64_t ldw,
+                        const int64_t* tokens, int64_t N, int64_t V, int64_t E,
+                        double temperature, float* logprobs, float* entropy, void* workspace,
+                        int64_t workspace_bytes, int dtype, void* stream);
+int64_t tpp_linear_logprobs_workspace(int64_t N, int64_t V, int64_t E);
+
 /* ---- persistent single-sequence decode step ------------------------------- */
 /* Row pitch of the persistent step's weights: `in` + TPP_PERSISTENT_ROW_PAD
  * elements.  The padding (never read) shifts consecutive rows by 16

@@ -117,6 +117,17 @@ SIGNATURES: dict[str, tuple] = {
     "tpp_kv_commit": (_i32, [_p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64, _p, _i64, _p,
                              _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64,
                              _i64, _i64, _i64, _i32, _p]),
+    "tpp_qk_norm_rope_packed": (_i32, [_p, _i64, _p, _p, _f32, _p, _p, _i64, _i64, _i32, _p, _i64,
+                                       _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _i64,
+                                       _i64, _i64, _i64, _i64, _i32, _p]),
+    "tpp_attention_packed": (_i32, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _p,
+                                    _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i64, _f32, _i32,
+                                    _p]),
+    "tpp_token_logprobs": (_i32, [_p, _i64, _i64, _i64, _p, C.c_double, _i64, _p, _p, _p, _p, _p,
+                                  _i32, _p]),
+    "tpp_linear_logprobs": (_i32, [_p, _i64, _p, _i64, _p, _i64, _i64, _i64, C.c_double, _p, _p,
+                                   _p, _i64, _i32, _p]),
+    "tpp_linear_logprobs_workspace": (_i64, [_i64, _i64, _i64]),
     "tpp_decode_advance": (_i32, [_p, _p, _i64, _i64, _p, _p, _i64, _p]),
 }
 
@@ -162,6 +173,16 @@ def call(name: str, *args) -> None:
     if st != TPP_OK:
         msg = lib().tpp_last_error().decode(errors="replace")
         raise TppError(name, st, msg)
+
+
+def call_on(t: torch.Tensor, name: str, *args) -> None:
+    """call(), with t's device as the current one."""
+    dev = t.get_device()
+    if dev == torch._C._cuda_getDevice():
+        call(name, *args)
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args)
 
 
 def dtype_code(t: torch.dtype) -> int:

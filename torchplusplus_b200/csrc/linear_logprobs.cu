@@ -1,0 +1,364 @@
+// Log probabilities of given tokens (and each row's entropy) straight from the LM head's
+// operands: softmax statistics of x W^T in the product's epilogue, the logits never
+// written.
+#include <math.h>
+#include "tc_common.cuh"
+
+namespace tpp {
+namespace {
+
+constexpr int BM = 128;        // tokens a tile
+constexpr int BK = 64;         // one 128-byte swizzle row of the operands
+constexpr int KS = 2;          // k-blocks a ring stage
+constexpr int kMaxBN = 256;    // vocabulary rows a tile at most (a multiple of 16)
+constexpr int kStages = 2;
+constexpr int kThreads = 384;  // 4 control warps, 8 of the epilogue
+constexpr int kEpiWarp0 = 4;
+constexpr uint32_t kSubA = BM * BK * 2;
+constexpr uint32_t kStageA = KS * kSubA;
+constexpr uint32_t kStageB = KS * kMaxBN * BK * 2;
+constexpr size_t kSmem = kStages * (kStageA + kStageB) + 2 * 3 * BM * 4 + 1024 + 256;
+static_assert(kSmem <= 227 * 1024, "shared memory plan exceeds 227 KB");
+
+struct HeadArgs {
+  const int64_t* tokens;
+  float* part;    // [tiles of the vocabulary][3][rows]: m, S, E of token_logprobs
+  float* target;  // [rows]: the token's logit
+  int N, V, E, BN;
+  int64_t rows;   // N rounded up to whole tiles
+  int flat;       // operands by 2-D maps, one request a k-block
+  float c;        // log2(e) / temperature
+  int* err;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+    linear_logprobs_kernel(const __grid_constant__ CUtensorMap tm_x,
+                           const __grid_constant__ CUtensorMap tm_w, HeadArgs p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~(uintptr_t)1023);
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + kStages * kStageA;
+  float* half1 = reinterpret_cast<float*>(sB + kStages * kStageB);  // [2 tiles][3][BM]
+  uint64_t* full = reinterpret_cast<uint64_t*>(half1 + 2 * 3 * BM);
+  uint64_t* empty = full + kStages;
+  uint64_t* tfull = empty + kStages;
+  uint64_t* tempty = tfull + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int BN = p.BN;
+  const int ntm = (p.N + BM - 1) / BM;
+  const int64_t ntiles = (int64_t)ntm * ((p.V + BN - 1) / BN);
+  const int nk = (p.E + BK * KS - 1) / (BK * KS);
+  const uint32_t sub_b = (uint32_t)BN * BK * 2;
+
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tm_x);
+    prefetch_tmap(&tm_w);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tfull[b], 1);
+      mbar_init(&tempty[b], 8);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_trigger();
+
+  bool ok = true;
+  if (warp == 0 && lane == 0) {
+    // ---------------- TMA producer ----------------
+    int it = 0;
+    for (int64_t t = blockIdx.x; t < ntiles && ok; t += gridDim.x) {
+      const int m0 = (int)(t % ntm) * BM, n0 = (int)(t / ntm) * BN;
+      for (int kb = 0; kb < nk && ok; ++kb, ++it) {
+        const int s = it % kStages;
+        if (it >= kStages) ok = mbar_wait(&empty[s], ((it / kStages) & 1) ^ 1, p.err, 51);
+        if (!ok) break;
+        mbar_arrive_expect_tx(&full[s], kStageA + KS * sub_b);
+        if (p.flat) {
+          for (int j = 0; j < KS; ++j) {
+            tma_load_2d(sA + s * kStageA + j * kSubA, &tm_x, &full[s], (kb * KS + j) * BK, m0);
+            tma_load_2d(sB + s * kStageB + j * sub_b, &tm_w, &full[s], (kb * KS + j) * BK, n0);
+          }
+        } else {
+          tma_load_3d(sA + s * kStageA, &tm_x, &full[s], 0, m0, kb * KS);
+          tma_load_3d(sB + s * kStageB, &tm_w, &full[s], 0, n0, kb * KS);
+        }
+      }
+    }
+  } else if (warp == 1 && lane == 0) {
+    // ---------------- MMA issuer ----------------
+    const uint32_t idesc = make_idesc_f16(BM, BN, IsBf16<T>::value, 0, 0);
+    int it = 0, j = 0;
+    for (int64_t t = blockIdx.x; t < ntiles && ok; t += gridDim.x, ++j) {
+      const int buf = j & 1;
+      if (j >= 2) ok = mbar_wait(&tempty[buf], ((j >> 1) & 1) ^ 1, p.err, 52);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t acc = tmem + (uint32_t)(buf * kMaxBN);
+      for (int kb = 0; kb < nk && ok; ++kb, ++it) {
+        const int s = it % kStages;
+        ok = mbar_wait(&full[s], (it / kStages) & 1, p.err, 53);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t a0 = smem_u32(sA + s * kStageA);
+        const uint32_t b0 = smem_u32(sB + s * kStageB);
+#pragma unroll
+        for (int k = 0; k < KS * BK / 16; ++k) {
+          const uint32_t j2 = k >> 2, kk = k & 3;
+          tc_mma_f16(acc, make_sdesc(a0 + j2 * kSubA + kk * 32, 16, 1024, 2),
+                     make_sdesc(b0 + j2 * sub_b + kk * 32, 16, 1024, 2), idesc, (kb | k) != 0);
+        }
+        tc_commit(&empty[s]);
+      }
+      tc_commit(&tfull[buf]);
+    }
+  } else if (warp >= kEpiWarp0) {
+    // ---------------- epilogue: one row and half the tile's columns a thread ----------------
+    const int quarter = warp & 3, hf = (warp - kEpiWarp0) >> 2;
+    const int rl = quarter * 32 + lane;
+    const int c_first = hf ? (BN / 16 + 1) / 2 * 16 : 0;  // this half's columns
+    const int half = hf ? BN - c_first : (BN / 16 + 1) / 2 * 16;
+    const float c = p.c;
+    const uint64_t c2 = f2_pack(c, c);
+    int j = 0;
+    for (int64_t t = blockIdx.x; t < ntiles; t += gridDim.x, ++j) {
+      const int row = (int)(t % ntm) * BM + rl, vt = (int)(t / ntm);
+      const int n0 = vt * BN + c_first, buf = j & 1;
+      const int nv = max(0, min(half, p.V - n0));  // columns inside the vocabulary
+      const int64_t at = row < p.N ? p.tokens[row] - n0 : -1;
+      const int tl = at >= 0 && at < nv ? (int)at : -1;  // the token's column here
+      const bool mine = __any_sync(0xffffffffu, tl >= 0);
+      // (after a wait that ran out the loop goes on, for the barrier below)
+      ok = ok && mbar_wait(&tfull[buf], (j >> 1) & 1, p.err, 54);
+      tc_fence_after();
+      const uint32_t trow =
+          tmem + (uint32_t)(buf * kMaxBN + c_first) + ((uint32_t)(quarter * 32) << 16);
+      float ref = -INFINITY, S = 0.f, En = 0.f;
+      for (int c0 = 0; c0 < nv; c0 += 16) {
+        uint32_t r[16];
+        tmem_ld16(trow + c0, r);
+        tmem_wait_ld();
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(r[i]);
+        const int left = nv - c0;  // (the same for the warp)
+        if (left < 16) {
+          // the vocabulary's end: what lies behind it weighs as much as its
+          // first column here, and is taken out again
+#pragma unroll
+          for (int i = 1; i < 16; ++i)
+            if (i >= left) x[i] = x[0];
+        }
+        float mx[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          mx[i] = fmaxf(fmaxf(x[i], x[4 + i]), fmaxf(x[8 + i], x[12 + i]));
+        const float cm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        if (c0 == 0) ref = cm;
+        if ((cm - ref) * c > 8.f) {
+          const float d = ref - cm, f = exp2f(c * d);
+          En = f == 0.f ? 0.f : (En + S * d) * f;
+          S *= f;
+          ref = cm;
+        }
+        const uint64_t r2 = f2_pack(-ref, -ref);
+        uint64_t s2 = 0ull, e2 = 0ull;
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const uint64_t q2 = f2_add(f2_pack(x[i], x[i + 1]), r2);
+          float d0, d1;
+          f2_unpack(f2_mul(q2, c2), d0, d1);
+          float w0 = ex2_ftz(d0), w1 = ex2_ftz(d1);
+          if (left < 16) {
+            w0 = i < left ? w0 : 0.f;
+            w1 = i + 1 < left ? w1 : 0.f;
+          }
+          const uint64_t w2 = f2_pack(w0, w1);
+          s2 = f2_add(s2, w2);
+          e2 = f2_fma(w2, q2, e2);
+        }
+        float a0, a1;
+        f2_unpack(s2, a0, a1);
+        S += a0 + a1;
+        f2_unpack(e2, a0, a1);
+        En += a0 + a1;
+        if (mine && (tl >> 4) == (c0 >> 4) && tl >= 0) {
+          float v = x[0];
+#pragma unroll
+          for (int i = 1; i < 16; ++i) v = (tl & 15) == i ? x[i] : v;
+          p.target[row] = v;
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tempty[buf]);
+      // the row's two halves, joined by the first
+      float* h1 = half1 + buf * 3 * BM;
+      if (hf == 1) {
+        h1[rl] = ref;
+        h1[BM + rl] = S;
+        h1[2 * BM + rl] = En;
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (hf == 0) {
+        const float rb = h1[rl], Sb = h1[BM + rl], Eb = h1[2 * BM + rl];
+        float* out = p.part + (int64_t)vt * 3 * p.rows + row;
+        float M = ref, S0 = S, E0 = En;
+        if (!(Sb == 0.f)) {  // (the second half may lie behind the vocabulary)
+          M = fmaxf(ref, rb);
+          const float da = ref - M, db = rb - M, fa = exp2f(c * da), fb = exp2f(c * db);
+          S0 = S * fa + Sb * fb;
+          E0 = (fa == 0.f ? 0.f : (En + S * da) * fa) + (fb == 0.f ? 0.f : (Eb + Sb * db) * fb);
+        }
+        out[0] = M;
+        out[p.rows] = S0;
+        out[2 * p.rows] = E0;
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
+// Joins the vocabulary's tiles: 32 rows a block, a tile a warp at a time.
+constexpr int kJoinWarps = 16;
+__global__ void __launch_bounds__(32 * kJoinWarps)
+    join_logprobs_kernel(const float* part, const float* target, const int64_t* tokens,
+                         int64_t rows, int nt, int N, int V, float c, float* logprobs,
+                         float* entropy) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ float sm[3][kJoinWarps][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = blockIdx.x * 32 + lane;
+  float M = -INFINITY, S = 0.f, E = 0.f;
+  auto add = [&](float m, float s, float e) {
+    const float big = fmaxf(M, m);
+    // (nothing so far: not -inf - -inf)
+    const float da = S == 0.f ? 0.f : M - big, db = s == 0.f ? 0.f : m - big;
+    const float fa = exp2f(c * da), fb = exp2f(c * db);
+    E = (fa == 0.f ? 0.f : (E + S * da) * fa) + (fb == 0.f ? 0.f : (e + s * db) * fb);
+    S = S * fa + s * fb;
+    M = big;
+  };
+  for (int t = warp; t < nt; t += kJoinWarps) {
+    const float* at = part + (int64_t)t * 3 * rows + row;
+    add(at[0], at[rows], at[2 * rows]);
+  }
+  sm[0][warp][lane] = M;
+  sm[1][warp][lane] = S;
+  sm[2][warp][lane] = E;
+  __syncthreads();
+  if (warp != 0 || row >= N) return;
+  for (int w = 1; w < kJoinWarps; ++w) add(sm[0][w][lane], sm[1][w][lane], sm[2][w][lane]);
+  constexpr float kLn2 = 0.69314718055994531f;
+  const float lz = log2f(S);
+  const int64_t tok = tokens[row];
+  logprobs[row] = tok >= 0 && tok < V ? ((target[row] - M) * c - lz) * kLn2 : 0.f;
+  entropy[row] = (lz - E / S * c) * kLn2;
+}
+
+// Vocabulary rows a tile: of the widths that fill the tensor core (a multiple of 16, at
+// least 128), the one whose tiles go evenly onto the SMs -- 151936 rows are 594 tiles of
+// 256, five rounds of 148 CTAs where four would nearly do, but five full rounds of 208.
+int tile_width(int64_t N, int64_t V) {
+  const int64_t ntm = (N + BM - 1) / BM, sms = num_sms();
+  int best = kMaxBN;
+  int64_t cost = -1;
+  for (int bn = kMaxBN; bn >= 128; bn -= 16) {
+    const int64_t tiles = ntm * ((V + bn - 1) / bn), rounds = (tiles + sms - 1) / sms;
+    const int64_t c = rounds * (bn + 8);  // 8: a tile's own cost
+    if (cost < 0 || c < cost) {
+      cost = c;
+      best = bn;
+    }
+  }
+  return best;
+}
+
+}  // namespace
+}  // namespace tpp
+
+using namespace tpp;
+
+extern "C" int64_t tpp_linear_logprobs_workspace(int64_t N, int64_t V, int64_t E) {
+  if (N <= 0 || V <= 0 || E <= 0) return 0;
+  const int64_t rows = (N + BM - 1) / BM * BM, bn = tile_width(N, V);
+  return 4 * rows * (3 * ((V + bn - 1) / bn) + 1);
+}
+
+extern "C" int tpp_linear_logprobs(const void* x, int64_t ldx, const void* w, int64_t ldw,
+                                   const int64_t* tokens, int64_t N, int64_t V, int64_t E,
+                                   double temperature, float* logprobs, float* entropy,
+                                   void* workspace, int64_t workspace_bytes, int dtype,
+                                   void* stream) {
+  if (N == 0) return TPP_OK;
+  TPP_REQUIRE(x && w && tokens && logprobs && entropy, TPP_ERR_SHAPE, "null pointer");
+  TPP_REQUIRE(N > 0 && N < (1ll << 31) - BM && V > 0 && V < (1ll << 31) - kMaxBN && E > 0 &&
+                  E < (1ll << 31) - BK * KS && ldx >= E && ldw >= E,
+              TPP_ERR_SHAPE, "bad sizes");
+  TPP_REQUIRE(temperature >= 1e-6 && isfinite(temperature), TPP_ERR_SHAPE,
+              "temperature must be positive");
+  TPP_REQUIRE(E % 8 == 0 && ldx % 8 == 0 && ldw % 8 == 0 && aligned16(x) && aligned16(w),
+              TPP_ERR_ALIGN, "rows must be 16-byte aligned and E a multiple of 8");
+  TPP_REQUIRE(workspace && workspace_bytes >= tpp_linear_logprobs_workspace(N, V, E) &&
+                  reinterpret_cast<uintptr_t>(workspace) % 4 == 0,
+              TPP_ERR_WORKSPACE, "workspace missing or too small");
+  HeadArgs a;
+  a.tokens = tokens;
+  a.N = (int)N; a.V = (int)V; a.E = (int)E;
+  a.BN = tile_width(N, V);
+  a.rows = (N + BM - 1) / BM * BM;
+  const int nt = (int)((V + a.BN - 1) / a.BN);
+  a.part = static_cast<float*>(workspace);
+  a.target = a.part + 3 * a.rows * nt;
+  a.flat = E % BK != 0;
+  a.c = (float)(1.4426950408889634 / temperature);
+  a.err = device_error_flag();
+  CUtensorMap tx, tw;
+  auto map = [&](CUtensorMap* m, const void* base, int64_t rows, int64_t ld, int box_rows) {
+    if (a.flat) {
+      const uint64_t dims[2] = {(uint64_t)E, (uint64_t)rows};
+      const uint64_t strides[1] = {(uint64_t)ld * 2};
+      const uint32_t box[2] = {BK, (uint32_t)box_rows};
+      return make_tmap(m, base, dtype, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    }
+    const uint64_t dims[3] = {BK, (uint64_t)rows, (uint64_t)(E / BK)};
+    const uint64_t strides[2] = {(uint64_t)ld * 2, BK * 2};
+    const uint32_t box[3] = {BK, (uint32_t)box_rows, KS};
+    return make_tmap(m, base, dtype, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  };
+  return TPP_DISPATCH_HALF(dtype, T, [&] {
+    int rc = map(&tx, x, N, ldx, BM);
+    if (rc == TPP_OK) rc = map(&tw, w, V, ldw, a.BN);
+    if (rc != TPP_OK) return rc;
+    auto kern = linear_logprobs_kernel<T>;
+    static std::atomic<bool> reserved[64];
+    rc = reserve_smem(reinterpret_cast<const void*>(kern), reserved, kSmem,
+                      "linear_logprobs_kernel");
+    if (rc != TPP_OK) return rc;
+    const int64_t tiles = (a.rows / BM) * nt;
+    const unsigned grid = (unsigned)(tiles < num_sms() ? tiles : num_sms());
+    rc = launch("linear_logprobs_kernel", kern, dim3(grid), dim3(kThreads), kSmem,
+                as_stream(stream), 0u, tx, tw, a);
+    if (rc != TPP_OK) return rc;
+    return launch("join_logprobs_kernel", join_logprobs_kernel, dim3((unsigned)((N + 31) / 32)),
+                  dim3(32 * kJoinWarps), 0, as_stream(stream), 0u, (const float*)a.part,
+                  (const float*)a.target, tokens, a.rows, nt, (int)N, (int)V, a.c, logprobs,
+                  entropy);
+  });
+}

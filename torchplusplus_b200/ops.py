@@ -962,6 +962,179 @@ def attention_tree_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     return out
 
 
+# ---------------------------------------------------------------- packed prompts
+def _one_device(t: torch.Tensor, *ts: torch.Tensor | None) -> None:
+    for o in (t, *ts):
+        if o is not None and (not o.is_cuda or o.get_device() != t.get_device()):
+            _cuda(o)
+            raise ValueError(f"operands on different devices: {t.device} and {o.device}")
+
+
+def _cu_seqlens(cu: torch.Tensor) -> int:
+    if cu.dtype is not torch.int32 or cu.dim() != 1 or cu.shape[0] < 1 or not cu.is_contiguous():
+        raise ValueError("cu_seqlens must be contiguous int32 [B + 1]")
+    return cu.shape[0] - 1
+
+
+def qk_norm_rope_packed(qkv: torch.Tensor, q_norm_w: torch.Tensor | None,
+                        k_norm_w: torch.Tensor | None, eps: float, cos: torch.Tensor,
+                        sin: torch.Tensor, cu_seqlens: torch.Tensor, Hq: int, Hkv: int,
+                        k_cache: torch.Tensor | None = None, v_cache: torch.Tensor | None = None,
+                        block_table: torch.Tensor | None = None,
+                        q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None
+                        ) -> tuple[torch.Tensor, torch.Tensor]:
+    """qkv [N,(Hq+2Hkv)*D], prompts packed row after row (sequence b: rows
+    cu_seqlens[b] .. cu_seqlens[b+1]-1, int32 [B+1] on the device, ascending) ->
+    q [N,Hq,D], k [N,Hkv,D], normed per head and rotated at each row's position in its
+    sequence (one outside the tables gives zero rows).  With caches [B,Hkv,Smax,D], or
+    pools [num_blocks,Hkv,64,D] and a block_table int32 [B,max_blocks], k and v are
+    also written to row `position` of sequence b (rows past the cache are skipped).
+    v is the last part of qkv as it is.  Rows of no sequence are not written."""
+    dt = _half_alike("qkv", qkv, q_norm_w, k_norm_w, k_cache, v_cache, q_out, k_out)
+    if qkv.dim() != 2 or Hq <= 0 or Hkv <= 0 or qkv.shape[1] % (Hq + 2 * Hkv):
+        raise ValueError("qkv must be [N, (Hq+2Hkv)*D]")
+    N_, W = qkv.shape
+    D = W // (Hq + 2 * Hkv)
+    _one_device(qkv, cos, sin, cu_seqlens, q_norm_w, k_norm_w, k_cache, v_cache, block_table)
+    B = _cu_seqlens(cu_seqlens)
+    for w in (q_norm_w, k_norm_w):
+        if w is not None and (w.shape != (D,) or not w.is_contiguous()):
+            raise ValueError(f"norm weights must be contiguous [{D}]")
+    if (k_cache is None) != (v_cache is None):
+        raise ValueError("k_cache and v_cache go together")
+    cs, rows, nb, tstride = (0, 0, 0, 0), 0, 0, 0
+    if k_cache is None:
+        if block_table is not None:
+            raise ValueError("block_table needs k_cache and v_cache")
+    elif block_table is not None:
+        nb, Hp, Dp = _paged_args(k_cache, v_cache, block_table, B)
+        if Hp != Hkv or Dp != D:
+            raise ValueError("the pools must match qkv's heads and head dim")
+        rows, tstride = 64 * block_table.shape[1], block_table.stride(0)
+    else:
+        cs = k_cache.stride()
+        if k_cache.dim() != 4 or k_cache.shape[:2] != (B, Hkv) or k_cache.shape[3] != D \
+                or v_cache.shape != k_cache.shape or v_cache.stride() != cs or cs[3] != 1:
+            raise ValueError("caches must be [B, Hkv, Smax, D] with identical layouts")
+        rows = k_cache.shape[2]
+    qkv = _rows16(qkv)
+    cos, sin, cs_stride, cs_dt = _table(cos, sin, D)
+    q_out = _tree_out(q_out, (N_, Hq, D), qkv)
+    k_out = _tree_out(k_out, (N_, Hkv, D), qkv)
+    N.call_on(qkv, "tpp_qk_norm_rope_packed", qkv.data_ptr(), qkv.stride(0), N.ptr(q_norm_w),
+              N.ptr(k_norm_w), eps, cos.data_ptr(), sin.data_ptr(), cs_stride, cos.shape[0],
+              cs_dt, cu_seqlens.data_ptr(), B, q_out.data_ptr(), k_out.data_ptr(),
+              N.ptr(k_cache), N.ptr(v_cache), cs[0], cs[1], cs[2], rows, nb, N.ptr(block_table),
+              tstride, N_, Hq, Hkv, D, dt, N.stream_of(qkv))
+    return q_out, k_out
+
+
+def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
+                     causal: bool = True, window_left: int = -1, scale: float | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of whole prompts packed row after row, each over itself: q [N,Hq,D],
+    k and v [N,Hkv,D] (any row and head strides; v may be the view of a projection),
+    sequence b in rows cu_seqlens[b] .. cu_seqlens[b+1]-1 (int32 [B+1] on the device,
+    ascending).  causal: keys up to the row itself; window_left >= 0: none further than
+    that before it.  Hq a multiple of Hkv, D 64 or 128.  Returns [N,Hq,D]; rows of no
+    sequence are not written.  What a row does not see does not affect it, NaN and
+    infinities included."""
+    dt = _half_alike("q", q, k, v, out)
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape:
+        raise ValueError("q must be [N, Hq, D], k and v [N, Hkv, D]")
+    N_, Hq, D = q.shape
+    Hkv = k.shape[1]
+    if k.shape[0] != N_ or k.shape[2] != D or Hkv == 0 or Hq % Hkv:
+        raise ValueError("k and v must be [N, Hkv, D] matching q, Hq a multiple of Hkv")
+    _one_device(q, k, v, cu_seqlens, out)
+    B = _cu_seqlens(cu_seqlens)
+    q, k, v = _rows16(q), _rows16(k), _rows16(v)
+    if out is None:
+        out = q.new_empty((N_, Hq, D))
+    elif out.shape != (N_, Hq, D) or out.stride(2) != 1:
+        raise ValueError("out must be [N, Hq, D] with a contiguous last dim")
+    qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), out.stride()
+    N.call_on(q, "tpp_attention_packed", q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
+              v.data_ptr(), vs[0], vs[1], cu_seqlens.data_ptr(), B, out.data_ptr(), os_[0],
+              os_[1], N_, Hq, Hkv, D, bool(causal), window_left,
+              D ** -0.5 if scale is None else scale, dt, N.stream_of(q))
+    return out
+
+
+def _scored(tokens: torch.Tensor, N_: int, temperature: float, *like: torch.Tensor
+            ) -> torch.Tensor:
+    if tokens.dtype is not torch.int64 or tokens.shape != (N_,):
+        raise ValueError("tokens must be int64 [N]")
+    _one_device(tokens, *like)
+    if not 1e-6 <= temperature < math.inf:
+        raise ValueError("temperature must be positive (at least 1e-6) and finite")
+    return tokens.contiguous()
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, temperature: float = 1.0,
+                   top: int = 0) -> tuple[torch.Tensor, ...]:
+    """Of each row of logits [N,V] (f16, bf16 or f32): the log probability of tokens[n]
+    (int64 [N]) under softmax(logits / temperature), float32 [N]; the distribution's
+    entropy in nats, float32 [N]; the token's rank, int64 [N] (1: no logit is above its
+    own); and the `top` (at most 32) most likely tokens' log probabilities, float32
+    [N,top], and ids, int64 [N,top], in descending order (ties: lower id first).  A token
+    outside [0, V) gives 0 and rank 0.  See tpp_token_logprobs for rows with -inf, +inf
+    and NaN."""
+    if logits.dim() != 2:
+        raise ValueError("logits must be [N, V]")
+    N_, V = logits.shape
+    dt = N.dtype_code(logits.dtype)
+    tokens = _scored(tokens, N_, temperature, logits)
+    if not 0 <= top <= min(32, V):
+        raise ValueError("top must be at most 32 and at most V")
+    if V == 0:
+        raise ValueError("logits must have at least one column")
+    if logits.stride(1) != 1 or (N_ > 1 and logits.stride(0) < V):
+        logits = logits.contiguous()
+    new = logits.new_empty
+    lp, ent = new(N_, dtype=torch.float32), new(N_, dtype=torch.float32)
+    rank = tokens.new_empty(N_)
+    tlp, tid = new((N_, top), dtype=torch.float32), tokens.new_empty((N_, top))
+    N.call_on(logits, "tpp_token_logprobs", logits.data_ptr(), max(logits.stride(0), V), N_, V,
+              tokens.data_ptr(), temperature, top, lp.data_ptr(), ent.data_ptr(),
+              rank.data_ptr(), tlp.data_ptr(), tid.data_ptr(), dt, N.stream_of(logits))
+    return lp, ent, rank, tlp, tid
+
+
+def linear_logprobs(x: torch.Tensor, weight: torch.Tensor, tokens: torch.Tensor,
+                    temperature: float = 1.0, workspace: torch.Tensor | None = None
+                    ) -> tuple[torch.Tensor, torch.Tensor]:
+    """token_logprobs' log probabilities and entropies, float32 [N] each, of the logits
+    x [N,E] @ weight [V,E].T in 32 bits, which are never written: scores of long prompts
+    without their [N,V] logits.  E a multiple of 8."""
+    dt = _half_alike("x", x, weight)
+    if x.dim() != 2 or weight.dim() != 2 or weight.shape[1] != x.shape[1]:
+        raise ValueError("x must be [N, E] and weight [V, E]")
+    N_, E = x.shape
+    V = weight.shape[0]
+    if V == 0 or E == 0 or E % 8:
+        raise ValueError("weight must have rows, and E must be a multiple of 8")
+    tokens = _scored(tokens, N_, temperature, x, weight)
+    x, weight = _rows16(x), _rows16(weight)
+    lp, ent = x.new_empty(N_, dtype=torch.float32), x.new_empty(N_, dtype=torch.float32)
+    nbytes = linear_logprobs_workspace_bytes(N_, V, E)
+    if workspace is None:
+        workspace = lp.new_empty(nbytes // 4)
+    else:
+        _one_device(x, workspace)
+        if not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
+    N.call_on(x, "tpp_linear_logprobs", x.data_ptr(), max(x.stride(0), E), weight.data_ptr(),
+              max(weight.stride(0), E), tokens.data_ptr(), N_, V, E, temperature, lp.data_ptr(),
+              ent.data_ptr(), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+              dt, N.stream_of(x))
+    return lp, ent
+
+
+def linear_logprobs_workspace_bytes(N_: int, V: int, E: int) -> int:
+    return N.lib().tpp_linear_logprobs_workspace(N_, V, E)
+
+
 def argmax(logits: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
     """Greedy token per row of logits [B, V] -> int64 [B]."""
     _cuda(logits)
