@@ -6,10 +6,8 @@
 namespace tpp {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
 constexpr int kU = 4;          // 16-byte vectors a thread has in flight
-constexpr int kCap = 2048;     // candidates for the alternatives; see below
+constexpr int kCap = 1024;     // candidates for the alternatives; see below
 constexpr int kMaxTop = 32;
 constexpr int kMaxCtas = 8;    // CTAs (one cluster) a row
 
@@ -102,6 +100,20 @@ template <typename T> struct Lane {
     const T2 m = __hmax2(__hmax2(as(u.x), as(u.y)), __hmax2(as(u.z), as(u.w)));
     return fmaxf(to_f32(m.x), to_f32(m.y));
   }
+  // how many of a chunk's elements exceed t: ones summed in the type (at most 16 a lane, exact)
+  struct Count {
+    T2 n{}, t;
+    __device__ __forceinline__ explicit Count(float v) {
+      const T e = from_f32<T>(v);
+      t.x = t.y = e;
+      n.x = n.y = from_f32<T>(0.f);
+    }
+    __device__ __forceinline__ void add(const uint4& u) {
+      n = __hadd2(__hadd2(n, __hadd2(__hgt2(as(u.x), t), __hgt2(as(u.y), t))),
+                  __hadd2(__hgt2(as(u.z), t), __hgt2(as(u.w), t)));
+    }
+    __device__ __forceinline__ int get() const { return (int)(to_f32(n.x) + to_f32(n.y)); }
+  };
 };
 template <> struct Lane<float> {
   static constexpr int E = 4;
@@ -113,6 +125,16 @@ template <> struct Lane<float> {
     return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)),
                  fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
   }
+  struct Count {
+    int n = 0;
+    float t;
+    __device__ __forceinline__ explicit Count(float v) : t(v) {}
+    __device__ __forceinline__ void add(const uint4& u) {
+      n += (__uint_as_float(u.x) > t) + (__uint_as_float(u.y) > t) + (__uint_as_float(u.z) > t) +
+           (__uint_as_float(u.w) > t);
+    }
+    __device__ __forceinline__ int get() const { return n; }
+  };
 };
 
 // One row a cluster of gridDim.y CTAs, each a slice of 16-byte vectors (of the row
@@ -124,16 +146,18 @@ template <> struct Lane<float> {
 // and two sums.  The differences are taken before the scale: masks of the type's lowest
 // value stay finite, and a row of nothing else is uniform.
 //
-// Alternatives: every warp's ceil(top / 8)-th largest of its threads' maxima over the
-// first chunk; the least of these eight is a lower bound of the slice's top-th largest
-// logit (at least `top` elements are no smaller).  What is no smaller there, and larger
-// later (a later equal one loses by its index), is kept: some 20 to 400 candidates, ranked at the
-// end by counting.  More than kCap (long runs of equal logits, ascending rows), or a NaN, and the
-// slice is searched `top` times over instead.
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(LogprobArgs p) {
-  constexpr int E = Lane<T>::E;
-  __shared__ uint64_t cand[TOP ? kCap : 1];
+// Alternatives: of each warp with a full first chunk, the r-th largest of its lanes'
+// maxima, r = ceil(top / such warps); the least of these is a lower bound of the slice's
+// top-th largest logit (at least `top` elements are no smaller).  What is no smaller there,
+// and larger later (a later equal one loses by its index), is a candidate.  After chunks
+// 1, 2, 4, 8 .. the candidates are ranked by counting and all but `top` dropped, which
+// raises the bound: some `top` new ones come in between.  More than kCap (long runs of equal
+// logits, ascending rows), or a NaN, and the slice is searched `top` times over instead.
+template <typename T, bool TOP, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT)
+    token_logprobs_kernel(LogprobArgs p) {
+  constexpr int E = Lane<T>::E, kWarps = NT / 32;
+  __shared__ __align__(16) uint64_t cand[TOP ? kCap : 1];
   __shared__ uint64_t list[TOP ? kMaxTop : 1];
   __shared__ uint64_t wbest[kWarps];
   __shared__ uint32_t wkey[2][kWarps];
@@ -148,73 +172,107 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(LogprobArgs
 
   const int64_t row_i = blockIdx.x;
   const T* row = static_cast<const T*>(p.logits) + row_i * p.ld;
-  const int64_t V = p.V;
+  const int V = (int)p.V;
   const int shift = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
   const T* base = row - shift;  // vector v holds elements v E - shift ...
-  const int64_t tok = p.tokens[row_i];
-  const bool has = tok >= 0 && tok < V;
-  const float xt = has ? to_f32(row[tok]) : INFINITY;
   // whole vectors [va, vb); the ends' elements go one by one
-  const int64_t nv = (shift + V + E - 1) / E;
-  const int64_t fa = shift > 0 ? 1 : 0, fb = (shift + V) / E;
-  const int64_t per = (nv + C - 1) / C;
-  const int64_t s0 = per * cr < nv ? per * cr : nv, s1 = s0 + per < nv ? s0 + per : nv;
-  const int64_t va = s0 > fa ? s0 : fa, vb = s1 < fb ? s1 : fb;
+  const int nv = (int)(((int64_t)shift + V + E - 1) / E);
+  const int fa = shift > 0 ? 1 : 0, fb = (int)(((int64_t)shift + V) / E);
+  const int per = (nv + C - 1) / C;
+  const int s0 = min(per * cr, nv), s1 = min(s0 + per, nv);
+  const int va = max(s0, fa), vb = min(s1, fb);
   // the slice's elements [e0, e1)
-  const int64_t e0 = s0 * E - shift > 0 ? s0 * E - shift : 0;
-  const int64_t e1 = s1 * E - shift < V ? (s1 * E - shift > 0 ? s1 * E - shift : 0) : V;
+  const int e0 = max(s0 * E - shift, 0), e1 = (int)min((int64_t)s1 * E - shift, (int64_t)V);
   // those outside its whole vectors: [e0, ea) and [eb, e1)
-  const int64_t ea = va < vb ? va * E - shift : e1, eb = va < vb ? vb * E - shift : e1;
+  const int ea = va < vb ? va * E - shift : e1, eb = va < vb ? vb * E - shift : e1;
 
-  const float c = p.c;
-  float ref = -INFINITY, S = 0.f, En = 0.f;
-  int greater = 0;
-  float T0 = INFINITY;  // what a candidate has to exceed, from the second chunk on
-
-  auto push = [&](float x, int64_t i) {
-    const int at = atomicAdd(&count, 1);
-    if (at < kCap) cand[at] = item_of(x, i);
-  };
   // chunk by chunk: kU vectors a thread, the next chunk's loads in flight
+  constexpr int step = NT * kU;
   uint4 nxt[kU];
-  const int64_t step = (int64_t)kThreads * kU;
-  auto fetch = [&](int64_t v0) {
+  auto fetch = [&](int v0) {
+    if (v0 + step <= vb) {
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int64_t v = v0 + u * kThreads + tid;
-      nxt[u] = v < vb ? ldg_nc_v4(base + v * E) : make_uint4(0, 0, 0, 0);
+      for (int u = 0; u < kU; ++u) nxt[u] = ldg_nc_v4(base + (int64_t)(v0 + u * NT + tid) * E);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const int v = v0 + u * NT + tid;
+        nxt[u] = v < vb ? ldg_nc_v4(base + (int64_t)v * E) : make_uint4(0, 0, 0, 0);
+      }
     }
   };
   fetch(va);
-  bool start = true;
-  for (int64_t v0 = va; start || v0 < vb; v0 += step) {
+
+  const int64_t tok = p.tokens[row_i];
+  const bool has = tok >= 0 && tok < V;
+  const float xt = has ? to_f32(row[tok]) : INFINITY;
+  const float c = p.c;
+  const uint64_t c2 = f2_pack(c, c);
+  float ref = -INFINITY, S = 0.f, En = 0.f;
+  int greater = 0;
+  float T0 = INFINITY;   // what a candidate has to exceed
+  float edge = 0.f;      // this thread's element of the ends, number ei
+  int ei = -1;
+  // the first chunk's bound as a key; at or below that of -inf everything is a candidate
+  // (below 0 comes -0, which equals it, and then the largest negative number)
+  constexpr uint32_t kLeastKey = 0x007fffffu, kZeroKey = 0x80000000u;
+  uint32_t first_key = 0;
+
+  auto push = [&](float x, int i) {
+    const int at = atomicAdd(&count, 1);
+    if (at < kCap) cand[at] = item_of(x, i);
+  };
+  // the candidates in order, all but the first `top` dropped; returns how many are left
+  // (more than kCap: too many, and none dropped)
+  auto narrow = [&]() {
+    __syncthreads();
+    const int n = count;
+    if (n > kCap) return n;
+    for (int i = tid; i < n; i += NT) {
+      const uint64_t me = cand[i];
+      int r = 0;
+      for (int j = 0; j < n; ++j) r += cand[j] > me;
+      if (r < p.top) list[r] = me;
+    }
+    __syncthreads();
+    const int left = min(n, p.top);
+    for (int i = tid; i < left; i += NT) cand[i] = list[i];
+    if (tid == 0) count = left;
+    __syncthreads();
+    return left;
+  };
+  // One chunk; FULL: every thread has kU vectors.
+  auto chunk = [&](int v0, auto full) {
+    constexpr bool FULL = decltype(full)::value;
     uint4 cur[kU];
 #pragma unroll
     for (int u = 0; u < kU; ++u) cur[u] = nxt[u];
     if (v0 + step < vb) fetch(v0 + step);
-    float cm = -INFINITY;  // of this thread's elements
-    const bool any = v0 + tid < vb;
+    const int mine = FULL ? kU : max(0, min(kU, (vb - v0 - tid + NT - 1) / NT));
+    float cm = -INFINITY;  // this thread's largest
 #pragma unroll
     for (int u = 0; u < kU; ++u)
-      if (v0 + u * kThreads + tid < vb) cm = fmaxf(cm, Lane<T>::most(cur[u]));
-    if (start) {
+      if (FULL || u < mine) cm = fmaxf(cm, Lane<T>::most(cur[u]));
+    if (v0 == va) {
       // the ends' elements (fewer than 2 E a row) belong to the first chunk, but not to
-      // the bound: one at the row's end loses to equal ones before it
-      float edge = 0.f;
-      int64_t ei = -1;
+      // the bound, and those of the row's end are candidates last: one loses to equal ones
+      // before it
       if (tid < ea - e0) ei = e0 + tid;
-      else if (tid - (ea - e0) < e1 - eb) ei = eb + tid - (ea - e0);
-      uint32_t key = any ? key_of(cm) : 0u, last = 0;
+      else if (tid - max(ea - e0, 0) < e1 - eb) ei = eb + tid - max(ea - e0, 0);
+      uint32_t key = key_of(cm), last = 0;
       if (ei >= 0) {
         edge = to_f32(row[ei]);
         cm = fmaxf(cm, edge);
       }
       const uint32_t first = __reduce_max_sync(0xffffffffu, key_of(cm));
-      const int rounds = TOP ? (p.top + kWarps - 1) / kWarps : 0;
-      for (int r = 0; r < rounds; ++r) {
-        last = __reduce_max_sync(0xffffffffu, key);
-        const uint32_t who = __ballot_sync(0xffffffffu, key == last);
-        if (lane == __ffs(who) - 1) key = 0;
+      const int whole = min(kWarps, (vb - va) / 32);  // warps with data in every lane
+      if (TOP && warp < whole) {
+        const int rounds = min(32, (p.top + whole - 1) / whole);
+        for (int r = 0; r < rounds; ++r) {
+          last = __reduce_max_sync(0xffffffffu, key);
+          const uint32_t who = __ballot_sync(0xffffffffu, key == last);
+          if (lane == __ffs(who) - 1) key = 0;
+        }
       }
       if (lane == 0) {
         wkey[0][warp] = first;
@@ -225,12 +283,15 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(LogprobArgs
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         big = max(big, wkey[0][w]);
-        least = min(least, wkey[1][w]);
+        if (w < whole) least = min(least, wkey[1][w]);
       }
       ref = value_of(big);
-      T0 = least == 0 ? -INFINITY : value_of(least);
+      // (reached, not exceeded, is enough in this chunk: the next value below)
+      first_key = whole * 32 < p.top ? 0u : least;
+      T0 = first_key <= kLeastKey ? -INFINITY
+                                  : value_of(first_key - (first_key == kZeroKey ? 2 : 1));
       if (ei >= 0) {
-        if (TOP && !(edge < T0)) push(edge, ei);
+        if (TOP && ei < eb && (first_key <= kLeastKey || edge > T0)) push(edge, ei);
         if (edge > xt) ++greater;
         if (edge != -INFINITY) {
           const float q = edge - ref, w = ex2_ftz(q * c);
@@ -245,36 +306,41 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(LogprobArgs
       S *= f;
       ref = cm;
     }
-    if (TOP && any && (start ? cm >= T0 : cm > T0)) {
+    const bool all = first_key <= kLeastKey && v0 == va;
+    if (TOP && (cm > T0 || all)) {
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
-        const int64_t v = v0 + u * kThreads + tid;
-        if (v >= vb) break;
-        const float vm = Lane<T>::most(cur[u]);
-        if (!(start ? vm >= T0 : vm > T0)) continue;
+        if (!FULL && u >= mine) break;
+        if (!(Lane<T>::most(cur[u]) > T0 || all)) continue;
         float f[E];
         Lane<T>::get(cur[u], f);
+        uint32_t hits = 0;
 #pragma unroll
-        for (int j = 0; j < E; ++j)
-          if (start ? f[j] >= T0 : f[j] > T0) push(f[j], v * E - shift + j);
+        for (int j = 0; j < E; ++j) hits |= (uint32_t)(f[j] > T0 || all) << j;
+        const int i0 = (v0 + u * NT + tid) * E - shift;
+        while (hits != 0) {
+          const int j = __ffs(hits) - 1;
+          hits &= hits - 1;
+          float x = f[0];
+#pragma unroll
+          for (int k = 1; k < E; ++k) x = j == k ? f[k] : x;
+          push(x, i0 + j);
+        }
       }
     }
     if (cm > xt) {
+      typename Lane<T>::Count above_t(xt);
 #pragma unroll
-      for (int u = 0; u < kU; ++u) {
-        if (v0 + u * kThreads + tid >= vb) break;
-        float f[E];
-        Lane<T>::get(cur[u], f);
-#pragma unroll
-        for (int j = 0; j < E; ++j) greater += f[j] > xt;
-      }
+      for (int u = 0; u < kU; ++u)
+        if (FULL || u < mine) above_t.add(cur[u]);
+      greater += above_t.get();
     }
     if (ref != -INFINITY) {
-      const uint64_t c2 = f2_pack(c, c), r2 = f2_pack(-ref, -ref);
+      const uint64_t r2 = f2_pack(-ref, -ref);
       uint64_t s2[2] = {0ull, 0ull}, e2[2] = {0ull, 0ull};
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
-        if (v0 + u * kThreads + tid >= vb) break;
+        if (!FULL && u >= mine) break;
         float f[E];
         Lane<T>::get(cur[u], f);
 #pragma unroll
@@ -296,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(LogprobArgs
       // nothing but -inf so far, which weighs nothing, or NaN
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
-        if (v0 + u * kThreads + tid >= vb) break;
+        if (!FULL && u >= mine) break;
         float f[E];
         Lane<T>::get(cur[u], f);
 #pragma unroll
@@ -304,8 +370,18 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(LogprobArgs
           if (isnan(f[j])) S = f[j];
       }
     }
-    start = false;
+  };
+  int done = 0, next = 1, v0 = va;
+  for (; v0 + step <= vb; v0 += step) {
+    chunk(v0, std::true_type{});
+    if (TOP && ++done == next && v0 + step < vb) {
+      next *= 2;
+      const int left = narrow();
+      if (left == p.top) T0 = value_of((uint32_t)(cand[left - 1] >> 32));
+    }
   }
+  if (v0 < vb || v0 == va) chunk(v0, std::false_type{});
+  if (TOP && ei >= eb && !(edge < T0)) push(edge, ei);
 
   // ---- the slice's weights and rank
   auto reduce = [&](Stat st) {
@@ -341,7 +417,7 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(LogprobArgs
     // -inf among the logits made 0 * -inf: once more, without those
     const float m = st.m;
     S = En = 0.f;
-    for (int64_t i = e0 + tid; i < e1; i += kThreads) {
+    for (int i = e0 + tid; i < e1; i += NT) {
       const float x = to_f32(row[i]);
       const float q = x - m, w = ex2_ftz(q * c);
       if (w == 0.f) continue;
@@ -354,18 +430,18 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(LogprobArgs
   if (odd) {
     greater = 0;
     const uint32_t kt = key_of(xt);
-    for (int64_t i = e0 + tid; i < e1; i += kThreads) greater += key_of(to_f32(row[i])) > kt;
+    for (int i = e0 + tid; i < e1; i += NT) greater += key_of(to_f32(row[i])) > kt;
   }
   greater = total(greater);  // (its barriers also order the candidates)
 
   // ---- the slice's alternatives, in order
   if constexpr (TOP) {
-    const int K = p.top, n = count;
-    if (odd || n > kCap) {
+    const int K = p.top, n = odd ? kCap + 1 : narrow();
+    if (n > kCap) {
       uint64_t prev = ~0ull;
       for (int k = 0; k < K; ++k) {
         uint64_t best = 0;
-        for (int64_t i = e0 + tid; i < e1; i += kThreads) {
+        for (int i = e0 + tid; i < e1; i += NT) {
           const uint64_t it = item_of(to_f32(row[i]), i);
           if (it < prev && it > best) best = it;
         }
@@ -379,15 +455,8 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(LogprobArgs
         if (tid == 0) list[k] = best;
         prev = best;  // (0, none left, stays 0)
       }
-    } else {
-      if (tid < K) list[tid] = 0;
-      __syncthreads();
-      for (int i = tid; i < n; i += kThreads) {
-        const uint64_t me = cand[i];
-        int r = 0;
-        for (int j = 0; j < n; ++j) r += cand[j] > me;
-        if (r < K) list[r] = me;
-      }
+    } else if (tid >= n && tid < K) {
+      list[tid] = 0;
     }
     __syncthreads();
   }
@@ -409,14 +478,14 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(LogprobArgs
     }
     if constexpr (TOP) {
       const int K = p.top, n = C * K;
-      if (tid < n) cand[tid] = peer_load(&list[tid % K], tid / K);
-      __syncthreads();
-      uint64_t me = tid < n ? cand[tid] : 0;
-      int r = 0;
-      if (me != 0)
+      for (int i = tid; i < n; i += NT) cand[i] = peer_load(&list[i % K], i / K);
+      cluster_sync();  // (its barrier is the CTA's too)
+      for (int i = tid; i < n; i += NT) {
+        const uint64_t me = cand[i];
+        int r = 0;
         for (int j = 0; j < n; ++j) r += cand[j] > me;
-      cluster_sync();
-      if (me != 0 && r < K) list[r] = me;
+        if (me != 0 && r < K) list[r] = me;
+      }
       __syncthreads();
     } else {
       cluster_sync();
@@ -469,18 +538,26 @@ extern "C" int tpp_token_logprobs(const void* logits, int64_t ld, int64_t N, int
   // CTAs a row: enough rows for three on every SM want one each
   int C = 1;
   while (C < kMaxCtas && N * C < 3 * (int64_t)num_sms()) C *= 2;
-  auto go = [&](auto tag) -> int {
+  auto go = [&](auto tag, auto threads) -> int {
     using T = decltype(tag);
+    constexpr int NT = decltype(threads)::value;
     TPP_REQUIRE(reinterpret_cast<uintptr_t>(logits) % sizeof(T) == 0, TPP_ERR_ALIGN,
                 "logits must be aligned to their type");
     return launch("token_logprobs_kernel",
-                  top > 0 ? token_logprobs_kernel<T, true> : token_logprobs_kernel<T, false>,
-                  dim3((unsigned)N, (unsigned)C), dim3(kThreads), 0, as_stream(stream),
+                  top > 0 ? token_logprobs_kernel<T, true, NT> : token_logprobs_kernel<T, false, NT>,
+                  dim3((unsigned)N, (unsigned)C), dim3(NT), 0, as_stream(stream),
                   C > 1 ? (unsigned)C : 0u, a);
   };
-  if (dtype == TPP_F16) return go(__half());
-  if (dtype == TPP_BF16) return go(__nv_bfloat16());
-  if (dtype == TPP_F32) return go(float());
+  auto size = [&](auto tag) -> int {
+    // a thread's chunk is 64 bytes: small slices want few threads, a row over several CTAs
+    // the latency of many, and eight CTAs on an SM hide each other's barriers
+    if (V * (int64_t)sizeof(tag) / C < 128 * 64) return go(tag, std::integral_constant<int, 64>{});
+    if (C < 8) return go(tag, std::integral_constant<int, 128>{});
+    return go(tag, std::integral_constant<int, 256>{});
+  };
+  if (dtype == TPP_F16) return size(__half());
+  if (dtype == TPP_BF16) return size(__nv_bfloat16());
+  if (dtype == TPP_F32) return size(float());
   set_error("tpp_token_logprobs: dtype must be f16, bf16 or f32");
   return TPP_ERR_DTYPE;
 }
