@@ -2,7 +2,7 @@
 // operands: softmax statistics of x W^T in the product's epilogue, the logits never
 // written.
 #include <math.h>
-#include "tc_common.cuh"
+#include "tc_issue.cuh"
 
 namespace tpp {
 namespace {
@@ -97,32 +97,33 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-  } else if (warp == 1 && lane == 0) {
-    // ---------------- MMA issuer ----------------
+  } else if (warp == 1) {
+    // ---------------- MMA issuer (the whole warp, see tc_issue.cuh) ----------------
     const uint32_t idesc = make_idesc_f16(BM, BN, IsBf16<T>::value, 0, 0);
+    const uint32_t tm = (uint32_t)same((int)tmem);
+    const uint32_t a_at = smem_u32(sA), b_at = smem_u32(sB);
+    const bool on = elect_lane();
     int it = 0, j = 0;
-    for (int64_t t = blockIdx.x; t < ntiles && ok; t += gridDim.x, ++j) {
+    for (int64_t t = blockIdx.x; t < ntiles; t += gridDim.x, ++j) {
       const int buf = j & 1;
-      if (j >= 2) ok = mbar_wait(&tempty[buf], ((j >> 1) & 1) ^ 1, p.err, 52);
-      if (!ok) break;
+      if (ok && j >= 2) ok = mbar_wait(&tempty[buf], ((j >> 1) & 1) ^ 1, p.err, 52);
+      if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
-      const uint32_t acc = tmem + (uint32_t)(buf * kMaxBN);
-      for (int kb = 0; kb < nk && ok; ++kb, ++it) {
+      const uint32_t acc = tm + (uint32_t)(buf * kMaxBN);
+      for (int kb = 0; kb < nk; ++kb, ++it) {
         const int s = it % kStages;
-        ok = mbar_wait(&full[s], (it / kStages) & 1, p.err, 53);
-        if (!ok) break;
+        if (ok) ok = mbar_wait(&full[s], (it / kStages) & 1, p.err, 53);
         tc_fence_after();
-        const uint32_t a0 = smem_u32(sA + s * kStageA);
-        const uint32_t b0 = smem_u32(sB + s * kStageB);
+        const uint32_t a0 = desc_lo(a_at + s * kStageA, 16), b0 = desc_lo(b_at + s * kStageB, 16);
 #pragma unroll
         for (int k = 0; k < KS * BK / 16; ++k) {
-          const uint32_t j2 = k >> 2, kk = k & 3;
-          tc_mma_f16(acc, make_sdesc(a0 + j2 * kSubA + kk * 32, 16, 1024, 2),
-                     make_sdesc(b0 + j2 * sub_b + kk * 32, 16, 1024, 2), idesc, (kb | k) != 0);
+          const uint32_t j2 = k >> 2, o = (k & 3) * 32 >> 4;
+          mma_ss(on, acc, a0 + j2 * (kSubA >> 4) + o, b0 + j2 * (sub_b >> 4) + o, idesc,
+                 (kb | k) != 0);
         }
-        tc_commit(&empty[s]);
+        commit(on, &empty[s]);
       }
-      tc_commit(&tfull[buf]);
+      commit(on, &tfull[buf]);
     }
   } else if (warp >= kEpiWarp0) {
     // ---------------- epilogue: one row and half the tile's columns a thread ----------------

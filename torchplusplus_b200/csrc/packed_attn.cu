@@ -23,7 +23,7 @@
 // are zeros and non-finite values are cleared (0 * NaN is NaN) and added to the
 // rows that see them at the end.
 #include <math.h>
-#include "tc_common.cuh"
+#include "tc_issue.cuh"
 #include "mma_common.cuh"
 
 namespace tpp {
@@ -42,20 +42,21 @@ struct Plan {
   static constexpr uint32_t kBox = 128 * 128;       // bytes of a box of 128 rows
   static constexpr uint32_t kTile = kBoxes * kBox;  // a Q, K or V tile
   static constexpr int kStages = D == 128 ? 4 : 8;
-  static constexpr size_t kSmem = 1024 + (2 + kStages) * kTile + 2 * BQ * 4 + kItems * 48 + 512;
+  static constexpr uint32_t kStage = 4 * 32 * 128;  // the epilogue's, 4 KB a warp
+  static constexpr size_t kSmem = 1024 + (2 + kStages) * kTile + kStage + 4 * BQ * 4 + kItems * 48 + 512;
   static_assert(kSmem <= 227 * 1024, "shared memory plan exceeds 227 KB");
 };
 
 struct PackedAttnArgs {
   const int32_t* cu;
   int B, N, Hkv, G, TT;
+  int inv_g;  // ceil(2^16 / G): r * inv_g >> 16 is r / G for r < 128
   int causal;
   int64_t window;
   float scale_log2;
   int sign;  // of the scale: scores are negated (-1) or all equal (0) first
   void* o;
   int64_t o_sn, o_sh;
-  int wide;  // o's rows allow 32-byte stores
   const void* v;
   int64_t v_sn, v_sh;
   int* err;
@@ -155,32 +156,16 @@ struct Walk {
   }
 };
 
-// Matrix descriptors (128-byte swizzle, 8-row groups 1 KB apart) as a low word, which a
-// step along the tile moves, and a high word that never changes.
-constexpr uint32_t kDescHi = (1024u >> 4) | 1u << 14 | 2u << 29;
-__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) {
-  return (addr >> 4) | (lbo >> 4) << 16;
+// Maxima that NaN passes through.
+__device__ __forceinline__ float nanmax(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc,
-                                       uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "mov.b64 a, {%1, %5};\n\t"
-      "mov.b64 b, {%2, %5};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
-      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(kDescHi)
-      : "memory");
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc,
-                                       uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "mov.b64 b, {%2, %5};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(kDescHi)
-      : "memory");
+__device__ __forceinline__ float nanmax(float a, float b, float c) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+  return m;
 }
 
 template <typename T>
@@ -196,11 +181,39 @@ __device__ __forceinline__ uint32_t times_zero_plus(uint32_t w, uint32_t acc) {
   }
 }
 
+// Adds the non-finite values that were cleared to the output row of query tile i's row rl,
+// as far as that row sees them (never but for broken inputs, hence apart).
+template <typename T, int D>
+__device__ __forceinline__ void add_hidden(const Work& w, int i, int rl, const PackedAttnArgs& p) {
+  const int tl = rl / p.G, g = rl - tl * p.G, tok = w.t0 + i * p.TT + tl;
+  if (tl >= p.TT || tok >= w.len) return;
+  T* out = static_cast<T*>(p.o) + (int64_t)(w.first + tok) * p.o_sn +
+           (int64_t)(w.kvh * p.G + g) * p.o_sh;
+#pragma unroll 1
+  for (int j = w.start(i); j < w.end(i); ++j) {
+    if (!w.part(j)) continue;
+#pragma unroll 1
+    for (int k = 0; k < BKV; ++k) {
+      const int key = (w.kb + j) * BKV + k;
+      if (key >= w.len || (p.causal && key > tok) || (p.window >= 0 && key < tok - p.window))
+        continue;
+      const T* v = static_cast<const T*>(p.v) + (int64_t)(w.first + key) * p.v_sn +
+                   (int64_t)w.kvh * p.v_sh;
+#pragma unroll 1
+      for (int c = 0; c < D; ++c) {
+        const float e = to_f32(v[c]);
+        if (!isfinite(e)) out[c] = from_f32<T>(to_f32(out[c]) + e);
+      }
+    }
+  }
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
     packed_attn_kernel(const __grid_constant__ CUtensorMap tm_q,
                        const __grid_constant__ CUtensorMap tm_k,
-                       const __grid_constant__ CUtensorMap tm_v, PackedAttnArgs p) {
+                       const __grid_constant__ CUtensorMap tm_v,
+                       const __grid_constant__ PackedAttnArgs p) {
   using P = Plan<D>;
   constexpr int S = P::kStages;
   extern __shared__ uint8_t smem_raw[];
@@ -208,23 +221,26 @@ __global__ void __launch_bounds__(kThreads, 1)
                                              ~(uintptr_t)1023);
   uint8_t* sQ = smem;                      // 2 tiles
   uint8_t* sKV = smem + 2 * P::kTile;      // ring: K_0, V_0, K_1, V_1, ... across items
-  float* sc = reinterpret_cast<float*>(sKV + S * P::kTile);  // [2][BQ] factors, then sums
-  Work* items = reinterpret_cast<Work*>(sc + 2 * BQ);
+  uint8_t* stage = sKV + S * P::kTile;
+  float* sc = reinterpret_cast<float*>(stage + P::kStage);  // [2][BQ] factors of O
+  float* sums = sc + 2 * BQ;                                 // [2][BQ]
+  Work* items = reinterpret_cast<Work*>(sums + 2 * BQ);
   uint64_t* bars = reinterpret_cast<uint64_t*>(items + kItems);
   uint64_t* q_full = bars;             // 2
   uint64_t* q_empty = q_full + 2;      // 2: the item's last S_i is done
   uint64_t* s_full = q_empty + 2;      // 2: S_i (and every product before it) is done
   uint64_t* p_ready = s_full + 2;      // 2: P_i written (4 warps), O_i rescaled (4 warps)
   uint64_t* sc_full = p_ready + 2;     // 2
-  uint64_t* sc_empty = sc_full + 2;    // 2
-  uint64_t* o_full = sc_empty + 2;     // 2: the item's last P_i V is done
+  uint64_t* l_full = sc_full + 2;      // 2
+  uint64_t* l_empty = l_full + 2;      // 2
+  uint64_t* o_full = l_empty + 2;      // 2: the item's last P_i V is done
   uint64_t* it_full = o_full + 2;      // kItems
   uint64_t* it_empty = it_full + kItems;
   uint64_t* kv_full = it_empty + kItems;  // S
   uint64_t* kv_empty = kv_full + S;       // S
   uint64_t* v_ok = kv_empty + S;          // S: a masked V tile is finite
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_ok + S);
-  int* odd_v = reinterpret_cast<int*>(tmem_slot + 1);  // the item's V had non-finite values
+  int* odd_v = reinterpret_cast<int*>(tmem_slot + 1);  // [2]: item whose V had non-finite values
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -238,7 +254,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&s_full[i], 1);
       mbar_init(&p_ready[i], 8);
       mbar_init(&sc_full[i], 4);
-      mbar_init(&sc_empty[i], 4);
+      mbar_init(&l_full[i], 4);
+      mbar_init(&l_empty[i], 4);
       mbar_init(&o_full[i], 1);
     }
     for (int i = 0; i < kItems; ++i) {
@@ -250,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&kv_empty[s], 1);
       mbar_init(&v_ok[s], 4);
     }
-    *odd_v = 0;
+    odd_v[0] = odd_v[1] = 0;
     fence_mbar_init();
   }
   if (warp == kMmaWarp) tmem_alloc(tmem_slot, 512);
@@ -274,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     return w;
   };
 
-  // (one instruction for a whole warpgroup; 2 x 184 + 80 + 64 = 4 x 128, what the launch has)
+  // (one instruction for a whole warpgroup; 2 x 176 + 96 + 64 = 4 x 128, what the launch has)
   if (warp >= kMmaWarp) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
   if (warp == kSchedWarp) {
@@ -297,7 +314,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == kTmaWarp) {
     // ---------------- loads ----------------
-    int nq[2] = {0, 0}, ring = 0;
+    uint32_t nq = 0;  // loads of each Q tile: bit i its parity, bit 2 + i whether any
+    int ring = 0;
     const uint32_t q_box = (uint32_t)(p.G * p.TT) * 128;
     for (int n = 0; ok; ++n) {
       const Work w = take(n);
@@ -313,16 +331,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++ring;
       };
       load(&tm_k, 0);
-#pragma unroll
+#pragma unroll 1
       for (int i = 0; i < 2; ++i) {
         if (w.end(i) <= w.start(i)) continue;
-        if (nq[i] > 0) ok = ok && mbar_wait(&q_empty[i], (nq[i] & 1) ^ 1, p.err, 64);
+        if (nq >> (2 + i) & 1) ok = ok && mbar_wait(&q_empty[i], (nq >> i & 1) ^ 1, p.err, 64);
         if (!ok) break;
         mbar_arrive_expect_tx(&q_full[i], P::kBoxes * q_box);
         for (int b = 0; b < P::kBoxes; ++b)
           tma_load_3d(sQ + i * P::kTile + b * P::kBox, &tm_q, &q_full[i], b * 64, w.kvh * p.G,
                       w.first + w.t0 + i * p.TT);
-        ++nq[i];
+        nq = (nq ^ 1u << i) | 4u << i;
       }
       for (int j = 0; j < w.nt && ok; ++j) {
         load(&tm_v, j);
@@ -333,91 +351,109 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------- products ----------------
     constexpr uint32_t idesc_s = make_idesc_f16(BQ, BKV, IsBf16<T>::value, 0, 0);
     constexpr uint32_t idesc_o = make_idesc_f16(BQ, D, IsBf16<T>::value, 0, 1);
-    int nq[2] = {0, 0}, np[2] = {0, 0}, ring = 0;  // ring: the next K or V tile's number
-    const uint32_t q_at = smem_u32(sQ), kv_at = smem_u32(sKV);
-    // S_i of the item's key tile in ring slot r; `last`: of this item and query tile
-    auto issue_s = [&](int i, int r, bool first, bool last) {
+    const bool on = elect_lane();
+    const uint32_t q_at = smem_u32(sQ), kv_at = smem_u32(sKV), tm = (uint32_t)same((int)tmem);
+    // a wait that ran out ends the loops at the next step, not at once
+    auto wait = [&](uint64_t* bar, int parity, int code) {
+      if (ok) ok = mbar_wait(bar, (uint32_t)parity & 1, p.err, code);
+    };
+    int ring = 1;  // the next V tile's number
+    // parities, a bit each: Q_i's loads, P_i's steps, the clearings of a ring slot's V
+    uint32_t nq = 0, np = 0, seen = 0;
+    // S_i of the item's key tile in ring slot s, which has landed; `last`: of this item and
+    // query tile
+    auto issue_s = [&](int i, int s, bool first, bool last) {
       if (first) {
-        ok = ok && mbar_wait(&q_full[i], nq[i] & 1, p.err, 65);
-        ++nq[i];
+        wait(&q_full[i], (int)(nq >> i), 65);
+        nq ^= 1u << i;
+        tc_fence_after();
       }
-      const int s = r % S;
-      ok = ok && mbar_wait(&kv_full[s], (r / S) & 1, p.err, 66);
-      if (!ok) return;
-      tc_fence_after();
       const uint32_t qa = desc_lo(q_at + i * P::kTile, 16), ka = desc_lo(kv_at + s * P::kTile, 16);
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
         const uint32_t o = ((kk >> 2) * P::kBox + (kk & 3) * 32) >> 4;
-        mma_ss(tmem + i * 128, qa + o, ka + o, idesc_s, kk != 0);
+        mma_ss(on, tm + i * 128, qa + o, ka + o, idesc_s, kk != 0);
       }
-      tc_commit(&s_full[i]);
-      if (last) tc_commit(&q_empty[i]);
+      commit(on, &s_full[i]);
+      if (last) commit(on, &q_empty[i]);
     };
-    uint32_t seen = 0;  // bit: parity of the clearings of a ring slot's V
-    Work cur = take(0);
-    bool more = ok && cur.len >= 0;
-    if (more && lane == 0) {
-#pragma unroll
+    // what this warp needs of an item
+    auto tiles = [&](int n) {
+      Work w = take(n);
+      w.len = same(w.len);
+      w.nt = same(w.nt);
+      w.start1 = same(w.start1);
+      w.end0 = same(w.end0);
+      w.end1 = same(w.end1);
+      w.low = same(w.low);
+      w.high = same(w.high);
+      return w;
+    };
+    Work cur = tiles(0);
+    bool more = __all_sync(0xffffffffu, ok) && cur.len >= 0;
+    if (more) {
+      wait(&kv_full[0], 0, 66);
+      tc_fence_after();
+#pragma unroll 1
       for (int i = 0; i < 2; ++i)
         if (cur.active(i, 0)) issue_s(i, 0, true, cur.end(i) == 1);
-      if (ok) tc_commit(&kv_empty[0]);
+      commit(on, &kv_empty[0]);
     }
-    ring = 1;
     for (int n = 1; more; ++n) {
-      const Work nxt = take(n);
-      if (!ok) break;
+      const Work nxt = tiles(n);
       const bool follows = nxt.len >= 0;
-      if (lane == 0) {
-        for (int j = 0; j < cur.nt && ok; ++j) {
-          const int rv = ring, rk = ring + 1, s = rv % S;  // V_j, then K_{j+1} or the next item's K_0
-          const bool part = cur.part(j);
+      more = follows;
+      for (int j = 0; j < cur.nt; ++j) {
+        // V_j, then K_{j+1} or the next item's K_0.  Their waits, and all else that does not
+        // hang on the softmax, come here, while the last step's products run: any wait
+        // takes 200 clocks (the softmax warps' exponentials fill the queue that barriers go
+        // through too)
+        const int rv = ring, rk = ring + 1, s = rv % S, sk = rk % S;
+        const bool part = cur.part(j), goes = j + 1 < cur.nt || follows;
+        wait(&kv_full[s], rv / S, 68);
+        if (goes) wait(&kv_full[sk], rk / S, 66);
+        if (part) wait(&v_ok[s], (int)(seen >> s), 69);
+        if (!__all_sync(0xffffffffu, ok)) {
+          more = false;
+          break;
+        }
+        const uint32_t va = desc_lo(kv_at + s * P::kTile, P::kBox);
+#pragma unroll 1
+        for (int i = 0; i < 2; ++i) {
+          if (cur.active(i, j)) {
+            wait(&p_ready[i], (int)(np >> i), 67);
+            tc_fence_after();
+            const uint32_t pa = tm + i * 128, oa = tm + 256 + i * 128;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (cur.active(i, j)) {
-              ok = ok && mbar_wait(&p_ready[i], np[i] & 1, p.err, 67);
-              ++np[i];
-              ok = ok && mbar_wait(&kv_full[s], (rv / S) & 1, p.err, 68);
-              if (part) ok = ok && mbar_wait(&v_ok[s], seen >> s & 1, p.err, 69);
-              if (!ok) break;
-              tc_fence_after();
-              const uint32_t va = desc_lo(kv_at + s * P::kTile, P::kBox);
-              const uint32_t pa = tmem + i * 128, oa = tmem + 256 + i * 128;
-#pragma unroll
-              for (int kk = 0; kk < BKV / 16; ++kk)
-                mma_ts(oa, pa + kk * 8, va + kk * (2048 >> 4), idesc_o,
-                       j > cur.start(i) || kk != 0);
-              if (j == cur.end(i) - 1) tc_commit(&o_full[i]);
-            }
-            if (j + 1 < cur.nt) {
-              if (cur.active(i, j + 1))
-                issue_s(i, rk, j + 1 == cur.start(i), j + 2 == cur.end(i));
-            } else if (follows && nxt.active(i, 0)) {
-              issue_s(i, rk, true, nxt.end(i) == 1);
-            }
+            for (int kk = 0; kk < BKV / 16; ++kk)
+              mma_ts(on, oa, pa + kk * 8, va + kk * (2048 >> 4), idesc_o,
+                     j > cur.start(i) || kk != 0);
+            np ^= 1u << i;
+            if (j == cur.end(i) - 1) commit(on, &o_full[i]);
           }
-          if (!ok) break;
-          if (part) seen ^= 1u << s;
-          tc_commit(&kv_empty[s]);
-          ring = rk;
-          if (j + 1 < cur.nt || follows) {
-            tc_commit(&kv_empty[rk % S]);
-            ring = rk + 1;
+          if (j + 1 < cur.nt) {
+            if (cur.active(i, j + 1)) issue_s(i, sk, j + 1 == cur.start(i), j + 2 == cur.end(i));
+          } else if (follows && nxt.active(i, 0)) {
+            issue_s(i, sk, true, nxt.end(i) == 1);
           }
         }
+        if (part) seen ^= 1u << s;
+        commit(on, &kv_empty[s]);
+        ring = rk;
+        if (goes) {
+          commit(on, &kv_empty[sk]);
+          ring = rk + 1;
+        }
       }
-      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-      ring = __shfl_sync(0xffffffffu, ring, 0);
-      more = ok && follows;
       cur = nxt;
     }
   }
   } else if (warp < kCorrWarp0) {
     // ---------------- softmax ----------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
     const int i = warp >> 2, rl = (warp & 3) * 32 + lane;
     const uint32_t tS = tmem + i * 128 + ((uint32_t)((warp & 3) * 32) << 16);
-    int ns = 0, nc = 0;
+    int ns = 0, nl = 0;
     for (int n = 0; ok; ++n) {
       const Work w = take(n);
       if (!ok || w.len < 0) break;
@@ -445,30 +481,34 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (w.part(j)) {
           const int key0 = (w.kb + j) * BKV;
           const int hi = (p.causal ? min(qpos, w.len - 1) : w.len - 1) - key0;
-          const int64_t lo64 = p.window >= 0 ? (int64_t)qpos - p.window - key0 : 0;
-          const int lo = (int)max((int64_t)0, lo64);
+          const int lo = p.window >= 0 ? (int)max((int64_t)0, qpos - p.window - key0) : 0;
 #pragma unroll
-          for (int k = 0; k < BKV; ++k)
-            if (k > hi || k < lo) sv[k] = -INFINITY;
+          for (int k0 = 0; k0 < BKV; k0 += 32) {
+            // the visible keys lo .. hi of these 32 as bits
+            const int h = min(max(hi - k0 + 1, 0), 32), b = min(max(lo - k0, 0), 32);
+            const uint32_t see = (uint32_t)((1ull << h) - 1) & ~(uint32_t)((1ull << b) - 1);
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (!(see & 1u << k)) sv[k0 + k] = -INFINITY;
+          }
         }
         float pm[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) pm[u] = fmaxf(sv[u], sv[8 + u]);
+        for (int u = 0; u < 8; ++u) pm[u] = nanmax(sv[u], sv[8 + u]);
 #pragma unroll
         for (int k = 16; k < BKV; k += 16)
 #pragma unroll
-          for (int u = 0; u < 8; ++u) pm[u] = fmax3(pm[u], sv[k + u], sv[k + 8 + u]);
-        const float mx = fmax3(fmax3(pm[0], pm[1], pm[2]), fmax3(pm[3], pm[4], pm[5]),
-                               fmaxf(pm[6], pm[7])) * p.scale_log2;
+          for (int u = 0; u < 8; ++u) pm[u] = nanmax(pm[u], sv[k + u], sv[k + 8 + u]);
+        const float mx = nanmax(nanmax(pm[0], pm[1], pm[2]), nanmax(pm[3], pm[4], pm[5]),
+                                nanmax(pm[6], pm[7])) * p.scale_log2;
         float corr = 1.f;
-        if (mx > m_ref + kMoves) {  // (the first finite one too)
+        if (!(mx <= m_ref + kMoves)) {  // (the first finite one too; NaN)
           corr = m_ref == -INFINITY ? 0.f : exp2f(m_ref - mx);
           l *= corr;
-          m_ref = mx;
+          m_ref = mx + (mx - mx);  // (infinite scores make a row NaN)
         }
-        if (nc > 0) ok = ok && mbar_wait(&sc_empty[i], (nc & 1) ^ 1, p.err, 71);
-        ++nc;
-        if (!ok) break;
+        // (the last factor has been read: its reader let P_i V of that step go, and S_i of
+        // this step came behind that)
         sc[i * BQ + rl] = corr;
         tc_fence_before();
         __syncwarp();
@@ -483,9 +523,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int k = 0; k < 32; k += 2) {
             float a0, a1;
             f2_unpack(f2_fma(f2_pack(sv[k0 + k], sv[k0 + k + 1]), sc2, nm2), a0, a1);
-            const float p0 = ex2_ftz(a0), p1 = ex2_ftz(a1);
-            ps[(k >> 1) & 3] = f2_add(ps[(k >> 1) & 3], f2_pack(p0, p1));
-            pk[k / 2] = pack2<T>(p0, p1);
+            a0 = ex2_ftz(a0);
+            a1 = ex2_ftz(a1);
+            ps[(k >> 1) & 3] = f2_add(ps[(k >> 1) & 3], f2_pack(a0, a1));
+            pk[k / 2] = pack2<T>(a0, a1);
           }
           tmem_st16(tS + k0 / 2, pk);
         }
@@ -498,19 +539,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         l += a0 + a1;
       }
       if (!ok) break;
-      ok = ok && mbar_wait(&sc_empty[i], (nc & 1) ^ 1, p.err, 72);
-      ++nc;
+      if (nl > 0) ok = ok && mbar_wait(&l_empty[i], (nl & 1) ^ 1, p.err, 72);
+      ++nl;
       if (!ok) break;
-      sc[i * BQ + rl] = l;
+      sums[i * BQ + rl] = l;
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sc_full[i]);
+      if (lane == 0) mbar_arrive(&l_full[i]);
     }
   } else {
     // ---------------- O ----------------
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     const int rl = (warp & 3) * 32 + lane;
     const uint32_t tO = tmem + 256 + ((uint32_t)((warp & 3) * 32) << 16);
-    int nc[2] = {0, 0}, no[2] = {0, 0}, ring = 1;  // ring: V_0's number
+    uint32_t nc = 0, no = 0;  // parities of the factors' and the ends' messages, bit i
+    int ring = 1;             // V_0's number
     for (int n = 0; ok; ++n) {
       const Work w = take(n);
       if (!ok || w.len < 0) break;
@@ -522,36 +564,33 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int s = ring % S;
           ok = ok && mbar_wait(&kv_full[s], (ring / S) & 1, p.err, 73);
           if (!ok) break;
-          uint8_t* tile = sKV + s * P::kTile;
-          const int key = (w.kb + j) * BKV + rl;
-          bool wrote = false;
-          if (key >= w.len) {
+          uint8_t* at = sKV + s * P::kTile + rl * 128;
+          bool wrote = (w.kb + j) * BKV + rl >= w.len;
+          // (chunks in the order that keeps eight rows on different banks)
+          if (wrote) {
 #pragma unroll
             for (int c = 0; c < D / 8; ++c)
-              *reinterpret_cast<uint4*>(tile + (c >> 3) * P::kBox + rl * 128 + (c & 7) * 16) =
+              *reinterpret_cast<uint4*>(at + (c >> 3) * P::kBox + ((c ^ rl) & 7) * 16) =
                   make_uint4(0, 0, 0, 0);
-            wrote = true;
           } else {
-            uint32_t acc = 0;
+            uint32_t acc[4] = {0, 0, 0, 0};  // 0 or NaN
 #pragma unroll
             for (int c = 0; c < D / 8; ++c) {
-              // (in the order that keeps eight rows on different banks)
-              const uint4 u = *reinterpret_cast<const uint4*>(
-                  tile + (c >> 3) * P::kBox + rl * 128 + ((c ^ rl) & 7) * 16);
-              acc = times_zero_plus<T>(u.x, acc);
-              acc = times_zero_plus<T>(u.y, acc);
-              acc = times_zero_plus<T>(u.z, acc);
-              acc = times_zero_plus<T>(u.w, acc);
+              const uint4 u = *reinterpret_cast<const uint4*>(at + (c >> 3) * P::kBox +
+                                                              ((c ^ rl) & 7) * 16);
+              acc[0] = times_zero_plus<T>(u.x, acc[0]);
+              acc[1] = times_zero_plus<T>(u.y, acc[1]);
+              acc[2] = times_zero_plus<T>(u.z, acc[2]);
+              acc[3] = times_zero_plus<T>(u.w, acc[3]);
             }
-            if ((acc & 0x7fff7fffu) != 0) {  // 0 or NaN
-              T* e = nullptr;
-              for (int c = 0; c < D / 8; ++c) {
-                e = reinterpret_cast<T*>(tile + (c >> 3) * P::kBox + rl * 128 + (c & 7) * 16);
-                for (int q = 0; q < 8; ++q)
-                  if (!isfinite(to_f32(e[q]))) e[q] = from_f32<T>(0.f);
+            if (((acc[0] | acc[1] | acc[2] | acc[3]) & 0x7fff7fffu) != 0) {
+#pragma unroll 1
+              for (int c = 0; c < D; ++c) {
+                T* e = reinterpret_cast<T*>(at + (c >> 6) * P::kBox) + (c & 63);
+                if (!isfinite(to_f32(*e))) *e = from_f32<T>(0.f);
               }
               wrote = true;
-              atomicExch(odd_v, n + 1);
+              atomicExch(odd_v + (n & 1), n + 1);
             }
           }
           if (wrote) fence_proxy_async_smem();
@@ -559,26 +598,24 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (lane == 0) mbar_arrive(&v_ok[s]);
           cleared = true;
         }
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < 2; ++i) {
           if (!w.active(i, j)) continue;
-          ok = ok && mbar_wait(&sc_full[i], nc[i] & 1, p.err, 74);
-          ++nc[i];
+          ok = ok && mbar_wait(&sc_full[i], nc >> i & 1, p.err, 74);
+          nc ^= 1u << i;
           if (!ok) break;
           tc_fence_after();
           const float f = sc[i * BQ + rl];
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sc_empty[i]);
           if (j > w.start(i) && __any_sync(0xffffffffu, f != 1.f)) {
             // S_i of this step was issued behind P_i V of the last: O_i is at rest
 #pragma unroll
-            for (int c = 0; c < D; c += 32) {
-              uint32_t r[32];
-              tmem_ld32(tO + i * 128 + c, r);
+            for (int c = 0; c < D; c += 16) {
+              uint32_t r[16];
+              tmem_ld16(tO + i * 128 + c, r);
               tmem_wait_ld();
 #pragma unroll
-              for (int q = 0; q < 32; ++q) r[q] = __float_as_uint(__uint_as_float(r[q]) * f);
-              tmem_st32(tO + i * 128 + c, r);
+              for (int q = 0; q < 16; ++q) r[q] = __float_as_uint(__uint_as_float(r[q]) * f);
+              tmem_st16(tO + i * 128 + c, r);
             }
             tmem_wait_st();
           }
@@ -589,77 +626,60 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       // the sums, both at once, so that the next item's softmax can go on
-      float inv[2] = {0.f, 0.f};
-#pragma unroll
+      float inv0 = 0.f, inv1 = 0.f;
+#pragma unroll 1
       for (int i = 0; i < 2; ++i) {
         if (w.end(i) <= w.start(i)) continue;
-        ok = ok && mbar_wait(&sc_full[i], nc[i] & 1, p.err, 75);
-        ++nc[i];
+        ok = ok && mbar_wait(&l_full[i], no >> i & 1, p.err, 75);
         if (!ok) break;
-        const float l = sc[i * BQ + rl];
-        inv[i] = l == 0.f ? 0.f : 1.f / l;
+        const float l = sums[i * BQ + rl];
+        (i ? inv1 : inv0) = l == 0.f ? 0.f : 1.f / l;
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sc_empty[i]);
+        if (lane == 0) mbar_arrive(&l_empty[i]);
       }
-      const bool add = ok && cleared && *reinterpret_cast<volatile int*>(odd_v) == n + 1;
-#pragma unroll
+#pragma unroll 1
       for (int i = 0; i < 2; ++i) {
         if (w.end(i) <= w.start(i)) continue;
-        ok = ok && mbar_wait(&o_full[i], no[i] & 1, p.err, 76);
-        ++no[i];
+        ok = ok && mbar_wait(&o_full[i], no >> i & 1, p.err, 76);
+        no ^= 1u << i;
         if (!ok) break;
         tc_fence_after();
-        const int tl = rl / p.G, g = rl - tl * p.G;
-        const int tok = w.t0 + i * p.TT + tl;
-        const bool mine = tl < p.TT && tok < w.len;
-        T* out = static_cast<T*>(p.o) + (int64_t)(w.first + tok) * p.o_sn +
-                 (int64_t)(w.kvh * p.G + g) * p.o_sh;
+        const float inv = i ? inv1 : inv0;
+        const int tok0 = w.t0 + i * p.TT, rows = min(p.TT, w.len - tok0);
+        T* out = static_cast<T*>(p.o) + (int64_t)(w.first + tok0) * p.o_sn +
+                 (int64_t)w.kvh * p.G * p.o_sh + (lane & 7) * 8;
+        // 64 dims at a time through this warp's 4 KB, so that a store covers whole rows
+        uint8_t* st = stage + (warp & 3) * 4096;
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          uint32_t r[32];
-          tmem_ld32(tO + i * 128 + c, r);
-          tmem_wait_ld();
-          float f[32];
+        for (int c = 0; c < D; c += 64) {
+          __syncwarp();
 #pragma unroll
-          for (int q = 0; q < 32; ++q) f[q] = __uint_as_float(r[q]) * inv[i];
-          if (add && mine) {
-            for (int j = w.start(i); j < w.end(i); ++j) {
-              if (!w.part(j)) continue;
-              for (int k = 0; k < BKV; ++k) {
-                const int key = (w.kb + j) * BKV + k;
-                if (key >= w.len || (p.causal && key > tok) ||
-                    (p.window >= 0 && key < tok - p.window))
-                  continue;
-                const T* v = static_cast<const T*>(p.v) + (int64_t)(w.first + key) * p.v_sn +
-                             (int64_t)w.kvh * p.v_sh + c;
+          for (int h = 0; h < 64; h += 16) {
+            uint32_t r[16];
+            tmem_ld16(tO + i * 128 + c + h, r);
+            tmem_wait_ld();
+            float f[16];
 #pragma unroll
-                for (int q = 0; q < 32; ++q) {
-                  const float e = to_f32(v[q]);
-                  if (!isfinite(e)) f[q] += e;
-                }
-              }
-            }
+            for (int q = 0; q < 16; ++q) f[q] = __uint_as_float(r[q]) * inv;
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+              *reinterpret_cast<uint4*>(st + lane * 128 + (((h >> 3) + q) ^ (lane & 7)) * 16) =
+                  pack8<T>(f + q * 8);
           }
-          if (mine) {
-            const uint4 a = pack8<T>(f), b = pack8<T>(f + 8), d = pack8<T>(f + 16),
-                        e = pack8<T>(f + 24);
-            if (p.wide) {
-              asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(out + c),
-                           "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z),
-                           "r"(b.w)
-                           : "memory");
-              asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(out + c + 16),
-                           "r"(d.x), "r"(d.y), "r"(d.z), "r"(d.w), "r"(e.x), "r"(e.y), "r"(e.z),
-                           "r"(e.w)
-                           : "memory");
-            } else {
-              uint4* o4 = reinterpret_cast<uint4*>(out + c);
-              o4[0] = a;
-              o4[1] = b;
-              o4[2] = d;
-              o4[3] = e;
-            }
+          __syncwarp();
+#pragma unroll 2
+          for (int q = 0; q < 8; ++q) {
+            const int r = q * 4 + (lane >> 3), row = (warp & 3) * 32 + r;
+            const int tl = row * p.inv_g >> 16;
+            const uint4 u = *reinterpret_cast<const uint4*>(st + r * 128 + ((lane ^ r) & 7) * 16);
+            if (tl < rows)
+              *reinterpret_cast<uint4*>(out + tl * p.o_sn + (row - tl * p.G) * p.o_sh + c) = u;
           }
+        }
+        // (set, if at all, before the last P V could be issued)
+        if (cleared && *reinterpret_cast<volatile int*>(odd_v + (n & 1)) == n + 1) {
+          __syncwarp();
+          add_hidden<T, D>(w, i, rl, p);
         }
         tc_fence_before();
       }
@@ -698,12 +718,12 @@ extern "C" int tpp_attention_packed(const void* q, int64_t q_sn, int64_t q_sh, c
   a.B = (int)B; a.N = (int)N; a.Hkv = (int)Hkv;
   a.G = (int)(Hq / Hkv);
   a.TT = BQ / a.G;
+  a.inv_g = (65536 + a.G - 1) / a.G;
   a.causal = causal != 0;
   a.window = window_left < 0 ? -1 : window_left < N ? window_left : N;
   a.sign = scale > 0 ? 1 : scale < 0 ? -1 : 0;
   a.scale_log2 = scale == 0 ? 1.f : fabsf(scale) * 1.4426950408889634f;
   a.o = o; a.o_sn = o_sn; a.o_sh = o_sh;
-  a.wide = ((o_sn | o_sh) & 15) == 0 && (reinterpret_cast<uintptr_t>(o) & 31) == 0;
   a.v = v; a.v_sn = v_sn; a.v_sh = v_sh;
   a.err = device_error_flag();
   CUtensorMap tq, tk, tv;
