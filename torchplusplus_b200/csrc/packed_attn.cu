@@ -7,15 +7,15 @@
 // tile's 128 rows are (token, head of the group), so short prompts and wide groups fill
 // it, and each K/V tile is read once for two query tiles.  512 threads:
 //   warps 0-3, 4-7 : softmax of query tile 0, 1: a thread owns a row, 128 scores a step
-//                    (running maximum that only moves when it grows by more than 2^8,
-//                    sums in 32 bits), P written over S in TMEM in the storage type.
-//   warps 8-11     : rescale O where a row's maximum moved, make masked V tiles finite,
-//                    and at the end write O / l.
+//                    (running maximum that only moves, and O with it, when it grows by
+//                    more than 2^8, sums in 32 bits), P over S in TMEM in the storage type.
+//   warps 8-11     : write O / l at an item's end, while the next one runs.
 //   warp 12        : MMA issuer.  S_i = Q_i K_j^T and O_i += P_i V_j, in the order
 //                    PV_0, S_0, PV_1, S_1: while one tile's softmax runs the tensor
 //                    core has the other tile's products, across items too.
 //   warp 13        : TMA: Q tiles, and K and V tiles of 128 keys through one ring.
 //   warp 14        : hands out the items, blocks with the most keys first.
+//   warp 15        : makes V tiles finite that some row sees only a part of.
 // TMEM: S/P 0 and 1 in columns [0, 256), O 0 and 1 in [256, 512).
 //
 // What a row does not see has no effect on it, NaN and infinities included: masked
@@ -42,8 +42,8 @@ struct Plan {
   static constexpr uint32_t kBox = 128 * 128;       // bytes of a box of 128 rows
   static constexpr uint32_t kTile = kBoxes * kBox;  // a Q, K or V tile
   static constexpr int kStages = D == 128 ? 4 : 8;
-  static constexpr uint32_t kStage = 4 * 32 * 128;  // the epilogue's, 4 KB a warp
-  static constexpr size_t kSmem = 1024 + (2 + kStages) * kTile + kStage + 4 * BQ * 4 + kItems * 48 + 512;
+  static constexpr uint32_t kStage = kTile;         // an output tile's
+  static constexpr size_t kSmem = 1024 + (2 + kStages) * kTile + kStage + 2 * BQ * 4 + kItems * 48 + 512;
   static_assert(kSmem <= 227 * 1024, "shared memory plan exceeds 227 KB");
 };
 
@@ -222,23 +222,23 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* sQ = smem;                      // 2 tiles
   uint8_t* sKV = smem + 2 * P::kTile;      // ring: K_0, V_0, K_1, V_1, ... across items
   uint8_t* stage = sKV + S * P::kTile;
-  float* sc = reinterpret_cast<float*>(stage + P::kStage);  // [2][BQ] factors of O
-  float* sums = sc + 2 * BQ;                                 // [2][BQ]
+  float* sums = reinterpret_cast<float*>(stage + P::kStage);  // [2][BQ]
   Work* items = reinterpret_cast<Work*>(sums + 2 * BQ);
   uint64_t* bars = reinterpret_cast<uint64_t*>(items + kItems);
   uint64_t* q_full = bars;             // 2
   uint64_t* q_empty = q_full + 2;      // 2: the item's last S_i is done
   uint64_t* s_full = q_empty + 2;      // 2: S_i (and every product before it) is done
-  uint64_t* p_ready = s_full + 2;      // 2: P_i written (4 warps), O_i rescaled (4 warps)
-  uint64_t* sc_full = p_ready + 2;     // 2
-  uint64_t* l_full = sc_full + 2;      // 2
+  uint64_t* p_ready = s_full + 2;      // 2: P_i written
+  uint64_t* l_full = p_ready + 2;      // 2: the item's sums
   uint64_t* l_empty = l_full + 2;      // 2
   uint64_t* o_full = l_empty + 2;      // 2: the item's last P_i V is done
-  uint64_t* it_full = o_full + 2;      // kItems
+  uint64_t* o_empty = o_full + 2;      // 2: its O_i has been read
+  uint64_t* it_full = o_empty + 2;      // kItems
   uint64_t* it_empty = it_full + kItems;
   uint64_t* kv_full = it_empty + kItems;  // S
   uint64_t* kv_empty = kv_full + S;       // S
-  uint64_t* v_ok = kv_empty + S;          // S: a masked V tile is finite
+  uint64_t* v_sent = kv_empty + S;        // S: a masked V tile is on its way
+  uint64_t* v_ok = v_sent + S;            // S: it is finite
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_ok + S);
   int* odd_v = reinterpret_cast<int*>(tmem_slot + 1);  // [2]: item whose V had non-finite values
 
@@ -252,20 +252,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_ready[i], 8);
-      mbar_init(&sc_full[i], 4);
+      mbar_init(&p_ready[i], 4);
       mbar_init(&l_full[i], 4);
       mbar_init(&l_empty[i], 4);
       mbar_init(&o_full[i], 1);
+      mbar_init(&o_empty[i], 4);
     }
     for (int i = 0; i < kItems; ++i) {
       mbar_init(&it_full[i], 1);
-      mbar_init(&it_empty[i], 14);
+      mbar_init(&it_empty[i], 15);
     }
     for (int s = 0; s < S; ++s) {
       mbar_init(&kv_full[s], 1);
       mbar_init(&kv_empty[s], 1);
-      mbar_init(&v_ok[s], 4);
+      mbar_init(&v_sent[s], 1);
+      mbar_init(&v_ok[s], 1);
     }
     odd_v[0] = odd_v[1] = 0;
     fence_mbar_init();
@@ -344,6 +345,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       for (int j = 0; j < w.nt && ok; ++j) {
         load(&tm_v, j);
+        if (ok && w.part(j)) mbar_arrive(&v_sent[(ring - 1) % S]);
         if (j + 1 < w.nt && ok) load(&tm_k, j + 1);
       }
     }
@@ -360,6 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int ring = 1;  // the next V tile's number
     // parities, a bit each: Q_i's loads, P_i's steps, the clearings of a ring slot's V
     uint32_t nq = 0, np = 0, seen = 0;
+    uint32_t no = 0;  // items of each query tile: bit i their parity, bit 2 + i whether any
     // S_i of the item's key tile in ring slot s, which has landed; `last`: of this item and
     // query tile
     auto issue_s = [&](int i, int s, bool first, bool last) {
@@ -421,6 +424,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
         for (int i = 0; i < 2; ++i) {
           if (cur.active(i, j)) {
+            if (j == cur.start(i)) {
+              if (no >> (2 + i) & 1) wait(&o_empty[i], (int)(no >> i) ^ 1, 78);
+              no = (no ^ 1u << i) | 4u << i;
+            }
             wait(&p_ready[i], (int)(np >> i), 67);
             tc_fence_after();
             const uint32_t pa = tm + i * 128, oa = tm + 256 + i * 128;
@@ -447,12 +454,66 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       cur = nxt;
     }
+  } else {
+    // ---------------- masked V tiles: zeros behind the sequence, elsewhere finite ----------------
+    // (this warp skips the other tiles, so a slot's phases could pass it by: that the load is
+    // on its way says that the slot's last phase is over, and the next one waits for v_ok)
+    int ring = 1;       // V_0's number
+    uint32_t seen = 0;  // bit: parity of the clearings of a ring slot's V
+    for (int n = 0; ok; ++n) {
+      const Work w = take(n);
+      if (!ok || w.len < 0) break;
+      for (int j = 0; j < w.nt && ok; ++j, ring += 2) {
+        if (!w.part(j)) continue;
+        const int s = ring % S;
+        ok = ok && mbar_wait(&v_sent[s], seen >> s & 1, p.err, 77);
+        seen ^= 1u << s;
+        ok = ok && mbar_wait(&kv_full[s], (ring / S) & 1, p.err, 73);
+        if (!ok) break;
+        bool wrote = false;
+#pragma unroll 1
+        for (int rl = lane; rl < BKV; rl += 32) {
+          uint8_t* at = sKV + s * P::kTile + rl * 128;
+          // (chunks in the order that keeps eight rows on different banks)
+          if ((w.kb + j) * BKV + rl >= w.len) {
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c)
+              *reinterpret_cast<uint4*>(at + (c >> 3) * P::kBox + ((c ^ rl) & 7) * 16) =
+                  make_uint4(0, 0, 0, 0);
+            wrote = true;
+            continue;
+          }
+          uint32_t acc[4] = {0, 0, 0, 0};  // 0 or NaN
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c) {
+            const uint4 u =
+                *reinterpret_cast<const uint4*>(at + (c >> 3) * P::kBox + ((c ^ rl) & 7) * 16);
+            acc[0] = times_zero_plus<T>(u.x, acc[0]);
+            acc[1] = times_zero_plus<T>(u.y, acc[1]);
+            acc[2] = times_zero_plus<T>(u.z, acc[2]);
+            acc[3] = times_zero_plus<T>(u.w, acc[3]);
+          }
+          if (((acc[0] | acc[1] | acc[2] | acc[3]) & 0x7fff7fffu) != 0) {
+#pragma unroll 1
+            for (int c = 0; c < D; ++c) {
+              T* e = reinterpret_cast<T*>(at + (c >> 6) * P::kBox) + (c & 63);
+              if (!isfinite(to_f32(*e))) *e = from_f32<T>(0.f);
+            }
+            wrote = true;
+            atomicExch(odd_v + (n & 1), n + 1);
+          }
+        }
+        if (wrote) fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_ok[s]);
+      }
+    }
   }
   } else if (warp < kCorrWarp0) {
     // ---------------- softmax ----------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
     const int i = warp >> 2, rl = (warp & 3) * 32 + lane;
-    const uint32_t tS = tmem + i * 128 + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t tS = tmem + i * 128 + ((uint32_t)((warp & 3) * 32) << 16), tO = tS + 256;
     int ns = 0, nl = 0;
     for (int n = 0; ok; ++n) {
       const Work w = take(n);
@@ -464,6 +525,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = ok && mbar_wait(&s_full[i], ns & 1, p.err, 70);
         ++ns;
         if (!ok) break;
+        __syncwarp();
         tc_fence_after();
         float sv[BKV];
         {
@@ -501,18 +563,25 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int u = 0; u < 8; ++u) pm[u] = nanmax(pm[u], sv[k + u], sv[k + 8 + u]);
         const float mx = nanmax(nanmax(pm[0], pm[1], pm[2]), nanmax(pm[3], pm[4], pm[5]),
                                 nanmax(pm[6], pm[7])) * p.scale_log2;
-        float corr = 1.f;
-        if (!(mx <= m_ref + kMoves)) {  // (the first finite one too; NaN)
-          corr = m_ref == -INFINITY ? 0.f : exp2f(m_ref - mx);
-          l *= corr;
-          m_ref = mx + (mx - mx);  // (infinite scores make a row NaN)
+        const bool moves = !(mx <= m_ref + kMoves);  // (the first finite one too; NaN)
+        if (__any_sync(0xffffffffu, moves)) {
+          const float f = !moves ? 1.f : m_ref == -INFINITY ? 0.f : exp2f(m_ref - mx);
+          l *= f;
+          m_ref = moves ? mx + (mx - mx) : m_ref;  // (infinite scores make a row NaN)
+          __syncwarp();  // (the transfers below are the whole warp's)
+          // S_i of this step was issued behind P_i V of the last: O_i is at rest
+          if (j > w.start(i)) {
+#pragma unroll 1
+            for (int c = 0; c < D; c += 8) {
+              uint32_t r[8];
+              tmem_ld8(tO + c, r);
+              tmem_wait_ld();
+#pragma unroll
+              for (int q = 0; q < 8; ++q) r[q] = __float_as_uint(__uint_as_float(r[q]) * f);
+              tmem_st8(tO + c, r);
+            }
+          }
         }
-        // (the last factor has been read: its reader let P_i V of that step go, and S_i of
-        // this step came behind that)
-        sc[i * BQ + rl] = corr;
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sc_full[i]);
         const float nm = m_ref == -INFINITY ? 0.f : -m_ref;
         const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), nm2 = f2_pack(nm, nm);
         uint64_t ps[4] = {0ull, 0ull, 0ull, 0ull};
@@ -551,80 +620,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     const int rl = (warp & 3) * 32 + lane;
     const uint32_t tO = tmem + 256 + ((uint32_t)((warp & 3) * 32) << 16);
-    uint32_t nc = 0, no = 0;  // parities of the factors' and the ends' messages, bit i
-    int ring = 1;             // V_0's number
+    uint32_t no = 0;  // parity of the items of each query tile, bit i
     for (int n = 0; ok; ++n) {
       const Work w = take(n);
       if (!ok || w.len < 0) break;
-      bool cleared = false;
-      for (int j = 0; j < w.nt && ok; ++j, ring += 2) {
-        const bool part = w.part(j);
-        if (part) {
-          // thread = key row: zeros behind the sequence, elsewhere finite values only
-          const int s = ring % S;
-          ok = ok && mbar_wait(&kv_full[s], (ring / S) & 1, p.err, 73);
-          if (!ok) break;
-          uint8_t* at = sKV + s * P::kTile + rl * 128;
-          bool wrote = (w.kb + j) * BKV + rl >= w.len;
-          // (chunks in the order that keeps eight rows on different banks)
-          if (wrote) {
-#pragma unroll
-            for (int c = 0; c < D / 8; ++c)
-              *reinterpret_cast<uint4*>(at + (c >> 3) * P::kBox + ((c ^ rl) & 7) * 16) =
-                  make_uint4(0, 0, 0, 0);
-          } else {
-            uint32_t acc[4] = {0, 0, 0, 0};  // 0 or NaN
-#pragma unroll
-            for (int c = 0; c < D / 8; ++c) {
-              const uint4 u = *reinterpret_cast<const uint4*>(at + (c >> 3) * P::kBox +
-                                                              ((c ^ rl) & 7) * 16);
-              acc[0] = times_zero_plus<T>(u.x, acc[0]);
-              acc[1] = times_zero_plus<T>(u.y, acc[1]);
-              acc[2] = times_zero_plus<T>(u.z, acc[2]);
-              acc[3] = times_zero_plus<T>(u.w, acc[3]);
-            }
-            if (((acc[0] | acc[1] | acc[2] | acc[3]) & 0x7fff7fffu) != 0) {
-#pragma unroll 1
-              for (int c = 0; c < D; ++c) {
-                T* e = reinterpret_cast<T*>(at + (c >> 6) * P::kBox) + (c & 63);
-                if (!isfinite(to_f32(*e))) *e = from_f32<T>(0.f);
-              }
-              wrote = true;
-              atomicExch(odd_v + (n & 1), n + 1);
-            }
-          }
-          if (wrote) fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&v_ok[s]);
-          cleared = true;
-        }
-#pragma unroll 1
-        for (int i = 0; i < 2; ++i) {
-          if (!w.active(i, j)) continue;
-          ok = ok && mbar_wait(&sc_full[i], nc >> i & 1, p.err, 74);
-          nc ^= 1u << i;
-          if (!ok) break;
-          tc_fence_after();
-          const float f = sc[i * BQ + rl];
-          if (j > w.start(i) && __any_sync(0xffffffffu, f != 1.f)) {
-            // S_i of this step was issued behind P_i V of the last: O_i is at rest
-#pragma unroll
-            for (int c = 0; c < D; c += 16) {
-              uint32_t r[16];
-              tmem_ld16(tO + i * 128 + c, r);
-              tmem_wait_ld();
-#pragma unroll
-              for (int q = 0; q < 16; ++q) r[q] = __float_as_uint(__uint_as_float(r[q]) * f);
-              tmem_st16(tO + i * 128 + c, r);
-            }
-            tmem_wait_st();
-          }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_ready[i]);
-        }
-      }
-      if (!ok) break;
       // the sums, both at once, so that the next item's softmax can go on
       float inv0 = 0.f, inv1 = 0.f;
 #pragma unroll 1
@@ -643,45 +642,47 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = ok && mbar_wait(&o_full[i], no >> i & 1, p.err, 76);
         no ^= 1u << i;
         if (!ok) break;
+        __syncwarp();
         tc_fence_after();
         const float inv = i ? inv1 : inv0;
         const int tok0 = w.t0 + i * p.TT, rows = min(p.TT, w.len - tok0);
         T* out = static_cast<T*>(p.o) + (int64_t)(w.first + tok0) * p.o_sn +
                  (int64_t)w.kvh * p.G * p.o_sh + (lane & 7) * 8;
-        // 64 dims at a time through this warp's 4 KB, so that a store covers whole rows
+        // through this warp's part of the staging tile, so that a store covers whole rows
         uint8_t* st = stage + (warp & 3) * 4096;
-#pragma unroll 1
-        for (int c = 0; c < D; c += 64) {
-          __syncwarp();
+        __syncwarp();
 #pragma unroll
-          for (int h = 0; h < 64; h += 16) {
-            uint32_t r[16];
-            tmem_ld16(tO + i * 128 + c + h, r);
-            tmem_wait_ld();
-            float f[16];
+        for (int c = 0; c < D; c += 32) {
+          uint32_t r[32];
+          tmem_ld32(tO + i * 128 + c, r);
+          tmem_wait_ld();
 #pragma unroll
-            for (int q = 0; q < 16; ++q) f[q] = __uint_as_float(r[q]) * inv;
+          for (int q = 0; q < 4; ++q) {
+            float f[8];
 #pragma unroll
-            for (int q = 0; q < 2; ++q)
-              *reinterpret_cast<uint4*>(st + lane * 128 + (((h >> 3) + q) ^ (lane & 7)) * 16) =
-                  pack8<T>(f + q * 8);
-          }
-          __syncwarp();
-#pragma unroll 2
-          for (int q = 0; q < 8; ++q) {
-            const int r = q * 4 + (lane >> 3), row = (warp & 3) * 32 + r;
-            const int tl = row * p.inv_g >> 16;
-            const uint4 u = *reinterpret_cast<const uint4*>(st + r * 128 + ((lane ^ r) & 7) * 16);
-            if (tl < rows)
-              *reinterpret_cast<uint4*>(out + tl * p.o_sn + (row - tl * p.G) * p.o_sh + c) = u;
+            for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(r[q * 8 + e]) * inv;
+            *reinterpret_cast<uint4*>(st + (c >> 6) * P::kBox + lane * 128 +
+                                      (((c & 63) / 8 + q) ^ (lane & 7)) * 16) = pack8<T>(f);
           }
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_empty[i]);
+#pragma unroll 4
+        for (int q = 0; q < 8 * P::kBoxes; ++q) {
+          const int r = (q & 7) * 4 + (lane >> 3), row = (warp & 3) * 32 + r;
+          const int tl = row * p.inv_g >> 16;
+          const uint4 u = *reinterpret_cast<const uint4*>(st + (q >> 3) * P::kBox + r * 128 +
+                                                          ((lane ^ r) & 7) * 16);
+          if (tl < rows)
+            *reinterpret_cast<uint4*>(out + tl * p.o_sn + (row - tl * p.G) * p.o_sh +
+                                      (q >> 3) * 64) = u;
+        }
         // (set, if at all, before the last P V could be issued)
-        if (cleared && *reinterpret_cast<volatile int*>(odd_v + (n & 1)) == n + 1) {
+        if (*reinterpret_cast<volatile int*>(odd_v + (n & 1)) == n + 1) {
           __syncwarp();
           add_hidden<T, D>(w, i, rl, p);
         }
-        tc_fence_before();
       }
     }
   }
