@@ -6,17 +6,16 @@
 // one sequence and all G = Hq / Hkv query heads of one kv head, TT = 128 / G: a query
 // tile's 128 rows are (token, head of the group), so short prompts and wide groups fill
 // it, and each K/V tile is read once for two query tiles.  512 threads:
-//   warps 0-3, 4-7 : softmax of query tile 0, 1: a thread owns a row, 128 scores a step
+//   warps 0-3, 4-7 : softmax of query tile 0, 1: a thread owns a row, a step's scores in registers
 //                    (running maximum that only moves, and O with it, when it grows by
-//                    more than 2^8, sums in 32 bits), P over S in TMEM in the storage type.
+//                    more than 2^8, sums in 32 bits), P in TMEM in the storage type.
 //   warps 8-11     : write O / l at an item's end, while the next one runs.
-//   warp 12        : MMA issuer.  S_i = Q_i K_j^T and O_i += P_i V_j, in the order
-//                    PV_0, S_0, PV_1, S_1: while one tile's softmax runs the tensor
-//                    core has the other tile's products, across items too.
-//   warp 13        : TMA: Q tiles, and K and V tiles of 128 keys through one ring.
-//   warp 14        : hands out the items, blocks with the most keys first.
+//   warps 12, 13   : products of query tile 0, 1: O_i += P_i V_j, then S_i = Q_i K^T of step
+//                    j + 2, across items too: a softmax finds the next S done when it has
+//                    written P.
+//   warp 14        : hands out the items, blocks with the most keys first, and loads: Q
+//                    tiles, and K and V tiles through one ring.
 //   warp 15        : makes V tiles finite that some row sees only a part of.
-// TMEM: S/P 0 and 1 in columns [0, 256), O 0 and 1 in [256, 512).
 //
 // What a row does not see has no effect on it, NaN and infinities included: masked
 // scores are -inf, and in tiles that any row sees a part of, V rows behind the sequence
@@ -30,20 +29,33 @@ namespace tpp {
 namespace {
 
 constexpr int BQ = 128;
-constexpr int BKV = 128;
 constexpr int kThreads = 512;
-constexpr int kCorrWarp0 = 8, kMmaWarp = 12, kTmaWarp = 13, kSchedWarp = 14;
-constexpr int kItems = 4;
+constexpr int kOutWarp0 = 8, kMmaWarp = 12, kTmaWarp = 14;  // (products: warps 12 and 13)
+constexpr int kItems = 8;
 constexpr float kMoves = 8.0f;  // growth of a row's maximum (log2) that moves its reference
 
+// TMEM (512 columns): O of both query tiles, then for each S (BKV columns) and, apart from
+// it, P (half as many), so that S of a later step is under way while a step's softmax runs:
+// that leaves 80 keys a step for 128 dims, 128 for 64.  (P over S with 128 keys: each
+// tile's products and softmax take turns, 3600 clocks for 128 keys of both tiles.)
 template <int D>
 struct Plan {
-  static constexpr int kBoxes = D / 64;             // 128-byte swizzle boxes a row
-  static constexpr uint32_t kBox = 128 * 128;       // bytes of a box of 128 rows
-  static constexpr uint32_t kTile = kBoxes * kBox;  // a Q, K or V tile
-  static constexpr int kStages = D == 128 ? 4 : 8;
-  static constexpr uint32_t kStage = kTile;         // an output tile's
-  static constexpr size_t kSmem = 1024 + (2 + kStages) * kTile + kStage + 2 * BQ * 4 + kItems * 48 + 512;
+  static constexpr int BKV = D == 128 ? 80 : 128;     // keys a step
+  static constexpr int kBoxes = D / 64;               // 128-byte swizzle boxes a row
+  static constexpr uint32_t kQBox = BQ * 128;         // bytes of a box of a Q or output tile
+  static constexpr uint32_t kQTile = kBoxes * kQBox;
+  static constexpr uint32_t kBox = BKV * 128;         // of a K or V tile
+  static constexpr uint32_t kTile = kBoxes * kBox;
+  static constexpr int kStages = D == 128 ? 6 : 8;
+  static constexpr uint32_t tO = 0, tS = 2 * D, kSCols = D == 128 ? 96 : 128,
+                            tP = tS + kSCols + BKV, kPCols = BKV / 2;
+  static_assert(tP + 2 * kPCols <= 512, "TMEM plan exceeds 512 columns");
+  // registers of a softmax, an output and a control thread: 4 x 128 are the launch's
+  static constexpr int kSoftRegs = D == 128 ? 152 : 176, kOutRegs = D == 128 ? 120 : 96,
+                       kCtrlRegs = D == 128 ? 88 : 64;
+  static_assert(2 * kSoftRegs + kOutRegs + kCtrlRegs == 512, "");
+  static constexpr size_t kSmem =
+      1024 + 3 * kQTile + kStages * kTile + 2 * BQ * 4 + kItems * 48 + 640;
   static_assert(kSmem <= 227 * 1024, "shared memory plan exceeds 227 KB");
 };
 
@@ -52,7 +64,7 @@ struct PackedAttnArgs {
   int B, N, Hkv, G, TT;
   int inv_g;  // ceil(2^16 / G): r * inv_g >> 16 is r / G for r < 128
   int causal;
-  int64_t window;
+  int window;  // at most N; -1: none
   float scale_log2;
   int sign;  // of the scale: scores are negated (-1) or all equal (0) first
   void* o;
@@ -72,11 +84,9 @@ struct Work {
 
   __device__ __forceinline__ int start(int i) const { return i ? start1 : 0; }
   __device__ __forceinline__ int end(int i) const { return i ? end1 : end0; }
-  __device__ __forceinline__ bool active(int i, int j) const {
-    return j >= start(i) && j < end(i);
-  }
   __device__ __forceinline__ bool part(int j) const { return j < low || j >= high; }
 };
+template <int BKV>
 __device__ __forceinline__ Work work_of(const int4& it, const PackedAttnArgs& p) {
   Work w{};
   w.first = it.x; w.len = it.y; w.t0 = it.z; w.kvh = it.w;
@@ -85,8 +95,7 @@ __device__ __forceinline__ Work work_of(const int4& it, const PackedAttnArgs& p)
   for (int i = 0; i < 2; ++i) {
     const int tok = w.t0 + i * p.TT, n = min(p.TT, w.len - tok);
     if (n <= 0) continue;
-    const int64_t lo = p.window >= 0 ? max((int64_t)0, tok - p.window) : 0;
-    const int kb = (int)(lo / BKV);
+    const int kb = p.window >= 0 ? max(0, tok - p.window) / BKV : 0;
     if (i == 0) w.kb = kb;
     const int end = ((p.causal ? tok + n : w.len) + BKV - 1) / BKV - w.kb;
     if (i == 0) w.end0 = end;
@@ -95,10 +104,15 @@ __device__ __forceinline__ Work work_of(const int4& it, const PackedAttnArgs& p)
     // key tile t: partly hidden behind the sequence, by causality, by the window
     w.high = min(w.high, (p.causal ? (tok + 1) / BKV : w.len / BKV) - w.kb);
     if (p.window >= 0 && tok + n - 1 > p.window)
-      w.low = max(w.low, (int)((tok + n - 1 - p.window + BKV - 1) / BKV) - w.kb);
+      w.low = max(w.low, (tok + n - 1 - p.window + BKV - 1) / BKV - w.kb);
   }
   return w;
 }
+
+// A CTA's steps (key tiles) are numbered on over its items.  K runs two steps ahead of V in
+// the ring: K_0, K_1, V_0, K_2, V_1, K_3 ..: the load of a step's K or V, by number.
+__device__ __forceinline__ int k_load(int g) { return g < 2 ? g : 2 * g - 1; }
+__device__ __forceinline__ int v_load(int g) { return 2 * g + 2; }
 
 // Walks the items in order: blocks of 2 TT tokens, the last ones of the longest
 // sequences first (a causal block's keys grow with its number), each for all kv heads.
@@ -106,7 +120,7 @@ struct Walk {
   const int32_t* cu;
   int B, N, per, Hkv;  // per: tokens a block
   int level;           // the blocks' number
-  int64_t base;        // items before this level
+  uint32_t base;       // items before this level (there are fewer than 2^31)
   int count;           // sequences that have it
 
   // sequence b's first row and length (whatever cu holds, inside [0, N])
@@ -119,11 +133,13 @@ struct Walk {
   }
   __device__ void recount(int lane) {
     count = 0;
+#pragma unroll 1
     for (int b = 0; b < B; b += 32)
       count += __popc(__ballot_sync(0xffffffffu, has(b + lane)));
   }
   __device__ void init(int lane) {
     int most = 0;
+#pragma unroll 1
     for (int b = lane; b < B; b += 32) most = max(most, span(b).y);
     most = __reduce_max_sync(0xffffffffu, most);
     level = (most + per - 1) / per - 1;
@@ -132,15 +148,17 @@ struct Walk {
   }
   // item number `at` (not before the last one asked for): first row, length, first
   // token of the block, kv head; length -1 behind the last
-  __device__ int4 item(int64_t at, int lane) {
-    while (level >= 0 && at >= base + (int64_t)count * Hkv) {
-      base += (int64_t)count * Hkv;
+  __device__ int4 item(uint32_t at, int lane) {
+#pragma unroll 1
+    while (level >= 0 && at >= base + (uint32_t)(count * Hkv)) {
+      base += (uint32_t)(count * Hkv);
       if (--level >= 0) recount(lane);
     }
     if (level < 0) return make_int4(0, -1, 0, 0);
-    const int64_t in = at - base;
-    int nth = (int)(in / Hkv);
-    const int kvh = (int)(in - (int64_t)nth * Hkv);
+    const uint32_t in = at - base;
+    int nth = (int)(in / (uint32_t)Hkv);
+    const int kvh = (int)(in - (uint32_t)nth * Hkv);
+#pragma unroll 1
     for (int b = 0; b < B; b += 32) {
       const uint32_t set = __ballot_sync(0xffffffffu, has(b + lane));
       const int n = __popc(set);
@@ -185,6 +203,7 @@ __device__ __forceinline__ uint32_t times_zero_plus(uint32_t w, uint32_t acc) {
 // as far as that row sees them (never but for broken inputs, hence apart).
 template <typename T, int D>
 __device__ __forceinline__ void add_hidden(const Work& w, int i, int rl, const PackedAttnArgs& p) {
+  constexpr int BKV = Plan<D>::BKV;
   const int tl = rl / p.G, g = rl - tl * p.G, tok = w.t0 + i * p.TT + tl;
   if (tl >= p.TT || tok >= w.len) return;
   T* out = static_cast<T*>(p.o) + (int64_t)(w.first + tok) * p.o_sn +
@@ -215,25 +234,27 @@ __global__ void __launch_bounds__(kThreads, 1)
                        const __grid_constant__ CUtensorMap tm_v,
                        const __grid_constant__ PackedAttnArgs p) {
   using P = Plan<D>;
-  constexpr int S = P::kStages;
+  constexpr int S = P::kStages, BKV = P::BKV;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~(uintptr_t)1023);
-  uint8_t* sQ = smem;                      // 2 tiles
-  uint8_t* sKV = smem + 2 * P::kTile;      // ring: K_0, V_0, K_1, V_1, ... across items
-  uint8_t* stage = sKV + S * P::kTile;
-  float* sums = reinterpret_cast<float*>(stage + P::kStage);  // [2][BQ]
+  uint8_t* sQ = smem;                   // 2 tiles
+  uint8_t* stage = sQ + 2 * P::kQTile;  // an output tile
+  uint8_t* sKV = stage + P::kQTile;     // ring of K and V tiles
+  float* sums = reinterpret_cast<float*>(sKV + S * P::kTile);  // [2][BQ]
   Work* items = reinterpret_cast<Work*>(sums + 2 * BQ);
   uint64_t* bars = reinterpret_cast<uint64_t*>(items + kItems);
-  uint64_t* q_full = bars;             // 2
-  uint64_t* q_empty = q_full + 2;      // 2: the item's last S_i is done
-  uint64_t* s_full = q_empty + 2;      // 2: S_i (and every product before it) is done
-  uint64_t* p_ready = s_full + 2;      // 2: P_i written
-  uint64_t* l_full = p_ready + 2;      // 2: the item's sums
-  uint64_t* l_empty = l_full + 2;      // 2
-  uint64_t* o_full = l_empty + 2;      // 2: the item's last P_i V is done
-  uint64_t* o_empty = o_full + 2;      // 2: its O_i has been read
-  uint64_t* it_full = o_empty + 2;      // kItems
+  uint64_t* q_full = bars;           // 2 each, of the query tiles:
+  uint64_t* q_empty = bars + 2;      // the item's last S_i is done
+  uint64_t* s_full = bars + 4;       // S_i is done
+  uint64_t* s_read = bars + 6;       // and in the softmax's registers
+  uint64_t* p_ready = bars + 8;      // P_i written
+  uint64_t* pv_done = bars + 10;     // P_i V done
+  uint64_t* l_full = bars + 12;      // the item's sums
+  uint64_t* l_empty = bars + 14;
+  uint64_t* o_full = bars + 16;      // the item's last P_i V is done
+  uint64_t* o_empty = bars + 18;     // its O_i has been read
+  uint64_t* it_full = bars + 20;     // kItems
   uint64_t* it_empty = it_full + kItems;
   uint64_t* kv_full = it_empty + kItems;  // S
   uint64_t* kv_empty = kv_full + S;       // S
@@ -241,6 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* v_ok = v_sent + S;            // S: it is finite
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_ok + S);
   int* odd_v = reinterpret_cast<int*>(tmem_slot + 1);  // [2]: item whose V had non-finite values
+  static_assert((20 + 2 * kItems + 4 * S) * 8 + 12 <= 640, "barriers exceed their room");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -252,7 +274,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
+      mbar_init(&s_read[i], 4);
       mbar_init(&p_ready[i], 4);
+      mbar_init(&pv_done[i], 1);
       mbar_init(&l_full[i], 4);
       mbar_init(&l_empty[i], 4);
       mbar_init(&o_full[i], 1);
@@ -260,11 +284,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < kItems; ++i) {
       mbar_init(&it_full[i], 1);
-      mbar_init(&it_empty[i], 15);
+      mbar_init(&it_empty[i], 17);  // 8 + 4 warps, 2 twice, 1
     }
     for (int s = 0; s < S; ++s) {
       mbar_init(&kv_full[s], 1);
-      mbar_init(&kv_empty[s], 1);
+      mbar_init(&kv_empty[s], 2);
       mbar_init(&v_sent[s], 1);
       mbar_init(&v_ok[s], 1);
     }
@@ -280,10 +304,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_trigger();
 
   bool ok = true;
-  // the n-th item (warp-uniform; every warp but the scheduler's reads each once)
+  // the n-th item (the same for the warp; every reader reads each once)
   auto take = [&](int n) {
     const int s = n % kItems;
-    ok = ok && mbar_wait(&it_full[s], (n / kItems) & 1, p.err, 61);
+    ok = ok && wait_short(&it_full[s], (n / kItems) & 1, p.err, 61);
     Work w{};
     w.len = -1;
     if (ok) w = items[s];
@@ -292,183 +316,187 @@ __global__ void __launch_bounds__(kThreads, 1)
     return w;
   };
 
-  // (one instruction for a whole warpgroup; 2 x 176 + 96 + 64 = 4 x 128, what the launch has)
+  // (one instruction for a whole warpgroup)
   if (warp >= kMmaWarp) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-  if (warp == kSchedWarp) {
-    // ---------------- items ----------------
-    Walk w{p.cu, p.B, p.N, 2 * p.TT, p.Hkv, 0, 0, 0};
-    w.init(lane);
-    for (int n = 0; ok; ++n) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(P::kCtrlRegs));
+  if (warp == kTmaWarp) {
+    // ---------------- items and loads ----------------
+    // Step gk of the K's, (wk, jk), runs two ahead of step gv of the V's, (wv, jv); an item is
+    // handed out when the K's come to it.
+    Walk walk{p.cu, p.B, p.N, 2 * p.TT, p.Hkv, 0, 0, 0};
+    walk.init(lane);
+    int nk = 0;
+    auto next_item = [&]() {
       // there and back: a CTA's early and late items of two rounds balance
-      const int64_t at = (int64_t)n * gridDim.x +
-                         (n & 1 ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
-      const int4 it = w.item(at, lane);
-      const int s = n % kItems;
-      if (n >= kItems) ok = ok && mbar_wait(&it_empty[s], ((n / kItems) & 1) ^ 1, p.err, 62);
-      if (!ok) break;
-      if (lane == 0) {
-        items[s] = work_of(it, p);
+      const uint32_t at = nk * gridDim.x + (nk & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+      const Work w = work_of<BKV>(walk.item(at, lane), p);
+      const int s = nk % kItems;
+      if (nk >= kItems) ok = ok && wait_short(&it_empty[s], ((nk / kItems) & 1) ^ 1, p.err, 62);
+      if (lane == 0 && ok) {
+        items[s] = w;
         mbar_arrive(&it_full[s]);
       }
-      if (it.y < 0) break;
-    }
-  } else if (warp == kTmaWarp) {
-    // ---------------- loads ----------------
-    uint32_t nq = 0;  // loads of each Q tile: bit i its parity, bit 2 + i whether any
-    int ring = 0;
-    const uint32_t q_box = (uint32_t)(p.G * p.TT) * 128;
-    for (int n = 0; ok; ++n) {
-      const Work w = take(n);
-      if (!ok || w.len < 0) break;
-      if (lane != 0) continue;
-      auto load = [&](const CUtensorMap* map, int j) {
-        const int s = ring % S;
-        if (ring >= S) ok = ok && mbar_wait(&kv_empty[s], ((ring / S) & 1) ^ 1, p.err, 63);
-        if (!ok) return;
-        mbar_arrive_expect_tx(&kv_full[s], P::kTile);
-        tma_load_4d(sKV + s * P::kTile, map, &kv_full[s], 0, w.first + (w.kb + j) * BKV, 0,
-                    w.kvh);
-        ++ring;
-      };
-      load(&tm_k, 0);
-#pragma unroll 1
-      for (int i = 0; i < 2; ++i) {
-        if (w.end(i) <= w.start(i)) continue;
-        if (nq >> (2 + i) & 1) ok = ok && mbar_wait(&q_empty[i], (nq >> i & 1) ^ 1, p.err, 64);
-        if (!ok) break;
-        mbar_arrive_expect_tx(&q_full[i], P::kBoxes * q_box);
-        for (int b = 0; b < P::kBoxes; ++b)
-          tma_load_3d(sQ + i * P::kTile + b * P::kBox, &tm_q, &q_full[i], b * 64, w.kvh * p.G,
-                      w.first + w.t0 + i * p.TT);
-        nq = (nq ^ 1u << i) | 4u << i;
-      }
-      for (int j = 0; j < w.nt && ok; ++j) {
-        load(&tm_v, j);
-        if (ok && w.part(j)) mbar_arrive(&v_sent[(ring - 1) % S]);
-        if (j + 1 < w.nt && ok) load(&tm_k, j + 1);
-      }
-    }
-  } else if (warp == kMmaWarp) {
-    // ---------------- products ----------------
-    constexpr uint32_t idesc_s = make_idesc_f16(BQ, BKV, IsBf16<T>::value, 0, 0);
-    constexpr uint32_t idesc_o = make_idesc_f16(BQ, D, IsBf16<T>::value, 0, 1);
-    const bool on = elect_lane();
-    const uint32_t q_at = smem_u32(sQ), kv_at = smem_u32(sKV), tm = (uint32_t)same((int)tmem);
-    // a wait that ran out ends the loops at the next step, not at once
-    auto wait = [&](uint64_t* bar, int parity, int code) {
-      if (ok) ok = mbar_wait(bar, (uint32_t)parity & 1, p.err, code);
-    };
-    int ring = 1;  // the next V tile's number
-    // parities, a bit each: Q_i's loads, P_i's steps, the clearings of a ring slot's V
-    uint32_t nq = 0, np = 0, seen = 0;
-    uint32_t no = 0;  // items of each query tile: bit i their parity, bit 2 + i whether any
-    // S_i of the item's key tile in ring slot s, which has landed; `last`: of this item and
-    // query tile
-    auto issue_s = [&](int i, int s, bool first, bool last) {
-      if (first) {
-        wait(&q_full[i], (int)(nq >> i), 65);
-        nq ^= 1u << i;
-        tc_fence_after();
-      }
-      const uint32_t qa = desc_lo(q_at + i * P::kTile, 16), ka = desc_lo(kv_at + s * P::kTile, 16);
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        const uint32_t o = ((kk >> 2) * P::kBox + (kk & 3) * 32) >> 4;
-        mma_ss(on, tm + i * 128, qa + o, ka + o, idesc_s, kk != 0);
-      }
-      commit(on, &s_full[i]);
-      if (last) commit(on, &q_empty[i]);
-    };
-    // what this warp needs of an item
-    auto tiles = [&](int n) {
-      Work w = take(n);
-      w.len = same(w.len);
-      w.nt = same(w.nt);
-      w.start1 = same(w.start1);
-      w.end0 = same(w.end0);
-      w.end1 = same(w.end1);
-      w.low = same(w.low);
-      w.high = same(w.high);
+      __syncwarp();
+      ++nk;
       return w;
     };
-    Work cur = tiles(0);
-    bool more = __all_sync(0xffffffffu, ok) && cur.len >= 0;
-    if (more) {
-      wait(&kv_full[0], 0, 66);
-      tc_fence_after();
+    uint32_t nq = 0;  // loads of each Q tile: bit i their parity, bit 2 + i whether any
+    const uint32_t q_box = (uint32_t)(p.G * p.TT) * 128;
+    Work wk = next_item(), wv = wk;
+    int nv = 0, jk = 0, jv = 0;
 #pragma unroll 1
-      for (int i = 0; i < 2; ++i)
-        if (cur.active(i, 0)) issue_s(i, 0, true, cur.end(i) == 1);
-      commit(on, &kv_empty[0]);
-    }
-    for (int n = 1; more; ++n) {
-      const Work nxt = tiles(n);
-      const bool follows = nxt.len >= 0;
-      more = follows;
-      for (int j = 0; j < cur.nt; ++j) {
-        // V_j, then K_{j+1} or the next item's K_0.  Their waits, and all else that does not
-        // hang on the softmax, come here, while the last step's products run: any wait
-        // takes 200 clocks (the softmax warps' exponentials fill the queue that barriers go
-        // through too)
-        const int rv = ring, rk = ring + 1, s = rv % S, sk = rk % S;
-        const bool part = cur.part(j), goes = j + 1 < cur.nt || follows;
-        wait(&kv_full[s], rv / S, 68);
-        if (goes) wait(&kv_full[sk], rk / S, 66);
-        if (part) wait(&v_ok[s], (int)(seen >> s), 69);
-        if (!__all_sync(0xffffffffu, ok)) {
-          more = false;
-          break;
-        }
-        const uint32_t va = desc_lo(kv_at + s * P::kTile, P::kBox);
+    for (int g = 0; (wk.len >= 0 || wv.len >= 0) && __all_sync(0xffffffffu, ok); ++g) {
+      // V of step g - 2, then K of step g
 #pragma unroll 1
-        for (int i = 0; i < 2; ++i) {
-          if (cur.active(i, j)) {
-            if (j == cur.start(i)) {
-              if (no >> (2 + i) & 1) wait(&o_empty[i], (int)(no >> i) ^ 1, 78);
-              no = (no ^ 1u << i) | 4u << i;
+      for (int k = g < 2 ? 1 : 0; k < 2; ++k) {
+        Work& w = k ? wk : wv;
+        int& j = k ? jk : jv;
+        if (w.len < 0) continue;
+        if (lane == 0) {
+          const int r = k ? k_load(g) : v_load(g - 2), s = r % S;
+          if (r >= S) ok = ok && wait_short(&kv_empty[s], ((r / S) & 1) ^ 1, p.err, 63);
+          if (ok) {
+            mbar_arrive_expect_tx(&kv_full[s], P::kTile);
+            tma_load_4d(sKV + s * P::kTile, k ? &tm_k : &tm_v, &kv_full[s], 0,
+                        w.first + (w.kb + j) * BKV, 0, w.kvh);
+            if (!k && w.part(j)) mbar_arrive(&v_sent[s]);
+          }
+          if (k && j == 0) {
+#pragma unroll 1
+            for (int i = 0; i < 2; ++i) {
+              if (w.end(i) <= w.start(i)) continue;
+              if (nq >> (2 + i) & 1)
+                ok = ok && wait_short(&q_empty[i], (nq >> i & 1) ^ 1, p.err, 64);
+              if (!ok) break;
+              mbar_arrive_expect_tx(&q_full[i], P::kBoxes * q_box);
+              for (int b = 0; b < P::kBoxes; ++b)
+                tma_load_3d(sQ + i * P::kQTile + b * P::kQBox, &tm_q, &q_full[i], b * 64,
+                            w.kvh * p.G, w.first + w.t0 + i * p.TT);
+              nq = (nq ^ 1u << i) | 4u << i;
             }
-            wait(&p_ready[i], (int)(np >> i), 67);
-            tc_fence_after();
-            const uint32_t pa = tm + i * 128, oa = tm + 256 + i * 128;
-#pragma unroll
-            for (int kk = 0; kk < BKV / 16; ++kk)
-              mma_ts(on, oa, pa + kk * 8, va + kk * (2048 >> 4), idesc_o,
-                     j > cur.start(i) || kk != 0);
-            np ^= 1u << i;
-            if (j == cur.end(i) - 1) commit(on, &o_full[i]);
-          }
-          if (j + 1 < cur.nt) {
-            if (cur.active(i, j + 1)) issue_s(i, sk, j + 1 == cur.start(i), j + 2 == cur.end(i));
-          } else if (follows && nxt.active(i, 0)) {
-            issue_s(i, sk, true, nxt.end(i) == 1);
           }
         }
-        if (part) seen ^= 1u << s;
-        commit(on, &kv_empty[s]);
-        ring = rk;
-        if (goes) {
-          commit(on, &kv_empty[sk]);
-          ring = rk + 1;
+        __syncwarp();
+        if (++j < w.nt) continue;
+        j = 0;
+        if (k) {
+          wk = next_item();
+        } else {
+          wv = items[++nv % kItems];  // (at most three behind the items handed out)
         }
       }
-      cur = nxt;
+    }
+  } else if (warp < kTmaWarp) {
+    // ---------------- products of query tile i ----------------
+    constexpr uint32_t idesc_s = make_idesc_f16(BQ, BKV, IsBf16<T>::value, 0, 0);
+    constexpr uint32_t idesc_o = make_idesc_f16(BQ, D, IsBf16<T>::value, 0, 1);
+    const int i = same(warp - kMmaWarp);
+    const bool on = elect_lane();
+    const uint32_t tm = (uint32_t)same((int)tmem);
+    const uint32_t kv_at = desc_lo(smem_u32(sKV), 0), qa = desc_lo(smem_u32(sQ) + i * P::kQTile, 16);
+    const uint32_t tS = tm + P::tS + i * P::kSCols, tPi = tm + P::tP + i * P::kPCols,
+                   tO = tm + P::tO + i * D;
+    // a wait that ran out ends the loop with its item, not at once
+    auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
+      if (ok) ok = wait_short(bar, parity & 1, p.err, code);
+    };
+    // what this warp needs of an item
+    struct Mine { int nt, start, end, low, high; };
+    auto mine = [&](int n) {
+      const Work w = take(n);
+      const bool go = __all_sync(0xffffffffu, ok) && same(w.len) >= 0;
+      return Mine{go ? same(w.nt) : 0, same(w.start(i)), same(w.end(i)), same(w.low), same(w.high)};
+    };
+    // S of step (ws, js) runs two ahead of P V of step (wp, jp)
+    Mine ws = mine(0), wp = mine(0);
+    int n_s = 0, n_p = 0, js = 0, jp = 0;
+    uint32_t nq = 0, ns = 1, np = 0, no = 1;  // parities of the next waits
+    bool s_any = false, o_any = false;
+    uint32_t seen = 0;                        // of the clearings of each ring slot's V
+    int sk = 0, sv = 2;                       // ring slots of the next K and V
+    uint32_t hk = 0, hv = 0;                  // and their parities
+    auto issue_s = [&]() {  // (K has landed)
+      if (js >= ws.start && js < ws.end) {
+        if (js == ws.start) {
+          wait(&q_full[i], nq, 65);
+          nq ^= 1;
+        }
+        if (s_any) wait(&s_read[i], ns, 66);  // the last S_i is in registers
+        s_any = true;
+        ns ^= 1;
+        tc_fence_after();
+        const uint32_t ka = kv_at + (16 >> 4 << 16) + sk * (P::kTile >> 4);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          mma_ss(on, tS, qa + (((kk >> 2) * P::kQBox + (kk & 3) * 32) >> 4),
+                 ka + (((kk >> 2) * P::kBox + (kk & 3) * 32) >> 4), idesc_s, kk != 0);
+        commit(on, &s_full[i]);
+        if (js == ws.end - 1) commit(on, &q_empty[i]);
+      }
+      commit(on, &kv_empty[sk]);
+      if (++js == ws.nt) {
+        ws = mine(++n_s);
+        js = 0;
+      }
+    };
+    for (int g = 0; g < 2 && ws.nt > 0; ++g) {
+      wait(&kv_full[g], 0, 67);
+      issue_s();
+      sk = g == 0 ? 1 : 3;
+    }
+    sk = 3;
+    while (wp.nt > 0) {
+      // V of this step, K of the one after the next: in time for the softmax, as a rule
+      const bool part = jp < wp.low || jp >= wp.high;
+      wait(&kv_full[sv], hv, 68);
+      if (part) wait(&v_ok[sv], seen >> sv, 70);
+      if (ws.nt > 0) wait(&kv_full[sk], hk, 69);
+      if (jp >= wp.start && jp < wp.end) {
+        if (jp == wp.start) {
+          if (o_any) wait(&o_empty[i], no, 71);
+          o_any = true;
+          no ^= 1;
+        }
+        wait(&p_ready[i], np, 72);
+        np ^= 1;
+        tc_fence_after();
+        const uint32_t va = kv_at + (P::kBox >> 4 << 16) + sv * (P::kTile >> 4);
+#pragma unroll
+        for (int kk = 0; kk < BKV / 16; ++kk)
+          mma_ts(on, tO, tPi + kk * 8, va + kk * (2048 >> 4), idesc_o,
+                 jp > wp.start || kk != 0);
+        commit(on, &pv_done[i]);
+        if (jp == wp.end - 1) commit(on, &o_full[i]);
+      }
+      if (part) seen ^= 1u << sv;
+      commit(on, &kv_empty[sv]);
+      sv += 2;
+      if (sv >= S) sv -= S, hv ^= 1;
+      if (ws.nt > 0) {
+        issue_s();
+        sk += 2;
+        if (sk >= S) sk -= S, hk ^= 1;
+      }
+      if (++jp == wp.nt) {
+        wp = mine(++n_p);
+        jp = 0;
+      }
     }
   } else {
     // ---------------- masked V tiles: zeros behind the sequence, elsewhere finite ----------------
     // (this warp skips the other tiles, so a slot's phases could pass it by: that the load is
     // on its way says that the slot's last phase is over, and the next one waits for v_ok)
-    int ring = 1;       // V_0's number
+    int g = 0;          // the step
     uint32_t seen = 0;  // bit: parity of the clearings of a ring slot's V
     for (int n = 0; ok; ++n) {
       const Work w = take(n);
       if (!ok || w.len < 0) break;
-      for (int j = 0; j < w.nt && ok; ++j, ring += 2) {
+      for (int j = 0; j < w.nt && ok; ++j, ++g) {
         if (!w.part(j)) continue;
-        const int s = ring % S;
-        ok = ok && mbar_wait(&v_sent[s], seen >> s & 1, p.err, 77);
+        const int r = v_load(g), s = r % S;
+        ok = ok && wait_short(&v_sent[s], seen >> s & 1, p.err, 77);
         seen ^= 1u << s;
-        ok = ok && mbar_wait(&kv_full[s], (ring / S) & 1, p.err, 73);
+        ok = ok && wait_short(&kv_full[s], (r / S) & 1, p.err, 73);
         if (!ok) break;
         bool wrote = false;
 #pragma unroll 1
@@ -509,11 +537,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   }
-  } else if (warp < kCorrWarp0) {
+  } else if (warp < kOutWarp0) {
     // ---------------- softmax ----------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(P::kSoftRegs));
     const int i = warp >> 2, rl = (warp & 3) * 32 + lane;
-    const uint32_t tS = tmem + i * 128 + ((uint32_t)((warp & 3) * 32) << 16), tO = tS + 256;
+    const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t tS = at + P::tS + i * P::kSCols, tP = at + P::tP + i * P::kPCols,
+                   tO = at + P::tO + i * D;
     int ns = 0, nl = 0;
     for (int n = 0; ok; ++n) {
       const Work w = take(n);
@@ -522,7 +552,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int qpos = w.t0 + i * p.TT + rl / p.G;
       float m_ref = -INFINITY, l = 0.f;
       for (int j = w.start(i); j < w.end(i); ++j) {
-        ok = ok && mbar_wait(&s_full[i], ns & 1, p.err, 70);
+        ok = ok && wait_short(&s_full[i], ns & 1, p.err, 70);
         ++ns;
         if (!ok) break;
         __syncwarp();
@@ -530,12 +560,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         float sv[BKV];
         {
           uint32_t* r = reinterpret_cast<uint32_t*>(sv);
-          tmem_ld32(tS, r);
-          tmem_ld32(tS + 32, r + 32);
-          tmem_ld32(tS + 64, r + 64);
-          tmem_ld32(tS + 96, r + 96);
+#pragma unroll
+          for (int k = 0; k + 32 <= BKV; k += 32) tmem_ld32(tS + k, r + k);
+          if (BKV % 32) tmem_ld16(tS + BKV - 16, r + BKV - 16);
           tmem_wait_ld();
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_read[i]);
         if (p.sign <= 0) {
 #pragma unroll
           for (int k = 0; k < BKV; ++k) sv[k] = p.sign < 0 ? -sv[k] : 0.f;
@@ -543,14 +575,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (w.part(j)) {
           const int key0 = (w.kb + j) * BKV;
           const int hi = (p.causal ? min(qpos, w.len - 1) : w.len - 1) - key0;
-          const int lo = p.window >= 0 ? (int)max((int64_t)0, qpos - p.window - key0) : 0;
+          const int lo = p.window >= 0 ? max(0, qpos - p.window - key0) : 0;
 #pragma unroll
-          for (int k0 = 0; k0 < BKV; k0 += 32) {
-            // the visible keys lo .. hi of these 32 as bits
-            const int h = min(max(hi - k0 + 1, 0), 32), b = min(max(lo - k0, 0), 32);
-            const uint32_t see = (uint32_t)((1ull << h) - 1) & ~(uint32_t)((1ull << b) - 1);
+          for (int k0 = 0; k0 < BKV; k0 += 16) {
+            // the visible keys lo .. hi of these 16 as bits
+            const int h = min(max(hi - k0 + 1, 0), 16), b = min(max(lo - k0, 0), 16);
+            const uint32_t see = ((1u << h) - 1) & ~((1u << b) - 1);
 #pragma unroll
-            for (int k = 0; k < 32; ++k)
+            for (int k = 0; k < 16; ++k)
               if (!(see & 1u << k)) sv[k0 + k] = -INFINITY;
           }
         }
@@ -563,13 +595,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int u = 0; u < 8; ++u) pm[u] = nanmax(pm[u], sv[k + u], sv[k + 8 + u]);
         const float mx = nanmax(nanmax(pm[0], pm[1], pm[2]), nanmax(pm[3], pm[4], pm[5]),
                                 nanmax(pm[6], pm[7])) * p.scale_log2;
+        // P_i V of the last step is done: P_i may be written, and O_i is at rest
+        if (ns > 1) ok = ok && wait_short(&pv_done[i], ns & 1, p.err, 74);
+        if (!ok) break;
+        tc_fence_after();
         const bool moves = !(mx <= m_ref + kMoves);  // (the first finite one too; NaN)
         if (__any_sync(0xffffffffu, moves)) {
           const float f = !moves ? 1.f : m_ref == -INFINITY ? 0.f : exp2f(m_ref - mx);
           l *= f;
           m_ref = moves ? mx + (mx - mx) : m_ref;  // (infinite scores make a row NaN)
           __syncwarp();  // (the transfers below are the whole warp's)
-          // S_i of this step was issued behind P_i V of the last: O_i is at rest
           if (j > w.start(i)) {
 #pragma unroll 1
             for (int c = 0; c < D; c += 8) {
@@ -586,10 +621,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), nm2 = f2_pack(nm, nm);
         uint64_t ps[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
-        for (int k0 = 0; k0 < BKV; k0 += 32) {
-          uint32_t pk[16];
+        for (int k0 = 0; k0 < BKV; k0 += 16) {
+          uint32_t pk[8];
 #pragma unroll
-          for (int k = 0; k < 32; k += 2) {
+          for (int k = 0; k < 16; k += 2) {
             float a0, a1;
             f2_unpack(f2_fma(f2_pack(sv[k0 + k], sv[k0 + k + 1]), sc2, nm2), a0, a1);
             a0 = ex2_ftz(a0);
@@ -597,7 +632,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             ps[(k >> 1) & 3] = f2_add(ps[(k >> 1) & 3], f2_pack(a0, a1));
             pk[k / 2] = pack2<T>(a0, a1);
           }
-          tmem_st16(tS + k0 / 2, pk);
+          tmem_st8(tP + k0 / 2, pk);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -608,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         l += a0 + a1;
       }
       if (!ok) break;
-      if (nl > 0) ok = ok && mbar_wait(&l_empty[i], (nl & 1) ^ 1, p.err, 72);
+      if (nl > 0) ok = ok && wait_short(&l_empty[i], (nl & 1) ^ 1, p.err, 72);
       ++nl;
       if (!ok) break;
       sums[i * BQ + rl] = l;
@@ -617,9 +652,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ---------------- O ----------------
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(P::kOutRegs));
     const int rl = (warp & 3) * 32 + lane;
-    const uint32_t tO = tmem + 256 + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t tO = tmem + P::tO + ((uint32_t)((warp & 3) * 32) << 16);
     uint32_t no = 0;  // parity of the items of each query tile, bit i
     for (int n = 0; ok; ++n) {
       const Work w = take(n);
@@ -629,7 +664,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
       for (int i = 0; i < 2; ++i) {
         if (w.end(i) <= w.start(i)) continue;
-        ok = ok && mbar_wait(&l_full[i], no >> i & 1, p.err, 75);
+        ok = ok && wait_short(&l_full[i], no >> i & 1, p.err, 75);
         if (!ok) break;
         const float l = sums[i * BQ + rl];
         (i ? inv1 : inv0) = l == 0.f ? 0.f : 1.f / l;
@@ -639,7 +674,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
       for (int i = 0; i < 2; ++i) {
         if (w.end(i) <= w.start(i)) continue;
-        ok = ok && mbar_wait(&o_full[i], no >> i & 1, p.err, 76);
+        ok = ok && wait_short(&o_full[i], no >> i & 1, p.err, 76);
         no ^= 1u << i;
         if (!ok) break;
         __syncwarp();
@@ -654,14 +689,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int c = 0; c < D; c += 32) {
           uint32_t r[32];
-          tmem_ld32(tO + i * 128 + c, r);
+          tmem_ld32(tO + i * D + c, r);
           tmem_wait_ld();
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             float f[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(r[q * 8 + e]) * inv;
-            *reinterpret_cast<uint4*>(st + (c >> 6) * P::kBox + lane * 128 +
+            *reinterpret_cast<uint4*>(st + (c >> 6) * P::kQBox + lane * 128 +
                                       (((c & 63) / 8 + q) ^ (lane & 7)) * 16) = pack8<T>(f);
           }
         }
@@ -672,7 +707,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int q = 0; q < 8 * P::kBoxes; ++q) {
           const int r = (q & 7) * 4 + (lane >> 3), row = (warp & 3) * 32 + r;
           const int tl = row * p.inv_g >> 16;
-          const uint4 u = *reinterpret_cast<const uint4*>(st + (q >> 3) * P::kBox + r * 128 +
+          const uint4 u = *reinterpret_cast<const uint4*>(st + (q >> 3) * P::kQBox + r * 128 +
                                                           ((lane ^ r) & 7) * 16);
           if (tl < rows)
             *reinterpret_cast<uint4*>(out + tl * p.o_sn + (row - tl * p.G) * p.o_sh +
@@ -721,7 +756,7 @@ extern "C" int tpp_attention_packed(const void* q, int64_t q_sn, int64_t q_sh, c
   a.TT = BQ / a.G;
   a.inv_g = (65536 + a.G - 1) / a.G;
   a.causal = causal != 0;
-  a.window = window_left < 0 ? -1 : window_left < N ? window_left : N;
+  a.window = (int)(window_left < 0 ? -1 : window_left < N ? window_left : N);
   a.sign = scale > 0 ? 1 : scale < 0 ? -1 : 0;
   a.scale_log2 = scale == 0 ? 1.f : fabsf(scale) * 1.4426950408889634f;
   a.o = o; a.o_sn = o_sn; a.o_sh = o_sh;
@@ -736,7 +771,8 @@ extern "C" int tpp_attention_packed(const void* q, int64_t q_sn, int64_t q_sh, c
   auto kv_map = [&](CUtensorMap* m, const void* base, int64_t sn, int64_t sh) {
     const uint64_t d[4] = {64, (uint64_t)N, (uint64_t)(D / 64), (uint64_t)Hkv};
     const uint64_t s[3] = {(uint64_t)sn * 2, 128, (uint64_t)sh * 2};
-    const uint32_t b[4] = {64, BKV, (uint32_t)(D / 64), 1};
+    const uint32_t b[4] = {64, (uint32_t)(D == 128 ? Plan<128>::BKV : Plan<64>::BKV),
+                           (uint32_t)(D / 64), 1};
     return make_tmap(m, base, dtype, 4, d, s, b, CU_TENSOR_MAP_SWIZZLE_128B);
   };
   if (rc == TPP_OK) rc = kv_map(&tk, k, k_sn, k_sh);
@@ -744,6 +780,7 @@ extern "C" int tpp_attention_packed(const void* q, int64_t q_sn, int64_t q_sh, c
   if (rc != TPP_OK) return rc;
   // items at most: a block of 2 TT tokens each, one more a sequence
   const int64_t items = (N / (2 * a.TT) + B) * Hkv;
+  TPP_REQUIRE(items < (1ll << 30), TPP_ERR_SHAPE, "too many rows, sequences and heads");
   const unsigned grid = (unsigned)(items < num_sms() ? items : num_sms());
   auto go = [&](auto tag, auto dim) -> int {
     using T = decltype(tag);

@@ -67,6 +67,15 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
       : "memory");
 }
+// mbar_wait in little code: a kernel of many roles and waits outgrows the instruction cache
+// (with the loops unrolled packed_attn_kernel had 210 KB, and every wait cost 250 clocks).
+__device__ __forceinline__ bool wait_short(uint64_t* bar, uint32_t parity, int* err, int code) {
+#pragma unroll 1
+  for (uint32_t i = 0; i < kWaitLimit; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  if (err) atomicExch(err, code);
+  return false;
+}
 // The same value from every lane, as the compiler can see.
 __device__ __forceinline__ int same(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
