@@ -36,23 +36,24 @@ constexpr float kMoves = 8.0f;  // growth of a row's maximum (log2) that moves i
 
 // TMEM (512 columns): O of both query tiles, then for each S (BKV columns) and, apart from
 // it, P (half as many), so that S of a later step is under way while a step's softmax runs:
-// that leaves 80 keys a step for 128 dims, 128 for 64.  (P over S with 128 keys: each
-// tile's products and softmax take turns, 3600 clocks for 128 keys of both tiles.)
+// that leaves 80 keys a step for 128 dims.  (P over S with 128 keys: each tile's products
+// and softmax take turns, 3600 clocks for 128 keys of both tiles, against 3100 now.)  For 64
+// dims 128 keys would fit, and 96 are faster: one prompt of 16384, 64: 912 us, 96: 770, 112:
+// 850, 128: 832.
 template <int D>
 struct Plan {
-  static constexpr int BKV = D == 128 ? 80 : 128;     // keys a step
+  static constexpr int BKV = D == 128 ? 80 : 96;      // keys a step
   static constexpr int kBoxes = D / 64;               // 128-byte swizzle boxes a row
   static constexpr uint32_t kQBox = BQ * 128;         // bytes of a box of a Q or output tile
   static constexpr uint32_t kQTile = kBoxes * kQBox;
   static constexpr uint32_t kBox = BKV * 128;         // of a K or V tile
   static constexpr uint32_t kTile = kBoxes * kBox;
   static constexpr int kStages = D == 128 ? 6 : 8;
-  static constexpr uint32_t tO = 0, tS = 2 * D, kSCols = D == 128 ? 96 : 128,
+  static constexpr uint32_t tO = 0, tS = 2 * D, kSCols = 96,
                             tP = tS + kSCols + BKV, kPCols = BKV / 2;
   static_assert(tP + 2 * kPCols <= 512, "TMEM plan exceeds 512 columns");
   // registers of a softmax, an output and a control thread: 4 x 128 are the launch's
-  static constexpr int kSoftRegs = D == 128 ? 152 : 176, kOutRegs = D == 128 ? 120 : 96,
-                       kCtrlRegs = D == 128 ? 88 : 64;
+  static constexpr int kSoftRegs = 152, kOutRegs = 120, kCtrlRegs = 88;
   static_assert(2 * kSoftRegs + kOutRegs + kCtrlRegs == 512, "");
   static constexpr size_t kSmem =
       1024 + 3 * kQTile + kStages * kTile + 2 * BQ * 4 + kItems * 48 + 640;

@@ -70,6 +70,7 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
 // mbar_wait in little code: a kernel of many roles and waits outgrows the instruction cache
 // (with the loops unrolled packed_attn_kernel had 210 KB, and every wait cost 250 clocks).
 __device__ __forceinline__ bool wait_short(uint64_t* bar, uint32_t parity, int* err, int code) {
+  if (mbar_try_wait(bar, parity)) return true;
 #pragma unroll 1
   for (uint32_t i = 0; i < kWaitLimit; ++i)
     if (mbar_try_wait(bar, parity)) return true;
