@@ -8,16 +8,13 @@ namespace tpp {
 namespace {
 
 constexpr int BM = 128;        // tokens a tile
-constexpr int BK = 64;         // one 128-byte swizzle row of the operands
-constexpr int KS = 2;          // k-blocks a ring stage
+constexpr int BK = 64;         // a ring stage: one 128-byte swizzle row of the operands
 constexpr int kMaxBN = 256;    // vocabulary rows a tile at most (a multiple of 16)
-constexpr int kStages = 2;
+constexpr int kMaxStages = 8;
 constexpr int kThreads = 384;  // 4 control warps, 8 of the epilogue
 constexpr int kEpiWarp0 = 4;
-constexpr uint32_t kSubA = BM * BK * 2;
-constexpr uint32_t kStageA = KS * kSubA;
-constexpr uint32_t kStageB = KS * kMaxBN * BK * 2;
-constexpr size_t kSmem = kStages * (kStageA + kStageB) + 2 * 3 * BM * 4 + 1024 + 256;
+constexpr size_t kRing = 216 * 1024;
+constexpr size_t kSmem = kRing + 2 * 3 * BM * 4 + 1024 + 256;
 static_assert(kSmem <= 227 * 1024, "shared memory plan exceeds 227 KB");
 
 struct HeadArgs {
@@ -26,7 +23,10 @@ struct HeadArgs {
   float* target;  // [rows]: the token's logit
   int N, V, E, BN;
   int64_t rows;   // N rounded up to whole tiles
-  int flat;       // operands by 2-D maps, one request a k-block
+  // Ring stages, as many as fit: 4 for whole tiles, 8 for a few tokens, where the rest of
+  // a tile's 128 rows is left unloaded (rows of x do not mix) and the weights are all that
+  // counts.  a_rows: rows of x loaded.
+  int stages, a_rows;
   float c;        // log2(e) / temperature
   int* err;
 };
@@ -38,12 +38,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~(uintptr_t)1023);
-  uint8_t* sA = smem;
-  uint8_t* sB = smem + kStages * kStageA;
-  float* half1 = reinterpret_cast<float*>(sB + kStages * kStageB);  // [2 tiles][3][BM]
+  float* half1 = reinterpret_cast<float*>(smem + kRing);  // [2 tiles][3][BM]
   uint64_t* full = reinterpret_cast<uint64_t*>(half1 + 2 * 3 * BM);
-  uint64_t* empty = full + kStages;
-  uint64_t* tfull = empty + kStages;
+  uint64_t* empty = full + kMaxStages;
+  uint64_t* tfull = empty + kMaxStages;
   uint64_t* tempty = tfull + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
 
@@ -51,14 +49,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int BN = p.BN;
   const int ntm = (p.N + BM - 1) / BM;
   const int64_t ntiles = (int64_t)ntm * ((p.V + BN - 1) / BN);
-  const int nk = (p.E + BK * KS - 1) / (BK * KS);
-  const uint32_t sub_b = (uint32_t)BN * BK * 2;
+  const int nk = (p.E + BK - 1) / BK, stages = p.stages;
+  // a stage: x rows (whole 1 KB), then W rows
+  const uint32_t a_bytes = (uint32_t)p.a_rows * 128, b_bytes = (uint32_t)BN * 128;
+  const uint32_t stage = a_bytes + b_bytes;
 
   if (threadIdx.x == 0) {
     prefetch_tmap(&tm_x);
     prefetch_tmap(&tm_w);
-    for (int s = 0; s < kStages; ++s) {
-      mbar_init(&full[s], 1);
+    for (int s = 0; s < kMaxStages; ++s) {
+      mbar_init(&full[s], 2);
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -76,24 +76,29 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_trigger();
 
   bool ok = true;
-  if (warp == 0 && lane == 0) {
-    // ---------------- TMA producer ----------------
-    int it = 0;
+  if ((warp == 0 || warp == 2) && lane == 0) {
+    // ---------------- TMA producers: x by one thread, W by another ----------------
+    // (a thread takes some 0.2 us a request, and a stage's products 0.3)
+    int s = 0;
+    uint32_t turn = 1;
+    bool first = true;
     for (int64_t t = blockIdx.x; t < ntiles && ok; t += gridDim.x) {
       const int m0 = (int)(t % ntm) * BM, n0 = (int)(t / ntm) * BN;
-      for (int kb = 0; kb < nk && ok; ++kb, ++it) {
-        const int s = it % kStages;
-        if (it >= kStages) ok = mbar_wait(&empty[s], ((it / kStages) & 1) ^ 1, p.err, 51);
+      for (int kb = 0; kb < nk; ++kb) {
+        if (!first) ok = ok && wait_short(&empty[s], turn, p.err, 51);
         if (!ok) break;
-        mbar_arrive_expect_tx(&full[s], kStageA + KS * sub_b);
-        if (p.flat) {
-          for (int j = 0; j < KS; ++j) {
-            tma_load_2d(sA + s * kStageA + j * kSubA, &tm_x, &full[s], (kb * KS + j) * BK, m0);
-            tma_load_2d(sB + s * kStageB + j * sub_b, &tm_w, &full[s], (kb * KS + j) * BK, n0);
-          }
+        uint8_t* at = smem + s * stage;
+        if (warp == 0) {
+          mbar_arrive_expect_tx(&full[s], a_bytes);
+          tma_load_2d(at, &tm_x, &full[s], kb * BK, m0);
         } else {
-          tma_load_3d(sA + s * kStageA, &tm_x, &full[s], 0, m0, kb * KS);
-          tma_load_3d(sB + s * kStageB, &tm_w, &full[s], 0, n0, kb * KS);
+          mbar_arrive_expect_tx(&full[s], b_bytes);
+          tma_load_2d(at + a_bytes, &tm_w, &full[s], kb * BK, n0);
+        }
+        if (++s == stages) {
+          s = 0;
+          turn ^= 1;
+          first = false;
         }
       }
     }
@@ -101,27 +106,30 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------- MMA issuer (the whole warp, see tc_issue.cuh) ----------------
     const uint32_t idesc = make_idesc_f16(BM, BN, IsBf16<T>::value, 0, 0);
     const uint32_t tm = (uint32_t)same((int)tmem);
-    const uint32_t a_at = smem_u32(sA), b_at = smem_u32(sB);
+    const uint32_t at = desc_lo(smem_u32(smem), 16);
     const bool on = elect_lane();
-    int it = 0, j = 0;
+    int s = 0, j = 0;
+    uint32_t turn = 0;
+#pragma unroll 1
     for (int64_t t = blockIdx.x; t < ntiles; t += gridDim.x, ++j) {
       const int buf = j & 1;
-      if (ok && j >= 2) ok = mbar_wait(&tempty[buf], ((j >> 1) & 1) ^ 1, p.err, 52);
+      if (ok && j >= 2) ok = wait_short(&tempty[buf], ((j >> 1) & 1) ^ 1, p.err, 52);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
       const uint32_t acc = tm + (uint32_t)(buf * kMaxBN);
-      for (int kb = 0; kb < nk; ++kb, ++it) {
-        const int s = it % kStages;
-        if (ok) ok = mbar_wait(&full[s], (it / kStages) & 1, p.err, 53);
+#pragma unroll 1
+      for (int kb = 0; kb < nk; ++kb) {
+        if (ok) ok = wait_short(&full[s], turn, p.err, 53);
         tc_fence_after();
-        const uint32_t a0 = desc_lo(a_at + s * kStageA, 16), b0 = desc_lo(b_at + s * kStageB, 16);
+        const uint32_t a0 = at + s * (stage >> 4), b0 = a0 + (a_bytes >> 4);
 #pragma unroll
-        for (int k = 0; k < KS * BK / 16; ++k) {
-          const uint32_t j2 = k >> 2, o = (k & 3) * 32 >> 4;
-          mma_ss(on, acc, a0 + j2 * (kSubA >> 4) + o, b0 + j2 * (sub_b >> 4) + o, idesc,
-                 (kb | k) != 0);
-        }
+        for (int k = 0; k < BK / 16; ++k)
+          mma_ss(on, acc, a0 + (k * 32 >> 4), b0 + (k * 32 >> 4), idesc, (kb | k) != 0);
         commit(on, &empty[s]);
+        if (++s == stages) {
+          s = 0;
+          turn ^= 1;
+        }
       }
       commit(on, &tfull[buf]);
     }
@@ -142,65 +150,95 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int tl = at >= 0 && at < nv ? (int)at : -1;  // the token's column here
       const bool mine = __any_sync(0xffffffffu, tl >= 0);
       // (after a wait that ran out the loop goes on, for the barrier below)
-      ok = ok && mbar_wait(&tfull[buf], (j >> 1) & 1, p.err, 54);
+      ok = ok && wait_short(&tfull[buf], (j >> 1) & 1, p.err, 54);
       tc_fence_after();
       const uint32_t trow =
           tmem + (uint32_t)(buf * kMaxBN + c_first) + ((uint32_t)(quarter * 32) << 16);
       float ref = -INFINITY, S = 0.f, En = 0.f;
-      for (int c0 = 0; c0 < nv; c0 += 16) {
-        uint32_t r[16];
-        tmem_ld16(trow + c0, r);
-        tmem_wait_ld();
-        float x[16];
+      // C columns from c0 on; the next ones' transfer runs meanwhile
+      auto take = [&](const uint32_t* r, int c0, auto size) {
+        constexpr int C = decltype(size)::value;
+        const float* x = reinterpret_cast<const float*>(r);
+        float mx[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(r[i]);
-        const int left = nv - c0;  // (the same for the warp)
-        if (left < 16) {
-          // the vocabulary's end: what lies behind it weighs as much as its
-          // first column here, and is taken out again
+        for (int i = 4; i < C; i += 8)
 #pragma unroll
-          for (int i = 1; i < 16; ++i)
-            if (i >= left) x[i] = x[0];
-        }
-        float mx[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          mx[i] = fmaxf(fmaxf(x[i], x[4 + i]), fmaxf(x[8 + i], x[12 + i]));
+          for (int u = 0; u < 4; ++u)
+            mx[u] = i + 4 + u < C ? fmax3(mx[u], x[i + u], x[i + 4 + u]) : fmaxf(mx[u], x[i + u]);
         const float cm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         if (c0 == 0) ref = cm;
-        if ((cm - ref) * c > 8.f) {
+        if ((cm - ref) * c > 8.f) {  // (rare)
           const float d = ref - cm, f = exp2f(c * d);
           En = f == 0.f ? 0.f : (En + S * d) * f;
           S *= f;
           ref = cm;
         }
         const uint64_t r2 = f2_pack(-ref, -ref);
-        uint64_t s2 = 0ull, e2 = 0ull;
+        uint64_t s2[2] = {0ull, 0ull}, e2[2] = {0ull, 0ull};
 #pragma unroll
-        for (int i = 0; i < 16; i += 2) {
+        for (int i = 0; i < C; i += 2) {
           const uint64_t q2 = f2_add(f2_pack(x[i], x[i + 1]), r2);
           float d0, d1;
           f2_unpack(f2_mul(q2, c2), d0, d1);
-          float w0 = ex2_ftz(d0), w1 = ex2_ftz(d1);
-          if (left < 16) {
-            w0 = i < left ? w0 : 0.f;
-            w1 = i + 1 < left ? w1 : 0.f;
-          }
-          const uint64_t w2 = f2_pack(w0, w1);
-          s2 = f2_add(s2, w2);
-          e2 = f2_fma(w2, q2, e2);
+          const uint64_t w2 = f2_pack(ex2_ftz(d0), ex2_ftz(d1));
+          s2[(i >> 1) & 1] = f2_add(s2[(i >> 1) & 1], w2);
+          e2[(i >> 1) & 1] = f2_fma(w2, q2, e2[(i >> 1) & 1]);
         }
         float a0, a1;
-        f2_unpack(s2, a0, a1);
+        f2_unpack(f2_add(s2[0], s2[1]), a0, a1);
         S += a0 + a1;
-        f2_unpack(e2, a0, a1);
+        f2_unpack(f2_add(e2[0], e2[1]), a0, a1);
         En += a0 + a1;
-        if (mine && (tl >> 4) == (c0 >> 4) && tl >= 0) {
-          float v = x[0];
+        if (mine) {
 #pragma unroll
-          for (int i = 1; i < 16; ++i) v = (tl & 15) == i ? x[i] : v;
-          p.target[row] = v;
+          for (int i = 0; i < C; ++i)
+            if (tl == c0 + i) p.target[row] = x[i];
         }
+      };
+      constexpr std::integral_constant<int, 32> k32{};
+      int c0 = 0;
+      if (nv >= 32) {
+        uint32_t r[2][32];
+        tmem_ld32(trow, r[0]);
+        for (; c0 + 64 <= nv; c0 += 64) {
+          tmem_wait_ld();
+          tmem_ld32(trow + c0 + 32, r[1]);
+          take(r[0], c0, k32);
+          tmem_wait_ld();
+          if (c0 + 96 <= nv) tmem_ld32(trow + c0 + 64, r[0]);
+          take(r[1], c0 + 32, k32);
+        }
+        if (c0 + 32 <= nv) {
+          tmem_wait_ld();
+          take(r[0], c0, k32);
+          c0 += 32;
+        }
+      }
+      if (c0 + 16 <= nv) {
+        uint32_t r[16];
+        tmem_ld16(trow + c0, r);
+        tmem_wait_ld();
+        take(r, c0, std::integral_constant<int, 16>{});
+        c0 += 16;
+      }
+#pragma unroll 1
+      for (; c0 < nv; ++c0) {  // the vocabulary's end
+        uint32_t r;
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(trow + c0));
+        tmem_wait_ld();
+        const float x = __uint_as_float(r);
+        if (c0 == 0) ref = x;
+        if ((x - ref) * c > 8.f) {
+          const float d = ref - x, f = exp2f(c * d);
+          En = f == 0.f ? 0.f : (En + S * d) * f;
+          S *= f;
+          ref = x;
+        }
+        const float q = x - ref, w = ex2_ftz(q * c);
+        S += w;
+        En += w * q;
+        if (tl == c0) p.target[row] = x;
+        __syncwarp();
       }
       tc_fence_before();
       __syncwarp();
@@ -310,7 +348,7 @@ extern "C" int tpp_linear_logprobs(const void* x, int64_t ldx, const void* w, in
   if (N == 0) return TPP_OK;
   TPP_REQUIRE(x && w && tokens && logprobs && entropy, TPP_ERR_SHAPE, "null pointer");
   TPP_REQUIRE(N > 0 && N < (1ll << 31) - BM && V > 0 && V < (1ll << 31) - kMaxBN && E > 0 &&
-                  E < (1ll << 31) - BK * KS && ldx >= E && ldw >= E,
+                  E < (1ll << 31) - BK && ldx >= E && ldw >= E,
               TPP_ERR_SHAPE, "bad sizes");
   TPP_REQUIRE(temperature >= 1e-6 && isfinite(temperature), TPP_ERR_SHAPE,
               "temperature must be positive");
@@ -327,24 +365,20 @@ extern "C" int tpp_linear_logprobs(const void* x, int64_t ldx, const void* w, in
   const int nt = (int)((V + a.BN - 1) / a.BN);
   a.part = static_cast<float*>(workspace);
   a.target = a.part + 3 * a.rows * nt;
-  a.flat = E % BK != 0;
+  a.a_rows = (int)(N < BM ? (N + 7) / 8 * 8 : BM);
+  const int64_t stage = (int64_t)(a.a_rows + a.BN) * 128;
+  a.stages = (int)((int64_t)kRing / stage < kMaxStages ? (int64_t)kRing / stage : kMaxStages);
   a.c = (float)(1.4426950408889634 / temperature);
   a.err = device_error_flag();
   CUtensorMap tx, tw;
   auto map = [&](CUtensorMap* m, const void* base, int64_t rows, int64_t ld, int box_rows) {
-    if (a.flat) {
-      const uint64_t dims[2] = {(uint64_t)E, (uint64_t)rows};
-      const uint64_t strides[1] = {(uint64_t)ld * 2};
-      const uint32_t box[2] = {BK, (uint32_t)box_rows};
-      return make_tmap(m, base, dtype, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
-    }
-    const uint64_t dims[3] = {BK, (uint64_t)rows, (uint64_t)(E / BK)};
-    const uint64_t strides[2] = {(uint64_t)ld * 2, BK * 2};
-    const uint32_t box[3] = {BK, (uint32_t)box_rows, KS};
-    return make_tmap(m, base, dtype, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    const uint64_t dims[2] = {(uint64_t)E, (uint64_t)rows};
+    const uint64_t strides[1] = {(uint64_t)ld * 2};
+    const uint32_t box[2] = {BK, (uint32_t)box_rows};
+    return make_tmap(m, base, dtype, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
   };
   return TPP_DISPATCH_HALF(dtype, T, [&] {
-    int rc = map(&tx, x, N, ldx, BM);
+    int rc = map(&tx, x, N, ldx, a.a_rows);
     if (rc == TPP_OK) rc = map(&tw, w, V, ldw, a.BN);
     if (rc != TPP_OK) return rc;
     auto kern = linear_logprobs_kernel<T>;
