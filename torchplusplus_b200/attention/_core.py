@@ -71,6 +71,29 @@ def attention_block(x: torch.Tensor, wqkv: torch.Tensor, wo: torch.Tensor,
     return ops.linear(o.reshape(B, S, Hq * D), wo, bo, residual=residual)
 
 
+def packed_attention_block(x: torch.Tensor, wqkv: torch.Tensor, wo: torch.Tensor,
+                           bo: torch.Tensor | None, Hq: int, Hkv: int, D: int,
+                           qn_w: torch.Tensor | None, kn_w: torch.Tensor | None, eps: float,
+                           cos: torch.Tensor, sin: torch.Tensor, cu_seqlens: torch.Tensor,
+                           kv_cache=None, window_left: int = -1,
+                           residual: torch.Tensor | None = None) -> torch.Tensor:
+    """attention_block over prompts of different lengths packed row after row: x [N, E],
+    sequence b in rows cu_seqlens[b] .. cu_seqlens[b+1]-1 (int32 on the device), causal,
+    whole prompts.  A KVCache of batch B receives each sequence's K and V from row 0 on;
+    its cache_len is left to the caller (the lengths differ)."""
+    qkv = ops.linear(x, wqkv)                                  # [N, (Hq+2Hkv) D]
+    kc = vc = None
+    if kv_cache is not None:
+        B = cu_seqlens.shape[0] - 1
+        kv_cache._ensure_allocated(B)
+        kc, vc = kv_cache.k_cache[:B], kv_cache.v_cache[:B]
+    q, k = ops.qk_norm_rope_packed(qkv, qn_w, kn_w, eps, cos, sin, cu_seqlens, Hq, Hkv,
+                                   k_cache=kc, v_cache=vc)
+    v = qkv[:, (Hq + Hkv) * D:].view(-1, Hkv, D)               # as the projection leaves it
+    o = ops.attention_packed(q, k, v, cu_seqlens, window_left=window_left)
+    return ops.linear(o.view(-1, Hq * D), wo, bo, residual=residual)
+
+
 def norm_eps(m) -> float:
     e = getattr(m, "eps", None)
     return 1e-6 if e is None else float(e)

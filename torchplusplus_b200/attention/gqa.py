@@ -8,7 +8,7 @@ import torch
 import torch.nn as nn
 
 from ..llmops.kvcache import KVCache
-from ._core import FusedQKV, attention_block, norm_eps
+from ._core import FusedQKV, attention_block, norm_eps, packed_attention_block
 
 
 class GroupedQueryAttention(nn.Module):
@@ -51,3 +51,17 @@ class GroupedQueryAttention(nn.Module):
             self.k_norm.weight if self.k_norm is not None else None,
             norm_eps(self.q_norm) if self.q_norm is not None else 1e-6, cos, sin,
             kv_cache=kv_cache, cache_pos=cache_pos, causal=True, residual=residual)
+
+    def forward_packed(self, x, cos, sin, cu_seqlens: torch.Tensor,
+                       kv_cache: Optional[KVCache] = None,
+                       residual: Optional[torch.Tensor] = None):
+        """forward over whole prompts of different lengths packed row after row: x [N, d_in],
+        cu_seqlens int32 [B+1] on the device (see _core.packed_attention_block)."""
+        w = self._qkv.get(self.Wq.weight, self.Wk.weight, self.Wv.weight)
+        return packed_attention_block(
+            x, w, self.out_projection.weight, self.out_projection.bias, self.num_heads,
+            self.n_kv_heads, self.head_dim,
+            self.q_norm.weight if self.q_norm is not None else None,
+            self.k_norm.weight if self.k_norm is not None else None,
+            norm_eps(self.q_norm) if self.q_norm is not None else 1e-6, cos, sin, cu_seqlens,
+            kv_cache=kv_cache, residual=residual)

@@ -13,7 +13,7 @@ from typing import Optional
 import torch
 import torch.nn as nn
 
-from ._core import FusedQKV, attention_block, norm_eps
+from ._core import FusedQKV, attention_block, norm_eps, packed_attention_block
 
 
 class SlidingWindowAttention(nn.Module):
@@ -51,3 +51,15 @@ class SlidingWindowAttention(nn.Module):
             norm_eps(self.q_norm) if self.q_norm is not None else 1e-6, cos, sin,
             kv_cache=kv_cache, cache_pos=cache_pos, causal=True,
             window_left=self.window_size - 1)
+
+    def forward_packed(self, x: torch.Tensor, cos, sin, cu_seqlens: torch.Tensor, kv_cache=None):
+        """forward over whole prompts of different lengths packed row after row: x
+        [N, embed_dim], cu_seqlens int32 [B+1] on the device."""
+        w = self._qkv.get(self.Wq.weight, self.Wk.weight, self.Wv.weight)
+        return packed_attention_block(
+            x, w, self.out_projection.weight, self.out_projection.bias, self.n_heads,
+            self.n_kv_heads, self.head_dim,
+            self.q_norm.weight if self.q_norm is not None else None,
+            self.k_norm.weight if self.k_norm is not None else None,
+            norm_eps(self.q_norm) if self.q_norm is not None else 1e-6, cos, sin, cu_seqlens,
+            kv_cache=kv_cache, window_left=self.window_size - 1)

@@ -228,6 +228,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
     __syncthreads();
     const int n = count;
     if (n > kCap) return n;
+#pragma unroll 1
     for (int i = tid; i < n; i += NT) {
       const uint64_t me = cand[i];
       int r = 0;
@@ -236,6 +237,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
     }
     __syncthreads();
     const int left = min(n, p.top);
+#pragma unroll 1
     for (int i = tid; i < left; i += NT) cand[i] = list[i];
     if (tid == 0) count = left;
     __syncthreads();
@@ -268,6 +270,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
       const int whole = min(kWarps, (vb - va) / 32);  // warps with data in every lane
       if (TOP && warp < whole) {
         const int rounds = min(32, (p.top + whole - 1) / whole);
+#pragma unroll 1
         for (int r = 0; r < rounds; ++r) {
           last = __reduce_max_sync(0xffffffffu, key);
           const uint32_t who = __ballot_sync(0xffffffffu, key == last);
@@ -371,34 +374,37 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
       }
     }
   };
-  int done = 0, next = 1, v0 = va;
-  for (; v0 + step <= vb; v0 += step) {
-    chunk(v0, std::true_type{});
-    if (TOP && ++done == next && v0 + step < vb) {
+  int done = 0, next = 1;
+#pragma unroll 1
+  for (int v0 = va; v0 < vb || v0 == va; v0 += step) {
+    if (TOP && done > 0 && done == next) {
       next *= 2;
       const int left = narrow();
       if (left == p.top) T0 = value_of((uint32_t)(cand[left - 1] >> 32));
     }
+    ++done;
+    if (v0 + step <= vb) chunk(v0, std::true_type{});
+    else chunk(v0, std::false_type{});
   }
-  if (v0 < vb || v0 == va) chunk(v0, std::false_type{});
   if (TOP && ei >= eb && !(edge < T0)) push(edge, ei);
 
   // ---- the slice's weights and rank
   auto reduce = [&](Stat st) {
-#pragma unroll
+#pragma unroll 1
     for (int o = 16; o > 0; o >>= 1) {
       Stat ot;
       ot.m = __shfl_xor_sync(0xffffffffu, st.m, o);
       ot.S = __shfl_xor_sync(0xffffffffu, st.S, o);
       ot.E = __shfl_xor_sync(0xffffffffu, st.E, o);
       // (both lanes of a pair add in the same order)
-      st = lane & o ? merge(ot, st, c) : merge(st, ot, c);
+      const bool up = lane & o;
+      st = merge(up ? ot : st, up ? st : ot, c);
     }
     __syncthreads();
     if (lane == 0) wstat[warp] = st;
     __syncthreads();
     st = wstat[0];
-#pragma unroll
+#pragma unroll 1
     for (int w = 1; w < kWarps; ++w) st = merge(st, wstat[w], c);
     return st;
   };
@@ -417,6 +423,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
     // -inf among the logits made 0 * -inf: once more, without those
     const float m = st.m;
     S = En = 0.f;
+#pragma unroll 1
     for (int i = e0 + tid; i < e1; i += NT) {
       const float x = to_f32(row[i]);
       const float q = x - m, w = ex2_ftz(q * c);
@@ -430,6 +437,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
   if (odd) {
     greater = 0;
     const uint32_t kt = key_of(xt);
+#pragma unroll 1
     for (int i = e0 + tid; i < e1; i += NT) greater += key_of(to_f32(row[i])) > kt;
   }
   greater = total(greater);  // (its barriers also order the candidates)
@@ -439,8 +447,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
     const int K = p.top, n = odd ? kCap + 1 : narrow();
     if (n > kCap) {
       uint64_t prev = ~0ull;
+#pragma unroll 1
       for (int k = 0; k < K; ++k) {
         uint64_t best = 0;
+#pragma unroll 1
         for (int i = e0 + tid; i < e1; i += NT) {
           const uint64_t it = item_of(to_f32(row[i]), i);
           if (it < prev && it > best) best = it;
@@ -472,14 +482,17 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
       cluster_sync();  // its shared memory lives until the first CTA has read it
       return;
     }
+#pragma unroll 1
     for (int r = 1; r < C; ++r) {
       st = merge(st, Stat{peer_load(&slice.m, r), peer_load(&slice.S, r), peer_load(&slice.E, r)}, c);
       greater += peer_load(&above, r);
     }
     if constexpr (TOP) {
       const int K = p.top, n = C * K;
+#pragma unroll 1
       for (int i = tid; i < n; i += NT) cand[i] = peer_load(&list[i % K], i / K);
       cluster_sync();  // (its barrier is the CTA's too)
+#pragma unroll 1
       for (int i = tid; i < n; i += NT) {
         const uint64_t me = cand[i];
         int r = 0;

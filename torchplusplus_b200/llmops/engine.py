@@ -116,6 +116,10 @@ class DecodeEngine:
         # None = greedy; else dict(temperature, top_k, top_p, seed) (set_sampling)
         self.sampling: Optional[dict] = None
         self._graph_sampling: Optional[dict] = None
+        # None, or dict(top): the scores of the tokens chosen (set_logprobs)
+        self.scoring: Optional[dict] = None
+        self._graph_scoring: Optional[dict] = None
+        self.scores: Optional[tuple] = None
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self.launches_per_step: int | None = None
         self.prompt_len = 0
@@ -164,6 +168,7 @@ class DecodeEngine:
         if self.persistent is not None and self.sampling is None:
             self.persistent.step(self.tokens, self.positions, self.seqlens, self.out_ids[0],
                                  self.logits[0])
+            self._record(ln["b"])
             return
         # several lanes run side by side as graph branches: each plans its
         # grids for its share of the SMs
@@ -219,6 +224,17 @@ class DecodeEngine:
             ops.rmsnorm_linear(x, self.lm_head_f, self.eps, out=ln["logits"])
         self._pick(ln["logits"], ln["positions"], ln["tokens"])
         ops.decode_advance(ln["tokens"], ln["out_ids"], ln["positions"], ln["seqlens"])
+        self._record(ln["b"])
+
+    def _record(self, b: slice) -> None:
+        """Writes the scores of the tokens just chosen to their places in `scores`."""
+        if self.scoring is None:
+            return
+        got = ops.token_logprobs(self.logits[b], self.tokens[b], top=self.scoring["top"])
+        at = self.positions[b].long()
+        row = torch.arange(at.shape[0], device=self.device)
+        for room, t in zip(self.scores, got):
+            room[b].index_put_((row, at), t)
 
     def _pick(self, logits: torch.Tensor, counters: torch.Tensor, out: torch.Tensor) -> None:
         """Next token per row: argmax, or an on-device draw (temperature /
@@ -244,6 +260,28 @@ class DecodeEngine:
 
     def set_greedy(self) -> None:
         self.sampling = None
+
+    def set_logprobs(self, top: Optional[int] = 0) -> None:
+        """Score the tokens chosen from now on under the model's own distribution
+        (temperature 1, whatever the sampling): `scores` holds, for each place of out_ids, the
+        token's log probability, the distribution's entropy and the token's rank, [B,
+        max_seq_len], and the `top` most likely tokens' log probabilities and ids, [B,
+        max_seq_len, top] (ops.token_logprobs; zeros where nothing was chosen since the last
+        prefill).  None: no more.  The decode graph is re-recorded when the setting changes."""
+        if top is None:
+            self.scoring = self.scores = None
+            return
+        if not 0 <= top <= min(32, self.cfg.vocab_size):
+            raise ValueError("top must be at most 32 and at most the vocabulary's size")
+        if self.scoring is not None and self.scoring["top"] == top:
+            return
+        self.scoring = dict(top=int(top))
+        shape, dev = (self.batch_size, self.max_seq_len), self.device
+        self.scores = (torch.zeros(shape, device=dev), torch.zeros(shape, device=dev),
+                       torch.zeros(shape, dtype=torch.int64, device=dev),
+                       torch.zeros(*shape, top, device=dev),
+                       torch.zeros(*shape, top, dtype=torch.int64, device=dev))
+        self._graph_scoring = None
 
     def step_eager(self) -> None:
         """One decode step launched directly (no graph); used by tests."""
@@ -280,12 +318,17 @@ class DecodeEngine:
         torch.cuda.current_stream(self.device).wait_stream(main)
         self.graph = g
         self._graph_sampling = None if self.sampling is None else dict(self.sampling)
+        self._graph_scoring = self.scoring
 
     # ------------------------------------------------------------ prefill
     @torch.inference_mode()
-    def prefill(self, input_ids: torch.Tensor) -> None:
-        """Runs the prompt through the model (tensor-core GEMMs + flash
-        attention, writing the caches) and samples the first new token."""
+    def prefill(self, input_ids) -> None:
+        """Runs the prompts through the model (tensor-core GEMMs + flash attention, writing the
+        caches) and samples the first new token: ids [B, S], or a list of B 1-D prompts of any
+        lengths of at least one token, which run packed row after row, without padding."""
+        if isinstance(input_ids, (list, tuple)):
+            self._prefill_packed(input_ids)
+            return
         B, S = input_ids.shape
         if B != self.batch_size or S >= self.max_seq_len:
             raise ValueError("prompt does not fit the engine's batch / capacity")
@@ -295,16 +338,45 @@ class DecodeEngine:
         x = ops.embedding(ids, self.emb)
         for blk, c in zip(self.model.transformer_blocs, self.caches):
             x = blk(x, self.cos, self.sin, c, 0)
-        h = ops.rmsnorm(x[:, -1], self.nf, self.eps)
-        ops.linear(h, self.lm_head, out=self.logits)
-        self._pick(self.logits, torch.full((B,), S - 1, dtype=torch.int32, device=self.device),
-                   self.tokens)
         self.out_ids[:, :S].copy_(ids)
-        self.out_ids[:, S].copy_(self.tokens)
-        self.positions.fill_(S)
-        self.seqlens.fill_(S + 1)
-        self.prompt_len = S
-        self._pos = S
+        self._first_token(x[:, -1], S, [S] * B)
+
+    def _prefill_packed(self, prompts) -> None:
+        from .scoring import pack
+        ids, cu, lens = pack(prompts, self.device)
+        S = max(lens)
+        if len(lens) != self.batch_size or S >= self.max_seq_len or min(lens) < 1:
+            raise ValueError("prompts do not fit the engine's batch / capacity")
+        x = self.model.forward_packed(ids, cu, self.caches)
+        for c in self.caches:
+            c.cache_len = S
+        a = 0
+        for b, n in enumerate(lens):
+            self.out_ids[b, :n].copy_(ids[a:a + n])
+            a += n
+        last = cu[1:].long() - 1
+        self._first_token(x[last], cu[1:] - cu[:-1], lens)
+
+    def _first_token(self, last: torch.Tensor, lengths, lens: List[int]) -> None:
+        """The first new token from the prompts' last rows; `lengths`: the prompts', one
+        number or int32 [B]."""
+        h = ops.rmsnorm(last, self.nf, self.eps)
+        ops.linear(h, self.lm_head, out=self.logits)
+        if isinstance(lengths, int):
+            self.positions.fill_(lengths)
+        else:
+            self.positions.copy_(lengths)
+        self._pick(self.logits, self.positions - 1, self.tokens)
+        rows = torch.arange(self.batch_size, device=self.device)
+        self.out_ids[rows, self.positions.long()] = self.tokens
+        torch.add(self.positions, 1, out=self.seqlens)
+        if self.scoring is not None:
+            for room in self.scores:
+                room.zero_()
+            self._record(slice(0, self.batch_size))
+        self.prompt_len = max(lens)
+        self._lens = lens
+        self._pos = max(lens)
 
     def _advance(self, steps: int) -> None:
         # every step writes one K/V row at the current position and the next
@@ -316,16 +388,21 @@ class DecodeEngine:
 
     def decode(self, steps: int) -> None:
         self._advance(steps)
-        if self.graph is None or self._graph_sampling != self.sampling:
+        if self.graph is None or self._graph_sampling != self.sampling or \
+                self._graph_scoring is not self.scoring:
             self.capture()
         for _ in range(steps):
             self.graph.replay()
 
     @torch.inference_mode()
-    def generate(self, input_ids: torch.Tensor, max_new_token: int,
+    def generate(self, input_ids, max_new_token: int,
                  eos_token_id: Optional[int] = None,
-                 stop_token_ids: Optional[list] = None, check_every: int = 16) -> torch.Tensor:
-        B, S = input_ids.shape
+                 stop_token_ids: Optional[list] = None, check_every: int = 16):
+        """ids [B, S] -> [B, S + new]; a list of B 1-D prompts -> a list of them with their
+        new tokens (the same number each)."""
+        packed = isinstance(input_ids, (list, tuple))
+        S = max(map(len, input_ids), default=0) if packed else input_ids.shape[1]
+        B = len(input_ids)
         if S + max_new_token > self.max_seq_len:
             raise ValueError("prompt + max_new_token exceeds the engine capacity")
         self.prefill(input_ids)
@@ -340,10 +417,14 @@ class DecodeEngine:
             remaining -= n
             done += n
             if stops:
-                cur = self.out_ids[:, S:S + 1 + done].cpu()
+                cur = torch.stack([self.out_ids[b, n:n + 1 + done]
+                                   for b, n in enumerate(self._lens)]).cpu() if packed \
+                    else self.out_ids[:, S:S + 1 + done].cpu()
                 hit = torch.zeros(B, dtype=torch.bool)
                 for t in stops:
                     hit |= (cur == t).any(dim=1)
                 if bool(hit.all()):
                     break
+        if packed:
+            return [self.out_ids[b, :n + 1 + done].clone() for b, n in enumerate(self._lens)]
         return self.out_ids[:, :S + 1 + done]

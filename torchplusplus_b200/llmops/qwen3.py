@@ -82,6 +82,11 @@ class Transformer(nn.Module):
         h = self.rms_norm2(x)
         return self.ffn(h, residual=x)
 
+    def forward_packed(self, x, cos, sin, cu_seqlens: torch.Tensor,
+                       kv_cache: Optional[KVCache] = None):
+        x = self.attn.forward_packed(self.rms_norm1(x), cos, sin, cu_seqlens, kv_cache, residual=x)
+        return self.ffn(self.rms_norm2(x), residual=x)
+
 
 class Qwen3(LLMInference):
 
@@ -137,6 +142,23 @@ class Qwen3(LLMInference):
         x = self.final_rmsnorm(x)
         return ops.linear(x, self.out_head.weight)
 
+    def forward_packed(self, ids: torch.Tensor, cu_seqlens: torch.Tensor,
+                       kv_caches: Optional[List[KVCache]] = None) -> torch.Tensor:
+        """Whole prompts of different lengths packed row after row (ids [N], sequence b in
+        rows cu_seqlens[b] .. cu_seqlens[b+1]-1, int32 on the device) -> the rows [N, E] before
+        the final norm.  With kv_caches each sequence's K and V go to its rows of them."""
+        x = ops.embedding(ids, self.tok_embed.weight)
+        for i, blk in enumerate(self.transformer_blocs):
+            x = blk.forward_packed(x, self.cos, self.sin, cu_seqlens,
+                                   kv_caches[i] if kv_caches is not None else None)
+        return x
+
+    def score(self, prompts, temperature: float = 1.0, top: Optional[int] = None):
+        """The log probability of every token of every prompt (a list of 1-D tensors of
+        token ids, of any lengths): llmops.scoring.score."""
+        from .scoring import score
+        return score(self, prompts, temperature, top)
+
     def engine(self, batch_size: int, max_seq_len: int, weight_format: str | None = None):
         """The model's decode engine (rebuilt when the batch, capacity or
         weight format changes).  weight_format: "native" or "fp8" (decode
@@ -152,16 +174,23 @@ class Qwen3(LLMInference):
         return e
 
     @torch.inference_mode()
-    def generate(self, input_ids: torch.Tensor, max_new_token: int = 100, temp: float = 1.0,
+    def generate(self, input_ids, max_new_token: int = 100, temp: float = 1.0,
                  top_p: float = 0.9, top_k: Optional[int] = None,
                  sampling_strategy: str = "top_p", stop_token_ids=None, eos_token_id=None,
                  stream: bool = False, stream_callback=None):
+        """input_ids [B, S], or a list of 1-D prompts of any lengths (their prefill is packed;
+        the result is then a list: each prompt with its new tokens)."""
+        packed = isinstance(input_ids, (list, tuple))
+        if packed and (stream or sampling_strategy not in ("greedy", "top_p", "top_k") or
+                       (sampling_strategy == "top_k" and top_k is None)):
+            raise ValueError("prompts of different lengths generate greedily, by top_p or by "
+                             "top_k, without a stream")
         if stream or sampling_strategy not in ("greedy", "top_p", "top_k") or \
                 (sampling_strategy == "top_k" and top_k is None):
             return super().generate(input_ids, max_new_token, temp, top_p, top_k,
                                     sampling_strategy, stop_token_ids, eos_token_id, stream,
                                     stream_callback)
-        B, S = input_ids.shape
+        B, S = (len(input_ids), max(map(len, input_ids), default=0)) if packed else input_ids.shape
         eng = self.engine(B, S + max_new_token)
         if sampling_strategy == "greedy":
             eng.set_greedy()
