@@ -222,6 +222,17 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
     const int at = atomicAdd(&count, 1);
     if (at < kCap) cand[at] = item_of(x, i);
   };
+  // how many of the first n candidates come before `me`
+  auto place = [&](uint64_t me, int n) {
+    int r = 0, j = 0;
+#pragma unroll 4
+    for (; j + 2 <= n; j += 2) {
+      const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(cand + j);
+      r += (o.x > me) + (o.y > me);
+    }
+    if (j < n) r += cand[j] > me;
+    return r;
+  };
   // the candidates in order, all but the first `top` dropped; returns how many are left
   // (more than kCap: too many, and none dropped)
   auto narrow = [&]() {
@@ -231,8 +242,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
 #pragma unroll 1
     for (int i = tid; i < n; i += NT) {
       const uint64_t me = cand[i];
-      int r = 0;
-      for (int j = 0; j < n; ++j) r += cand[j] > me;
+      const int r = place(me, n);
       if (r < p.top) list[r] = me;
     }
     __syncthreads();
@@ -495,8 +505,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
 #pragma unroll 1
       for (int i = tid; i < n; i += NT) {
         const uint64_t me = cand[i];
-        int r = 0;
-        for (int j = 0; j < n; ++j) r += cand[j] > me;
+        const int r = place(me, n);
         if (me != 0 && r < K) list[r] = me;
       }
       __syncthreads();
