@@ -964,9 +964,10 @@ def attention_tree_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
 
 # ---------------------------------------------------------------- packed prompts
 def _one_device(t: torch.Tensor, *ts: torch.Tensor | None) -> None:
-    for o in (t, *ts):
-        if o is not None and (not o.is_cuda or o.get_device() != t.get_device()):
-            _cuda(o)
+    dev = t.get_device()  # (-1 on the CPU)
+    for o in ts:
+        if o is not None and o.get_device() != dev:
+            _cuda(t, o)
             raise ValueError(f"operands on different devices: {t.device} and {o.device}")
 
 
@@ -1012,13 +1013,16 @@ def qk_norm_rope_packed(qkv: torch.Tensor, q_norm_w: torch.Tensor | None,
             raise ValueError("the pools must match qkv's heads and head dim")
         rows, tstride = 64 * block_table.shape[1], block_table.stride(0)
     else:
-        cs = k_cache.stride()
-        if k_cache.dim() != 4 or k_cache.shape[:2] != (B, Hkv) or k_cache.shape[3] != D \
-                or v_cache.shape != k_cache.shape or v_cache.stride() != cs or cs[3] != 1:
+        cs, shape = k_cache.stride(), k_cache.shape
+        if len(shape) != 4 or shape[0] != B or shape[1] != Hkv or shape[3] != D \
+                or v_cache.shape != shape or v_cache.stride() != cs or cs[3] != 1:
             raise ValueError("caches must be [B, Hkv, Smax, D] with identical layouts")
-        rows = k_cache.shape[2]
+        rows = shape[2]
     qkv = _rows16(qkv)
-    cos, sin, cs_stride, cs_dt = _table(cos, sin, D)
+    cs_dt, cs_stride = N.DTYPE_CODE.get(cos.dtype), D
+    if cs_dt is None or cos.shape != sin.shape or cos.dtype is not sin.dtype or cos.dim() != 2 \
+            or cos.shape[1] != D or not (cos.is_contiguous() and sin.is_contiguous()):
+        cos, sin, cs_stride, cs_dt = _table(cos, sin, D)
     q_out = _tree_out(q_out, (N_, Hq, D), qkv)
     k_out = _tree_out(k_out, (N_, Hkv, D), qkv)
     N.call_on(qkv, "tpp_qk_norm_rope_packed", qkv.data_ptr(), qkv.stride(0), N.ptr(q_norm_w),
