@@ -63,6 +63,7 @@ struct Plan {
 struct PackedAttnArgs {
   const int32_t* cu;
   int B, N, Hkv, G, TT;
+  int tok_w;  // tokens of 32 rows of a query tile (0: not a whole number)
   int inv_g;  // ceil(2^16 / G): r * inv_g >> 16 is r / G for r < 128
   int causal;
   int window;  // at most N; -1: none
@@ -233,6 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     packed_attn_kernel(const __grid_constant__ CUtensorMap tm_q,
                        const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v,
+                       const __grid_constant__ CUtensorMap tm_o,
                        const __grid_constant__ PackedAttnArgs p) {
   using P = Plan<D>;
   constexpr int S = P::kStages, BKV = P::BKV;
@@ -499,38 +501,43 @@ __global__ void __launch_bounds__(kThreads, 1)
         seen ^= 1u << s;
         ok = ok && wait_short(&kv_full[s], (r / S) & 1, p.err, 73);
         if (!ok) break;
-        bool wrote = false;
+        // rows of the sequence, then rows behind it (each 128 bytes a box)
+        const int valid = min(BKV, w.len - (w.kb + j) * BKV);
+        uint8_t* at = sKV + s * P::kTile;
+        bool wrote = valid < BKV;
+        uint32_t acc[4] = {0, 0, 0, 0};  // 0 or NaN
 #pragma unroll 1
-        for (int rl = lane; rl < BKV; rl += 32) {
-          uint8_t* at = sKV + s * P::kTile + rl * 128;
-          // (chunks in the order that keeps eight rows on different banks)
-          if ((w.kb + j) * BKV + rl >= w.len) {
-#pragma unroll
-            for (int c = 0; c < D / 8; ++c)
-              *reinterpret_cast<uint4*>(at + (c >> 3) * P::kBox + ((c ^ rl) & 7) * 16) =
-                  make_uint4(0, 0, 0, 0);
-            wrote = true;
-            continue;
-          }
-          uint32_t acc[4] = {0, 0, 0, 0};  // 0 or NaN
-#pragma unroll
-          for (int c = 0; c < D / 8; ++c) {
-            const uint4 u =
-                *reinterpret_cast<const uint4*>(at + (c >> 3) * P::kBox + ((c ^ rl) & 7) * 16);
-            acc[0] = times_zero_plus<T>(u.x, acc[0]);
-            acc[1] = times_zero_plus<T>(u.y, acc[1]);
-            acc[2] = times_zero_plus<T>(u.z, acc[2]);
-            acc[3] = times_zero_plus<T>(u.w, acc[3]);
-          }
-          if (((acc[0] | acc[1] | acc[2] | acc[3]) & 0x7fff7fffu) != 0) {
+        for (int b = 0; b < P::kBoxes; ++b, at += P::kBox) {
+          constexpr int kAtOnce = 10;
 #pragma unroll 1
-            for (int c = 0; c < D; ++c) {
-              T* e = reinterpret_cast<T*>(at + (c >> 6) * P::kBox) + (c & 63);
-              if (!isfinite(to_f32(*e))) *e = from_f32<T>(0.f);
+          for (int e0 = lane * 16; e0 < valid * 128; e0 += kAtOnce * 512) {
+            uint4 u[kAtOnce];
+#pragma unroll
+            for (int q = 0; q < kAtOnce; ++q)
+              u[q] = e0 + q * 512 < valid * 128 ? *reinterpret_cast<const uint4*>(at + e0 + q * 512)
+                                                : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int q = 0; q < kAtOnce; ++q) {
+              acc[0] = times_zero_plus<T>(u[q].x, acc[0]);
+              acc[1] = times_zero_plus<T>(u[q].y, acc[1]);
+              acc[2] = times_zero_plus<T>(u[q].z, acc[2]);
+              acc[3] = times_zero_plus<T>(u[q].w, acc[3]);
             }
-            wrote = true;
-            atomicExch(odd_v + (n & 1), n + 1);
           }
+#pragma unroll 1
+          for (int e0 = valid * 128 + lane * 16; e0 < (int)P::kBox; e0 += 512)
+            *reinterpret_cast<uint4*>(at + e0) = make_uint4(0, 0, 0, 0);
+        }
+        if (__any_sync(0xffffffffu, ((acc[0] | acc[1] | acc[2] | acc[3]) & 0x7fff7fffu) != 0)) {
+          at = sKV + s * P::kTile;
+#pragma unroll 1
+          for (int e0 = lane; e0 < P::kBoxes * valid * 64; e0 += 32) {
+            const int b = e0 / (valid * 64);
+            T* e = reinterpret_cast<T*>(at + b * P::kBox) + (e0 - b * valid * 64);
+            if (!isfinite(to_f32(*e))) *e = from_f32<T>(0.f);
+          }
+          wrote = true;
+          atomicExch(odd_v + (n & 1), n + 1);
         }
         if (wrote) fence_proxy_async_smem();
         __syncwarp();
@@ -681,46 +688,69 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         tc_fence_after();
         const float inv = i ? inv1 : inv0;
-        const int tok0 = w.t0 + i * p.TT, rows = min(p.TT, w.len - tok0);
-        T* out = static_cast<T*>(p.o) + (int64_t)(w.first + tok0) * p.o_sn +
-                 (int64_t)w.kvh * p.G * p.o_sh + (lane & 7) * 8;
         // through this warp's part of the staging tile, so that a store covers whole rows
+        const int tok0 = w.t0 + i * p.TT, rows = min(p.TT, w.len - tok0);
         uint8_t* st = stage + (warp & 3) * 4096;
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         __syncwarp();
 #pragma unroll
-        for (int c = 0; c < D; c += 32) {
-          uint32_t r[32];
+        for (int c = 0; c < D; c += 64) {
+          uint32_t r[64];
           tmem_ld32(tO + i * D + c, r);
+          tmem_ld32(tO + i * D + c + 32, r + 32);
           tmem_wait_ld();
+          if (c + 64 == D) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&o_empty[i]);
+          }
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
+          for (int q = 0; q < 8; ++q) {
             float f[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(r[q * 8 + e]) * inv;
             *reinterpret_cast<uint4*>(st + (c >> 6) * P::kQBox + lane * 128 +
-                                      (((c & 63) / 8 + q) ^ (lane & 7)) * 16) = pack8<T>(f);
+                                      (q ^ (lane & 7)) * 16) = pack8<T>(f);
           }
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&o_empty[i]);
-#pragma unroll 4
-        for (int q = 0; q < 8 * P::kBoxes; ++q) {
-          const int r = (q & 7) * 4 + (lane >> 3), row = (warp & 3) * 32 + r;
-          const int tl = row * p.inv_g >> 16;
-          const uint4 u = *reinterpret_cast<const uint4*>(st + (q >> 3) * P::kQBox + r * 128 +
-                                                          ((lane ^ r) & 7) * 16);
-          if (tl < rows)
-            *reinterpret_cast<uint4*>(out + tl * p.o_sn + (row - tl * p.G) * p.o_sh +
-                                      (q >> 3) * 64) = u;
+        // this warp's tokens: all of them in one request a box, or their rows one by one
+        const int t_lo = p.tok_w * (warp & 3);
+        if (p.tok_w > 0 && t_lo + p.tok_w <= rows) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            for (int b = 0; b < P::kBoxes; ++b)
+              asm volatile(
+                  "cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];"
+                  ::"l"(reinterpret_cast<uint64_t>(&tm_o)), "r"(b * 64), "r"(w.kvh * p.G),
+                  "r"(w.first + tok0 + t_lo), "r"(smem_u32(st + b * P::kQBox))
+                  : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+        } else {
+          __syncwarp();
+          T* out = static_cast<T*>(p.o) + (int64_t)(w.first + tok0) * p.o_sn +
+                   (int64_t)w.kvh * p.G * p.o_sh + (lane & 7) * 8;
+#pragma unroll 2
+          for (int q = 0; q < 8 * P::kBoxes; ++q) {
+            const int r = (q & 7) * 4 + (lane >> 3), row = (warp & 3) * 32 + r;
+            const int tl = row * p.inv_g >> 16;
+            const uint4 u = *reinterpret_cast<const uint4*>(st + (q >> 3) * P::kQBox + r * 128 +
+                                                            ((lane ^ r) & 7) * 16);
+            if (tl < rows)
+              *reinterpret_cast<uint4*>(out + tl * p.o_sn + (row - tl * p.G) * p.o_sh +
+                                        (q >> 3) * 64) = u;
+          }
         }
         // (set, if at all, before the last P V could be issued)
         if (*reinterpret_cast<volatile int*>(odd_v + (n & 1)) == n + 1) {
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
           __syncwarp();
           add_hidden<T, D>(w, i, rl, p);
         }
       }
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   __syncwarp();
   tc_fence_before();
@@ -756,6 +786,7 @@ extern "C" int tpp_attention_packed(const void* q, int64_t q_sn, int64_t q_sh, c
   a.G = (int)(Hq / Hkv);
   a.TT = BQ / a.G;
   a.inv_g = (65536 + a.G - 1) / a.G;
+  a.tok_w = 32 % a.G == 0 ? 32 / a.G : 0;
   a.causal = causal != 0;
   a.window = (int)(window_left < 0 ? -1 : window_left < N ? window_left : N);
   a.sign = scale > 0 ? 1 : scale < 0 ? -1 : 0;
@@ -763,7 +794,7 @@ extern "C" int tpp_attention_packed(const void* q, int64_t q_sn, int64_t q_sh, c
   a.o = o; a.o_sn = o_sn; a.o_sh = o_sh;
   a.v = v; a.v_sn = v_sn; a.v_sh = v_sh;
   a.err = device_error_flag();
-  CUtensorMap tq, tk, tv;
+  CUtensorMap tq, tk, tv, to;
   const uint64_t qd[3] = {(uint64_t)D, (uint64_t)Hq, (uint64_t)N};
   const uint64_t qs[2] = {(uint64_t)q_sh * 2, (uint64_t)q_sn * 2};
   const uint32_t qb[3] = {64, (uint32_t)a.G, (uint32_t)a.TT};
@@ -776,6 +807,9 @@ extern "C" int tpp_attention_packed(const void* q, int64_t q_sn, int64_t q_sh, c
                            (uint32_t)(D / 64), 1};
     return make_tmap(m, base, dtype, 4, d, s, b, CU_TENSOR_MAP_SWIZZLE_128B);
   };
+  const uint64_t os[2] = {(uint64_t)o_sh * 2, (uint64_t)o_sn * 2};
+  const uint32_t ob[3] = {64, (uint32_t)(a.tok_w ? a.G : 1), (uint32_t)(a.tok_w ? a.tok_w : 1)};
+  if (rc == TPP_OK) rc = make_tmap(&to, o, dtype, 3, qd, os, ob, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc == TPP_OK) rc = kv_map(&tk, k, k_sn, k_sh);
   if (rc == TPP_OK) rc = kv_map(&tv, v, v_sn, v_sh);
   if (rc != TPP_OK) return rc;
@@ -792,7 +826,7 @@ extern "C" int tpp_attention_packed(const void* q, int64_t q_sn, int64_t q_sh, c
                                "packed_attn_kernel");
     if (e != TPP_OK) return e;
     return launch("packed_attn_kernel", kern, dim3(grid), dim3(kThreads), Plan<DH>::kSmem,
-                  as_stream(stream), 0u, tq, tk, tv, a);
+                  as_stream(stream), 0u, tq, tk, tv, to, a);
   };
   return TPP_DISPATCH_HALF(dtype, T, [&] {
     return D == 128 ? go(T(), std::integral_constant<int, 128>{})
