@@ -113,9 +113,9 @@ def test_attention_long(Hq, Hkv, D, dtype):
     check_attention(*operands(4, N, Hq, Hkv, D, dtype), cu)
 
 
-@pytest.mark.parametrize("seed,n", [(5, 31), (6, 33), (7, 700)])
+@pytest.mark.parametrize("seed,n", [(5, 31), (6, 33), (7, 700), (8, 3000)])
 def test_attention_many_sequences(seed, n):
-    lens = torch.randint(0, 200 if n < 100 else 40, (n,),
+    lens = torch.randint(0, 200 if n < 100 else 40 if n < 1000 else 5, (n,),
                          generator=torch.Generator().manual_seed(seed)).tolist()
     cu, N = packed(lens)
     check_attention(*operands(seed, N, 4, 2, 64, BF16), cu)
@@ -237,6 +237,31 @@ def test_attention_on_a_side_stream_and_in_a_graph():
     graph.replay()
     check_attention(q, k, v, cu, got=out)
     assert (out[480:] == 0).all()
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(4, 2), (6, 2)])
+def test_attention_into_its_queries(Hq, Hkv):
+    from torchplusplus_b200 import ops
+    cu, N = packed([300, 5, 131])
+    q, k, v = operands(16, N, Hq, Hkv, 64, BF16)
+    want = ops.attention_packed(q, k, v, cu)
+    assert ops.attention_packed(q, k, v, cu, out=q) is q and torch.equal(q, want)
+
+
+def test_attention_of_lengths_that_do_not_ascend():
+    """Whatever cu_seqlens holds, only rows of q, k and v are read and rows of out written."""
+    from torchplusplus_b200 import ops
+    q, k, v = operands(17, 400, 4, 2, 128, BF16)
+    out = torch.zeros(420, 4, 128, dtype=BF16, device="cuda")
+    cu = torch.tensor([-5, 100, 50, 1 << 30, -(1 << 31), 20, 500], dtype=torch.int32, device="cuda")
+    ops.attention_packed(q, k, v, cu, out=out[:400])
+    assert (out[400:] == 0).all() and ops.device_error() == 0
+    # [0, 100), none, [50, 400), none, [0, 20) and [20, 400): the rows of no two of them
+    cos = torch.ones(400, 128, device="cuda")
+    qkv = torch.randn(400, 8 * 128, generator=gen(17), device="cuda").to(BF16)
+    kc = torch.zeros(6, 2, 64, 128, dtype=BF16, device="cuda")
+    ops.qk_norm_rope_packed(qkv, None, None, 1e-6, cos, cos, cu, 4, 2, kc, kc.clone())
+    torch.cuda.synchronize()
 
 
 def test_attention_of_no_rows():
@@ -374,6 +399,7 @@ def test_refusals():
         (ValueError, lambda: ops.attention_packed(q, k, v, cu[:0])),
         (RuntimeError, lambda: ops.attention_packed(q, k, v, cu.cpu())),
         (ValueError, lambda: ops.attention_packed(q, k, v, cu, out=q[:10])),
+        (ValueError, lambda: ops.attention_packed(q, k, v, cu, out=q[:1].expand(N, -1, -1))),
         (TppError, lambda: ops.attention_packed(*operands(1, N, 2, 2, 96, BF16), cu)),
         (TppError, lambda: ops.attention_packed(*operands(1, N, 129, 1, 64, BF16), cu)),
         (TppError, lambda: ops.attention_packed(q, k, v, cu, scale=math.inf)),

@@ -547,8 +547,8 @@ extern "C" int tpp_token_logprobs(const void* logits, int64_t ld, int64_t N, int
                                   void* stream) {
   if (N == 0) return TPP_OK;
   TPP_REQUIRE(logits && tokens && logprobs && entropy && ranks, TPP_ERR_SHAPE, "null pointer");
-  TPP_REQUIRE(N > 0 && N < (1ll << 31) && V > 0 && V < (1ll << 31) && ld >= V, TPP_ERR_SHAPE,
-              "bad sizes");
+  TPP_REQUIRE(N > 0 && N < (1ll << 31) && V > 0 && V < (1ll << 31) - 4096 && ld >= V,
+              TPP_ERR_SHAPE, "bad sizes");
   TPP_REQUIRE(temperature > 0 && isfinite(temperature) && temperature >= 1e-6, TPP_ERR_SHAPE,
               "temperature must be positive");
   TPP_REQUIRE(top >= 0 && top <= kMaxTop && top <= V, TPP_ERR_SHAPE,

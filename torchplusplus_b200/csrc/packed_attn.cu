@@ -124,6 +124,7 @@ struct Walk {
   int level;           // the blocks' number
   uint32_t base;       // items before this level (there are fewer than 2^31)
   int count;           // sequences that have it
+  int seek, before;    // the last item's: of 32 sequences the first, those with it before
 
   // sequence b's first row and length (whatever cu holds, inside [0, N])
   __device__ __forceinline__ int2 span(int b) const {
@@ -134,7 +135,7 @@ struct Walk {
     return b < B && span(b).y > (int64_t)level * per;
   }
   __device__ void recount(int lane) {
-    count = 0;
+    count = seek = before = 0;
 #pragma unroll 1
     for (int b = 0; b < B; b += 32)
       count += __popc(__ballot_sync(0xffffffffu, has(b + lane)));
@@ -158,19 +159,20 @@ struct Walk {
     }
     if (level < 0) return make_int4(0, -1, 0, 0);
     const uint32_t in = at - base;
-    int nth = (int)(in / (uint32_t)Hkv);
+    const int nth = (int)(in / (uint32_t)Hkv);
     const int kvh = (int)(in - (uint32_t)nth * Hkv);
 #pragma unroll 1
-    for (int b = 0; b < B; b += 32) {
-      const uint32_t set = __ballot_sync(0xffffffffu, has(b + lane));
+    for (; seek < B; seek += 32) {  // (items ascend, so the last one's place is a start)
+      const uint32_t set = __ballot_sync(0xffffffffu, has(seek + lane));
       const int n = __popc(set);
-      if (nth < n) {
-        const bool me = (set >> lane & 1) && __popc(set & ((1u << lane) - 1)) == nth;
+      if (nth < before + n) {
+        const bool me =
+            (set >> lane & 1) && before + __popc(set & ((1u << lane) - 1)) == nth;
         const int src = __ffs(__ballot_sync(0xffffffffu, me)) - 1;
-        const int2 s = span(b + src);
+        const int2 s = span(seek + src);
         return make_int4(s.x, s.y, level * per, kvh);
       }
-      nth -= n;
+      before += n;
     }
     return make_int4(0, -1, 0, 0);
   }
@@ -326,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------- items and loads ----------------
     // Step gk of the K's, (wk, jk), runs two ahead of step gv of the V's, (wv, jv); an item is
     // handed out when the K's come to it.
-    Walk walk{p.cu, p.B, p.N, 2 * p.TT, p.Hkv, 0, 0, 0};
+    Walk walk{p.cu, p.B, p.N, 2 * p.TT, p.Hkv, 0, 0, 0, 0, 0};
     walk.init(lane);
     int nk = 0;
     auto next_item = [&]() {
@@ -794,6 +796,10 @@ extern "C" int tpp_attention_packed(const void* q, int64_t q_sn, int64_t q_sh, c
   a.o = o; a.o_sn = o_sn; a.o_sh = o_sh;
   a.v = v; a.v_sn = v_sn; a.v_sh = v_sh;
   a.err = device_error_flag();
+  // items at most: a block of 2 TT tokens each, one more a sequence
+  const int64_t items = (N / (2 * a.TT) + B) * Hkv;
+  TPP_REQUIRE(items < (1ll << 30), TPP_ERR_SHAPE, "too many rows, sequences and heads");
+  const unsigned grid = (unsigned)(items < num_sms() ? items : num_sms());
   CUtensorMap tq, tk, tv, to;
   const uint64_t qd[3] = {(uint64_t)D, (uint64_t)Hq, (uint64_t)N};
   const uint64_t qs[2] = {(uint64_t)q_sh * 2, (uint64_t)q_sn * 2};
@@ -813,10 +819,6 @@ extern "C" int tpp_attention_packed(const void* q, int64_t q_sn, int64_t q_sh, c
   if (rc == TPP_OK) rc = kv_map(&tk, k, k_sn, k_sh);
   if (rc == TPP_OK) rc = kv_map(&tv, v, v_sn, v_sh);
   if (rc != TPP_OK) return rc;
-  // items at most: a block of 2 TT tokens each, one more a sequence
-  const int64_t items = (N / (2 * a.TT) + B) * Hkv;
-  TPP_REQUIRE(items < (1ll << 30), TPP_ERR_SHAPE, "too many rows, sequences and heads");
-  const unsigned grid = (unsigned)(items < num_sms() ? items : num_sms());
   auto go = [&](auto tag, auto dim) -> int {
     using T = decltype(tag);
     constexpr int DH = decltype(dim)::value;

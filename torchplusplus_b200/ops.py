@@ -996,7 +996,8 @@ def qk_norm_rope_packed(qkv: torch.Tensor, q_norm_w: torch.Tensor | None,
         raise ValueError("qkv must be [N, (Hq+2Hkv)*D]")
     N_, W = qkv.shape
     D = W // (Hq + 2 * Hkv)
-    _one_device(qkv, cos, sin, cu_seqlens, q_norm_w, k_norm_w, k_cache, v_cache, block_table)
+    _one_device(qkv, cos, sin, cu_seqlens, q_norm_w, k_norm_w, k_cache, v_cache, block_table,
+                q_out, k_out)
     B = _cu_seqlens(cu_seqlens)
     for w in (q_norm_w, k_norm_w):
         if w is not None and (w.shape != (D,) or not w.is_contiguous()):
@@ -1015,8 +1016,10 @@ def qk_norm_rope_packed(qkv: torch.Tensor, q_norm_w: torch.Tensor | None,
     else:
         cs, shape = k_cache.stride(), k_cache.shape
         if len(shape) != 4 or shape[0] != B or shape[1] != Hkv or shape[3] != D \
-                or v_cache.shape != shape or v_cache.stride() != cs or cs[3] != 1:
-            raise ValueError("caches must be [B, Hkv, Smax, D] with identical layouts")
+                or v_cache.shape != shape or v_cache.stride() != cs or cs[3] != 1 \
+                or any(s == 0 and n > 1 for s, n in zip(cs, shape)):
+            raise ValueError("caches must be [B, Hkv, Smax, D] with identical layouts, no two "
+                             "rows in one place")
         rows = shape[2]
     qkv = _rows16(qkv)
     cs_dt, cs_stride = N.DTYPE_CODE.get(cos.dtype), D
@@ -1042,7 +1045,7 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     ascending).  causal: keys up to the row itself; window_left >= 0: none further than
     that before it.  Hq a multiple of Hkv, D 64 or 128.  Returns [N,Hq,D]; rows of no
     sequence are not written.  What a row does not see does not affect it, NaN and
-    infinities included."""
+    infinities included.  out may be q, but share no memory with k and v."""
     dt = _half_alike("q", q, k, v, out)
     if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape:
         raise ValueError("q must be [N, Hq, D], k and v [N, Hkv, D]")
@@ -1055,8 +1058,10 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     q, k, v = _rows16(q), _rows16(k), _rows16(v)
     if out is None:
         out = q.new_empty((N_, Hq, D))
-    elif out.shape != (N_, Hq, D) or out.stride(2) != 1:
-        raise ValueError("out must be [N, Hq, D] with a contiguous last dim")
+    elif out.shape != (N_, Hq, D) or out.stride(2) != 1 \
+            or any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
+        raise ValueError("out must be [N, Hq, D] with a contiguous last dim, no two rows in one "
+                         "place")
     qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), out.stride()
     N.call_on(q, "tpp_attention_packed", q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
               v.data_ptr(), vs[0], vs[1], cu_seqlens.data_ptr(), B, out.data_ptr(), os_[0],
