@@ -164,9 +164,15 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
   __shared__ Stat wstat[kWarps], slice;
   __shared__ int wcount[kWarps];
   __shared__ int count, above;
+  // With whole rows a CTA (128 threads) a chunk's hit costs its warp as little as possible:
+  // the thread's vectors are noted and looked at when the candidates are narrowed.  (Where a
+  // row has several CTAs, latency counts, and they are looked at on the spot.)
+  constexpr bool LATER = TOP && NT == 128;
+  constexpr int kHits = 512;
+  __shared__ int hit[LATER ? kHits : 1], hits;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int C = gridDim.y, cr = C > 1 ? (int)cluster_rank() : 0;
-  if (tid == 0) count = 0;
+  if (tid == 0) count = hits = 0;
   pdl_wait();
   pdl_trigger();
 
@@ -217,6 +223,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
   // (below 0 comes -0, which equals it, and then the largest negative number)
   constexpr uint32_t kLeastKey = 0x007fffffu, kZeroKey = 0x80000000u;
   uint32_t first_key = 0;
+  bool everything = false;
 
   auto push = [&](float x, int i) {
     const int at = atomicAdd(&count, 1);
@@ -237,6 +244,22 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
   // (more than kCap: too many, and none dropped)
   auto narrow = [&]() {
     __syncthreads();
+    if (LATER) {
+      const int noted = hits;
+      if (noted > kHits) return kCap + 1;
+#pragma unroll 1
+      for (int e = tid; e < noted * kU; e += NT) {
+        const int v = hit[e / kU] + e % kU * NT;
+        if (v >= vb) continue;
+        float f[E];
+        Lane<T>::get(ldg_nc_v4(base + (int64_t)v * E), f);
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          if (f[j] > T0 || (everything && v < va + step)) push(f[j], v * E - shift + j);
+      }
+      __syncthreads();
+      if (tid == 0) hits = 0;
+    }
     const int n = count;
     if (n > kCap) return n;
 #pragma unroll 1
@@ -301,10 +324,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
       ref = value_of(big);
       // (reached, not exceeded, is enough in this chunk: the next value below)
       first_key = whole * 32 < p.top ? 0u : least;
-      T0 = first_key <= kLeastKey ? -INFINITY
-                                  : value_of(first_key - (first_key == kZeroKey ? 2 : 1));
+      everything = first_key <= kLeastKey;
+      T0 = everything ? -INFINITY : value_of(first_key - (first_key == kZeroKey ? 2 : 1));
       if (ei >= 0) {
-        if (TOP && ei < eb && (first_key <= kLeastKey || edge > T0)) push(edge, ei);
+        if (TOP && ei < eb && (everything || edge > T0)) push(edge, ei);
         if (edge > xt) ++greater;
         if (edge != -INFINITY) {
           const float q = edge - ref, w = ex2_ftz(q * c);
@@ -319,8 +342,12 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
       S *= f;
       ref = cm;
     }
-    const bool all = first_key <= kLeastKey && v0 == va;
-    if (TOP && (cm > T0 || all)) {
+    const bool all = everything && v0 == va;
+    if (LATER && (cm > T0 || all)) {
+      const int at = atomicAdd(&hits, 1);
+      if (at < kHits) hit[at] = v0 + tid;
+    }
+    if (TOP && !LATER && (cm > T0 || all)) {
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
         if (!FULL && u >= mine) break;
