@@ -201,6 +201,22 @@ def test_attention_non_finite_values(D, bad, causal, window):
         assert (got[hit] == bad).all() or not got[hit].isfinite().any()
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n", [1, 30, 90])
+def test_attention_non_finite_values_in_every_sequence(n, D):
+    """Many short sequences a CTA: what one's V holds is known when its rows are written."""
+    B = 4000
+    cu, N = packed([n] * B)
+    q, k, v = operands(22, N, 4, 2, D, BF16, 0.5)
+    at = torch.arange(B, device="cuda") * n + n // 2
+    v[at, :, 7] = math.inf
+    from torchplusplus_b200 import ops
+    got = ops.attention_packed(q, k, v, cu).view(B, n, 4, D)
+    assert (got[:, n // 2:, :, 7] == math.inf).all()
+    assert got[:, :n // 2, :, 7].isfinite().all()
+    assert got[..., :7].isfinite().all() and got[..., 8:].isfinite().all()
+
+
 def test_attention_non_finite_keys_stay_hidden():
     cu, N = packed([100, 200])
     q, k, v = operands(13, N, 2, 2, 128, BF16)

@@ -176,3 +176,10 @@ def test_sliding_window_module_packed():
             # both round the probabilities, the attention's and the projection's outputs to bf16
             assert (got[s:s + n] - want).abs().max() <= 2e-2 * max(1.0, want.abs().max().item())
             s += n
+
+
+def test_generate_refuses_prompts_of_no_tokens():
+    m = make()
+    for bad in ([], [torch.tensor([3, 4]), torch.tensor([], dtype=torch.int64)]):
+        with pytest.raises(ValueError):
+            m.generate(bad, max_new_token=4, sampling_strategy="greedy")

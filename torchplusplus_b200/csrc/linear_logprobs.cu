@@ -1,6 +1,16 @@
 // Log probabilities of given tokens (and each row's entropy) straight from the LM head's
 // operands: softmax statistics of x W^T in the product's epilogue, the logits never
 // written.
+//
+// Persistent CTAs over tiles of 128 tokens x BN vocabulary rows, tokens first (a tile row of W
+// stays in L2 meanwhile), the accumulators double-buffered in TMEM: a thread reads half a
+// token's logits of a tile and leaves (largest, sum of weights, sum of weights times
+// difference), 12 bytes for BN logits, which join_logprobs_kernel adds up.  Measured, bf16:
+// 4096 x 1024 x 151936 816-832 us in bursts, 1560 TFLOP/s (950 in long runs at the power
+// limit's clock); 4096 x 2048 x 32003 344 us, as fast; to 128 tokens 76 us, 4.1 TB/s of
+// weights: bound by the tensor core, and by HBM's latency at the start and end (some 12 us) and
+// its rate between.  Stages of 128 or 256 columns for few tokens, for longer requests: the
+// same 76 and 89 us.
 #include <math.h>
 #include "tc_issue.cuh"
 

@@ -35,7 +35,9 @@ struct PackedRopeArgs {
 // [8l, 8l+8) of both halves of each row, so rotate-half stays inside a lane and only
 // the sum of squares crosses lanes; the norm's weight is folded into the lane's cos and
 // sin once for all R rows.  fp32 throughout, one rounding at the store.  Bound by HBM
-// at many tokens (R rows' loads in flight a lane), by latency at few (R = 1).
+// at many tokens (R rows' loads in flight a lane), by latency at few (R = 1).  Measured, bf16,
+// D 128: 64 prompts to 1024, 32 + 2 x 8 heads into a paged cache 242 us, 5.04 TB/s, 77 % of a
+// copy's rate (R = 2: 258, 8: 295); one of 130, 16 + 2 x 8 heads: 4.3 us.
 template <typename T, typename CS, int G, int R>
 __global__ void __launch_bounds__(256) qk_norm_rope_packed_kernel(PackedRopeArgs p) {
   pdl_wait();

@@ -266,8 +266,8 @@ class DecodeEngine:
         (temperature 1, whatever the sampling): `scores` holds, for each place of out_ids, the
         token's log probability, the distribution's entropy and the token's rank, [B,
         max_seq_len], and the `top` most likely tokens' log probabilities and ids, [B,
-        max_seq_len, top] (ops.token_logprobs; zeros where nothing was chosen since the last
-        prefill).  None: no more.  The decode graph is re-recorded when the setting changes."""
+        max_seq_len, top] (ops.token_logprobs; zeros where the engine chose nothing since its
+        last prefill).  None: no more.  The decode graph is re-recorded when the setting changes."""
         if top is None:
             self.scoring = self.scores = None
             return

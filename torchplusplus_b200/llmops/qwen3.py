@@ -185,12 +185,14 @@ class Qwen3(LLMInference):
                        (sampling_strategy == "top_k" and top_k is None)):
             raise ValueError("prompts of different lengths generate greedily, by top_p or by "
                              "top_k, without a stream")
+        if packed and min(map(len, input_ids), default=0) < 1:
+            raise ValueError("prompts must have at least one token")
         if stream or sampling_strategy not in ("greedy", "top_p", "top_k") or \
                 (sampling_strategy == "top_k" and top_k is None):
             return super().generate(input_ids, max_new_token, temp, top_p, top_k,
                                     sampling_strategy, stop_token_ids, eos_token_id, stream,
                                     stream_callback)
-        B, S = (len(input_ids), max(map(len, input_ids), default=0)) if packed else input_ids.shape
+        B, S = (len(input_ids), max(map(len, input_ids))) if packed else input_ids.shape
         eng = self.engine(B, S + max_new_token)
         if sampling_strategy == "greedy":
             eng.set_greedy()
