@@ -9,8 +9,9 @@
 // 4096 x 1024 x 151936 816-832 us in bursts, 1560 TFLOP/s (950 in long runs at the power
 // limit's clock); 4096 x 2048 x 32003 344 us, as fast; to 128 tokens 76 us, 4.1 TB/s of
 // weights: bound by the tensor core, and by HBM's latency at the start and end (some 12 us) and
-// its rate between.  Stages of 128 or 256 columns for few tokens, for longer requests: the
-// same 76 and 89 us.
+// its rate between.  (Stages of 128 or 256 columns for few tokens, for longer requests, take
+// 76 and 89 us.)
+#include <float.h>
 #include <math.h>
 #include "tc_issue.cuh"
 
@@ -23,6 +24,17 @@ constexpr int kMaxBN = 256;    // vocabulary rows a tile at most (a multiple of 
 constexpr int kMaxStages = 8;
 constexpr int kThreads = 384;  // 4 control warps, 8 of the epilogue
 constexpr int kEpiWarp0 = 4;
+// Stages a chain of products sums in the tensor core; longer ones are parts that the epilogue
+// adds.  The tensor core's sums do not round to nearest, so a chain's logits are biased
+// the more the longer it is: of 2048 columns in one chain (32003 vocabulary rows, temperature
+// 0.8) the entropies were 2.8e-6 off, relative, in chains of 512 6e-7, 384 4e-7, 256 2.4e-7.  At
+// 4096 x 1024 x 151936 one chain takes 814 us, of 512 816, 384 838, 256 925.  A single chain's
+// logits go straight from TMEM to the weights (PARTS false), which is faster where the epilogue
+// counts: 2000 x 256 x 50000 68 us, 85 through registers.
+constexpr int kChain = 8;
+// registers of a control and an epilogue thread that holds its logits meanwhile: 168 at launch
+constexpr int kCtrlRegs = 72, kEpiRegs = 216;
+static_assert(128 * kCtrlRegs + 256 * kEpiRegs == kThreads * 168, "");
 constexpr size_t kRing = 216 * 1024;
 constexpr size_t kSmem = kRing + 2 * 3 * BM * 4 + 1024 + 256;
 static_assert(kSmem <= 227 * 1024, "shared memory plan exceeds 227 KB");
@@ -41,7 +53,7 @@ struct HeadArgs {
   int* err;
 };
 
-template <typename T>
+template <typename T, bool PARTS>
 __global__ void __launch_bounds__(kThreads, 1)
     linear_logprobs_kernel(const __grid_constant__ CUtensorMap tm_x,
                            const __grid_constant__ CUtensorMap tm_w, HeadArgs p) {
@@ -86,6 +98,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_trigger();
 
   bool ok = true;
+  if (warp < kEpiWarp0) {
+  if constexpr (PARTS)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCtrlRegs));
   if ((warp == 0 || warp == 2) && lane == 0) {
     // ---------------- TMA producers: x by one thread, W by another ----------------
     // (a thread takes some 0.2 us a request, and a stage's products 0.3)
@@ -121,29 +136,37 @@ __global__ void __launch_bounds__(kThreads, 1)
     int s = 0, j = 0;
     uint32_t turn = 0;
 #pragma unroll 1
-    for (int64_t t = blockIdx.x; t < ntiles; t += gridDim.x, ++j) {
-      const int buf = j & 1;
-      if (ok && j >= 2) ok = wait_short(&tempty[buf], ((j >> 1) & 1) ^ 1, p.err, 52);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      tc_fence_after();
-      const uint32_t acc = tm + (uint32_t)(buf * kMaxBN);
+    for (int64_t t = blockIdx.x; t < ntiles; t += gridDim.x) {
 #pragma unroll 1
-      for (int kb = 0; kb < nk; ++kb) {
-        if (ok) ok = wait_short(&full[s], turn, p.err, 53);
+      for (int kb = 0; kb < nk; ++j) {  // chain by chain
+        const int buf = j & 1, end = min(kb + kChain, nk);
+        if (ok && j >= 2) ok = wait_short(&tempty[buf], ((j >> 1) & 1) ^ 1, p.err, 52);
         tc_fence_after();
-        const uint32_t a0 = at + s * (stage >> 4), b0 = a0 + (a_bytes >> 4);
+        const uint32_t acc = tm + (uint32_t)(buf * kMaxBN);
+        bool more = false;
+#pragma unroll 1
+        for (; kb < end; ++kb) {
+          if (ok) ok = wait_short(&full[s], turn, p.err, 53);
+          tc_fence_after();
+          const uint32_t a0 = at + s * (stage >> 4), b0 = a0 + (a_bytes >> 4);
 #pragma unroll
-        for (int k = 0; k < BK / 16; ++k)
-          mma_ss(on, acc, a0 + (k * 32 >> 4), b0 + (k * 32 >> 4), idesc, (kb | k) != 0);
-        commit(on, &empty[s]);
-        if (++s == stages) {
-          s = 0;
-          turn ^= 1;
+          for (int k = 0; k < BK / 16; ++k)
+            mma_ss(on, acc, a0 + (k * 32 >> 4), b0 + (k * 32 >> 4), idesc, more || k != 0);
+          more = true;
+          commit(on, &empty[s]);
+          if (++s == stages) {
+            s = 0;
+            turn ^= 1;
+          }
         }
+        commit(on, &tfull[buf]);
       }
-      commit(on, &tfull[buf]);
+      if (!__all_sync(0xffffffffu, ok)) break;
     }
-  } else if (warp >= kEpiWarp0) {
+  }
+  } else {
+    if constexpr (PARTS)
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
     // ---------------- epilogue: one row and half the tile's columns a thread ----------------
     const int quarter = warp & 3, hf = (warp - kEpiWarp0) >> 2;
     const int rl = quarter * 32 + lane;
@@ -151,24 +174,31 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int half = hf ? BN - c_first : (BN / 16 + 1) / 2 * 16;
     const float c = p.c;
     const uint64_t c2 = f2_pack(c, c);
-    int j = 0;
-    for (int64_t t = blockIdx.x; t < ntiles; t += gridDim.x, ++j) {
+    int j = 0, tile = 0;
+    for (int64_t t = blockIdx.x; t < ntiles; t += gridDim.x, ++tile) {
       const int row = (int)(t % ntm) * BM + rl, vt = (int)(t / ntm);
-      const int n0 = vt * BN + c_first, buf = j & 1;
+      const int n0 = vt * BN + c_first;
       const int nv = max(0, min(half, p.V - n0));  // columns inside the vocabulary
       const int64_t at = row < p.N ? p.tokens[row] - n0 : -1;
       const int tl = at >= 0 && at < nv ? (int)at : -1;  // the token's column here
       const bool mine = __any_sync(0xffffffffu, tl >= 0);
-      // (after a wait that ran out the loop goes on, for the barrier below)
-      ok = ok && wait_short(&tfull[buf], (j >> 1) & 1, p.err, 54);
-      tc_fence_after();
-      const uint32_t trow =
-          tmem + (uint32_t)(buf * kMaxBN + c_first) + ((uint32_t)(quarter * 32) << 16);
       float ref = -INFINITY, S = 0.f, En = 0.f;
-      // C columns from c0 on; the next ones' transfer runs meanwhile
-      auto take = [&](const uint32_t* r, int c0, auto size) {
+      auto arrived = [&]() {
+        // (after a wait that ran out the loop goes on, for the barrier below)
+        ok = ok && wait_short(&tfull[j & 1], (j >> 1) & 1, p.err, 54);
+        __syncwarp();
+        tc_fence_after();
+        return tmem + (uint32_t)((j & 1) * kMaxBN + c_first) + ((uint32_t)(quarter * 32) << 16);
+      };
+      auto release = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tempty[j & 1]);
+        ++j;
+      };
+      // C columns from c0 on
+      auto take = [&](const float* x, int c0, auto size) {
         constexpr int C = decltype(size)::value;
-        const float* x = reinterpret_cast<const float*>(r);
         float mx[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
         for (int i = 4; i < C; i += 8)
@@ -206,55 +236,98 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       };
       constexpr std::integral_constant<int, 32> k32{};
-      int c0 = 0;
-      if (nv >= 32) {
-        uint32_t r[2][32];
-        tmem_ld32(trow, r[0]);
-        for (; c0 + 64 <= nv; c0 += 64) {
-          tmem_wait_ld();
-          tmem_ld32(trow + c0 + 32, r[1]);
-          take(r[0], c0, k32);
-          tmem_wait_ld();
-          if (c0 + 96 <= nv) tmem_ld32(trow + c0 + 64, r[0]);
-          take(r[1], c0 + 32, k32);
-        }
-        if (c0 + 32 <= nv) {
-          tmem_wait_ld();
-          take(r[0], c0, k32);
-          c0 += 32;
-        }
-      }
-      if (c0 + 16 <= nv) {
-        uint32_t r[16];
-        tmem_ld16(trow + c0, r);
-        tmem_wait_ld();
-        take(r, c0, std::integral_constant<int, 16>{});
-        c0 += 16;
-      }
+      constexpr std::integral_constant<int, 16> k16{};
+      if constexpr (PARTS) {
+        // the logits stay in registers: the parts, added in 32 bits
+        float x[kMaxBN / 2];
 #pragma unroll 1
-      for (; c0 < nv; ++c0) {  // the vocabulary's end
-        uint32_t r;
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(trow + c0));
-        tmem_wait_ld();
-        const float x = __uint_as_float(r);
-        if (c0 == 0) ref = x;
-        if ((x - ref) * c > 8.f) {
-          const float d = ref - x, f = exp2f(c * d);
-          En = f == 0.f ? 0.f : (En + S * d) * f;
-          S *= f;
-          ref = x;
+        for (int kb = 0; kb < nk; kb += kChain) {
+          const uint32_t from = arrived();
+          if (kb == 0) {
+#pragma unroll
+            for (int c0 = 0; c0 < kMaxBN / 2; c0 += 32)
+              if (c0 < half) tmem_ld32(from + c0, reinterpret_cast<uint32_t*>(x) + c0);
+            tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int c0 = 0; c0 < kMaxBN / 2; c0 += 32) {
+              if (c0 >= half) break;
+              uint32_t r[32];
+              tmem_ld32(from + c0, r);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; i += 2)
+                f2_unpack(f2_add(f2_pack(x[c0 + i], x[c0 + i + 1]),
+                                 f2_pack(__uint_as_float(r[i]), __uint_as_float(r[i + 1]))),
+                          x[c0 + i], x[c0 + i + 1]);
+            }
+          }
+          release();
         }
-        const float q = x - ref, w = ex2_ftz(q * c);
-        S += w;
-        En += w * q;
-        if (tl == c0) p.target[row] = x;
-        __syncwarp();
+#pragma unroll
+        for (int c0 = 0; c0 < kMaxBN / 2; c0 += 32) {
+          if (c0 + 32 <= nv) {
+            take(x + c0, c0, k32);
+          } else if (c0 < nv) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)  // (weight 0, and finite against any reference)
+              if (c0 + i >= nv) x[c0 + i] = -FLT_MAX;
+            take(x + c0, c0, k16);
+            if (c0 + 16 < nv) take(x + c0 + 16, c0 + 16, k16);
+          }
+        }
+      } else {
+        const uint32_t trow = arrived();
+        // a block's transfer runs beside the one before's weights
+        auto as_f = [](const uint32_t* r) { return reinterpret_cast<const float*>(r); };
+        int c0 = 0;
+        if (nv >= 32) {
+          uint32_t r[2][32];
+          tmem_ld32(trow, r[0]);
+          for (; c0 + 64 <= nv; c0 += 64) {
+            tmem_wait_ld();
+            tmem_ld32(trow + c0 + 32, r[1]);
+            take(as_f(r[0]), c0, k32);
+            tmem_wait_ld();
+            if (c0 + 96 <= nv) tmem_ld32(trow + c0 + 64, r[0]);
+            take(as_f(r[1]), c0 + 32, k32);
+          }
+          if (c0 + 32 <= nv) {
+            tmem_wait_ld();
+            take(as_f(r[0]), c0, k32);
+            c0 += 32;
+          }
+        }
+        if (c0 + 16 <= nv) {
+          uint32_t r[16];
+          tmem_ld16(trow + c0, r);
+          tmem_wait_ld();
+          take(as_f(r), c0, k16);
+          c0 += 16;
+        }
+#pragma unroll 1
+        for (; c0 < nv; ++c0) {  // the vocabulary's end
+          uint32_t r;
+          asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(trow + c0));
+          tmem_wait_ld();
+          const float x = __uint_as_float(r);
+          if (c0 == 0) ref = x;
+          if ((x - ref) * c > 8.f) {
+            const float d = ref - x, f = exp2f(c * d);
+            En = f == 0.f ? 0.f : (En + S * d) * f;
+            S *= f;
+            ref = x;
+          }
+          const float q = x - ref, w = ex2_ftz(q * c);
+          S += w;
+          En += w * q;
+          if (tl == c0) p.target[row] = x;
+          __syncwarp();
+        }
+        release();
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&tempty[buf]);
       // the row's two halves, joined by the first
-      float* h1 = half1 + buf * 3 * BM;
+      float* h1 = half1 + (tile & 1) * 3 * BM;
       if (hf == 1) {
         h1[rl] = ref;
         h1[BM + rl] = S;
@@ -391,9 +464,10 @@ extern "C" int tpp_linear_logprobs(const void* x, int64_t ldx, const void* w, in
     int rc = map(&tx, x, N, ldx, a.a_rows);
     if (rc == TPP_OK) rc = map(&tw, w, V, ldw, a.BN);
     if (rc != TPP_OK) return rc;
-    auto kern = linear_logprobs_kernel<T>;
-    static std::atomic<bool> reserved[64];
-    rc = reserve_smem(reinterpret_cast<const void*>(kern), reserved, kSmem,
+    const bool parts = E > kChain * BK;
+    auto kern = parts ? linear_logprobs_kernel<T, true> : linear_logprobs_kernel<T, false>;
+    static std::atomic<bool> reserved[2][64];
+    rc = reserve_smem(reinterpret_cast<const void*>(kern), reserved[parts], kSmem,
                       "linear_logprobs_kernel");
     if (rc != TPP_OK) return rc;
     const int64_t tiles = (a.rows / BM) * nt;
