@@ -356,17 +356,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 1) tmem_dealloc(tmem, 512);
 }
 
-// Joins the vocabulary's tiles: 32 rows a block, a tile a warp at a time.
-constexpr int kJoinWarps = 16;
+// Joins the vocabulary's tiles: 32 rows a block, a tile a warp at a time, kJoinAhead tiles'
+// loads in flight (for a few tokens there is one block, and latency is all it costs).
+constexpr int kJoinWarps = 32, kJoinAhead = 8;  // (32: a warp a row in the end)
 __global__ void __launch_bounds__(32 * kJoinWarps)
     join_logprobs_kernel(const float* part, const float* target, const int64_t* tokens,
                          int64_t rows, int nt, int N, int V, float c, float* logprobs,
                          float* entropy) {
   pdl_wait();
   pdl_trigger();
-  __shared__ float sm[3][kJoinWarps][32];
+  __shared__ float sm[3][kJoinWarps][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int row = blockIdx.x * 32 + lane;
+  int row = blockIdx.x * 32 + lane;
   float M = -INFINITY, S = 0.f, E = 0.f;
   auto add = [&](float m, float s, float e) {
     const float big = fmaxf(M, m);
@@ -377,16 +378,36 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
     S = S * fa + s * fb;
     M = big;
   };
-  for (int t = warp; t < nt; t += kJoinWarps) {
-    const float* at = part + (int64_t)t * 3 * rows + row;
-    add(at[0], at[rows], at[2 * rows]);
+  for (int t0 = warp; t0 < nt; t0 += kJoinWarps * kJoinAhead) {
+    float m[kJoinAhead], s[kJoinAhead], e[kJoinAhead];
+#pragma unroll
+    for (int u = 0; u < kJoinAhead; ++u) {
+      const int t = t0 + u * kJoinWarps;
+      const float* at = part + (int64_t)min(t, nt - 1) * 3 * rows + row;
+      m[u] = at[0];
+      s[u] = t < nt ? at[rows] : 0.f;
+      e[u] = t < nt ? at[2 * rows] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < kJoinAhead; ++u) add(m[u], s[u], e[u]);
   }
   sm[0][warp][lane] = M;
   sm[1][warp][lane] = S;
   sm[2][warp][lane] = E;
   __syncthreads();
-  if (warp != 0 || row >= N) return;
-  for (int w = 1; w < kJoinWarps; ++w) add(sm[0][w][lane], sm[1][w][lane], sm[2][w][lane]);
+  // a row a warp, a part a lane
+  row = blockIdx.x * 32 + warp;
+  if (row >= N) return;
+  M = sm[0][lane][warp];
+  S = sm[1][lane][warp];
+  E = sm[2][lane][warp];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float m = __shfl_down_sync(0xffffffffu, M, o), t = __shfl_down_sync(0xffffffffu, S, o),
+                e = __shfl_down_sync(0xffffffffu, E, o);
+    add(m, t, e);
+  }
+  if (lane != 0) return;
   constexpr float kLn2 = 0.69314718055994531f;
   const float lz = log2f(S);
   const int64_t tok = tokens[row];
