@@ -30,20 +30,22 @@ struct PackedRopeArgs {
   int Hq, Hkv;
 };
 
+constexpr int kBlock = 128;  // (blocks are short: 96 threads 216 us where 128 take 211, 256: 238, 512: 252)
+
 // y = rope(x * rsqrt(mean(x^2) + eps) * w): a unit is R head rows of one kind (q, k
 // or, with a cache, v) of one token.  G = D/16 lanes own it, lane l elements
 // [8l, 8l+8) of both halves of each row, so rotate-half stays inside a lane and only
 // the sum of squares crosses lanes; the norm's weight is folded into the lane's cos and
 // sin once for all R rows.  fp32 throughout, one rounding at the store.  Bound by HBM
 // at many tokens (R rows' loads in flight a lane), by latency at few (R = 1).  Measured, bf16,
-// D 128: 64 prompts to 1024, 32 + 2 x 8 heads into a paged cache 242 us, 5.04 TB/s, 77 % of a
-// copy's rate (R = 2: 258, 8: 295); one of 130, 16 + 2 x 8 heads: 4.3 us.
+// D 128: 64 prompts to 1024, 32 + 2 x 8 heads into a paged cache 211 us, 5.8 TB/s, 88 % of a
+// copy's rate (R = 2: 236, 8: 224); one of 130, 16 + 2 x 8 heads: 4.3 us.
 template <typename T, typename CS, int G, int R>
-__global__ void __launch_bounds__(256) qk_norm_rope_packed_kernel(PackedRopeArgs p) {
+__global__ void __launch_bounds__(kBlock) qk_norm_rope_packed_kernel(PackedRopeArgs p) {
   pdl_wait();
   pdl_trigger();
   constexpr int D = G * 16;
-  const uint32_t unit = blockIdx.x * (256 / G) + threadIdx.x / G;
+  const uint32_t unit = blockIdx.x * (kBlock / G) + threadIdx.x / G;
   const int lane = threadIdx.x % G;
   const bool valid = unit < p.units;  // (lanes past the end take part in the shuffles)
   const int gq = (p.Hq + R - 1) / R, gk = (p.Hkv + R - 1) / R;
@@ -172,7 +174,7 @@ int packed_rope_launch(PackedRopeArgs a, int64_t N, int64_t D, cudaStream_t st) 
     return launch("qk_norm_rope_packed_kernel",
                   four ? qk_norm_rope_packed_kernel<T, CS, G, 4>
                        : qk_norm_rope_packed_kernel<T, CS, G, 1>,
-                  dim3((unsigned)((units + 256 / G - 1) / (256 / G))), dim3(256), 0, st, 0u, a);
+                  dim3((unsigned)((units + kBlock / G - 1) / (kBlock / G))), dim3(kBlock), 0, st, 0u, a);
   };
   switch (D) {
     case 16: return go(std::integral_constant<int, 1>{});
