@@ -600,6 +600,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // the visible keys lo .. hi of these 16 as bits
             const int h = min(max(hi - k0 + 1, 0), 16), b = min(max(lo - k0, 0), 16);
             const uint32_t see = ((1u << h) - 1) & ~((1u << b) - 1);
+            if (__all_sync(0xffffffffu, see == 0xffffu)) continue;
 #pragma unroll
             for (int k = 0; k < 16; ++k)
               if (!(see & 1u << k)) sv[k0 + k] = -INFINITY;
