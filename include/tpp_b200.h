@@ -553,7 +553,8 @@ int tpp_token_logprobs(const void* logits, int64_t ld, int64_t N, int64_t V,
 
 /* The log probabilities and entropies of tpp_token_logprobs for the logits
  * x [N, E] . w [V, E]^T, summed in 32 bits and never written (row strides ldx, ldw; f16
- * or bf16; E a multiple of 8, rows 16-byte aligned).  An infinite or NaN logit makes its row NaN.
+ * or bf16; E a multiple of 8, rows 16-byte aligned).  A NaN or +inf logit makes its row
+ * NaN, one of -inf may.
  * workspace: tpp_linear_logprobs_workspace bytes, 4-byte aligned. */
 int tpp_linear_logprobs(const void* x, int64_t ldx, const void* w, int64_t ldw,
                         const int64_t* tokens, int64_t N, int64_t V, int64_t E,
