@@ -167,19 +167,25 @@ def exported_symbols() -> list[str]:
     return list(SIGNATURES)
 
 
+def _failed(name: str, st: int) -> None:
+    raise TppError(name, st, lib().tpp_last_error().decode(errors="replace"))
+
+
 def call(name: str, *args) -> None:
     """Calls a status-returning entry point and raises TppError on failure."""
     st = getattr(lib(), name)(*args)
     if st != TPP_OK:
-        msg = lib().tpp_last_error().decode(errors="replace")
-        raise TppError(name, st, msg)
+        _failed(name, st)
 
 
 def call_on(t: torch.Tensor, name: str, *args) -> None:
     """call(), with t's device as the current one."""
     dev = t.get_device()
     if dev == torch._C._cuda_getDevice():
-        call(name, *args)
+        # (call() itself would pass the arguments on once more)
+        st = getattr(_lib or lib(), name)(*args)
+        if st != TPP_OK:
+            _failed(name, st)
     else:
         with torch.cuda.device(dev):
             call(name, *args)

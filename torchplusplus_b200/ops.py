@@ -1017,7 +1017,7 @@ def qk_norm_rope_packed(qkv: torch.Tensor, q_norm_w: torch.Tensor | None,
         cs, shape = k_cache.stride(), k_cache.shape
         if len(shape) != 4 or shape[0] != B or shape[1] != Hkv or shape[3] != D \
                 or v_cache.shape != shape or v_cache.stride() != cs or cs[3] != 1 \
-                or any(s == 0 and n > 1 for s, n in zip(cs, shape)):
+                or 0 in cs and any(s == 0 and n > 1 for s, n in zip(cs, shape)):
             raise ValueError("caches must be [B, Hkv, Smax, D] with identical layouts, no two "
                              "rows in one place")
         rows = shape[2]
@@ -1057,7 +1057,7 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     B = _cu_seqlens(cu_seqlens)
     q, k, v = _rows16(q), _rows16(k), _rows16(v)
     if out is None:
-        out = q.new_empty((N_, Hq, D))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != (N_, Hq, D) or out.stride(2) != 1 \
             or any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
         raise ValueError("out must be [N, Hq, D] with a contiguous last dim, no two rows in one "
