@@ -6,11 +6,11 @@
 // stays in L2 meanwhile), the accumulators double-buffered in TMEM: a thread reads half a
 // token's logits of a tile and leaves (largest, sum of weights, sum of weights times
 // difference), 12 bytes for BN logits, which join_logprobs_kernel adds up.  Measured, bf16:
-// 4096 x 1024 x 151936 816-832 us in bursts, 1560 TFLOP/s (950 in long runs at the power
-// limit's clock); 4096 x 2048 x 32003 344 us, as fast; to 128 tokens 76 us, 4.1 TB/s of
-// weights: bound by the tensor core, and by HBM's latency at the start and end (some 12 us) and
-// its rate between.  (Stages of 128 or 256 columns for few tokens, for longer requests, take
-// 76 and 89 us.)
+// 4096 x 1024 x 151936 800-825 us in bursts, 1546-1590 TFLOP/s (950 in long runs at the power
+// limit's clock); 4096 x 2048 x 32003 338-349, as fast; to 128 tokens 62-64, 5.0 TB/s of
+// weights.  Bound by the tensor core (95 % of its cycles); for few tokens by HBM (5.5 TB/s in
+// mid-course) and some 7 us of start and join.  (Stages of 128 or 256 columns for few
+// tokens, for longer requests, gave nothing: the same time, and 12 us more.)
 #include <float.h>
 #include <math.h>
 #include "tc_issue.cuh"
@@ -388,8 +388,20 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
       s[u] = t < nt ? at[rows] : 0.f;
       e[u] = t < nt ? at[2 * rows] : 0.f;
     }
+    // (one exponential a tile, where add() takes two)
+    float big = M;
 #pragma unroll
-    for (int u = 0; u < kJoinAhead; ++u) add(m[u], s[u], e[u]);
+    for (int u = 0; u < kJoinAhead; ++u) big = fmaxf(big, m[u]);
+    const float d0 = S == 0.f ? 0.f : M - big, f0 = ex2_ftz(c * d0);
+    E = f0 == 0.f ? 0.f : (E + S * d0) * f0;
+    S *= f0;
+    M = big;
+#pragma unroll
+    for (int u = 0; u < kJoinAhead; ++u) {
+      const float d = s[u] == 0.f ? 0.f : m[u] - big, f = ex2_ftz(c * d);
+      E += f == 0.f ? 0.f : (e[u] + s[u] * d) * f;
+      S += s[u] * f;
+    }
   }
   sm[0][warp][lane] = M;
   sm[1][warp][lane] = S;

@@ -154,9 +154,10 @@ template <> struct Lane<float> {
 // raises the bound: some `top` new ones come in between.  More than kCap, or kHits chunks of a thread (long runs of
 // equal logits, ascending rows), or a NaN, and the slice is searched `top` times over instead.
 //
-// Measured, bf16: 4096 x 151936 LPTOP0 us without alternatives (5.6 TB/s), LPTOP20 with 20;
-// 4096 x 32003 with 20: 100; a single row of 151936 over 8 CTAs with 5: 14.5.  Bound by HBM without
-// alternatives, by issue slots with them (the candidates' handling), a single row by latency.
+// Measured, bf16: 4096 x 151936 224 us without alternatives (5.55 TB/s, 85 % of a copy's rate), 288
+// with 20; 4096 x 32003 62 and 100; a single row of 151936 over 8 CTAs 10.6, with 5 14.6.
+// Bound by HBM without alternatives (issue slots 69 % busy), by issue slots and barriers with
+// them, a single row by latency.  Narrowing after chunks 1, 3, 9 .. takes as long, 1, 8, 64: 313.
 template <typename T, bool TOP, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT)
     token_logprobs_kernel(LogprobArgs p) {

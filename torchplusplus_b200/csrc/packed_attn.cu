@@ -23,12 +23,15 @@
 // rows that see them at the end.
 //
 // Measured (bf16, heads over kv heads, D 128 unless said otherwise): one prompt of 32768,
-// 16/8: 3.2 ms, 1360 TFLOP/s of the visible pairs' products (3.7 in long runs at the power
-// limit's clock); 6 to 8191, 32/8: 1.69 ms; 32 to 512, 16/8: 51 us (their bytes: 22); one of
-// 130: 11 us; 64-dim heads, one of 16384, 16/8: 0.77 ms.  What bounds it: in long prompts the
-// chain S -> softmax -> P V of each query tile (a step of both, 80 keys, takes some 1900
-// clocks, its products 1280), in short ones an item's start, its masked steps (V tiles looked
-// at by one warp) and its output.
+// 16/8: 3.2-3.4 ms, 1300-1360 TFLOP/s of the visible pairs' products (3.8 in long runs at the
+// power limit's clock); 6 to 8191, 32/8: 1.69 ms; 32 to 512, 16/8: 52 us (their bytes: 22); one
+// of 130: 11 us; 64-dim heads, one of 16384, 16/8: 0.77-0.9 ms by clock.  In long prompts a step
+// of both tiles (80 keys) takes some 2250 clocks, its products 1280: the tiles' softmaxes run
+// side by side, and their exponentials (1450 for both; the units' own rate gives 1280) are
+// followed by 800 to 950 of barriers, transfers and maxima.  Taking turns, so that one tile's
+// fill the other's gaps, is slower (2430 to 2560: a warp alone takes 11 clocks an
+// exponential, two together 9 each).  In short prompts an item's start, its masked steps (3300
+// clocks) and its output count.
 #include <math.h>
 #include "tc_issue.cuh"
 #include "mma_common.cuh"
