@@ -438,3 +438,33 @@ def test_refusals():
         with pytest.raises(err):
             call()
     assert ops.device_error() == 0
+
+
+def test_all_operators_on_two_streams_at_once():
+    """Calls that overlap on the device give what they give one after another."""
+    from torchplusplus_b200 import ops
+    cu, N = packed([700, 3, 1500, 64])
+    q, k, v = operands(31, N, 16, 8, 128, BF16)
+    g = gen(32)
+    qkv, w = randn(g, N, 32 * 128, dtype=BF16), randn(g, 128, dtype=BF16)
+    cos, sin = randn(g, 1500, 128), randn(g, 1500, 128)
+    x, head = randn(g, 300, 1024, dtype=BF16), randn(g, 30001, 1024, dtype=BF16) / 32
+    tok = torch.randint(0, 30001, (300,), generator=g, device="cuda")
+    logits = randn(g, 300, 30001, dtype=BF16)
+    calls = [lambda: (ops.attention_packed(q, k, v, cu),),
+             lambda: ops.qk_norm_rope_packed(qkv, w, w, 1e-6, cos, sin, cu, 16, 8),
+             lambda: ops.linear_logprobs(x, head, tok),
+             lambda: ops.token_logprobs(logits, tok, top=20)]
+    want = [c() for c in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for turn in range(12):
+        for at, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                n = (turn + at * (1 + turn // 4)) % 4
+                got.append((n, calls[n]()))
+    torch.cuda.synchronize()
+    for n, out in got:
+        assert all(torch.equal(a, b) for a, b in zip(out, want[n])), n
+    assert ops.device_error() == 0
