@@ -964,7 +964,9 @@ def attention_tree_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
 
 # ---------------------------------------------------------------- packed prompts
 def _one_device(t: torch.Tensor, *ts: torch.Tensor | None) -> None:
-    dev = t.get_device()  # (-1 on the CPU)
+    dev = t.get_device()
+    if dev < 0:  # (the CPU)
+        _cuda(t)
     for o in ts:
         if o is not None and o.get_device() != dev:
             _cuda(t, o)
