@@ -1,0 +1,65 @@
+"""Packed-prompt operators at the edges of what their documentation allows, against their
+definitions in 64 bits."""
+import pytest
+import torch
+
+from .test_packed_gpu import BF16, F16, F32, gen, packed, randn, rope_oracle
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ norm, positions, cache
+def check_rope(lens, head, tail, Hq, Hkv, D, dtype, cache, norm):
+    from torchplusplus_b200 import ops
+    cu, N = packed(lens, head, tail)
+    g = gen(40)
+    qkv = randn(g, N, (Hq + 2 * Hkv) * D, dtype=dtype)
+    qn = (1 + 0.2 * randn(g, D)).to(dtype) if "q" in norm else None
+    kn = (1 + 0.2 * randn(g, D)).to(dtype) if "k" in norm else None
+    ang = torch.rand(max(lens), D, generator=g, device="cuda") * 6
+    cos, sin = ang.cos().half(), ang.sin().half()
+    B, cols = len(lens), -(-max(lens) // 64)
+    kc = vc = table = want = None
+    if cache == "rows":
+        kc, vc = (randn(g, B, Hkv, max(lens), D, dtype=dtype) for _ in range(2))
+    elif cache == "paged":
+        kc, vc = (randn(g, B * cols, Hkv, 64, D, dtype=dtype) for _ in range(2))
+        table = torch.randperm(B * cols, generator=g, device="cuda").view(B, cols).to(torch.int32)
+    if kc is not None:
+        want = kc.clone(), vc.clone()
+    q = torch.full((N, Hq, D), 9.0, dtype=dtype, device="cuda")
+    k = torch.full((N, Hkv, D), 9.0, dtype=dtype, device="cuda")
+    ops.qk_norm_rope_packed(qkv, qn, kn, 1e-6, cos, sin, cu, Hq, Hkv, k_cache=kc, v_cache=vc,
+                            block_table=table, q_out=q, k_out=k)
+    (qr, qt, kr, kt), seq, pos = rope_oracle(qkv, qn, kn, 1e-6, cos, sin, cu, Hq, Hkv)
+    has = seq >= 0
+    assert ((q.double() - qr).abs() <= qt)[has].all() and ((k.double() - kr).abs() <= kt)[has].all()
+    assert (q[~has] == 9).all() and (k[~has] == 9).all()
+    if kc is not None:
+        v = qkv[:, (Hq + Hkv) * D:].view(N, Hkv, D)
+        b, at = seq[has], pos[has]
+        if table is not None:
+            b, at = table.long()[b, at // 64], at % 64
+        want[0][b, :, at], want[1][b, :, at] = k[has], v[has]
+        assert torch.equal(kc, want[0]) and torch.equal(vc, want[1])
+
+
+@pytest.mark.parametrize("norm", ["q", "k", "qk", ""])
+@pytest.mark.parametrize("cache", ["none", "rows", "paged"])
+@pytest.mark.parametrize("Hq,Hkv,D,dtype", [(4, 2, 128, BF16), (3, 1, 64, F16), (5, 3, 32, BF16),
+                                            (2, 2, 256, F16), (3, 2, 16, BF16)])
+def test_rope_of_either_norm(norm, cache, Hq, Hkv, D, dtype):
+    check_rope([5, 0, 64, 66], 3, 4, Hq, Hkv, D, dtype, cache, norm)
+
+
+# From N (Hq + Hkv, 2 Hkv with a cache) D / 16 = 4 * 2048 * 148 on a unit of lanes takes four
+# heads; these group sizes leave it one, two, three or all four of its last ones.
+@pytest.mark.parametrize("norm", ["q", "k", "qk", ""])
+@pytest.mark.parametrize("cache", ["none", "rows", "paged"])
+@pytest.mark.parametrize("Hq,Hkv,D,dtype", [(7, 3, 128, BF16), (8, 2, 128, F16), (5, 1, 256, BF16),
+                                            (14, 4, 64, F16)])
+def test_rope_of_many_rows(norm, cache, Hq, Hkv, D, dtype):
+    rows = -(-4 * 2048 * 160 * 16 // ((Hq + Hkv * (1 if cache == "none" else 2)) * D))
+    lens = [rows // 2, 1, rows // 3, 0, 130]
+    lens.append(rows - sum(lens) + 37)
+    check_rope(lens, 2, 3, Hq, Hkv, D, dtype, cache, norm)

@@ -108,6 +108,9 @@ __global__ void __launch_bounds__(kBlock) qk_norm_rope_packed_kernel(PackedRopeA
     table8<CS>(cs + D / 2, c);
     table8<CS>(sn + D / 2, d);
   }
+  // (a warp's units are of several kinds and only one may have a norm: every lane takes part
+  // in the sums' shuffles, whatever its own)
+  const bool norms = p.qn != nullptr || p.kn != nullptr;
   const T* nw = static_cast<const T*>(kind == 0 ? p.qn : p.kn);
   if (nw != nullptr) {
     float g1[8], g2[8];
@@ -128,7 +131,7 @@ __global__ void __launch_bounds__(kBlock) qk_norm_rope_packed_kernel(PackedRopeA
     unpack8<T>(lo[i], x);
     unpack8<T>(hi[i], y);
     float inv = 1.f;
-    if (nw != nullptr) {
+    if (norms) {
       float s0 = 0.f, s1 = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -138,7 +141,7 @@ __global__ void __launch_bounds__(kBlock) qk_norm_rope_packed_kernel(PackedRopeA
       s0 += s1;
 #pragma unroll
       for (int o = G / 2; o > 0; o >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
-      inv = known ? rsqrtf(s0 / (float)D + p.eps) : 0.f;  // (eps may be 0)
+      if (nw != nullptr) inv = known ? rsqrtf(s0 / (float)D + p.eps) : 0.f;  // (eps may be 0)
     }
     float u[8], v[8];
 #pragma unroll
