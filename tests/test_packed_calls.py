@@ -37,3 +37,39 @@ def test_cpu_tensors_never_reach_the_library(calls, name):
     with pytest.raises(RuntimeError, match="need CUDA tensors"):
         cpu_calls()[name]()
     assert calls == []
+
+
+class OnGpu(torch.Tensor):
+    """A host tensor that says it is on GPU 0 (whatever is made from it too)."""
+    is_cuda = property(lambda self: True)
+
+    def get_device(self):
+        return 0
+
+
+def on_gpu(t):
+    return t.as_subclass(OnGpu)
+
+
+def within(t, address, stride, N, E):
+    """Whether rows of E elements lie inside t's memory."""
+    lo = t.untyped_storage().data_ptr()
+    end = address + ((N - 1) * stride + E) * t.element_size()
+    return lo <= address and end <= lo + t.untyped_storage().nbytes()
+
+
+@pytest.mark.parametrize("step", [8, 24, 56])
+@pytest.mark.parametrize("which", ["x", "weight"])
+def test_linear_logprobs_of_rows_that_overlap(calls, which, step):
+    """Rows that share memory (a row stride below their length) are copied apart."""
+    N_, V, E = 5, 7, 64
+    rows = dict(x=N_, weight=V)
+    got = dict(x=on_gpu(torch.zeros(N_, E, dtype=BF16)), weight=on_gpu(torch.zeros(V, E, dtype=BF16)))
+    room = on_gpu(torch.zeros((rows[which] - 1) * step + E, dtype=BF16))
+    got[which] = room.as_strided((rows[which], E), (step, 1))
+    ops.linear_logprobs(got["x"], got["weight"], on_gpu(torch.zeros(N_, dtype=torch.int64)))
+    (_, args), = calls
+    address, stride = args[0 if which == "x" else 2], args[1 if which == "x" else 3]
+    assert stride >= E
+    # (a copy's memory has been freed by now; the operand's own must not be read that far)
+    assert address != room.data_ptr() or within(room, address, stride, rows[which], E)

@@ -63,3 +63,22 @@ def test_rope_of_many_rows(norm, cache, Hq, Hkv, D, dtype):
     lens = [rows // 2, 1, rows // 3, 0, 130]
     lens.append(rows - sum(lens) + 37)
     check_rope(lens, 2, 3, Hq, Hkv, D, dtype, cache, norm)
+
+
+# ------------------------------------------------------------------ scores
+@pytest.mark.parametrize("step", [8, 24, 56])
+@pytest.mark.parametrize("which", ["x", "weight"])
+def test_head_of_rows_that_overlap(which, step):
+    """A row stride below the rows' length (a view of a signal's windows)."""
+    from torchplusplus_b200 import ops
+    g = gen(41)
+    N, V, E = 33, 150, 64
+    rows = dict(x=N, weight=V)
+    got = dict(x=randn(g, N, E, dtype=BF16), weight=randn(g, V, E, dtype=BF16))
+    room = randn(g, (rows[which] - 1) * step + E, dtype=BF16)
+    got[which] = room.as_strided((rows[which], E), (step, 1))
+    tok = torch.randint(0, V, (N,), generator=g, device="cuda")
+    out = ops.linear_logprobs(got["x"], got["weight"], tok)
+    got[which] = got[which].contiguous()
+    want = ops.linear_logprobs(got["x"], got["weight"], tok)
+    assert all(torch.equal(a, b) for a, b in zip(out, want))

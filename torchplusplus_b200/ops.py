@@ -1112,6 +1112,12 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, temperature: floa
     return lp, ent, rank, tlp, tid
 
 
+def _matrix(t: torch.Tensor) -> torch.Tensor:
+    """_rows16 of [rows, E], whose rows lie at least E apart."""
+    t = _rows16(t)
+    return t.contiguous() if t.shape[0] > 1 and t.stride(0) < t.shape[1] else t
+
+
 def linear_logprobs(x: torch.Tensor, weight: torch.Tensor, tokens: torch.Tensor,
                     temperature: float = 1.0, workspace: torch.Tensor | None = None
                     ) -> tuple[torch.Tensor, torch.Tensor]:
@@ -1126,7 +1132,7 @@ def linear_logprobs(x: torch.Tensor, weight: torch.Tensor, tokens: torch.Tensor,
     if V == 0 or E == 0 or E % 8:
         raise ValueError("weight must have rows, and E must be a multiple of 8")
     tokens = _scored(tokens, N_, temperature, x, weight)
-    x, weight = _rows16(x), _rows16(weight)
+    x, weight = _matrix(x), _matrix(weight)
     lp, ent = x.new_empty(N_, dtype=torch.float32), x.new_empty(N_, dtype=torch.float32)
     nbytes = linear_logprobs_workspace_bytes(N_, V, E)
     if workspace is None:
