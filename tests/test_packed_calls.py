@@ -73,3 +73,27 @@ def test_linear_logprobs_of_rows_that_overlap(calls, which, step):
     assert stride >= E
     # (a copy's memory has been freed by now; the operand's own must not be read that far)
     assert address != room.data_ptr() or within(room, address, stride, rows[which], E)
+
+
+def pitched(rows, *shape, dtype=BF16):
+    """Rows of `shape` at a pitch that is no multiple of 16 bytes."""
+    n = torch.Size(shape).numel()
+    return on_gpu(torch.zeros(rows, n + 5, dtype=dtype))[:, :n].view(rows, *shape)
+
+
+def test_the_stride_of_a_single_row_does_not_matter(calls):
+    """A tensor of one row may lie in memory of any pitch: no stride that the library would
+    refuse (a multiple of 8 elements) gets there."""
+    cu = on_gpu(torch.tensor([0, 1], dtype=torch.int32))
+    one = on_gpu(torch.zeros(1, dtype=torch.int64))
+    ops.linear_logprobs(pitched(3, 64)[:1], pitched(3, 64)[:1], one)
+    ops.attention_packed(pitched(2, 4, 64)[:1], pitched(2, 2, 64)[:1], pitched(2, 2, 64)[:1], cu,
+                         out=pitched(2, 4, 64)[:1])
+    table = on_gpu(torch.ones(8, 64))
+    for kc, vc in ((None, None), (pitched(2, 2, 8, 64)[:1], pitched(2, 2, 8, 64)[:1])):
+        ops.qk_norm_rope_packed(pitched(2, 8 * 64)[:1], None, None, 1e-6, table, table, cu, 4, 2, kc, vc)
+    strides = {"tpp_linear_logprobs": [1, 3], "tpp_attention_packed": [1, 2, 4, 5, 7, 8, 12, 13],
+               "tpp_qk_norm_rope_packed": [1, 7, 16, 17, 18]}
+    assert len(calls) == 4
+    for name, args in calls:
+        assert not [args[i] for i in strides[name] if args[i] % 8], name

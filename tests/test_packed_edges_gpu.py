@@ -82,3 +82,33 @@ def test_head_of_rows_that_overlap(which, step):
     got[which] = got[which].contiguous()
     want = ops.linear_logprobs(got["x"], got["weight"], tok)
     assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+# ------------------------------------------------------------------ single rows at any pitch
+def pitched(g, rows, *shape, dtype=BF16):
+    """Rows of `shape` at a pitch that is no multiple of 16 bytes."""
+    n = torch.Size(shape).numel()
+    return randn(g, rows, n + 5, dtype=dtype)[:, :n].view(rows, *shape)
+
+
+def test_single_rows_at_any_pitch():
+    from torchplusplus_b200 import ops
+    g = gen(42)
+    cu = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    x, w = pitched(g, 3, 64)[:1], pitched(g, 3, 64)[:1]
+    tok = torch.zeros(1, dtype=torch.int64, device="cuda")
+    out = ops.linear_logprobs(x, w, tok)
+    assert out[0].item() == 0 and out[1].item() == 0  # one token: certain
+    q, k, v, o = (pitched(g, 2, h, 64)[:1] for h in (4, 2, 2, 4))
+    rest = o.untyped_storage()[-2 * (4 * 64 + 10):].tolist()
+    assert ops.attention_packed(q, k, v, cu, out=o) is o
+    assert torch.equal(o, v.repeat_interleave(2, 1)) and o.untyped_storage()[-2 * (4 * 64 + 10):].tolist() == rest
+    t = randn(g, 8, 64)
+    qkv = pitched(g, 2, 8 * 64)[:1]
+    kc, vc = pitched(g, 2, 2, 8, 64)[:1], pitched(g, 2, 2, 8, 64)[:1]
+    want = kc.clone(), vc.clone()
+    got = ops.qk_norm_rope_packed(qkv, None, None, 1e-6, t, t, cu, 4, 2, kc, vc)
+    ref = ops.qk_norm_rope_packed(qkv.clone(), None, None, 1e-6, t, t, cu, 4, 2, *want)
+    for a, b in ((got[0], ref[0]), (got[1], ref[1]), (kc, want[0]), (vc, want[1])):
+        assert torch.equal(a, b)
+    assert ops.device_error() == 0

@@ -707,12 +707,23 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
     """t itself if its last dim is contiguous, every row starts on 16 bytes and no
     rows share memory, a contiguous copy otherwise."""
     if not t.data_ptr() & 15:
-        if t.is_contiguous() and not t.shape[-1] & 7:
+        if t.is_contiguous() and not t.shape[-1] & 7 \
+                and (1 not in t.shape or not any(s & 7 for s in t.stride()[:-1])):
             return t
         *lead, last = t.stride()
         if last == 1 and not any(s & 7 or s == 0 for s in lead):
             return t
     return t.clone(memory_format=torch.contiguous_format)
+
+
+def _strides8(t: torch.Tensor) -> tuple:
+    """t's strides; those of dims of one entry, which no address takes, as a contiguous
+    tensor has them (they may be anything, and the kernels want multiples of 8)."""
+    st, shape = t.stride(), t.shape
+    if 1 not in shape:
+        return st
+    return tuple(math.prod(shape[i + 1:]) if n == 1 else s
+                 for i, (n, s) in enumerate(zip(shape, st)))
 
 
 def _i32(t: torch.Tensor, shape: tuple, what: str) -> None:
@@ -1022,7 +1033,7 @@ def qk_norm_rope_packed(qkv: torch.Tensor, q_norm_w: torch.Tensor | None,
                 or 0 in cs and any(s == 0 and n > 1 for s, n in zip(cs, shape)):
             raise ValueError("caches must be [B, Hkv, Smax, D] with identical layouts, no two "
                              "rows in one place")
-        rows = shape[2]
+        cs, rows = _strides8(k_cache), shape[2]
     qkv = _rows16(qkv)
     cs_dt, cs_stride = N.DTYPE_CODE.get(cos.dtype), D
     if cs_dt is None or cos.shape != sin.shape or cos.dtype is not sin.dtype or cos.dim() != 2 \
@@ -1064,7 +1075,7 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
             or any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
         raise ValueError("out must be [N, Hq, D] with a contiguous last dim, no two rows in one "
                          "place")
-    qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), out.stride()
+    qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), _strides8(out)
     N.call_on(q, "tpp_attention_packed", q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
               v.data_ptr(), vs[0], vs[1], cu_seqlens.data_ptr(), B, out.data_ptr(), os_[0],
               os_[1], N_, Hq, Hkv, D, bool(causal), window_left,
