@@ -555,7 +555,8 @@ int tpp_token_logprobs(const void* logits, int64_t ld, int64_t N, int64_t V,
  * x [N, E] . w [V, E]^T, summed in 32 bits and never written (row strides ldx, ldw; f16
  * or bf16; E a multiple of 8, rows 16-byte aligned).  A NaN or +inf logit makes its row
  * NaN, one of -inf may.
- * workspace: tpp_linear_logprobs_workspace bytes, 4-byte aligned. */
+ * workspace: tpp_linear_logprobs_workspace bytes (of the device that is current then, as it
+ * must be in the call), 4-byte aligned. */
 int tpp_linear_logprobs(const void* x, int64_t ldx, const void* w, int64_t ldw,
                         const int64_t* tokens, int64_t N, int64_t V, int64_t E,
                         double temperature, float* logprobs, float* entropy, void* workspace,

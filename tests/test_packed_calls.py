@@ -15,6 +15,7 @@ def calls(monkeypatch):
     made = []
     monkeypatch.setattr(N, "call_on", lambda t, name, *args: made.append((name, args)))
     monkeypatch.setattr(N, "stream_of", lambda t: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
     return made
 
 
@@ -97,3 +98,56 @@ def test_the_stride_of_a_single_row_does_not_matter(calls):
     assert len(calls) == 4
     for name, args in calls:
         assert not [args[i] for i in strides[name] if args[i] % 8], name
+
+
+class TwoGpus:
+    """A library for two devices whose workspaces differ in size."""
+    need = {0: 1024, 1: 4096}
+
+    def __init__(self):
+        self.current, self.called = 0, []
+
+    def tpp_linear_logprobs_workspace(self, N_, V, E):
+        return self.need[self.current]
+
+    def tpp_linear_logprobs(self, *args):
+        nbytes = args[12]
+        self.called.append((self.current, nbytes))
+        return 0 if nbytes >= self.need[self.current] else 7
+
+    def tpp_last_error(self):
+        return b"workspace missing or too small"
+
+
+@pytest.fixture
+def two_gpus(monkeypatch):
+    gpus = TwoGpus()
+
+    class device:
+        def __init__(self, dev):
+            self.dev = dev
+
+        def __enter__(self):
+            self.old, gpus.current = gpus.current, self.dev
+
+        def __exit__(self, *_):
+            gpus.current = self.old
+    monkeypatch.setattr(N, "_lib", gpus)
+    monkeypatch.setattr(N, "stream_of", lambda t: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: gpus.current, raising=False)
+    monkeypatch.setattr(torch.cuda, "device", device)
+    return gpus
+
+
+class OnGpu1(OnGpu):
+    def get_device(self):
+        return 1
+
+
+def test_linear_logprobs_workspace_is_of_the_operands_device(two_gpus):
+    """Its size goes by the SMs of the device that the call runs on, not of the current one."""
+    x, w = (torch.zeros(5, 64, dtype=BF16).as_subclass(OnGpu1) for _ in range(2))
+    ops.linear_logprobs(x, w, torch.zeros(5, dtype=torch.int64).as_subclass(OnGpu1))
+    assert two_gpus.called == [(1, 4096)] and two_gpus.current == 0
+    assert ops.linear_logprobs_workspace_bytes(5, 5, 64) == 1024
+    assert ops.linear_logprobs_workspace_bytes(5, 5, 64, torch.device("cuda", 1)) == 4096

@@ -178,6 +178,14 @@ def call(name: str, *args) -> None:
         _failed(name, st)
 
 
+def value_on(dev: int, name: str, *args):
+    """What an entry point returns, with device number dev as the current one."""
+    if dev == torch._C._cuda_getDevice():
+        return getattr(_lib or lib(), name)(*args)
+    with torch.cuda.device(dev):
+        return getattr(lib(), name)(*args)
+
+
 def call_on(t: torch.Tensor, name: str, *args) -> None:
     """call(), with t's device as the current one."""
     dev = t.get_device()

@@ -1145,7 +1145,7 @@ def linear_logprobs(x: torch.Tensor, weight: torch.Tensor, tokens: torch.Tensor,
     tokens = _scored(tokens, N_, temperature, x, weight)
     x, weight = _matrix(x), _matrix(weight)
     lp, ent = x.new_empty(N_, dtype=torch.float32), x.new_empty(N_, dtype=torch.float32)
-    nbytes = linear_logprobs_workspace_bytes(N_, V, E)
+    nbytes = N.value_on(x.get_device(), "tpp_linear_logprobs_workspace", N_, V, E)
     if workspace is None:
         workspace = lp.new_empty(nbytes // 4)
     else:
@@ -1159,8 +1159,13 @@ def linear_logprobs(x: torch.Tensor, weight: torch.Tensor, tokens: torch.Tensor,
     return lp, ent
 
 
-def linear_logprobs_workspace_bytes(N_: int, V: int, E: int) -> int:
-    return N.lib().tpp_linear_logprobs_workspace(N_, V, E)
+def linear_logprobs_workspace_bytes(N_: int, V: int, E: int,
+                                    device: torch.device | None = None) -> int:
+    """Bytes of linear_logprobs' workspace on `device` (None: the current one; the tiles go by
+    its number of SMs)."""
+    if device is None or device.index is None:
+        return N.lib().tpp_linear_logprobs_workspace(N_, V, E)
+    return N.value_on(device.index, "tpp_linear_logprobs_workspace", N_, V, E)
 
 
 def argmax(logits: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
