@@ -3,6 +3,7 @@ definitions in 64 bits."""
 import pytest
 import torch
 
+from .test_logprobs_gpu import check_head, operands as head_operands
 from .test_packed_gpu import BF16, F16, F32, gen, packed, randn, rope_oracle
 
 pytestmark = pytest.mark.gpu
@@ -112,3 +113,18 @@ def test_single_rows_at_any_pitch():
     for a, b in ((got[0], ref[0]), (got[1], ref[1]), (kc, want[0]), (vc, want[1])):
         assert torch.equal(a, b)
     assert ops.device_error() == 0
+
+
+# Vocabularies that end inside a block of 16 logits, products of one chain and of several.
+@pytest.mark.parametrize("E,V", [(64, 1003), (1024, 1003), (1024, 37), (520, 300)])
+@pytest.mark.parametrize("temperature", [1e-6, 1e30, 1e37, 1e38, 1e39, 1e300])
+def test_head_at_any_temperature(E, V, temperature):
+    check_head(*head_operands(43, 40, E, V, BF16), temperature)
+
+
+@pytest.mark.parametrize("E,V", [(64, 1003), (1024, 1003), (1024, 37), (520, 300)])
+@pytest.mark.parametrize("size", [2.0 ** 50, 2.0 ** 58, 2.0 ** 60])
+def test_head_of_large_logits(E, V, size):
+    """Logits of up to some 2^122, both signs: their differences stay finite."""
+    x, w, tok = head_operands(44, 40, E, V, BF16)
+    check_head(x * size, w * size, tok)

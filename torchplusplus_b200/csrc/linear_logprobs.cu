@@ -11,7 +11,6 @@
 // weights.  Bound by the tensor core (95 % of its cycles); for few tokens by HBM (5.5 TB/s in
 // mid-course) and some 7 us of start and join.  (Stages of 128 or 256 columns for few
 // tokens, for longer requests, gave nothing: the same time, and 12 us more.)
-#include <float.h>
 #include <math.h>
 #include "tc_issue.cuh"
 
@@ -196,8 +195,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&tempty[j & 1]);
         ++j;
       };
-      // C columns from c0 on
-      auto take = [&](const float* x, int c0, auto size) {
+      // C columns from c0 on, of which the first n weigh anything
+      auto take = [&](const float* x, int c0, auto size, int n) {
         constexpr int C = decltype(size)::value;
         float mx[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
@@ -220,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint64_t q2 = f2_add(f2_pack(x[i], x[i + 1]), r2);
           float d0, d1;
           f2_unpack(f2_mul(q2, c2), d0, d1);
-          const uint64_t w2 = f2_pack(ex2_ftz(d0), ex2_ftz(d1));
+          const uint64_t w2 = f2_pack(i < n ? ex2_ftz(d0) : 0.f, i + 1 < n ? ex2_ftz(d1) : 0.f);
           s2[(i >> 1) & 1] = f2_add(s2[(i >> 1) & 1], w2);
           e2[(i >> 1) & 1] = f2_fma(w2, q2, e2[(i >> 1) & 1]);
         }
@@ -267,13 +266,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int c0 = 0; c0 < kMaxBN / 2; c0 += 32) {
           if (c0 + 32 <= nv) {
-            take(x + c0, c0, k32);
+            take(x + c0, c0, k32, 32);
           } else if (c0 < nv) {
+            // (behind the vocabulary: a logit of the row again, so that nothing moves, without
+            // weight; a number of its own would weigh at high temperatures, or overflow)
 #pragma unroll
-            for (int i = 0; i < 32; ++i)  // (weight 0, and finite against any reference)
-              if (c0 + i >= nv) x[c0 + i] = -FLT_MAX;
-            take(x + c0, c0, k16);
-            if (c0 + 16 < nv) take(x + c0 + 16, c0 + 16, k16);
+            for (int i = 1; i < 32; ++i)
+              if (c0 + i >= nv) x[c0 + i] = x[c0];
+            take(x + c0, c0, k16, nv - c0);
+            if (c0 + 16 < nv) take(x + c0 + 16, c0 + 16, k16, nv - c0 - 16);
           }
         }
       } else {
@@ -287,14 +288,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (; c0 + 64 <= nv; c0 += 64) {
             tmem_wait_ld();
             tmem_ld32(trow + c0 + 32, r[1]);
-            take(as_f(r[0]), c0, k32);
+            take(as_f(r[0]), c0, k32, 32);
             tmem_wait_ld();
             if (c0 + 96 <= nv) tmem_ld32(trow + c0 + 64, r[0]);
-            take(as_f(r[1]), c0 + 32, k32);
+            take(as_f(r[1]), c0 + 32, k32, 32);
           }
           if (c0 + 32 <= nv) {
             tmem_wait_ld();
-            take(as_f(r[0]), c0, k32);
+            take(as_f(r[0]), c0, k32, 32);
             c0 += 32;
           }
         }
@@ -302,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t r[16];
           tmem_ld16(trow + c0, r);
           tmem_wait_ld();
-          take(as_f(r), c0, k16);
+          take(as_f(r), c0, k16, 16);
           c0 += 16;
         }
 #pragma unroll 1
