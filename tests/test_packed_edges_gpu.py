@@ -128,3 +128,20 @@ def test_head_of_large_logits(E, V, size):
     """Logits of up to some 2^122, both signs: their differences stay finite."""
     x, w, tok = head_operands(44, 40, E, V, BF16)
     check_head(x * size, w * size, tok)
+
+
+def test_head_of_log_probabilities_next_to_the_largest_number():
+    """A log probability of -3.2e38 is a float32, and 1.44 times it (in bits) is none."""
+    from torchplusplus_b200 import ops
+    x = torch.zeros(2, 8, dtype=BF16, device="cuda")
+    w = torch.zeros(40, 8, dtype=BF16, device="cuda")
+    x[:, 0] = 2.0 ** 63
+    w[3, 0], w[5, 0] = 2.0 ** 63 * 1.875, -(2.0 ** 63) * 1.875
+    tok = torch.tensor([5, 3], device="cuda")
+    lp, ent = ops.linear_logprobs(x, w, tok)
+    assert lp.tolist() == [-2.0 ** 127 * 1.875, 0.0] and ent.tolist() == [0.0, 0.0]
+    lp, ent = ops.linear_logprobs(x, w, tok, temperature=2.0)
+    assert lp.tolist() == [-2.0 ** 126 * 1.875, 0.0] and ent.tolist() == [0.0, 0.0]
+    # and as far off at a temperature below 1
+    lp, _ = ops.linear_logprobs(x / 2 ** 10, w, tok, temperature=2.0 ** -10)
+    assert lp.tolist() == [-2.0 ** 127 * 1.875, 0.0]

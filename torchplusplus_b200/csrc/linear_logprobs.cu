@@ -362,8 +362,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 constexpr int kJoinWarps = 32, kJoinAhead = 8;  // (32: a warp a row in the end)
 __global__ void __launch_bounds__(32 * kJoinWarps)
     join_logprobs_kernel(const float* part, const float* target, const int64_t* tokens,
-                         int64_t rows, int nt, int N, int V, float c, float* logprobs,
-                         float* entropy) {
+                         int64_t rows, int nt, int N, int V, float c, float inv_t,
+                         float* logprobs, float* entropy) {
   pdl_wait();
   pdl_trigger();
   __shared__ float sm[3][kJoinWarps][33];
@@ -424,7 +424,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
   constexpr float kLn2 = 0.69314718055994531f;
   const float lz = log2f(S);
   const int64_t tok = tokens[row];
-  logprobs[row] = tok >= 0 && tok < V ? ((target[row] - M) * c - lz) * kLn2 : 0.f;
+  // (not in bits, where the farthest logits' would overflow)
+  logprobs[row] = tok >= 0 && tok < V ? (target[row] - M) * inv_t - lz * kLn2 : 0.f;
   entropy[row] = (lz - E / S * c) * kLn2;
 }
 
@@ -511,7 +512,7 @@ extern "C" int tpp_linear_logprobs(const void* x, int64_t ldx, const void* w, in
     if (rc != TPP_OK) return rc;
     return launch("join_logprobs_kernel", join_logprobs_kernel, dim3((unsigned)((N + 31) / 32)),
                   dim3(32 * kJoinWarps), 0, as_stream(stream), 0u, (const float*)a.part,
-                  (const float*)a.target, tokens, a.rows, nt, (int)N, (int)V, a.c, logprobs,
-                  entropy);
+                  (const float*)a.target, tokens, a.rows, nt, (int)N, (int)V, a.c,
+                  (float)(1 / temperature), logprobs, entropy);
   });
 }
