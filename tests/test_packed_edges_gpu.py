@@ -1,10 +1,12 @@
 """Packed-prompt operators at the edges of what their documentation allows, against their
 definitions in 64 bits."""
+import math
+
 import pytest
 import torch
 
 from .test_logprobs_gpu import check_head, operands as head_operands
-from .test_packed_gpu import BF16, F16, F32, gen, packed, randn, rope_oracle
+from .test_packed_gpu import BF16, F16, F32, attention_oracle, gen, packed, randn, rope_oracle
 
 pytestmark = pytest.mark.gpu
 
@@ -145,3 +147,28 @@ def test_head_of_log_probabilities_next_to_the_largest_number():
     # and as far off at a temperature below 1
     lp, _ = ops.linear_logprobs(x / 2 ** 10, w, tok, temperature=2.0 ** -10)
     assert lp.tolist() == [-2.0 ** 127 * 1.875, 0.0]
+
+
+# ------------------------------------------------------------------ attention
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("bits", [20.0, 25.2, 28.0])
+def test_attention_f16_of_many_small_weights(D, bits, causal):
+    """A first key of weight 1 (and value 0) before thousands of 2^-bits (and value 1): what
+    each gives is below f16's smallest number, their sum is not.
+
+    Tolerance: as the oracle's, but for what a weight loses below the smallest normal number:
+    weights are held 2^7 times as large as against the row's largest, so 2^-32 each."""
+    from torchplusplus_b200 import ops
+    cu, N = packed([6000, 1, 500])
+    q = torch.zeros(N, 4, D, dtype=F16, device="cuda")
+    k = torch.zeros(N, 2, D, dtype=F16, device="cuda")
+    v = torch.ones(N, 2, D, dtype=F16, device="cuda")
+    q[:, :, 0] = 1
+    for a in cu.tolist()[:-1]:
+        k[a, :, 0], v[a] = bits * math.log(2), 0
+    got = ops.attention_packed(q, k, v, cu, causal=causal, scale=1.0)
+    ref, tol = attention_oracle(q, k, v, cu, causal=causal, scale=1.0)
+    for a, b in zip(cu.tolist()[:-1], cu.tolist()[1:]):
+        tol[a:b] -= (b - a) * (2.0 ** -25 - 2.0 ** -32)  # (of values of 1)
+    assert ((got.double() - ref).abs() <= tol).all(), ((got.double() - ref).abs() / tol).max().item()

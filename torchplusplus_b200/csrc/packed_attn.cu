@@ -8,7 +8,8 @@
 // it, and each K/V tile is read once for two query tiles.  512 threads:
 //   warps 0-3, 4-7 : softmax of query tile 0, 1: a thread owns a row, a step's scores in registers
 //                    (running maximum that only moves, and O with it, when it grows by
-//                    more than 2^8, sums in 32 bits), P in TMEM in the storage type.
+//                    more than 2^8, sums in 32 bits), P in TMEM in the storage type, as the
+//                    product with V takes it (off by at most half a step, see kLift).
 //   warps 8-11     : write O / l at an item's end, while the next one runs.
 //   warps 12, 13   : products of query tile 0, 1: O_i += P_i V_j, then S_i = Q_i K^T of step
 //                    j + 2, across items too: a softmax finds the next S done when it has
@@ -44,6 +45,13 @@ constexpr int kThreads = 512;
 constexpr int kOutWarp0 = 8, kMmaWarp = 12, kTmaWarp = 14;  // (products: warps 12 and 13)
 constexpr int kItems = 8;
 constexpr float kMoves = 8.0f;  // growth of a row's maximum (log2) that moves its reference
+// P = 2^kLift exp(s - reference): f16 numbers end at 2^-24 below (steps of as much, 1024 of them
+// to the first of full precision), and thousands of keys that each weigh less may weigh something
+// together.  With 2^7 P stays below 2^(kMoves + 7) = 2^15, and what a weight loses is at most
+// 2^-32 of the row's largest.  (O and the sum of the weights carry the same factor.)  bf16 has
+// the range of 32 bits.
+template <typename T>
+constexpr float kLift = std::is_same<T, __half>::value ? 7.0f : 0.0f;
 
 // TMEM (512 columns): O of both query tiles, then for each S (BKV columns) and, apart from
 // it, P (half as many), so that S of a later step is under way while a step's softmax runs:
@@ -640,7 +648,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        const float nm = m_ref == -INFINITY ? 0.f : -m_ref;
+        const float nm = m_ref == -INFINITY ? 0.f : kLift<T> - m_ref;
         const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), nm2 = f2_pack(nm, nm);
         uint64_t ps[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
