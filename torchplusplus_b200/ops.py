@@ -717,13 +717,10 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
 
 
 def _strides8(t: torch.Tensor) -> tuple:
-    """t's strides; those of dims of one entry, which no address takes, as a contiguous
-    tensor has them (they may be anything, and the kernels want multiples of 8)."""
-    st, shape = t.stride(), t.shape
-    if 1 not in shape:
-        return st
-    return tuple(math.prod(shape[i + 1:]) if n == 1 else s
-                 for i, (n, s) in enumerate(zip(shape, st)))
+    """t's strides; those of dims of one entry, which no address takes and which may be
+    anything, as a contiguous tensor has them (the kernels want multiples of 8)."""
+    return tuple(math.prod(t.shape[i + 1:]) if n == 1 else s
+                 for i, (n, s) in enumerate(zip(t.shape, t.stride())))
 
 
 def _i32(t: torch.Tensor, shape: tuple, what: str) -> None:
@@ -1033,7 +1030,9 @@ def qk_norm_rope_packed(qkv: torch.Tensor, q_norm_w: torch.Tensor | None,
                 or 0 in cs and any(s == 0 and n > 1 for s, n in zip(cs, shape)):
             raise ValueError("caches must be [B, Hkv, Smax, D] with identical layouts, no two "
                              "rows in one place")
-        cs, rows = _strides8(k_cache), shape[2]
+        rows = shape[2]
+        if (cs[0] | cs[1] | cs[2]) & 7:
+            cs = _strides8(k_cache)
     qkv = _rows16(qkv)
     cs_dt, cs_stride = N.DTYPE_CODE.get(cos.dtype), D
     if cs_dt is None or cos.shape != sin.shape or cos.dtype is not sin.dtype or cos.dim() != 2 \
@@ -1075,7 +1074,9 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
             or any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
         raise ValueError("out must be [N, Hq, D] with a contiguous last dim, no two rows in one "
                          "place")
-    qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), _strides8(out)
+    qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), out.stride()
+    if (os_[0] | os_[1]) & 7:
+        os_ = _strides8(out)
     N.call_on(q, "tpp_attention_packed", q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
               v.data_ptr(), vs[0], vs[1], cu_seqlens.data_ptr(), B, out.data_ptr(), os_[0],
               os_[1], N_, Hq, Hkv, D, bool(causal), window_left,
