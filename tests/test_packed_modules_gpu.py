@@ -1,0 +1,93 @@
+"""forward_packed of the attention modules and the model: what does not fit is refused, as
+forward refuses it."""
+import pytest
+import torch
+
+from torchplusplus_b200.attention.gqa import GroupedQueryAttention
+from torchplusplus_b200.attention.swa import SlidingWindowAttention
+from torchplusplus_b200.dlops.rope import compute_rope_params
+from torchplusplus_b200.llmops.kvcache import KVCache
+
+from .test_packed_model_gpu import make, prompts
+
+pytestmark = pytest.mark.gpu
+DEV, BF16 = "cuda", torch.bfloat16
+
+
+def module(kind):
+    torch.manual_seed(0)
+    if kind == "gqa":
+        return GroupedQueryAttention(256, 4, 2, dtype=BF16).to(DEV)
+    return SlidingWindowAttention(33, 256, 4, dtype=BF16, n_kv_heads=2).to(DEV)
+
+
+def packed(lens, tail=0):
+    cu = torch.tensor([0] + lens).cumsum(0).to(torch.int32).to(DEV)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    return torch.randn(sum(lens) + tail, 256, generator=g, device=DEV).to(BF16), cu
+
+
+def cache(batch, rows):
+    return KVCache(rows, 2, 64, BF16, torch.device(DEV), batch_size=batch)
+
+
+@pytest.mark.parametrize("kind", ["gqa", "swa"])
+@torch.inference_mode()
+def test_prompts_longer_than_the_cache_or_the_tables(kind):
+    a = module(kind)
+    cos, sin = compute_rope_params(64, 1e6, 100, device=DEV)
+    x, cu = packed([60, 3, 90])
+    for kw in (dict(), dict(max_seqlen=90)):
+        with pytest.raises(ValueError, match="KV cache overflow"):
+            a.forward_packed(x, cos, sin, cu, cache(3, 89), **kw)
+        with pytest.raises(ValueError, match="rotary table"):
+            a.forward_packed(x, cos[:89], sin[:89], cu, cache(3, 90), **kw)
+        with pytest.raises(ValueError, match="rotary table"):
+            a.forward_packed(x, cos[:89], sin[:89], cu, **kw)
+        # all rows together are more than the cache and the tables hold, each prompt is not
+        kv = cache(3, 90)
+        got = a.forward_packed(x, cos[:90], sin[:90], cu, kv, **kw)
+        assert torch.equal(got, a.forward_packed(x, cos, sin, cu)) and kv.k_cache[2, :, 89].any()
+
+
+@torch.inference_mode()
+def test_rows_of_no_prompt_do_not_count():
+    a = module("gqa")
+    cos, sin = compute_rope_params(64, 1e6, 40, device=DEV)
+    x, cu = packed([40, 3], tail=50)
+    got = a.forward_packed(x, cos, sin, cu, cache(2, 40))
+    assert torch.equal(got[:43], a.forward_packed(x[:43], cos, sin, cu))
+    none = torch.zeros(1, dtype=torch.int32, device=DEV)
+    assert a.forward_packed(x, cos, sin, none).shape == x.shape
+
+
+@torch.inference_mode()
+def test_recorded_calls_say_their_longest_prompt():
+    """A call that is being recorded cannot look at the lengths on the device."""
+    a = module("gqa")
+    cos, sin = compute_rope_params(64, 1e6, 60, device=DEV)
+    x, cu = packed([60, 3])
+    want = a.forward_packed(x, cos, sin, cu)
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        with pytest.raises(ValueError, match="max_seqlen"):
+            a.forward_packed(x, cos, sin, cu)
+        got = a.forward_packed(x, cos, sin, cu, max_seqlen=60)
+    g.replay()
+    assert torch.equal(got, want)
+
+
+@torch.inference_mode()
+def test_model_prompts_longer_than_its_tables_or_caches():
+    m = make()  # (a context of 512)
+    ids = torch.cat(prompts([513, 2])).to(DEV)
+    cu = torch.tensor([0, 513, 515], dtype=torch.int32, device=DEV)
+    with pytest.raises(ValueError, match="rotary table"):
+        m.forward_packed(ids, cu)
+    ids, cu = ids[1:], (cu - 1).clamp_min(0)
+    whole = m.forward_packed(ids, cu)
+    assert torch.equal(m.forward_packed(ids, cu, max_seqlen=512), whole)
+    caches = [KVCache(511, 2, 64, BF16, torch.device(DEV), batch_size=2) for _ in range(2)]
+    with pytest.raises(ValueError, match="KV cache overflow"):
+        m.forward_packed(ids, cu, caches)

@@ -71,16 +71,36 @@ def attention_block(x: torch.Tensor, wqkv: torch.Tensor, wo: torch.Tensor,
     return ops.linear(o.reshape(B, S, Hq * D), wo, bo, residual=residual)
 
 
+def longest_prompt(cu_seqlens: torch.Tensor, rows: int, room: int) -> int:
+    """A length that no prompt of a packed batch of `rows` rows exceeds: all its rows where so
+    many fit `room` anyway, else the longest prompt's, read from the device."""
+    if rows <= room or cu_seqlens.shape[0] < 2:
+        return min(rows, room)
+    if torch.cuda.is_current_stream_capturing():
+        raise ValueError("a recorded call has to be given max_seqlen")
+    return int((cu_seqlens[1:] - cu_seqlens[:-1]).max())
+
+
 def packed_attention_block(x: torch.Tensor, wqkv: torch.Tensor, wo: torch.Tensor,
                            bo: torch.Tensor | None, Hq: int, Hkv: int, D: int,
                            qn_w: torch.Tensor | None, kn_w: torch.Tensor | None, eps: float,
                            cos: torch.Tensor, sin: torch.Tensor, cu_seqlens: torch.Tensor,
                            kv_cache=None, window_left: int = -1,
-                           residual: torch.Tensor | None = None) -> torch.Tensor:
+                           residual: torch.Tensor | None = None,
+                           max_seqlen: int | None = None) -> torch.Tensor:
     """attention_block over prompts of different lengths packed row after row: x [N, E],
     sequence b in rows cu_seqlens[b] .. cu_seqlens[b+1]-1 (int32 on the device), causal,
     whole prompts.  A KVCache of batch B receives each sequence's K and V from row 0 on;
-    its cache_len is left to the caller (the lengths differ)."""
+    its cache_len is left to the caller (the lengths differ).  max_seqlen: the longest prompt's
+    length, if the caller has it; it is otherwise read from the device where N rows are more
+    than the rotary tables or the cache hold."""
+    room = cos.shape[0] if kv_cache is None else min(cos.shape[0], kv_cache.max_seq_len)
+    if max_seqlen is None:
+        max_seqlen = longest_prompt(cu_seqlens, x.shape[0], room)
+    if max_seqlen > cos.shape[0]:
+        raise ValueError("a prompt exceeds the rotary tables")
+    if max_seqlen > room:
+        raise ValueError("KV cache overflow")
     qkv = ops.linear(x, wqkv)                                  # [N, (Hq+2Hkv) D]
     kc = vc = None
     if kv_cache is not None:

@@ -54,9 +54,11 @@ class GroupedQueryAttention(nn.Module):
 
     def forward_packed(self, x, cos, sin, cu_seqlens: torch.Tensor,
                        kv_cache: Optional[KVCache] = None,
-                       residual: Optional[torch.Tensor] = None):
+                       residual: Optional[torch.Tensor] = None,
+                       max_seqlen: Optional[int] = None):
         """forward over whole prompts of different lengths packed row after row: x [N, d_in],
-        cu_seqlens int32 [B+1] on the device (see _core.packed_attention_block)."""
+        cu_seqlens int32 [B+1] on the device, max_seqlen the longest one's length, if known
+        (see _core.packed_attention_block)."""
         w = self._qkv.get(self.Wq.weight, self.Wk.weight, self.Wv.weight)
         return packed_attention_block(
             x, w, self.out_projection.weight, self.out_projection.bias, self.num_heads,
@@ -64,4 +66,4 @@ class GroupedQueryAttention(nn.Module):
             self.q_norm.weight if self.q_norm is not None else None,
             self.k_norm.weight if self.k_norm is not None else None,
             norm_eps(self.q_norm) if self.q_norm is not None else 1e-6, cos, sin, cu_seqlens,
-            kv_cache=kv_cache, residual=residual)
+            kv_cache=kv_cache, residual=residual, max_seqlen=max_seqlen)

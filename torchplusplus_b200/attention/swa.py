@@ -52,9 +52,11 @@ class SlidingWindowAttention(nn.Module):
             kv_cache=kv_cache, cache_pos=cache_pos, causal=True,
             window_left=self.window_size - 1)
 
-    def forward_packed(self, x: torch.Tensor, cos, sin, cu_seqlens: torch.Tensor, kv_cache=None):
+    def forward_packed(self, x: torch.Tensor, cos, sin, cu_seqlens: torch.Tensor, kv_cache=None,
+                       max_seqlen: Optional[int] = None):
         """forward over whole prompts of different lengths packed row after row: x
-        [N, embed_dim], cu_seqlens int32 [B+1] on the device."""
+        [N, embed_dim], cu_seqlens int32 [B+1] on the device, max_seqlen the longest one's
+        length, if known (see _core.packed_attention_block)."""
         w = self._qkv.get(self.Wq.weight, self.Wk.weight, self.Wv.weight)
         return packed_attention_block(
             x, w, self.out_projection.weight, self.out_projection.bias, self.n_heads,
@@ -62,4 +64,5 @@ class SlidingWindowAttention(nn.Module):
             self.q_norm.weight if self.q_norm is not None else None,
             self.k_norm.weight if self.k_norm is not None else None,
             norm_eps(self.q_norm) if self.q_norm is not None else 1e-6, cos, sin, cu_seqlens,
-            kv_cache=kv_cache, window_left=self.window_size - 1)
+            kv_cache=kv_cache, window_left=self.window_size - 1,
+            max_seqlen=max_seqlen)

@@ -347,7 +347,7 @@ class DecodeEngine:
         S = max(lens)
         if len(lens) != self.batch_size or S >= self.max_seq_len or min(lens) < 1:
             raise ValueError("prompts do not fit the engine's batch / capacity")
-        x = self.model.forward_packed(ids, cu, self.caches)
+        x = self.model.forward_packed(ids, cu, self.caches, max_seqlen=S)
         for c in self.caches:
             c.cache_len = S
         a = 0

@@ -22,7 +22,7 @@ import torch
 import torch.nn as nn
 
 from .. import ops
-from ..attention._core import FusedQKV
+from ..attention._core import FusedQKV, longest_prompt
 from ..attention.gqa import GroupedQueryAttention
 from ..dlops.linear import LinearSILU
 from ..dlops.normalization import RmsNormFused
@@ -83,8 +83,9 @@ class Transformer(nn.Module):
         return self.ffn(h, residual=x)
 
     def forward_packed(self, x, cos, sin, cu_seqlens: torch.Tensor,
-                       kv_cache: Optional[KVCache] = None):
-        x = self.attn.forward_packed(self.rms_norm1(x), cos, sin, cu_seqlens, kv_cache, residual=x)
+                       kv_cache: Optional[KVCache] = None, max_seqlen: Optional[int] = None):
+        x = self.attn.forward_packed(self.rms_norm1(x), cos, sin, cu_seqlens, kv_cache, residual=x,
+                                     max_seqlen=max_seqlen)
         return self.ffn(self.rms_norm2(x), residual=x)
 
 
@@ -143,14 +144,20 @@ class Qwen3(LLMInference):
         return ops.linear(x, self.out_head.weight)
 
     def forward_packed(self, ids: torch.Tensor, cu_seqlens: torch.Tensor,
-                       kv_caches: Optional[List[KVCache]] = None) -> torch.Tensor:
+                       kv_caches: Optional[List[KVCache]] = None,
+                       max_seqlen: Optional[int] = None) -> torch.Tensor:
         """Whole prompts of different lengths packed row after row (ids [N], sequence b in
         rows cu_seqlens[b] .. cu_seqlens[b+1]-1, int32 on the device) -> the rows [N, E] before
-        the final norm.  With kv_caches each sequence's K and V go to its rows of them."""
+        the final norm.  With kv_caches each sequence's K and V go to its rows of them.
+        max_seqlen: the longest prompt's length, if known (read from the device otherwise where
+        N rows are more than the rotary tables or the caches hold)."""
+        if max_seqlen is None:
+            max_seqlen = longest_prompt(cu_seqlens, ids.shape[0], min(
+                [self.cos.shape[0]] + [c.max_seq_len for c in kv_caches or ()]))
         x = ops.embedding(ids, self.tok_embed.weight)
         for i, blk in enumerate(self.transformer_blocs):
             x = blk.forward_packed(x, self.cos, self.sin, cu_seqlens,
-                                   kv_caches[i] if kv_caches is not None else None)
+                                   kv_caches[i] if kv_caches is not None else None, max_seqlen)
         return x
 
     def score(self, prompts, temperature: float = 1.0, top: Optional[int] = None):

@@ -55,7 +55,7 @@ def score(model, prompts: Sequence[torch.Tensor], temperature: float = 1.0,
     if len(ids) == 0:
         parts = None
     else:
-        h = model.final_rmsnorm(model.forward_packed(ids, cu))
+        h = model.final_rmsnorm(model.forward_packed(ids, cu, max_seqlen=max(lens)))
         # the token that each row predicts; -1 behind the last (its score is dropped)
         nxt = torch.cat([ids[1:], ids.new_full((1,), -1)])
         w = model.out_head.weight
