@@ -78,6 +78,21 @@ def test_recorded_calls_say_their_longest_prompt():
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("kind", ["gqa", "swa"])
+@torch.inference_mode()
+def test_without_rotary_tables(kind):
+    a = module(kind)
+    lens = [100, 1, 70]
+    x, cu = packed(lens)
+    got = a.forward_packed(x, None, None, cu).float()
+    s = 0
+    for n in lens:
+        want = a(x[None, s:s + n], None, None)[0].float()
+        # both round the probabilities, the attention's and the projection's outputs to bf16
+        assert (got[s:s + n] - want).abs().max() <= 2e-2 * max(1.0, want.abs().max().item())
+        s += n
+
+
 @torch.inference_mode()
 def test_model_prompts_longer_than_its_tables_or_caches():
     m = make()  # (a context of 512)

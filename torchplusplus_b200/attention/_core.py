@@ -35,6 +35,15 @@ class FusedQKV:
         return self._w
 
 
+def rotary_tables(cos: torch.Tensor | None, sin: torch.Tensor | None, D: int, like: torch.Tensor
+                  ) -> tuple[torch.Tensor, torch.Tensor]:
+    """cos and sin, or identity tables where there is no rotary embedding."""
+    if cos is None:
+        cos = torch.ones((1, D), dtype=like.dtype, device=like.device).expand(1 << 20, D)
+        sin = torch.zeros((1, D), dtype=like.dtype, device=like.device).expand(1 << 20, D)
+    return cos, sin
+
+
 def attention_block(x: torch.Tensor, wqkv: torch.Tensor, wo: torch.Tensor,
                     bo: torch.Tensor | None, Hq: int, Hkv: int, D: int,
                     qn_w: torch.Tensor | None, kn_w: torch.Tensor | None, eps: float,
@@ -43,9 +52,7 @@ def attention_block(x: torch.Tensor, wqkv: torch.Tensor, wo: torch.Tensor,
                     window_left: int = -1, residual: torch.Tensor | None = None) -> torch.Tensor:
     B, S, _ = x.shape
     qkv = ops.linear(x, wqkv)                                  # [B, S, (Hq+2Hkv) D]
-    if cos is None:  # no rotary embedding: identity tables
-        cos = torch.ones((1, D), dtype=x.dtype, device=x.device).expand(1 << 20, D)
-        sin = torch.zeros((1, D), dtype=x.dtype, device=x.device).expand(1 << 20, D)
+    cos, sin = rotary_tables(cos, sin, D, x)
     if kv_cache is not None:
         start = int(cache_pos) if cache_pos is not None else kv_cache.cache_len
         kv_cache._ensure_allocated(B)
@@ -84,7 +91,8 @@ def longest_prompt(cu_seqlens: torch.Tensor, rows: int, room: int) -> int:
 def packed_attention_block(x: torch.Tensor, wqkv: torch.Tensor, wo: torch.Tensor,
                            bo: torch.Tensor | None, Hq: int, Hkv: int, D: int,
                            qn_w: torch.Tensor | None, kn_w: torch.Tensor | None, eps: float,
-                           cos: torch.Tensor, sin: torch.Tensor, cu_seqlens: torch.Tensor,
+                           cos: torch.Tensor | None, sin: torch.Tensor | None,
+                           cu_seqlens: torch.Tensor,
                            kv_cache=None, window_left: int = -1,
                            residual: torch.Tensor | None = None,
                            max_seqlen: int | None = None) -> torch.Tensor:
@@ -94,6 +102,7 @@ def packed_attention_block(x: torch.Tensor, wqkv: torch.Tensor, wo: torch.Tensor
     its cache_len is left to the caller (the lengths differ).  max_seqlen: the longest prompt's
     length, if the caller has it; it is otherwise read from the device where N rows are more
     than the rotary tables or the cache hold."""
+    cos, sin = rotary_tables(cos, sin, D, x)
     room = cos.shape[0] if kv_cache is None else min(cos.shape[0], kv_cache.max_seq_len)
     if max_seqlen is None:
         max_seqlen = longest_prompt(cu_seqlens, x.shape[0], room)
