@@ -1,5 +1,8 @@
 """What the packed-prompt wrappers hand to the library, and what they refuse before it, on the
 CPU: the library's calls are recorded, none is made."""
+import re
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -151,3 +154,19 @@ def test_linear_logprobs_workspace_is_of_the_operands_device(two_gpus):
     assert two_gpus.called == [(1, 4096)] and two_gpus.current == 0
     assert ops.linear_logprobs_workspace_bytes(5, 5, 64) == 1024
     assert ops.linear_logprobs_workspace_bytes(5, 5, 64, torch.device("cuda", 1)) == 4096
+
+
+def wait_codes(path):
+    """The codes that a kernel source's bounded waits set when they run out."""
+    text = re.sub(r"//[^\n]*", "", path.read_text())
+    return [int(c) for c in re.findall(r"\w*wait\w*\([^;]*?, *(\d+)\)[;) ]", text)
+            + re.findall(r"expired\w*\([^;]*?, *(\d+)\)", text)]
+
+
+@pytest.mark.parametrize("name", ["packed_attn.cu", "linear_logprobs.cu"])
+def test_a_wait_that_ran_out_can_be_told_from_the_others(name):
+    csrc = Path(ops.__file__).parent / "csrc"
+    mine = wait_codes(csrc / name)
+    assert len(mine) >= 4 and len(set(mine)) == len(mine)
+    others = {c for p in csrc.glob("*.cu") if p.name != name for c in wait_codes(p)}
+    assert not others & set(mine)

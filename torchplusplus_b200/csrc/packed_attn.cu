@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // the n-th item (the same for the warp; every reader reads each once)
   auto take = [&](int n) {
     const int s = n % kItems;
-    ok = ok && wait_short(&it_full[s], (n / kItems) & 1, p.err, 61);
+    ok = ok && wait_short(&it_full[s], (n / kItems) & 1, p.err, 81);
     Work w{};
     w.len = -1;
     if (ok) w = items[s];
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t at = nk * gridDim.x + (nk & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
       const Work w = work_of<BKV>(walk.item(at, lane), p);
       const int s = nk % kItems;
-      if (nk >= kItems) ok = ok && wait_short(&it_empty[s], ((nk / kItems) & 1) ^ 1, p.err, 62);
+      if (nk >= kItems) ok = ok && wait_short(&it_empty[s], ((nk / kItems) & 1) ^ 1, p.err, 82);
       if (lane == 0 && ok) {
         items[s] = w;
         mbar_arrive(&it_full[s]);
@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (w.len < 0) continue;
         if (lane == 0) {
           const int r = k ? k_load(g) : v_load(g - 2), s = r % S;
-          if (r >= S) ok = ok && wait_short(&kv_empty[s], ((r / S) & 1) ^ 1, p.err, 63);
+          if (r >= S) ok = ok && wait_short(&kv_empty[s], ((r / S) & 1) ^ 1, p.err, 83);
           if (ok) {
             mbar_arrive_expect_tx(&kv_full[s], P::kTile);
             tma_load_4d(sKV + s * P::kTile, k ? &tm_k : &tm_v, &kv_full[s], 0,
@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < 2; ++i) {
               if (w.end(i) <= w.start(i)) continue;
               if (nq >> (2 + i) & 1)
-                ok = ok && wait_short(&q_empty[i], (nq >> i & 1) ^ 1, p.err, 64);
+                ok = ok && wait_short(&q_empty[i], (nq >> i & 1) ^ 1, p.err, 84);
               if (!ok) break;
               mbar_arrive_expect_tx(&q_full[i], P::kBoxes * q_box);
               for (int b = 0; b < P::kBoxes; ++b)
@@ -443,10 +443,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto issue_s = [&]() {  // (K has landed)
       if (js >= ws.start && js < ws.end) {
         if (js == ws.start) {
-          wait(&q_full[i], nq, 65);
+          wait(&q_full[i], nq, 85);
           nq ^= 1;
         }
-        if (s_any) wait(&s_read[i], ns, 66);  // the last S_i is in registers
+        if (s_any) wait(&s_read[i], ns, 86);  // the last S_i is in registers
         s_any = true;
         ns ^= 1;
         tc_fence_after();
@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     };
     for (int g = 0; g < 2 && ws.nt > 0; ++g) {
-      wait(&kv_full[g], 0, 67);
+      wait(&kv_full[g], 0, 87);
       issue_s();
       sk = g == 0 ? 1 : 3;
     }
@@ -473,16 +473,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     while (wp.nt > 0) {
       // V of this step, K of the one after the next: in time for the softmax, as a rule
       const bool part = jp < wp.low || jp >= wp.high;
-      wait(&kv_full[sv], hv, 68);
-      if (part) wait(&v_ok[sv], seen >> sv, 70);
-      if (ws.nt > 0) wait(&kv_full[sk], hk, 69);
+      wait(&kv_full[sv], hv, 88);
+      if (part) wait(&v_ok[sv], seen >> sv, 89);
+      if (ws.nt > 0) wait(&kv_full[sk], hk, 90);
       if (jp >= wp.start && jp < wp.end) {
         if (jp == wp.start) {
-          if (o_any) wait(&o_empty[i], no, 71);
+          if (o_any) wait(&o_empty[i], no, 91);
           o_any = true;
           no ^= 1;
         }
-        wait(&p_ready[i], np, 72);
+        wait(&p_ready[i], np, 92);
         np ^= 1;
         tc_fence_after();
         const uint32_t va = kv_at + (P::kBox >> 4 << 16) + sv * (P::kTile >> 4);
@@ -519,9 +519,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int j = 0; j < w.nt && ok; ++j, ++g) {
         if (!w.part(j)) continue;
         const int r = v_load(g), s = r % S;
-        ok = ok && wait_short(&v_sent[s], seen >> s & 1, p.err, 77);
+        ok = ok && wait_short(&v_sent[s], seen >> s & 1, p.err, 93);
         seen ^= 1u << s;
-        ok = ok && wait_short(&kv_full[s], (r / S) & 1, p.err, 73);
+        ok = ok && wait_short(&kv_full[s], (r / S) & 1, p.err, 94);
         if (!ok) break;
         // rows of the sequence, then rows behind it (each 128 bytes a box)
         const int valid = min(BKV, w.len - (w.kb + j) * BKV);
@@ -582,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int qpos = w.t0 + i * p.TT + rl / p.G;
       float m_ref = -INFINITY, l = 0.f;
       for (int j = w.start(i); j < w.end(i); ++j) {
-        ok = ok && wait_short(&s_full[i], ns & 1, p.err, 70);
+        ok = ok && wait_short(&s_full[i], ns & 1, p.err, 95);
         ++ns;
         if (!ok) break;
         __syncwarp();
@@ -627,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float mx = nanmax(nanmax(pm[0], pm[1], pm[2]), nanmax(pm[3], pm[4], pm[5]),
                                 nanmax(pm[6], pm[7])) * p.scale_log2;
         // P_i V of the last step is done: P_i may be written, and O_i is at rest
-        if (ns > 1) ok = ok && wait_short(&pv_done[i], ns & 1, p.err, 74);
+        if (ns > 1) ok = ok && wait_short(&pv_done[i], ns & 1, p.err, 96);
         if (!ok) break;
         tc_fence_after();
         const bool moves = !(mx <= m_ref + kMoves);  // (the first finite one too; NaN)
@@ -674,7 +674,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         l += a0 + a1;
       }
       if (!ok) break;
-      if (nl > 0) ok = ok && wait_short(&l_empty[i], (nl & 1) ^ 1, p.err, 72);
+      if (nl > 0) ok = ok && wait_short(&l_empty[i], (nl & 1) ^ 1, p.err, 97);
       ++nl;
       if (!ok) break;
       sums[i * BQ + rl] = l;
@@ -695,7 +695,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
       for (int i = 0; i < 2; ++i) {
         if (w.end(i) <= w.start(i)) continue;
-        ok = ok && wait_short(&l_full[i], no >> i & 1, p.err, 75);
+        ok = ok && wait_short(&l_full[i], no >> i & 1, p.err, 98);
         if (!ok) break;
         const float l = sums[i * BQ + rl];
         (i ? inv1 : inv0) = l == 0.f ? 0.f : 1.f / l;
@@ -705,7 +705,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
       for (int i = 0; i < 2; ++i) {
         if (w.end(i) <= w.start(i)) continue;
-        ok = ok && wait_short(&o_full[i], no >> i & 1, p.err, 76);
+        ok = ok && wait_short(&o_full[i], no >> i & 1, p.err, 99);
         no ^= 1u << i;
         if (!ok) break;
         __syncwarp();
