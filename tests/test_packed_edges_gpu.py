@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from .test_logprobs_gpu import check_head, operands as head_operands
+from .test_logprobs_gpu import check, check_head, operands as head_operands
 from .test_packed_gpu import BF16, F16, F32, attention_oracle, gen, packed, randn, rope_oracle
 
 pytestmark = pytest.mark.gpu
@@ -172,3 +172,75 @@ def test_attention_f16_of_many_small_weights(D, bits, causal):
     for a, b in zip(cu.tolist()[:-1], cu.tolist()[1:]):
         tol[a:b] -= (b - a) * (2.0 ** -25 - 2.0 ** -32)  # (of values of 1)
     assert ((got.double() - ref).abs() <= tol).all(), ((got.double() - ref).abs() / tol).max().item()
+
+
+# 111 to 443 rows take two or four CTAs each, with 128 threads from 128 * 64 bytes a CTA on:
+# noted hits and the join over the CTAs together.
+@pytest.mark.parametrize("N,V", [(130, 33013), (221, 17011), (222, 17011), (300, 12007), (443, 9001)])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_logprobs_of_rows_over_some_ctas(N, V, dtype):
+    ix = torch.arange(V, device="cuda")
+    low = torch.finfo(dtype).min
+    rows = [
+        torch.zeros(V),                                                    # all equal
+        ix / V * 60 - 30, 30 - ix / V * 60,                                # in order
+        torch.where(ix % 3 == 0, -math.inf, torch.where(ix % 37 == 5, 1.0, 0.0)),
+        torch.where(ix < V - 2, -math.inf, 2.0),                           # two tokens left
+        torch.where(ix < 5, 3.0 * (ix % 2), low),
+        torch.full((V,), -math.inf),
+        torch.where(ix == V // 2, math.nan, ix % 11),
+        torch.where(ix == V - 1, math.inf, ix % 11),
+        torch.where(ix % 2 == 0, 0.0, -0.0),
+        torch.where(ix == V - 1, 60.0, ix % 13),
+        torch.where((ix > V // 2) & (ix < V // 2 + 40), 9.0, ix % 5 * 1.0),  # across CTAs
+    ]
+    x = (torch.randn(N, V, generator=gen(45), device="cuda") * 3).to(dtype)
+    for i, r in enumerate(rows):
+        x[7 * i + 1] = r.to(device="cuda", dtype=dtype)
+    tok = torch.randint(0, V, (N,), generator=gen(46), device="cuda")
+    for top in (0, 1, 9, 32):
+        check(x, tok, top=top)
+
+
+@pytest.mark.parametrize("off,ld", [(3, 17019), (1, 17013)])
+def test_logprobs_of_strided_rows_over_some_ctas(off, ld):
+    room = (torch.randn(150, ld, generator=gen(47), device="cuda") * 3).to(BF16)
+    check(room[:, off:off + 17011], torch.randint(0, 17011, (150,), generator=gen(48), device="cuda"), top=7)
+
+
+# ------------------------------------------------------------------ lengths that make no sense
+def guarded(*shape, value):
+    """A tensor in the middle of a larger one full of `value`, and that one."""
+    n = torch.Size(shape).numel()
+    room = torch.full((n + 2 * 65536,), value, dtype=BF16, device="cuda")
+    return room[65536:65536 + n].view(shape), room
+
+
+def test_lengths_that_do_not_ascend_write_rows_only():
+    """Whatever cu_seqlens holds, attention reads its spans cut to [0, N), and both operators
+    write rows of their outputs and caches only."""
+    from torchplusplus_b200 import ops
+    N, Hq, Hkv, D = 400, 4, 2, 128
+    g = gen(49)
+    q, k, v = randn(g, N, Hq, D, dtype=BF16), randn(g, N, Hkv, D, dtype=BF16), randn(g, N, Hkv, D, dtype=BF16)
+    qkv = randn(g, N, (Hq + 2 * Hkv) * D, dtype=BF16)
+    cos = torch.ones(N, D, device="cuda")
+    wild = [-7, 100, 60, 60, -9, -2, -(1 << 31), -5, 0, 0]    # rows 0 to 99 once
+    late = [1 << 30, 500, 450, 250, 1 << 30, (1 << 31) - 1]   # rows 250 to 399 once
+    for cu, a, b in ((wild, 0, 100), (late, 250, 400)):
+        cu = torch.tensor(cu, dtype=torch.int32, device="cuda")
+        out, room = guarded(N, Hq, D, value=7.0)
+        ops.attention_packed(q, k, v, cu, out=out)
+        span = torch.tensor([a, b], dtype=torch.int32, device="cuda")
+        ref, tol = attention_oracle(q, k, v, span)
+        assert ((out.double() - ref).abs() <= tol)[a:b].all()
+        out[a:b] = 7
+        assert (room == 7).all() and ops.device_error() == 0
+        # the norm and its cache: rows of its own outputs, and nothing else
+        B = cu.shape[0] - 1
+        got = [guarded(*s, value=7.0) for s in ((N, Hq, D), (N, Hkv, D), (B, Hkv, 64, D), (B, Hkv, 64, D))]
+        ops.qk_norm_rope_packed(qkv, None, None, 1e-6, cos, cos, cu, Hq, Hkv, got[2][0], got[3][0],
+                                q_out=got[0][0], k_out=got[1][0])
+        for t, room in got:
+            t.fill_(7)
+            assert (room == 7).all()
