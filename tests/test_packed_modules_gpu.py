@@ -106,3 +106,39 @@ def test_model_prompts_longer_than_its_tables_or_caches():
     caches = [KVCache(511, 2, 64, BF16, torch.device(DEV), batch_size=2) for _ in range(2)]
     with pytest.raises(ValueError, match="KV cache overflow"):
         m.forward_packed(ids, cu, caches)
+
+
+def test_scores_asked_for_in_inference_mode():
+    """What set_logprobs allocates there is written by steps outside it too."""
+    m = make()
+    want = None
+    for inside in (False, True):
+        eng = m.engine(2, 64)
+        with torch.inference_mode(inside):
+            eng.set_logprobs(None)
+            eng.set_logprobs(2)
+        eng.set_greedy()
+        eng.prefill(prompts([20, 7]))
+        eng.decode(3)
+        eng.step_eager()
+        got = [s.clone() for s in eng.scores]
+        want = want or got
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert (got[2][0, 20:25] == 1).all() and (got[2][1, 7:12] == 1).all()
+
+
+@pytest.mark.parametrize("batch", [2, 5])
+def test_scores_of_a_batch_in_lanes(batch):
+    """Each lane scores its own sequences, side by side in the graph."""
+    from torchplusplus_b200.llmops.engine import DecodeEngine
+    m = make()
+    ps = prompts([20, 33, 7, 50, 1][:batch])
+    for lanes in (1, 2):
+        eng = DecodeEngine(m, batch, 96, lanes=lanes)
+        eng.set_logprobs(4)
+        out = eng.generate(ps, 12)
+        for b, (p, o) in enumerate(zip(ps, out)):
+            n = len(p)
+            now = torch.arange(n, n + 12, device=DEV)
+            assert torch.equal(eng.scores[4][b, now, 0], o[n:]) and (eng.scores[2][b, now] == 1).all()
+            assert (eng.scores[0][b, now] < 0).all() and (eng.scores[0][b, n + 12:] == 0).all()

@@ -226,6 +226,7 @@ class DecodeEngine:
         ops.decode_advance(ln["tokens"], ln["out_ids"], ln["positions"], ln["seqlens"])
         self._record(ln["b"])
 
+    @torch.inference_mode()  # (scores allocated there may be written nowhere else)
     def _record(self, b: slice) -> None:
         """Writes the scores of the tokens just chosen to their places in `scores`."""
         if self.scoring is None:
