@@ -554,7 +554,7 @@ int tpp_token_logprobs(const void* logits, int64_t ld, int64_t N, int64_t V,
 /* The log probabilities and entropies of tpp_token_logprobs for the logits
  * x [N, E] . w [V, E]^T, summed in 32 bits and never written (row strides ldx, ldw; f16
  * or bf16; E a multiple of 8, rows 16-byte aligned).  A NaN or +inf logit makes its row
- * NaN, one of -inf may.
+ * NaN; one of -inf may, and logits further apart than the largest float32 (3.4e38).
  * workspace: tpp_linear_logprobs_workspace bytes (of the device that is current then, as it
  * must be in the call), 4-byte aligned. */
 int tpp_linear_logprobs(const void* x, int64_t ldx, const void* w, int64_t ldw,

@@ -432,6 +432,11 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
 // Vocabulary rows a tile: of the widths that fill the tensor core (a multiple of 16, at
 // least 128), the one whose tiles go evenly onto the SMs -- 151936 rows are 594 tiles of
 // 256, five rounds of 148 CTAs where four would nearly do, but five full rounds of 208.
+// Measured (bf16, us; widths 128, 208, 224, 240, 256, then the choice): 7 x 1024 x 151936 63.7,
+// 59.9, 57.7, 59.8, 60.4: 208; 4096 x 1024 x 32003 244, 183, 181, 177, 181: 240; 2000 x 256 x
+// 50000 73, 63, 61, 61, 60: 240.  Not always the best: 1000 x 1024 x 32003 66.6, 49.8, 47.7, 48.9,
+// 46.3, and it takes 176, 52.8 (a tile's own cost of 16 columns would give 256 there, and the
+// same widths in the other cases).
 int tile_width(int64_t N, int64_t V) {
   const int64_t ntm = (N + BM - 1) / BM, sms = num_sms();
   int best = kMaxBN;

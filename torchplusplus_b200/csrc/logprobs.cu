@@ -158,6 +158,9 @@ template <> struct Lane<float> {
 // with 20; 4096 x 32003 62 and 100; a single row of 151936 over 8 CTAs 10.6, with 5 14.6.
 // Bound by HBM without alternatives (issue slots 69 % busy), by issue slots and barriers with
 // them, a single row by latency.  Narrowing after chunks 1, 3, 9 .. takes as long, 1, 8, 64: 313.
+// A row with -inf is read once more, an element a thread at a time, and one whose first chunk's
+// bound is -inf `top` times more: 10 % of the 4096 x 151936 at -inf 2290 us, 2380 with 20
+// alternatives; all but 100 of each row 2290, and 45 ms (8 such rows: 139 us, of others 17).
 template <typename T, bool TOP, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT)
     token_logprobs_kernel(LogprobArgs p) {
@@ -589,7 +592,11 @@ extern "C" int tpp_token_logprobs(const void* logits, int64_t ld, int64_t N, int
   const LogprobArgs a{logits, ld, V, tokens, (float)(1.4426950408889634 / temperature),
                       (float)(1 / temperature), (int)top,
                       logprobs, entropy, ranks, top_logprobs, top_tokens};
-  // CTAs a row: enough rows for three on every SM want one each
+  // CTAs a row: enough rows for three on every SM want one each.  Measured (bf16, top 20, us with
+  // 1, 2, 4, 8 CTAs): one of 151936 39.5, 27.6, 21.2, 16.7; 130 46, 33, 28, 46 (takes 4); 300 51, 52,
+  // 53, 98 (2); 1200 113, 116, 147, 349 (1).  Not the best between, and for small rows: 110 of
+  // 151936 46, 33, 28, 44 (8); 600 84, 72, 85, 182 (1), without alternatives 64, 44, 47, 93; one of
+  // 32003 15.9, 13.2, 11.3, 17.0 (8).
   int C = 1;
   while (C < kMaxCtas && N * C < 3 * (int64_t)num_sms()) C *= 2;
   auto go = [&](auto tag, auto threads) -> int {

@@ -45,20 +45,18 @@ constexpr int kThreads = 512;
 constexpr int kOutWarp0 = 8, kMmaWarp = 12, kTmaWarp = 14;  // (products: warps 12 and 13)
 constexpr int kItems = 8;
 constexpr float kMoves = 8.0f;  // growth of a row's maximum (log2) that moves its reference
-// P = 2^kLift exp(s - reference): f16 numbers end at 2^-24 below (steps of as much, 1024 of them
-// to the first of full precision), and thousands of keys that each weigh less may weigh something
-// together.  With 2^7 P stays below 2^(kMoves + 7) = 2^15, and what a weight loses is at most
-// 2^-32 of the row's largest.  (O and the sum of the weights carry the same factor.)  bf16 has
-// the range of 32 bits.
+// P = 2^kLift exp(s - reference), and so are O and the sums.  f16 numbers end at 2^-24, and
+// thousands of keys that weigh less each may weigh something together: with 2^7, P stays
+// below 2^(kMoves + 7) = 2^15, and a weight loses at most 2^-32 of the row's largest (2^-25 without,
+// in one prompt of 6000 rows up to all of an output).  bf16 has the range of 32 bits.
 template <typename T>
 constexpr float kLift = std::is_same<T, __half>::value ? 7.0f : 0.0f;
 
 // TMEM (512 columns): O of both query tiles, then for each S (BKV columns) and, apart from
 // it, P (half as many), so that S of a later step is under way while a step's softmax runs:
-// that leaves 80 keys a step for 128 dims.  (P over S with 128 keys: each tile's products
-// and softmax take turns, 3600 clocks for 128 keys of both tiles, against 3100 now.)  For 64
-// dims 128 keys would fit, and 96 are faster: one prompt of 16384, 64: 912 us, 96: 770, 112:
-// 850, 128: 832.
+// that leaves 80 keys a step for 128 dims.  (With P over S, 128 keys a step, each tile's products
+// and softmax take turns.)  For 64 dims 128 keys would fit, and 96 are faster: one prompt of
+// 16384, 64: 912 us, 96: 770, 112: 850, 128: 832.
 template <int D>
 struct Plan {
   static constexpr int BKV = D == 128 ? 80 : 96;      // keys a step
