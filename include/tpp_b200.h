@@ -531,7 +531,7 @@ int tpp_qk_norm_rope_packed(const void* qkv, int64_t qkv_sn, const void* qn_w,
  * [N, Hkv, D], o [N, Hq, D] by row and head strides (multiples of 8 elements).  causal: keys up to the
  * row itself; window_left >= 0: keys from the row's position - window_left on.  D 64 or
  * 128, Hq / Hkv <= 128.  What a row does not see does not affect it, NaN and
- * infinities included. */
+ * infinities included.  Scaled scores from 9e7 in magnitude on may make a row NaN. */
 int tpp_attention_packed(const void* q, int64_t q_sn, int64_t q_sh, const void* k, int64_t k_sn,
                          int64_t k_sh, const void* v, int64_t v_sn, int64_t v_sh,
                          const int32_t* cu_seqlens, int64_t B, void* o, int64_t o_sn,

@@ -6,7 +6,8 @@ import pytest
 import torch
 
 from .test_logprobs_gpu import check, check_head, operands as head_operands
-from .test_packed_gpu import BF16, F16, F32, attention_oracle, gen, packed, randn, rope_oracle
+from .test_packed_gpu import (BF16, F16, F32, attention_oracle, check_attention, gen, packed, randn,
+                              rope_oracle)
 
 pytestmark = pytest.mark.gpu
 
@@ -244,3 +245,21 @@ def test_lengths_that_do_not_ascend_write_rows_only():
         for t, room in got:
             t.fill_(7)
             assert (room == 7).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("power", [19, 21, 23, 24, 25, 26])
+def test_attention_of_large_scores(D, power, dtype):
+    """Scores of 2^19 to 2^26 (in bits) whose maximum grows by up to 8 from step to step: where a
+    float32 ends at whole numbers, weights stay finite in the storage type."""
+    cu, N = packed([300, 40])
+    for grow in (4, 8):
+        q = torch.zeros(N, 2, D, dtype=dtype, device="cuda")
+        k = torch.zeros(N, 1, D, dtype=dtype, device="cuda")
+        q[:, :, 0], q[:, :, 1] = 2.0 ** (power - 13), 1
+        k[:, :, 0] = 2.0 ** 13
+        k[:, :, 1] = (64 + torch.arange(N, device="cuda") // 80 * grow).to(dtype)[:, None]
+        v = randn(gen(50), N, 1, D, dtype=dtype)
+        check_attention(q, k, v, cu, scale=math.log(2))
+        check_attention(q, k, v, cu, scale=math.log(2), causal=False)

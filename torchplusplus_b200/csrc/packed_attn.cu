@@ -45,12 +45,15 @@ constexpr int kThreads = 512;
 constexpr int kOutWarp0 = 8, kMmaWarp = 12, kTmaWarp = 14;  // (products: warps 12 and 13)
 constexpr int kItems = 8;
 constexpr float kMoves = 8.0f;  // growth of a row's maximum (log2) that moves its reference
-// P = 2^kLift exp(s - reference), and so are O and the sums.  f16 numbers end at 2^-24, and
+// A row's reference lies kLift (log2) below the maximum that set it.  f16 numbers end at 2^-24, and
 // thousands of keys that weigh less each may weigh something together: with 2^7, P stays
 // below 2^(kMoves + 7) = 2^15, and a weight loses at most 2^-32 of the row's largest (2^-25 without,
-// in one prompt of 6000 rows up to all of an output).  bf16 has the range of 32 bits.
+// in one prompt of 6000 rows up to all of an output).  bf16 has the range of 32 bits.  Maxima
+// from kFar on are their own references: where steps of float32 come near to 1, the room that
+// is left up to 2^16 is for roundings.
 template <typename T>
 constexpr float kLift = std::is_same<T, __half>::value ? 7.0f : 0.0f;
+constexpr float kFar = 1048576.0f;  // 2^20
 
 // TMEM (512 columns): O of both query tiles, then for each S (BKV columns) and, apart from
 // it, P (half as many), so that S of a later step is under way while a step's softmax runs:
@@ -628,11 +631,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (ns > 1) ok = ok && wait_short(&pv_done[i], ns & 1, p.err, 96);
         if (!ok) break;
         tc_fence_after();
-        const bool moves = !(mx <= m_ref + kMoves);  // (the first finite one too; NaN)
+        const float lift = fabsf(mx) < kFar ? kLift<T> : 0.f;
+        const bool moves = !(mx <= m_ref + (kMoves + lift));  // (the first finite one too; NaN)
         if (__any_sync(0xffffffffu, moves)) {
-          const float f = !moves ? 1.f : m_ref == -INFINITY ? 0.f : exp2f(m_ref - mx);
+          const float to = mx - lift;
+          const float f = !moves ? 1.f : m_ref == -INFINITY ? 0.f : exp2f(m_ref - to);
           l *= f;
-          m_ref = moves ? mx + (mx - mx) : m_ref;  // (infinite scores make a row NaN)
+          m_ref = moves ? to + (mx - mx) : m_ref;  // (infinite scores make a row NaN)
           __syncwarp();  // (the transfers below are the whole warp's)
           if (j > w.start(i)) {
 #pragma unroll 1
@@ -646,7 +651,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        const float nm = m_ref == -INFINITY ? 0.f : kLift<T> - m_ref;
+        const float nm = m_ref == -INFINITY ? 0.f : -m_ref;
         const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), nm2 = f2_pack(nm, nm);
         uint64_t ps[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll

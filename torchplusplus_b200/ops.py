@@ -1057,7 +1057,8 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     ascending).  causal: keys up to the row itself; window_left >= 0: none further than
     that before it.  Hq a multiple of Hkv, D 64 or 128.  Returns [N,Hq,D]; rows of no
     sequence are not written.  What a row does not see does not affect it, NaN and
-    infinities included.  out may be q, but share no memory with k and v."""
+    infinities included.  out may be q, but share no memory with k and v.  Scaled scores
+    from 9e7 in magnitude on may make a row NaN."""
     dt = _half_alike("q", q, k, v, out)
     if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape:
         raise ValueError("q must be [N, Hq, D], k and v [N, Hkv, D]")
