@@ -25,8 +25,8 @@
 //
 // Measured (bf16, heads over kv heads, D 128 unless said otherwise): one prompt of 32768,
 // 16/8: 3.2-3.4 ms, 1300-1360 TFLOP/s of the visible pairs' products (3.8 in long runs at the
-// power limit's clock); 6 to 8191, 32/8: 1.69 ms; 32 to 512, 16/8: 52 us (their bytes: 22); one
-// of 130: 11 us; 64-dim heads, one of 16384, 16/8: 0.77-0.9 ms by clock.  In long prompts a step
+// power limit's clock); 6 to 8191, 32/8, f16: 1.7-1.8 ms; 32 to 512, 16/8: 52-56 us (their bytes:
+// 22); one of 130: 9-11 us; 64-dim heads, one of 16384, 16/8: 0.77-0.9 ms by clock.  In long prompts a step
 // of both tiles (80 keys) takes some 2250 clocks, its products 1280: the tiles' softmaxes run
 // side by side, and their exponentials (1450 for both; the units' own rate gives 1280) are
 // followed by 800 to 950 of barriers, transfers and maxima.  Taking turns, so that one tile's
